@@ -81,6 +81,14 @@ SIGNATURES = {
     "fovi_norm_block_workspace_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
     "fovi_norm_block_backward": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
     "fovi_launch_count": (C.c_int64, []),
+    "fovi_layer_norm_forward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int64, _P, _P, C.c_float, _P, C.c_int, _P, _P]),
+    "fovi_layer_norm_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int]),
+    "fovi_layer_norm_backward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "fovi_rotary": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int64), _P, C.c_int64, C.c_int, C.POINTER(C.c_int32), _P, C.c_int,
+                              C.c_int, C.c_int, _P, _P]),
+    "fovi_attention_workspace_bytes": (C.c_int64, [C.c_int] * 8),
+    "fovi_attention_forward": (C.c_int, [_P, _P, _P] + [C.c_int] * 7 + [C.POINTER(C.c_int64), _P, _P, C.c_float, _P, _P, _P, C.c_int64, _P]),
+    "fovi_attention_backward": (C.c_int, [_P] * 5 + [C.c_int] * 7 + [C.POINTER(C.c_int64), _P, _P, C.c_float] + [_P] * 5 + [C.c_int64, _P]),
 }
 
 if not os.path.exists(LIB_PATH):

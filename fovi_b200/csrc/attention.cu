@@ -1,0 +1,386 @@
+// Cross attention of queries q [B, Lq, H, D] to an encoder's states k, v [B, Lk, Hkv, D], and its gradients, in float32 arithmetic on the CUDA cores:
+// float32 inputs, and every shape, stride and alignment that the tensor-core kernels do not take.
+//   s = scale * q k^T (masked keys: -inf),  p = softmax(s),  o = p v;  a row without a key gives 0
+//   delta = rowsum(dy * o),  ds = p * (dy v^T - delta),  dq = scale * ds k,  dk = scale * ds^T q,  dv = p^T dy, the last two summed over the heads that
+//   share a state head
+// Tiles of 64 x 64 scores, 16 x 16 threads with 4 x 4 each, operands in shared memory as float32.  The forward pass goes over the keys once with the running
+// maximum and sum of every row; the backward pass recomputes p from the row's logarithm of the sum.  dq goes by query tiles and dk, dv by key tiles,
+// each by one CTA in a fixed order: no atomics, the same bits every time.  Masked keys are read as zeros, whatever they hold.
+#include <cuda_bf16.h>
+
+#include "attention.cuh"
+
+using fovi::AttnArgs;
+using fovi::key_end;
+
+namespace {
+
+constexpr int T = 64;                    // queries and keys of a tile
+constexpr int THREADS = 256;
+constexpr int PP = T + 4;                // pitch of a tile of scores
+constexpr float INF = __builtin_huge_valf();
+
+template <int DP> constexpr int PITCH = DP + 4;        // rows 4 floats apart modulo 32 banks: eight threads' float4 reads of one column do not collide
+
+__device__ __forceinline__ bool key_ok(const AttnArgs& a, int b, int key, int end) {
+  return key < end && (!a.mask || __ldg(a.mask + (int64_t)b * a.Lk + key));
+}
+
+// Rows [r0, r0 + 64) of one head as float32, zeros behind n and D, and where `ok` says no.
+template <typename E, int DP>
+__device__ __forceinline__ void load_tile(float* dst, const E* src, int64_t sl, int r0, int n, int D, const unsigned char* ok = nullptr) {
+  for (int i = threadIdx.x; i < T * DP; i += THREADS) {
+    const int r = i / DP, d = i - r * DP;
+    dst[r * PITCH<DP> + d] = r0 + r < n && d < D && (!ok || ok[r]) ? ld_as_float(src + (int64_t)(r0 + r) * sl + d) : 0.f;
+  }
+}
+
+// acc[i][j] = <A row ty + 16 i, B row tx + 16 j>
+template <int DP>
+__device__ __forceinline__ void dot_tile(const float* A, const float* B, float (&acc)[4][4]) {
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = *reinterpret_cast<const float4*>(A + (ty + 16 * i) * PITCH<DP> + d);
+      y[i] = *reinterpret_cast<const float4*>(B + (tx + 16 * i) * PITCH<DP> + d);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]); acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]); acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+      }
+  }
+}
+
+// acc[i][c] += sum over r of P[ty + 16 i][r] * V[r][channel c of this thread], channels 64 jj + 4 tx .. + 3
+template <int DP>
+__device__ __forceinline__ void mix_tile(const float* P, const float* V, float (&acc)[4][DP / 16]) {
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll 2
+  for (int r = 0; r < T; r += 4) {
+    float p[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(p[i]) = *reinterpret_cast<const float4*>(P + (ty + 16 * i) * PP + r);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int jj = 0; jj < DP / 64; ++jj) {
+        const float4 v = *reinterpret_cast<const float4*>(V + (r + q) * PITCH<DP> + 64 * jj + 4 * tx);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[i][4 * jj] = fmaf(p[i][q], v.x, acc[i][4 * jj]); acc[i][4 * jj + 1] = fmaf(p[i][q], v.y, acc[i][4 * jj + 1]);
+          acc[i][4 * jj + 2] = fmaf(p[i][q], v.z, acc[i][4 * jj + 2]); acc[i][4 * jj + 3] = fmaf(p[i][q], v.w, acc[i][4 * jj + 3]);
+        }
+      }
+  }
+}
+
+// The sixteen threads of a row are half a warp.
+__device__ __forceinline__ float row_max(float v) {
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float row_sum(float v) {
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename E, int DP>
+__device__ __forceinline__ void store_tile(E* dst, int64_t pitch, int r0, int n, int D, const float (&acc)[4][DP / 16], const float (&f)[4]) {
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + ty + 16 * i;
+    if (r >= n) continue;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      const int d = 64 * (c >> 2) + 4 * tx + (c & 3);
+      if (d < D) dst[r * pitch + d] = from_float<E>(acc[i][c] * f[i]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ forward: a CTA per (64 queries, head, sample)
+template <typename E, int DP>
+__global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a) {
+  extern __shared__ float4 smem4[];
+  float* Q = reinterpret_cast<float*>(smem4);
+  float *K = Q + T * PITCH<DP>, *V = K + T * PITCH<DP>, *P = V + T * PITCH<DP>;
+  __shared__ unsigned char ok[T];
+  const int n_qt = (a.Lq + T - 1) / T, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int qt = blockIdx.x % n_qt, h = blockIdx.x / n_qt % a.H, b = blockIdx.x / n_qt / a.H, end = key_end(a, b);
+  const E* k = (const E*)a.k + b * a.k_sb + (h / a.group) * a.k_sh;
+  const E* v = (const E*)a.v + b * a.v_sb + (h / a.group) * a.v_sh;
+  load_tile<E, DP>(Q, (const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, qt * T, a.Lq, a.D);
+  float m[4], l[4], acc[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INF; l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+  }
+  for (int k0 = 0; k0 < end; k0 += T) {
+    __syncthreads();
+    if (threadIdx.x < T) ok[threadIdx.x] = key_ok(a, b, k0 + threadIdx.x, end);
+    __syncthreads();
+    load_tile<E, DP>(K, k, a.k_sl, k0, a.Lk, a.D, ok);
+    load_tile<E, DP>(V, v, a.v_sl, k0, a.Lk, a.D, ok);
+    __syncthreads();
+    float s[4][4];
+    dot_tile<DP>(Q, K, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float top = -INF;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = ok[tx + 16 * j] ? s[i][j] * a.scale_log2 : -INF;
+        top = fmaxf(top, s[i][j]);
+      }
+      const float m_new = fmaxf(m[i], row_max(top)), base = m_new == -INF ? 0.f : m_new;      // no key yet: exp2(-inf - 0) = 0
+      const float f = exp2f(m[i] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = exp2f(s[i][j] - base);
+        P[(ty + 16 * i) * PP + tx + 16 * j] = p;
+        sum += p;
+      }
+      l[i] = l[i] * f + row_sum(sum);
+      m[i] = m_new;
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) acc[i][c] *= f;
+    }
+    __syncthreads();
+    mix_tile<DP>(P, V, acc);
+  }
+  float inv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    inv[i] = m[i] == -INF ? 0.f : 1.f / l[i];
+    const int r = qt * T + ty + 16 * i;
+    if (a.lse && tx == 0 && r < a.Lq) a.lse[((int64_t)b * a.H + h) * a.Lq + r] = m[i] == -INF ? INF : m[i] + log2f(l[i]);
+  }
+  store_tile<E, DP>((E*)a.out + ((int64_t)b * a.Lq * a.H + h) * a.D, (int64_t)a.H * a.D, qt * T, a.Lq, a.D, acc, inv);
+}
+
+// ------------------------------------------------------------------------------------------------------------ backward
+// A warp per row: delta = <dy, o>.
+template <typename E>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);        // b, l, h
+  if (row >= (int64_t)a.B * a.Lq * a.H) return;
+  const int h = (int)(row % a.H), lane = threadIdx.x & 31;
+  const int64_t bl = row / a.H, b = bl / a.Lq, l = bl - b * a.Lq;
+  const E* o = (const E*)a.o + row * a.D;
+  const E* g = (const E*)a.dy + b * a.g_sb + l * a.g_sl + h * a.g_sh;
+  float s = 0.f;
+  for (int d = lane; d < a.D; d += 32) s = fmaf(ld_as_float(o + d), ld_as_float(g + d), s);
+  for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+  if (lane == 0) a.delta[(b * a.H + h) * a.Lq + l] = s;
+}
+
+// A CTA per (64 queries, head, sample): dq.
+template <typename E, int DP>
+__global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
+  extern __shared__ float4 smem4[];
+  float* Q = reinterpret_cast<float*>(smem4);
+  float *G = Q + T * PITCH<DP>, *K = G + T * PITCH<DP>, *V = K + T * PITCH<DP>, *P = V + T * PITCH<DP>;
+  __shared__ unsigned char ok[T];
+  const int n_qt = (a.Lq + T - 1) / T, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int qt = blockIdx.x % n_qt, h = blockIdx.x / n_qt % a.H, b = blockIdx.x / n_qt / a.H, end = key_end(a, b);
+  const E* k = (const E*)a.k + b * a.k_sb + (h / a.group) * a.k_sh;
+  const E* v = (const E*)a.v + b * a.v_sb + (h / a.group) * a.v_sh;
+  load_tile<E, DP>(Q, (const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, qt * T, a.Lq, a.D);
+  load_tile<E, DP>(G, (const E*)a.dy + b * a.g_sb + h * a.g_sh, a.g_sl, qt * T, a.Lq, a.D);
+  float lse[4], delta[4], acc[4][DP / 16], f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = qt * T + ty + 16 * i;
+    const int64_t at = ((int64_t)b * a.H + h) * a.Lq + r;
+    lse[i] = r < a.Lq ? __ldg(a.lse + at) : INF;
+    delta[i] = r < a.Lq ? a.delta[at] : 0.f;
+    f[i] = a.scale;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+  }
+  for (int k0 = 0; k0 < end; k0 += T) {
+    __syncthreads();
+    if (threadIdx.x < T) ok[threadIdx.x] = key_ok(a, b, k0 + threadIdx.x, end);
+    __syncthreads();
+    load_tile<E, DP>(K, k, a.k_sl, k0, a.Lk, a.D, ok);
+    load_tile<E, DP>(V, v, a.v_sl, k0, a.Lk, a.D, ok);
+    __syncthreads();
+    float s[4][4], dp[4][4];
+    dot_tile<DP>(Q, K, s);
+    dot_tile<DP>(G, V, dp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = ok[tx + 16 * j] ? exp2f(s[i][j] * a.scale_log2 - lse[i]) : 0.f;
+        P[(ty + 16 * i) * PP + tx + 16 * j] = ok[tx + 16 * j] ? p * (dp[i][j] - delta[i]) : 0.f;
+      }
+    __syncthreads();
+    mix_tile<DP>(P, K, acc);
+  }
+  store_tile<E, DP>((E*)a.dq + ((int64_t)b * a.Lq * a.H + h) * a.D, (int64_t)a.H * a.D, qt * T, a.Lq, a.D, acc, f);
+}
+
+// A CTA per (64 keys, state head, sample): dk and dv, over all queries of all heads that read the state head.
+template <typename E, int DP>
+__global__ void __launch_bounds__(THREADS) attn_dkv_kernel(const AttnArgs a) {
+  extern __shared__ float4 smem4[];
+  float* K = reinterpret_cast<float*>(smem4);
+  float *V = K + T * PITCH<DP>, *Q = V + T * PITCH<DP>, *G = Q + T * PITCH<DP>, *P = G + T * PITCH<DP>, *S = P + T * PP;
+  __shared__ unsigned char ok[T];
+  const int n_kt = (a.Lk + T - 1) / T, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int kt = blockIdx.x % n_kt, hk = blockIdx.x / n_kt % a.Hkv, b = blockIdx.x / n_kt / a.Hkv, end = key_end(a, b);
+  float dk[4][DP / 16], dv[4][DP / 16], f[4], one[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = a.scale; one[i] = 1.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
+  }
+  if (threadIdx.x < T) ok[threadIdx.x] = key_ok(a, b, kt * T + threadIdx.x, end);
+  __syncthreads();
+  load_tile<E, DP>(K, (const E*)a.k + b * a.k_sb + hk * a.k_sh, a.k_sl, kt * T, a.Lk, a.D, ok);
+  load_tile<E, DP>(V, (const E*)a.v + b * a.v_sb + hk * a.v_sh, a.v_sl, kt * T, a.Lk, a.D, ok);
+  const int first = kt * T < end ? hk * a.group : (hk + 1) * a.group;         // a tile behind the sample's length has gradients of zero
+  for (int h = first; h < (hk + 1) * a.group; ++h)
+    for (int q0 = 0; q0 < a.Lq; q0 += T) {
+      __syncthreads();
+      load_tile<E, DP>(Q, (const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, q0, a.Lq, a.D);
+      load_tile<E, DP>(G, (const E*)a.dy + b * a.g_sb + h * a.g_sh, a.g_sl, q0, a.Lq, a.D);
+      __syncthreads();
+      float s[4][4], dp[4][4];
+      dot_tile<DP>(K, Q, s);
+      dot_tile<DP>(V, G, dp);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = q0 + tx + 16 * j;
+        const int64_t at = ((int64_t)b * a.H + h) * a.Lq + r;
+        const float lse = r < a.Lq ? __ldg(a.lse + at) : INF, delta = r < a.Lq ? a.delta[at] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = ok[ty + 16 * i];
+          const float p = in ? exp2f(s[i][j] * a.scale_log2 - lse) : 0.f;
+          P[(ty + 16 * i) * PP + tx + 16 * j] = p;
+          S[(ty + 16 * i) * PP + tx + 16 * j] = in ? p * (dp[i][j] - delta) : 0.f;
+        }
+      }
+      __syncthreads();
+      mix_tile<DP>(P, G, dv);
+      mix_tile<DP>(S, Q, dk);
+    }
+  // a masked key's weights are zeros, but zero times a query that is not a number is none: its gradients are set to zero
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (!ok[ty + 16 * i]) {
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
+    }
+  const int64_t at = ((int64_t)b * a.Lk * a.Hkv + hk) * a.D, pitch = (int64_t)a.Hkv * a.D;
+  store_tile<E, DP>((E*)a.dk + at, pitch, kt * T, a.Lk, a.D, dk, f);
+  store_tile<E, DP>((E*)a.dv + at, pitch, kt * T, a.Lk, a.D, dv, one);
+}
+
+// ------------------------------------------------------------------------------------------------------------ host
+template <int DP> constexpr size_t FWD_SMEM = (3 * T * PITCH<DP> + T * PP) * sizeof(float);
+template <int DP> constexpr size_t DQ_SMEM = (4 * T * PITCH<DP> + T * PP) * sizeof(float);
+template <int DP> constexpr size_t DKV_SMEM = (4 * T * PITCH<DP> + 2 * T * PP) * sizeof(float);
+
+template <typename Kernel>
+int launch(Kernel kernel, int64_t blocks, size_t smem, cudaStream_t st, const AttnArgs& a, const char* name) {
+  if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;
+  if (smem) FOVI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<(int)blocks, THREADS, smem, st>>>(a);
+  return fovi::after_launch(name);
+}
+
+template <typename E, int DP>
+int forward(const AttnArgs& a, cudaStream_t st) {
+  return launch(attn_forward_kernel<E, DP>, (int64_t)((a.Lq + T - 1) / T) * a.H * a.B, FWD_SMEM<DP>, st, a, "attn_forward_kernel");
+}
+
+template <typename E, int DP>
+int backward(const AttnArgs& a, cudaStream_t st) {
+  int rc = launch(attn_delta_kernel<E>, ((int64_t)a.B * a.Lq * a.H + 7) / 8, 0, st, a, "attn_delta_kernel");
+  if (!rc && a.dq) rc = launch(attn_dq_kernel<E, DP>, (int64_t)((a.Lq + T - 1) / T) * a.H * a.B, DQ_SMEM<DP>, st, a, "attn_dq_kernel");
+  if (!rc && a.dk) rc = launch(attn_dkv_kernel<E, DP>, (int64_t)((a.Lk + T - 1) / T) * a.Hkv * a.B, DKV_SMEM<DP>, st, a, "attn_dkv_kernel");
+  return rc;
+}
+
+bool shape_ok(int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides, int n) {
+  if (!fovi::valid_dtype(dtype) || B < 0 || Lq < 0 || Lk < 0 || H < 1 || Hkv < 1 || D < 1 || H % Hkv || !strides) return false;
+  for (int i = 0; i < n; ++i)
+    if (strides[i] < 0) return false;
+  return true;
+}
+
+AttnArgs arguments(const void* q, const void* k, const void* v, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* s, const int32_t* lengths,
+                   const uint8_t* mask, float scale) {
+  AttnArgs a = {};
+  a.q = q; a.k = k; a.v = v; a.lengths = lengths; a.mask = mask;
+  a.q_sb = s[0]; a.q_sl = s[1]; a.q_sh = s[2]; a.k_sb = s[3]; a.k_sl = s[4]; a.k_sh = s[5]; a.v_sb = s[6]; a.v_sl = s[7]; a.v_sh = s[8];
+  a.B = B; a.Lq = Lq; a.Lk = Lk; a.H = H; a.Hkv = Hkv; a.D = D; a.group = H / Hkv;
+  a.scale = scale; a.scale_log2 = scale * 1.44269504088896340736f;
+  return a;
+}
+
+}  // namespace
+
+extern "C" int64_t fovi_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, int backward) {
+  const int64_t none = 0;
+  if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, &none, 0)) return -1;
+  return backward ? (int64_t)B * H * Lq * 4 : 0;
+}
+
+extern "C" int fovi_attention_forward(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides,
+                                      const int32_t* key_lengths, const uint8_t* key_mask, float scale, void* o, float* lse, void* work, int64_t work_bytes,
+                                      void* stream) {
+  if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, strides, 9)) return FOVI_ERR_INVALID_ARGUMENT;
+  if (D > fovi::ATT_MAX_DIM) return FOVI_ERR_UNSUPPORTED;
+  if ((int64_t)B * Lq == 0) return FOVI_OK;
+  if (!q || !o || (Lk > 0 && (!k || !v))) return FOVI_ERR_INVALID_ARGUMENT;
+  const int64_t need = fovi_attention_workspace_bytes(dtype, B, Lq, Lk, H, Hkv, D, 0);
+  if (need > 0 && (!work || work_bytes < need)) return FOVI_ERR_INVALID_ARGUMENT;
+  AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
+  a.out = o; a.lse = lse;
+  auto st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == FOVI_BF16) return D <= 64 ? forward<__nv_bfloat16, 64>(a, st) : forward<__nv_bfloat16, 128>(a, st);
+  return D <= 64 ? forward<float, 64>(a, st) : forward<float, 128>(a, st);
+}
+
+extern "C" int fovi_attention_backward(const void* q, const void* k, const void* v, const void* o, const void* dy, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D,
+                                       const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, float scale, const float* lse, void* dq, void* dk,
+                                       void* dv, void* work, int64_t work_bytes, void* stream) {
+  if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, strides, 12) || !dk != !dv) return FOVI_ERR_INVALID_ARGUMENT;
+  if (D > fovi::ATT_MAX_DIM) return FOVI_ERR_UNSUPPORTED;
+  auto st = reinterpret_cast<cudaStream_t>(stream);
+  if ((int64_t)B * Lq == 0) {       // no query: no gradient reaches the states
+    const size_t bytes = (size_t)B * Lk * Hkv * D * fovi::dtype_size(dtype);
+    if (dk && bytes) {
+      FOVI_CUDA(cudaMemsetAsync(dk, 0, bytes, st));
+      FOVI_CUDA(cudaMemsetAsync(dv, 0, bytes, st));
+    }
+    return FOVI_OK;
+  }
+  if (!q || !o || !dy || !lse || (Lk > 0 && (!k || !v))) return FOVI_ERR_INVALID_ARGUMENT;
+  const int64_t need = fovi_attention_workspace_bytes(dtype, B, Lq, Lk, H, Hkv, D, 1);
+  if (need > 0 && (!work || work_bytes < need)) return FOVI_ERR_INVALID_ARGUMENT;
+  AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
+  a.o = o; a.dy = dy; a.lse = const_cast<float*>(lse); a.dq = dq; a.dk = Lk > 0 ? dk : nullptr; a.dv = dv; a.delta = static_cast<float*>(work);
+  a.g_sb = strides[9]; a.g_sl = strides[10]; a.g_sh = strides[11];
+  if (dtype == FOVI_BF16) return D <= 64 ? backward<__nv_bfloat16, 64>(a, st) : backward<__nv_bfloat16, 128>(a, st);
+  return D <= 64 ? backward<float, 64>(a, st) : backward<float, 128>(a, st);
+}

@@ -1,6 +1,8 @@
 """Tensor-level wrappers over the C ABI: plans own device tables, functions take torch CUDA
 tensors, pass raw pointers and the current stream, and allocate outputs with torch."""
 import ctypes as C
+import functools
+import math
 import os
 import warnings
 
@@ -43,7 +45,7 @@ def _dt(t):
 # the host routines; its launches fail in torch.cuda.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-_I64x4 = C.c_int64 * 4
+_I64x3, _I64x4, _I64x9, _I64x12 = (C.c_int64 * n for n in (3, 4, 9, 12))
 
 
 def _stream():
@@ -795,6 +797,187 @@ def column_sum(x):
     with _on(x.device):
         check(lib.fovi_column_sum(_ptr(x), _dt(x.dtype), x.numel() // Cc, Cc, _ptr(out), _stream()), "fovi_column_sum")
     return out
+
+
+def _f32_param(t, n, name):
+    """A parameter as the token kernels read it: float32, contiguous, n values; None passes."""
+    if t is None:
+        return None
+    if t.numel() != n:
+        raise ValueError(f"{name} has {t.numel()} values, {n} are wanted")
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.detach().to(torch.float32).contiguous()
+
+
+def _rows(x, c):
+    """x [..., C] as (rows of C contiguous values a fixed stride apart, their number, the stride); a copy where its strides do not give that."""
+    n = x.numel() // c if c else 0
+    if x.is_contiguous():
+        return x, n, c
+    x2 = x.reshape(n, c)
+    if x2.stride(1) != 1 and c > 1:
+        x2 = x2.contiguous()
+    return x2, n, x2.stride(0)
+
+
+def _same_device(first, *others):
+    _need_cuda(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and on {t.device}: all of a call's tensors are on one device")
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None, want_stats=False):
+    """Layer norm over the last axis of x [..., C] (float32 or bf16); weight, bias [C].  Returns y of x's shape, contiguous, in `out_dtype` (default: x's), and with
+    `want_stats` also the float32 [rows, 2] mean and 1/std that layer_norm_backward takes."""
+    _same_device(x, weight, bias)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer norm needs a last axis of at least one value, got the shape {tuple(x.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"eps is {eps}")
+    c = x.shape[-1]
+    w, b = _f32_param(weight, c, "weight"), _f32_param(bias, c, "bias")
+    xr, n, stride = _rows(x, c)
+    y = torch.empty(x.shape, dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=x.device) if want_stats else None
+    with _on(x.device):
+        check(lib.fovi_layer_norm_forward(_ptr(xr), _dt(x.dtype), n, c, stride, None if w is None else _ptr(w), None if b is None else _ptr(b), eps, _ptr(y),
+                                          _dt(y.dtype), None if stats is None else _ptr(stats), _stream()), "fovi_layer_norm_forward")
+    return (y, stats) if want_stats else y
+
+
+def layer_norm_backward(x, grad, weight, stats, need=(True, True, True)):
+    """Gradients of layer_norm with respect to (x, weight, bias), from the gradient of its result and its stats; None where `need` says no.  Those of the parameters are
+    float32 [C], summed in a fixed order."""
+    _same_device(x, grad, weight, stats)
+    c = x.shape[-1]
+    if grad.shape != x.shape:
+        raise ValueError(f"the gradient has the shape {tuple(grad.shape)}, the result {tuple(x.shape)}")
+    if stats.dtype != torch.float32 or not stats.is_contiguous() or stats.numel() * c != 2 * x.numel():
+        raise ValueError("stats is not what layer_norm gave for x")
+    w = _f32_param(weight, c, "weight")
+    xr, n, stride = _rows(x, c)
+    gr, _, g_stride = _rows(grad, c)
+    dev = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+    dw, db = (torch.empty(c, dtype=torch.float32, device=dev) if m else None for m in need[1:])
+    size = lib.fovi_layer_norm_workspace_bytes(n, c) if need[1] or need[2] else 0
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    with _on(dev):
+        check(lib.fovi_layer_norm_backward(_ptr(xr), _dt(x.dtype), n, c, stride, _ptr(gr), _dt(grad.dtype), g_stride, None if w is None else _ptr(w), _ptr(stats),
+                                           None if dx is None else _ptr(dx), None if dw is None else _ptr(dw), None if db is None else _ptr(db),
+                                           None if work is None else _ptr(work), size, _stream()), "fovi_layer_norm_backward")
+    return dx, dw, db
+
+
+@functools.lru_cache(maxsize=256)
+def _sections(pairs_per_axis):
+    return (C.c_int32 * len(pairs_per_axis))(*pairs_per_axis)
+
+
+def rotary(x, positions, frequencies, pairs_per_axis, prefix=0, interleaved=False, inverse=False):
+    """x [B, L, H, D] turned by positions [L - prefix, axes] or [B, L - prefix, axes] and frequencies [P], both float32; the first pairs_per_axis[0] pairs belong to axis 0,
+    and so on (see fovi_rotary).  Returns a contiguous tensor of x's type."""
+    _same_device(x, positions, frequencies)
+    if x.dim() != 4 or x.shape[2] < 1 or x.shape[3] < 1:
+        raise ValueError(f"x has the shape {tuple(x.shape)}; [batch, tokens, heads, channels] is wanted")
+    B, L, H, D = x.shape
+    pairs = tuple(int(n) for n in pairs_per_axis)
+    axes = len(pairs)
+    if not 1 <= axes <= 4 or min(pairs) < 0 or 2 * sum(pairs) > D:
+        raise ValueError(f"pairs_per_axis {pairs}: one to four axes whose pairs fit the {D} channels of a head")
+    if not 0 <= prefix <= L:
+        raise ValueError(f"prefix is {prefix}, x has {L} tokens")
+    if tuple(positions.shape) not in ((L - prefix, axes), (B, L - prefix, axes)):
+        raise ValueError(f"positions have the shape {tuple(positions.shape)}; {(L - prefix, axes)} or {(B, L - prefix, axes)} is wanted")
+    if positions.dtype != torch.float32 or frequencies.dtype != torch.float32:
+        raise TypeError("positions and frequencies are float32")
+    if frequencies.numel() != sum(pairs):
+        raise ValueError(f"{frequencies.numel()} frequencies for {sum(pairs)} pairs")
+    if x.stride(3) != 1 and D > 1:
+        x = x.contiguous()
+    shared = positions.dim() == 2 or positions.stride(0) == 0
+    if not (positions if positions.dim() == 2 or not shared else positions[:1]).is_contiguous():
+        positions, shared = positions.contiguous(), positions.dim() == 2
+    frequencies = frequencies.contiguous()
+    y = torch.empty((B, L, H, D), dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        check(lib.fovi_rotary(_ptr(x), _dt(x.dtype), B, L, H, D, _I64x3(*x.stride()[:3]), _ptr(positions), 0 if shared else positions.stride(0), axes, _sections(pairs),
+                              _ptr(frequencies), prefix, bool(interleaved), bool(inverse), _ptr(y), _stream()), "fovi_rotary")
+    return y
+
+
+def _attention_inputs(q, k, v, key_lengths, key_mask, scale):
+    """Checked arguments of an attention call: tensors with contiguous channels, (B, Lq, Lk, H, Hkv, D), scale."""
+    _same_device(q, k, v, key_lengths, key_mask)
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: [B, Lq, H, D] and two of [B, Lk, Hkv, D] are wanted")
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise ValueError(f"{H} query heads cannot share {Hkv} state heads")
+    if not 1 <= D <= 128:
+        raise ValueError(f"{D} channels a head; 1 to 128 are supported")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError(f"q, k and v have the types {q.dtype}, {k.dtype}, {v.dtype}; one type is wanted")
+    if key_lengths is not None:
+        if key_lengths.shape != (B,) or key_lengths.is_floating_point() or key_lengths.dtype == torch.bool:
+            raise ValueError(f"key_lengths: whole numbers, one for each of {B} samples")
+        if key_lengths.dtype != torch.int32 or not key_lengths.is_contiguous():
+            key_lengths = key_lengths.clamp(0, Lk).to(torch.int32).contiguous()
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or key_mask.shape != (B, Lk):
+            raise ValueError(f"key_mask: truth values (true: the key is read) of the shape {(B, Lk)}")
+        key_mask = key_mask.contiguous()
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale is {scale}")
+    if D > 1:
+        q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+    return q, k, v, key_lengths, key_mask, (B, Lq, Lk, H, Hkv, D), scale
+
+
+def attention(q, k, v, key_lengths=None, key_mask=None, scale=None, want_lse=False):
+    """softmax(scale * q k^T) v: q [B, Lq, H, D] over k, v [B, Lk, Hkv, D] (float32 or bf16, any strides), Hkv a divisor of H, D <= 128; scale: 1 / sqrt(D) by
+    default.  Keys at and behind key_lengths [B], and where key_mask [B, Lk] is false, are not read; a row without a key gives 0.  Returns contiguous [B, Lq, H, D]
+    of q's type and with `want_lse` also what attention_backward takes, float32 [B, H, Lq]."""
+    q, k, v, lengths, mask, dims, scale = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
+    B, Lq, Lk, H, Hkv, D = dims
+    dev, dt = q.device, _dt(q.dtype)
+    o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=dev) if want_lse else None
+    size = lib.fovi_attention_workspace_bytes(dt, *dims, 0)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+    with _on(dev):
+        check(lib.fovi_attention_forward(_ptr(q), _ptr(k), _ptr(v), dt, *dims, _I64x9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
+                                         None if lengths is None else _ptr(lengths), None if mask is None else _ptr(mask), scale, _ptr(o),
+                                         None if lse is None else _ptr(lse), None if work is None else _ptr(work), size, _stream()), "fovi_attention_forward")
+    return (o, lse) if want_lse else o
+
+
+def attention_backward(q, k, v, o, grad, lse, key_lengths=None, key_mask=None, scale=None, need=(True, True, True)):
+    """Gradients of attention with respect to (q, k, v), contiguous, from its result, its lse and the gradient of its result.  need: which are wanted (those of k and v are made
+    together)."""
+    q, k, v, lengths, mask, dims, scale = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
+    B, Lq, Lk, H, Hkv, D = dims
+    _same_device(q, o, grad, lse)
+    if grad.shape != q.shape or o.shape != q.shape or o.dtype != q.dtype or not o.is_contiguous() or tuple(lse.shape) != (B, H, Lq) or not lse.is_contiguous():
+        raise ValueError("o, lse: not what attention gave for these inputs; grad: of o's shape")
+    dev, dt = q.device, _dt(q.dtype)
+    if grad.dtype != q.dtype:
+        grad = grad.to(q.dtype)
+    if grad.stride(3) != 1 and D > 1:
+        grad = grad.contiguous()
+    dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev) if need[0] else None
+    dk, dv = (torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev) if need[1] or need[2] else None for _ in range(2))
+    size = lib.fovi_attention_workspace_bytes(dt, *dims, 1)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+    with _on(dev):
+        check(lib.fovi_attention_backward(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(grad), dt, *dims,
+                                          _I64x12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *grad.stride()[:3]),
+                                          None if lengths is None else _ptr(lengths), None if mask is None else _ptr(mask), scale, _ptr(lse),
+                                          None if dq is None else _ptr(dq), None if dk is None else _ptr(dk), None if dv is None else _ptr(dv),
+                                          None if work is None else _ptr(work), size, _stream()), "fovi_attention_backward")
+    return dq, dk if need[1] else None, dv if need[2] else None
 
 
 def launch_count():

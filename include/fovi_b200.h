@@ -453,6 +453,45 @@ int64_t fovi_knn_norm_stat_groups(int mode, int B, int C, int N, int groups);
 int fovi_knn_norm_forward(const void* x, int x_dtype, int layout, int B, int C, int N, int mode, int groups, const float* weight,
                           const float* bias, float eps, int relu, float* stats, void* y, int y_dtype, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Operators on tokens [B, L, ...]: what stands behind a patch embedding in a vision transformer
+ * (fovi/arch/vit.py:351-381, knnvit.py:420-464): layer norm, rotary positions, attention.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Layer norm over the last axis.  x: `rows` rows of C elements, x_stride elements apart; y: contiguous [rows, C];
+ * weight, bias: DEVICE float32 [C] or NULL; stats: [rows][2] float32, mean and 1/std of every row, or NULL.
+ * y = (x - mean) / sqrt(var + eps) * weight + bias, biased variance, float32 arithmetic. */
+int fovi_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int C, int64_t x_stride, const float* weight, const float* bias, float eps, void* y,
+                            int y_dtype, float* stats, void* stream);
+/* Its gradients from dy (y_dtype, rows dy_stride elements apart) and the forward's stats: dx (x_dtype, contiguous), dweight, dbias (float32 [C]); each may
+ * be NULL.  work: fovi_layer_norm_workspace_bytes bytes, where dweight or dbias is wanted.  Sums in a fixed order: the same bits every time. */
+int64_t fovi_layer_norm_workspace_bytes(int64_t rows, int C);
+int fovi_layer_norm_backward(const void* x, int x_dtype, int64_t rows, int C, int64_t x_stride, const void* dy, int y_dtype, int64_t dy_stride,
+                             const float* weight, const float* stats, void* dx, float* dweight, float* dbias, void* work, int64_t work_bytes, void* stream);
+
+/* Rotary positions with up to four axes.  x: [B, L, H, D], element strides x_strides[3] of batch, token and head, channels contiguous; y: contiguous, same type.
+ * Pair p turns by position[axis of p] * frequencies[p]; the first pairs_per_axis[0] pairs belong to axis 0, the next to axis 1, and so on (HOST [axes], sum P,
+ * 2P <= D); a pair is the channels (p, p + P), or (2p, 2p + 1) with `interleaved`.  Channels from 2P on and the first `prefix` tokens pass unchanged.
+ * positions: DEVICE float32 [L - prefix, axes], pos_batch_stride elements from one sample's to the next's (0: one table for all); frequencies: DEVICE float32 [P].
+ * inverse: turn the other way (the gradient). */
+int fovi_rotary(const void* x, int dtype, int B, int L, int H, int D, const int64_t* x_strides, const float* positions, int64_t pos_batch_stride, int axes,
+                const int32_t* pairs_per_axis, const float* frequencies, int prefix, int interleaved, int inverse, void* y, void* stream);
+
+/* Cross attention: q [B, Lq, H, D] over k, v [B, Lk, Hkv, D], Hkv a divisor of H (head h reads state head h / (H / Hkv)), D <= 128.
+ * strides: element strides of batch, token and head of q, k, v (and dy), channels contiguous.  A key is masked where it lies at or behind key_lengths[b] (DEVICE
+ * int32 [B], taken into 0 .. Lk; or NULL) or key_mask[b, key] is 0 (DEVICE bytes, contiguous [B, Lk]; or NULL); what k and v hold there has no effect, not a number
+ * included.  o: contiguous [B, Lq, H, D]; a row without a key gives 0.  lse: float32 [B, H, Lq] for the backward pass, or NULL: the base-2 logarithm of the row's
+ * sum of exp(scale * q k), +inf for a row without a key.  work: fovi_attention_workspace_bytes bytes (backward: 0 or 1), 16-byte aligned.  Softmax statistics, sums and accumulators
+ * are float32; bf16 inputs' weights are rounded to bf16 in front of the second product. */
+int64_t fovi_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, int backward);
+int fovi_attention_forward(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides,
+                           const int32_t* key_lengths, const uint8_t* key_mask, float scale, void* o, float* lse, void* work, int64_t work_bytes, void* stream);
+/* The gradients dq (like o), dk and dv (contiguous [B, Lk, Hkv, D], both or neither), summed over the heads that share a state head; strides: [12], dy last.  dq, or dk and
+ * dv, may be NULL.  Fixed order of all sums: the same bits every time. */
+int fovi_attention_backward(const void* q, const void* k, const void* v, const void* o, const void* dy, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D,
+                            const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, float scale, const float* lse, void* dq, void* dk, void* dv,
+                            void* work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
