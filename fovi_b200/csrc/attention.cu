@@ -8,7 +8,7 @@
 // each by one CTA in a fixed order: no atomics, the same bits every time.  Masked keys are read as zeros, whatever they hold.
 #include <cuda_bf16.h>
 
-#include "attention.cuh"
+#include "attention_tc.cuh"
 
 using fovi::AttnArgs;
 using fovi::key_end;
@@ -357,6 +357,7 @@ extern "C" int fovi_attention_forward(const void* q, const void* k, const void* 
   AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
   a.out = o; a.lse = lse;
   auto st = reinterpret_cast<cudaStream_t>(stream);
+  if (fovi::attention_tc_takes(a, dtype, false)) return fovi::launch_attention_tc_forward(a, st, false);
   if (dtype == FOVI_BF16) return D <= 64 ? forward<__nv_bfloat16, 64>(a, st) : forward<__nv_bfloat16, 128>(a, st);
   return D <= 64 ? forward<float, 64>(a, st) : forward<float, 128>(a, st);
 }
@@ -383,4 +384,15 @@ extern "C" int fovi_attention_backward(const void* q, const void* k, const void*
   a.g_sb = strides[9]; a.g_sl = strides[10]; a.g_sh = strides[11];
   if (dtype == FOVI_BF16) return D <= 64 ? backward<__nv_bfloat16, 64>(a, st) : backward<__nv_bfloat16, 128>(a, st);
   return D <= 64 ? backward<float, 64>(a, st) : backward<float, 128>(a, st);
+}
+
+extern "C" int fovi_attention_check(void* stream) { return fovi::attention_tc_check(reinterpret_cast<cudaStream_t>(stream)); }
+
+extern "C" int fovi_attention_forward_selftest_wait_timeout(const void* q, const void* k, const void* v, int B, int Lq, int Lk, int H, int Hkv, int D,
+                                                            const int64_t* strides, float scale, void* o, void* stream) {
+  if (!shape_ok(FOVI_BF16, B, Lq, Lk, H, Hkv, D, strides, 9) || !q || !k || !v || !o || (int64_t)B * Lq * Lk == 0) return FOVI_ERR_INVALID_ARGUMENT;
+  AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, nullptr, nullptr, scale);
+  a.out = o;
+  if (!fovi::attention_tc_takes(a, FOVI_BF16, false)) return FOVI_ERR_UNSUPPORTED;
+  return fovi::launch_attention_tc_forward(a, reinterpret_cast<cudaStream_t>(stream), true);
 }

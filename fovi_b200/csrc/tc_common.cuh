@@ -233,8 +233,8 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), int grid, int block, siz
 // Tiled 3-D bf16 tensor map (box b0 x b1 x b2 of a tensor d0 x d1 x d2 with byte strides for d1, d2).
 int encode_3d(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_bytes,
               uint64_t stride2_bytes, uint32_t b0, uint32_t b1, uint32_t b2, bool swizzle128);
-// Tiled 4-D bf16 tensor map without swizzle (strides: bytes of dimensions 1 to 3).
-int encode_4d(CUtensorMap* m, const void* ptr, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4]);
+// Tiled 4-D bf16 tensor map, without swizzle unless asked for (strides: bytes of dimensions 1 to 3).
+int encode_4d(CUtensorMap* m, const void* ptr, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4], bool swizzle128 = false);
 // CTA-pair variant of the 64-channel mode (knnconv_tc2.cu).  Returns FOVI_ERR_UNSUPPORTED when it does not apply.
 int launch_knnconv_tc_pair(const fovi_knnconv_plan* p, const void* X, const void* Wt, const float* bias, void* Y, int y_dtype,
                            int B, int relu, cudaStream_t st, int skip_loads, uint32_t wait_limit, const OutMode& om);

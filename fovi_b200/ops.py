@@ -906,6 +906,21 @@ def rotary(x, positions, frequencies, pairs_per_axis, prefix=0, interleaved=Fals
     return y
 
 
+def _rows_for_copies(t):
+    """t [B, L, H, D] with contiguous channels, and for bf16 heads of a multiple of 8 channels in a form that the tensor copies take (rows on 16-byte boundaries, tokens not expanded):
+    a copy where it is not.  The copy costs a pass over t; without it the call would go to the kernel without tensor cores."""
+    D = t.shape[3]
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    if t.stride(3) != 1 and D > 1:
+        return t.contiguous()
+    if t.dtype == torch.bfloat16 and D % 8 == 0 and t.numel():
+        (B, L, H), (sb, sl, sh) = t.shape[:3], t.stride()[:3]
+        if t.data_ptr() % 16 or (L > 1 and (sl % 8 or sl == 0)) or (H > 1 and sh % 8) or (B > 1 and sb % 8):
+            return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 def _attention_inputs(q, k, v, key_lengths, key_mask, scale):
     """Checked arguments of an attention call: tensors with contiguous channels, (B, Lq, Lk, H, Hkv, D), scale."""
     _same_device(q, k, v, key_lengths, key_mask)
@@ -931,9 +946,7 @@ def _attention_inputs(q, k, v, key_lengths, key_mask, scale):
     scale = D ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"scale is {scale}")
-    if D > 1:
-        q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
-    return q, k, v, key_lengths, key_mask, (B, Lq, Lk, H, Hkv, D), scale
+    return _rows_for_copies(q), _rows_for_copies(k), _rows_for_copies(v), key_lengths, key_mask, (B, Lq, Lk, H, Hkv, D), scale
 
 
 def attention(q, k, v, key_lengths=None, key_mask=None, scale=None, want_lse=False):
@@ -965,8 +978,7 @@ def attention_backward(q, k, v, o, grad, lse, key_lengths=None, key_mask=None, s
     dev, dt = q.device, _dt(q.dtype)
     if grad.dtype != q.dtype:
         grad = grad.to(q.dtype)
-    if grad.stride(3) != 1 and D > 1:
-        grad = grad.contiguous()
+    grad = _rows_for_copies(grad)
     dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev) if need[0] else None
     dk, dv = (torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev) if need[1] or need[2] else None for _ in range(2))
     size = lib.fovi_attention_workspace_bytes(dt, *dims, 1)
@@ -978,6 +990,11 @@ def attention_backward(q, k, v, o, grad, lse, key_lengths=None, key_mask=None, s
                                           None if dq is None else _ptr(dq), None if dk is None else _ptr(dk), None if dv is None else _ptr(dv),
                                           None if work is None else _ptr(work), size, _stream()), "fovi_attention_backward")
     return dq, dk if need[1] else None, dv if need[2] else None
+
+
+def attention_check():
+    """Synchronise the current stream and raise if an attention launch on the current device gave up on a bounded wait since the last check."""
+    check(lib.fovi_attention_check(_stream()), "fovi_attention_check")
 
 
 def launch_count():

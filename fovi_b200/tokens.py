@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 
 from . import ops
 
-__all__ = ["layer_norm", "rotary", "cross_attention", "TokenNorm", "AxialRotary", "CrossAttention", "FixationReader"]
+__all__ = ["layer_norm", "rotary", "cross_attention", "TokenNorm", "AxialRotary", "CrossAttention", "FixationReader", "check"]
 
 
 def _wants_grad(*tensors):
@@ -107,6 +107,11 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
     if _wants_grad(q, k, v):
         return _AttentionFunction.apply(q, k, v, key_lengths, key_mask, scale)
     return ops.attention(q, k, v, key_lengths, key_mask, scale)
+
+
+def check():
+    """Synchronise the current stream and raise if an attention launch on the current device since the last check, forward or backward, gave up on a bounded wait."""
+    ops.attention_check()
 
 
 # ------------------------------------------------------------------------------------------------------------ modules

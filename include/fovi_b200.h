@@ -491,6 +491,12 @@ int fovi_attention_forward(const void* q, const void* k, const void* v, int dtyp
 int fovi_attention_backward(const void* q, const void* k, const void* v, const void* o, const void* dy, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D,
                             const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, float scale, const float* lse, void* dq, void* dk, void* dv,
                             void* work, int64_t work_bytes, void* stream);
+/* Synchronises `stream` and returns FOVI_ERR_DEVICE_TIMEOUT if an attention launch on the current device since the last check gave up on a bounded wait (its result is then
+ * incomplete); clears the word. */
+int fovi_attention_check(void* stream);
+/* Diagnostic: the tensor-core forward kernel with its loads withheld and a short wait limit, so that its first wait gives up; o is left unwritten or undefined. */
+int fovi_attention_forward_selftest_wait_timeout(const void* q, const void* k, const void* v, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides,
+                                                 float scale, void* o, void* stream);
 
 #ifdef __cplusplus
 }
