@@ -91,6 +91,7 @@ SIGNATURES = {
     "fovi_attention_backward": (C.c_int, [_P] * 5 + [C.c_int] * 7 + [C.POINTER(C.c_int64), _P, _P, C.c_float] + [_P] * 5 + [C.c_int64, _P]),
     "fovi_attention_check": (C.c_int, [_P]),
     "fovi_attention_forward_selftest_wait_timeout": (C.c_int, [_P, _P, _P] + [C.c_int] * 6 + [C.POINTER(C.c_int64), C.c_float, _P, _P]),
+    "fovi_attention_backward_selftest_wait_timeout": (C.c_int, [_P] * 5 + [C.c_int] * 6 + [C.POINTER(C.c_int64), C.c_float] + [_P] * 5 + [C.c_int64, _P]),
 }
 
 if not os.path.exists(LIB_PATH):

@@ -336,13 +336,17 @@ AttnArgs arguments(const void* q, const void* k, const void* v, int B, int Lq, i
   a.scale = scale; a.scale_log2 = scale * 1.44269504088896340736f;
   return a;
 }
+void gradients(AttnArgs& a, const void* o, const void* dy, const int64_t* s, const float* lse, void* dq, void* dk, void* dv, void* work) {
+  a.o = o; a.dy = dy; a.lse = const_cast<float*>(lse); a.dq = dq; a.dk = a.Lk > 0 ? dk : nullptr; a.dv = dv; a.delta = static_cast<float*>(work);
+  a.g_sb = s[9]; a.g_sl = s[10]; a.g_sh = s[11];
+}
 
 }  // namespace
 
 extern "C" int64_t fovi_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, int backward) {
   const int64_t none = 0;
   if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, &none, 0)) return -1;
-  return backward ? (int64_t)B * H * Lq * 4 : 0;
+  return backward ? fovi::attention_tc_backward_bytes(B, Lq, H) : 0;          // the plain kernels need a part of it
 }
 
 extern "C" int fovi_attention_forward(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides,
@@ -380,8 +384,8 @@ extern "C" int fovi_attention_backward(const void* q, const void* k, const void*
   const int64_t need = fovi_attention_workspace_bytes(dtype, B, Lq, Lk, H, Hkv, D, 1);
   if (need > 0 && (!work || work_bytes < need)) return FOVI_ERR_INVALID_ARGUMENT;
   AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
-  a.o = o; a.dy = dy; a.lse = const_cast<float*>(lse); a.dq = dq; a.dk = Lk > 0 ? dk : nullptr; a.dv = dv; a.delta = static_cast<float*>(work);
-  a.g_sb = strides[9]; a.g_sl = strides[10]; a.g_sh = strides[11];
+  gradients(a, o, dy, strides, lse, dq, dk, dv, work);
+  if (fovi::attention_tc_takes(a, dtype, true)) return fovi::launch_attention_tc_backward(a, work, st, false);
   if (dtype == FOVI_BF16) return D <= 64 ? backward<__nv_bfloat16, 64>(a, st) : backward<__nv_bfloat16, 128>(a, st);
   return D <= 64 ? backward<float, 64>(a, st) : backward<float, 128>(a, st);
 }
@@ -395,4 +399,16 @@ extern "C" int fovi_attention_forward_selftest_wait_timeout(const void* q, const
   a.out = o;
   if (!fovi::attention_tc_takes(a, FOVI_BF16, false)) return FOVI_ERR_UNSUPPORTED;
   return fovi::launch_attention_tc_forward(a, reinterpret_cast<cudaStream_t>(stream), true);
+}
+
+extern "C" int fovi_attention_backward_selftest_wait_timeout(const void* q, const void* k, const void* v, const void* o, const void* dy, int B, int Lq, int Lk, int H, int Hkv,
+                                                             int D, const int64_t* strides, float scale, const float* lse, void* dq, void* dk, void* dv, void* work,
+                                                             int64_t work_bytes, void* stream) {
+  if (!shape_ok(FOVI_BF16, B, Lq, Lk, H, Hkv, D, strides, 12) || !q || !k || !v || !o || !dy || !lse || !dk != !dv || (int64_t)B * Lq * Lk == 0 || !work ||
+      work_bytes < fovi_attention_workspace_bytes(FOVI_BF16, B, Lq, Lk, H, Hkv, D, 1))
+    return FOVI_ERR_INVALID_ARGUMENT;
+  AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, nullptr, nullptr, scale);
+  gradients(a, o, dy, strides, lse, dq, dk, dv, work);
+  if (!fovi::attention_tc_takes(a, FOVI_BF16, true)) return FOVI_ERR_UNSUPPORTED;
+  return fovi::launch_attention_tc_backward(a, work, reinterpret_cast<cudaStream_t>(stream), true);
 }

@@ -20,7 +20,7 @@ using fovi::key_end;
 
 namespace {
 
-__device__ int g_status;           // wait site at which a kernel gave up, see fovi_attention_check
+__device__ int g_status;           // wait site at which a kernel gave up, see fovi_attention_check: one word per device
 constexpr int AT_THREADS = 192;
 constexpr float AT_INF = __builtin_huge_valf();
 
@@ -82,12 +82,12 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       for (int c = 0; c < DC; ++c) tma_load_4d(sq + c * F::QBOX, &tm_q, qf, 64 * c, q0, h * t.q.mul_h, b * t.q.mul_b);
       uint32_t ks = 0, kp = 0, vs = 0, vp = 0;
       for (int j = 0; j < tiles; ++j) {
-        if (!mbar_wait(smem_u32(&hdr->k_empty[ks]), kp ^ 1u, abort_flag, &g_status, 1, t.wait_limit)) break;
+        if (!mbar_wait(smem_u32(&hdr->k_empty[ks]), kp ^ 1u, abort_flag, t.status, 1, t.wait_limit)) break;
         const uint32_t kf = smem_u32(&hdr->k_full[ks]);
         mbar_expect_tx(kf, F::TILE);
         for (int c = 0; c < DC; ++c) tma_load_4d(sk + ks * F::TILE + c * F::BOX, &tm_k, kf, 64 * c, j * KT, hk * t.k.mul_h, b * t.k.mul_b);
         if (++ks == F::NK) { ks = 0; kp ^= 1u; }
-        if (!mbar_wait(smem_u32(&hdr->v_empty[vs]), vp ^ 1u, abort_flag, &g_status, 2, t.wait_limit)) break;
+        if (!mbar_wait(smem_u32(&hdr->v_empty[vs]), vp ^ 1u, abort_flag, t.status, 2, t.wait_limit)) break;
         const uint32_t vf = smem_u32(&hdr->v_full[vs]);
         mbar_expect_tx(vf, F::TILE);
         for (int c = 0; c < DC; ++c) tma_load_4d(sv + vs * F::TILE + c * F::BOX, &tm_v, vf, 64 * c, j * KT, hk * t.v.mul_h, b * t.v.mul_b);
@@ -102,10 +102,10 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const uint32_t id_s = at_idesc(KT, false), id_o = at_idesc(dsteps * 16, true);
     const uint32_t u_sq = warp_uniform(sq), u_sk = warp_uniform(sk), u_sv = warp_uniform(sv), u_tmem = warp_uniform(tmem);
     uint32_t ks = 0, kp = 0, vs = 0, vp = 0;
-    bool ok = tiles == 0 || mbar_wait_warp(smem_u32(&hdr->q_full), 0, abort_flag, &g_status, 3, t.wait_limit);
+    bool ok = tiles == 0 || mbar_wait_warp(smem_u32(&hdr->q_full), 0, abort_flag, t.status, 3, t.wait_limit);
     auto scores = [&](int j) {
-      if (!mbar_wait_warp(smem_u32(&hdr->k_full[ks]), kp, abort_flag, &g_status, 4, t.wait_limit)) return false;
-      if (j > 0 && !mbar_wait_warp(smem_u32(&hdr->s_free), (j - 1) & 1, abort_flag, &g_status, 5, t.wait_limit)) return false;
+      if (!mbar_wait_warp(smem_u32(&hdr->k_full[ks]), kp, abort_flag, t.status, 4, t.wait_limit)) return false;
+      if (j > 0 && !mbar_wait_warp(smem_u32(&hdr->s_free), (j - 1) & 1, abort_flag, t.status, 5, t.wait_limit)) return false;
       tc_fence_after();
       if (elect_one()) {
         mma_rows(u_tmem, u_sq, F::QBOX, u_sk + ks * F::TILE, F::BOX, dsteps, id_s);
@@ -119,8 +119,8 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     if (ok && tiles > 0) ok = scores(0);
     for (int j = 0; j < tiles && ok; ++j) {
       if (j + 1 < tiles) ok = scores(j + 1);
-      ok = ok && mbar_wait_warp(smem_u32(&hdr->v_full[vs]), vp, abort_flag, &g_status, 6, t.wait_limit);
-      ok = ok && mbar_wait_warp(smem_u32(&hdr->p_full), j & 1, abort_flag, &g_status, 7, t.wait_limit);
+      ok = ok && mbar_wait_warp(smem_u32(&hdr->v_full[vs]), vp, abort_flag, t.status, 6, t.wait_limit);
+      ok = ok && mbar_wait_warp(smem_u32(&hdr->p_full), j & 1, abort_flag, t.status, 7, t.wait_limit);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -151,7 +151,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       bool whole = true;
 #pragma unroll
       for (int i = 0; i < KT / 32; ++i) { bits[i] = key_bits(a, mask, j * KT + 32 * i, end, lane); whole = whole && bits[i] == 0xffffffffu; }
-      ok = mbar_wait_warp(smem_u32(&hdr->s_full), j & 1, abort_flag, &g_status, 8, t.wait_limit);
+      ok = mbar_wait_warp(smem_u32(&hdr->s_full), j & 1, abort_flag, t.status, 8, t.wait_limit);
       if (!ok) break;
       tc_fence_after();
       float x[KT];
@@ -189,7 +189,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
       if (j > 0) {                      // the product with the previous P is done: P and O are this thread's
-        ok = mbar_wait_warp(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, &g_status, 9, t.wait_limit);
+        ok = mbar_wait_warp(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit);
         if (!ok) break;
         tc_fence_after();
         if (__any_sync(0xffffffffu, move)) {
@@ -209,7 +209,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         for (int i = 0; i < KT / 2; i += 32) tc_st32(lanes + F::P_COL + i, reinterpret_cast<uint32_t*>(x) + i);
       }
       if (!whole) {                     // rows of V that must not be read: a zero weight times what they hold need not be zero
-        ok = mbar_wait_warp(smem_u32(&hdr->v_full[j % F::NV]), (j / F::NV) & 1, abort_flag, &g_status, 10, t.wait_limit);
+        ok = mbar_wait_warp(smem_u32(&hdr->v_full[j % F::NV]), (j / F::NV) & 1, abort_flag, t.status, 10, t.wait_limit);
         if (!ok) break;
         if (threadIdx.x < KT) {
           const int r = threadIdx.x;
@@ -229,7 +229,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&hdr->p_full));
     }
-    if (ok && tiles > 0) ok = mbar_wait_warp(smem_u32(&hdr->o_full), (tiles - 1) & 1, abort_flag, &g_status, 11, t.wait_limit);
+    if (ok && tiles > 0) ok = mbar_wait_warp(smem_u32(&hdr->o_full), (tiles - 1) & 1, abort_flag, t.status, 11, t.wait_limit);
     if (ok && !idle) {
       tc_fence_after();
       const bool none = m == -AT_INF;
@@ -255,6 +255,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
           }
         }
+        __syncwarp();
       }
       if (a.lse && row < a.Lq) a.lse[((int64_t)b * a.H + h) * a.Lq + row] = zero ? AT_INF : m * c + log2f(sum);
     }
@@ -271,17 +272,6 @@ bool rows_ok(const void* p, int64_t sb, int64_t sl, int64_t sh, int B, int L, in
          sl < (int64_t)1 << 38 && sh < (int64_t)1 << 38 && sb < (int64_t)1 << 38;
 }
 
-// [64 channels x rows] boxes of a [B, L, H, D] tensor.
-int encode_rows(CUtensorMap* m, fovi::TcView* view, const void* p, int64_t sb, int64_t sl, int64_t sh, int B, int L, int H, int D, int rows) {
-  view->mul_h = H > 1 && sh > 0;
-  view->mul_b = B > 1 && sb > 0;
-  const uint64_t one = (uint64_t)(D + 7) / 8 * 16;        // the stride of an axis of extent 1 is never used
-  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)L, view->mul_h ? (uint64_t)H : 1, view->mul_b ? (uint64_t)B : 1};
-  const uint64_t strides[3] = {L > 1 ? (uint64_t)sl * 2 : one, view->mul_h ? (uint64_t)sh * 2 : one, view->mul_b ? (uint64_t)sb * 2 : one};
-  const uint32_t box[4] = {64, (uint32_t)rows, 1, 1};
-  return fovi::encode_4d(m, p, dims, strides, box, true);
-}
-
 template <int DC>
 int forward(const AttnArgs& a, cudaStream_t st, bool selftest) {
   using F = Fwd<DC>;
@@ -290,9 +280,10 @@ int forward(const AttnArgs& a, cudaStream_t st, bool selftest) {
   t.a = a;
   t.wait_limit = selftest ? 4096u : WAIT_LIMIT;
   t.skip_loads = selftest;
-  int rc = encode_rows(&tq, &t.q, a.q, a.q_sb, a.q_sl, a.q_sh, a.B, a.Lq, a.H, a.D, AT_M);
-  if (!rc) rc = encode_rows(&tk, &t.k, a.k, a.k_sb, a.k_sl, a.k_sh, a.B, a.Lk, a.Hkv, a.D, F::KT);
-  if (!rc) rc = encode_rows(&tv, &t.v, a.v, a.v_sb, a.v_sl, a.v_sh, a.B, a.Lk, a.Hkv, a.D, F::KT);
+  int rc = fovi::attention_tc_status(&t.status);
+  if (!rc) rc = fovi::encode_rows(&tq, &t.q, a.q, a.q_sb, a.q_sl, a.q_sh, a.B, a.Lq, a.H, a.D, AT_M);
+  if (!rc) rc = fovi::encode_rows(&tk, &t.k, a.k, a.k_sb, a.k_sl, a.k_sh, a.B, a.Lk, a.Hkv, a.D, F::KT);
+  if (!rc) rc = fovi::encode_rows(&tv, &t.v, a.v, a.v_sb, a.v_sl, a.v_sh, a.B, a.Lk, a.Hkv, a.D, F::KT);
   if (rc) return rc;
   const int64_t blocks = (int64_t)((a.Lq + AT_M - 1) / AT_M) * a.H * a.B;
   if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;
@@ -302,6 +293,16 @@ int forward(const AttnArgs& a, cudaStream_t st, bool selftest) {
 }
 
 }  // namespace
+
+int fovi::encode_rows(CUtensorMap* m, TcView* view, const void* p, int64_t sb, int64_t sl, int64_t sh, int B, int L, int H, int D, int rows) {
+  view->mul_h = H > 1 && sh > 0;
+  view->mul_b = B > 1 && sb > 0;
+  const uint64_t one = (uint64_t)(D + 7) / 8 * 16;        // the stride of an axis of extent 1 is never used
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)L, view->mul_h ? (uint64_t)H : 1, view->mul_b ? (uint64_t)B : 1};
+  const uint64_t strides[3] = {L > 1 ? (uint64_t)sl * 2 : one, view->mul_h ? (uint64_t)sh * 2 : one, view->mul_b ? (uint64_t)sb * 2 : one};
+  const uint32_t box[4] = {64, (uint32_t)rows, 1, 1};
+  return fovi::encode_4d(m, p, dims, strides, box, true);
+}
 
 bool fovi::attention_tc_takes(const AttnArgs& a, int dtype, bool backward) {
   return dtype == FOVI_BF16 && a.D % 8 == 0 && a.D <= ATT_MAX_DIM && a.Lk > 0 && a.scale_log2 > 0.f && rows_ok(a.q, a.q_sb, a.q_sl, a.q_sh, a.B, a.Lq, a.H) &&
@@ -313,6 +314,11 @@ bool fovi::attention_tc_takes(const AttnArgs& a, int dtype, bool backward) {
 
 int fovi::launch_attention_tc_forward(const AttnArgs& a, cudaStream_t st, bool selftest) {
   return a.D <= 64 ? forward<1>(a, st, selftest) : forward<2>(a, st, selftest);
+}
+
+int fovi::attention_tc_status(int** word) {
+  FOVI_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_status));
+  return FOVI_OK;
 }
 
 int fovi::attention_tc_check(cudaStream_t st) {

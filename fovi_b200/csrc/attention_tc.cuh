@@ -9,13 +9,19 @@ struct TcView { int mul_h, mul_b; };
 struct AttnTcArgs {
   AttnArgs a;
   TcView q, k, v, g;
+  int* status;             // wait site at which a kernel gave up
   uint32_t wait_limit;
   int skip_loads;          // self-test: the loads are withheld, so the first wait must give up
 };
 
 bool attention_tc_takes(const AttnArgs& a, int dtype, bool backward);
 int launch_attention_tc_forward(const AttnArgs& a, cudaStream_t st, bool selftest);
+int64_t attention_tc_backward_bytes(int B, int Lq, int H);
+int launch_attention_tc_backward(const AttnArgs& a, void* work, cudaStream_t st, bool selftest);
 int attention_tc_check(cudaStream_t st);
+int attention_tc_status(int** word);        // the current device's status word
+// Boxes of 64 channels x `rows` tokens of a [B, L, H, D] tensor.
+int encode_rows(CUtensorMap* m, TcView* view, const void* p, int64_t sb, int64_t sl, int64_t sh, int B, int L, int H, int D, int rows);
 }  // namespace fovi
 
 namespace {
@@ -44,6 +50,11 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* r) {
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
         "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
         "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Values written to shared memory by threads, seen by the MMAs.

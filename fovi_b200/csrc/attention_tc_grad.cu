@@ -1,0 +1,453 @@
+// Gradients of cross attention on the tensor cores (bf16, see attention_tc.cu for the shapes).
+//   p = 2^(scale log2(e) s - lse),  ds = p * (dp - delta),  s = q k^T, dp = dy v^T
+//   dq = scale * sum over keys of ds k          dv = sum over queries of p dy,   dk = scale * sum over queries of ds q
+// Two kernels of one form: a CTA owns 128 rows (queries for dq; keys for dk and dv), whose two operand tiles stay in shared memory, and goes over tiles of CT columns
+// (the keys; the queries of all heads that read the state head).  Per tile
+//   S = R1 C1^T, dP = R2 C2^T          SS MMAs, M = 128, N = CT, into tensor memory; for dk and dv these are the transposed scores, rows = keys
+//   P, dS                              eight warps, a thread per row and half the columns: registers, then back to tensor memory as bf16
+//   acc1 += dS C1 (dq, dk),  acc2 += P C2 (dv)          TS MMAs, the column tiles read MN-major: nothing is transposed, nothing goes through shared memory
+// Each gradient is summed by one CTA in a fixed order: no atomics, the same bits every time, no float32 buffer of dq, for 7 products instead of 5.
+// One CTA per SM with all 512 columns of tensor memory, over many row tiles (persistent): the next tile's S and dP are computed while this one's elements are worked on,
+// and the next row tile's operands arrive meanwhile.  A last tile of fewer columns costs only its own (N and the steps over its columns follow).
+// Rows of K whose key is masked are set to zero in shared memory in front of dS K; for dk and dv a masked key is a row, whose results are zeros by a select.
+#include <cuda_bf16.h>
+
+#include "attention_tc.cuh"
+
+using fovi::AttnArgs;
+using fovi::AttnTcArgs;
+using fovi::key_end;
+
+namespace {
+
+constexpr int EW_WARPS = 8, GR_THREADS = (EW_WARPS + 2) * 32;
+constexpr float AT_INF = __builtin_huge_valf();
+
+template <int DC> struct Grad {
+  static constexpr int CT = DC == 1 ? 128 : 64, HALF = CT / 2;       // columns of a tile, of a thread
+  static constexpr int NS = DC == 1 ? 4 : 3;                         // column tiles in flight
+  static constexpr uint32_t RBOX = AT_M * 128u, RTILE = DC * RBOX, CBOX = CT * 128u, CTILE = DC * CBOX;
+  static constexpr uint32_t ROWS = 4 * RTILE;                        // two row tiles of two operands
+  static constexpr uint32_t SMEM = 1024 + ROWS + NS * 2 * CTILE + NS * 2 * CT * 4 + 256;         // slack for the alignment, tiles, row statistics, barriers
+  static constexpr uint32_t DP = CT, P = 2 * CT, DS = 2 * CT + CT / 2, ACC1 = DC == 1 ? 384 : 256, ACC2 = ACC1 + 64 * DC;
+};
+
+struct GradHeader {
+  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_free, drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct GradArgs {
+  AttnTcArgs t;
+  const float *nl, *nd;        // [B, H, pitch]: -lse and -delta, -inf and 0 behind the last query
+  int pitch, items, tiles;     // tiles: row tiles of a head
+};
+
+struct Item { int row0, h, b, end, n; };     // h: query head (dq) or state head (dk, dv); n: column tiles
+
+template <int DC, bool KEYS>
+__device__ __forceinline__ Item item_at(const GradArgs& g, int i) {
+  const AttnArgs& a = g.t.a;
+  const int heads = KEYS ? a.Hkv : a.H;
+  Item it;
+  it.row0 = i % g.tiles * AT_M; it.h = i / g.tiles % heads; it.b = i / g.tiles / heads;
+  it.end = key_end(a, it.b);
+  it.n = KEYS ? (it.row0 < it.end ? a.group * ((a.Lq + Grad<DC>::CT - 1) / Grad<DC>::CT) : 0) : (it.end + Grad<DC>::CT - 1) / Grad<DC>::CT;
+  return it;
+}
+
+// (row tile, column tile) pairs in the order in which every role meets them; row tiles without columns are passed over.
+template <int DC, bool KEYS>
+struct Walk {
+  int i, j, seq;               // seq: how many row tiles with columns came before
+  Item it;
+  __device__ __forceinline__ explicit Walk(const GradArgs& g) : i(blockIdx.x), j(0), seq(0) { settle(g); }
+  __device__ __forceinline__ void settle(const GradArgs& g) {
+    for (; i < g.items; i += gridDim.x) {
+      it = item_at<DC, KEYS>(g, i);
+      if (it.n > 0) return;
+    }
+  }
+  __device__ __forceinline__ bool more(const GradArgs& g) const { return i < g.items; }
+  __device__ __forceinline__ void next(const GradArgs& g) {
+    if (++j < it.n) return;
+    j = 0; ++seq; i += gridDim.x;
+    settle(g);
+  }
+};
+
+// Columns of tile j: first one, and how many there are.
+template <int DC, bool KEYS>
+__device__ __forceinline__ int columns(const AttnArgs& a, const Item& it, int j, int& c0, int& h) {
+  constexpr int CT = Grad<DC>::CT;
+  const int per = KEYS ? (a.Lq + CT - 1) / CT : it.n;
+  const int q = KEYS ? j / per : 0;
+  c0 = (j - q * per) * CT;
+  h = KEYS ? it.h * a.group + q : it.h;
+  return min(CT, (KEYS ? a.Lq : it.end) - c0);
+}
+
+template <int DC, bool KEYS>
+__global__ void __launch_bounds__(GR_THREADS, 1)
+attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                    const __grid_constant__ CUtensorMap tm_g, const GradArgs g) {
+  using G = Grad<DC>;
+  constexpr int CT = G::CT, HALF = G::HALF;
+  const AttnTcArgs& t = g.t;
+  const AttnArgs& a = t.a;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  const uint32_t srow = base, scol = srow + G::ROWS, sstat = scol + G::NS * 2 * G::CTILE;
+  static_assert(sizeof(GradHeader) <= 256 && G::SMEM <= 232448, "shared memory of a block");
+  GradHeader* hdr = reinterpret_cast<GradHeader*>(smem_raw + (sstat - raw) + G::NS * 2 * CT * 4);
+  volatile int* abort_flag = &hdr->abort_flag;
+  int* status = t.status;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->row_full[i]), 1); mbar_init(smem_u32(&hdr->row_empty[i]), 1); }
+    for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&hdr->full[i]), 1); mbar_init(smem_u32(&hdr->empty[i]), 1); }
+    mbar_init(smem_u32(&hdr->s_full), 1); mbar_init(smem_u32(&hdr->s_free), EW_WARPS); mbar_init(smem_u32(&hdr->p_full), EW_WARPS);
+    mbar_init(smem_u32(&hdr->mixed), 1); mbar_init(smem_u32(&hdr->acc_free), EW_WARPS); mbar_init(smem_u32(&hdr->drain), 1);
+    hdr->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == EW_WARPS) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hdr->tmem_base)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = hdr->tmem_base;
+
+  if (warp == EW_WARPS + 1) {
+    // ------------------------------------------------------------ copies
+    if (lane == 0 && !t.skip_loads) {
+      uint32_t s = 0, sp = 0;
+      for (Walk<DC, KEYS> w(g); w.more(g); w.next(g)) {
+        if (w.j == 0) {
+          const uint32_t f = w.seq & 1, fp = w.seq >> 1 & 1, bar = smem_u32(&hdr->row_full[f]), dst = srow + f * 2 * G::RTILE;
+          if (!mbar_wait(smem_u32(&hdr->row_empty[f]), fp ^ 1u, abort_flag, status, 21, t.wait_limit)) break;
+          mbar_expect_tx(bar, 2 * G::RTILE);
+          for (int c = 0; c < DC; ++c) {
+            if (KEYS) {
+              tma_load_4d(dst + c * G::RBOX, &tm_k, bar, 64 * c, w.it.row0, w.it.h * t.k.mul_h, w.it.b * t.k.mul_b);
+              tma_load_4d(dst + G::RTILE + c * G::RBOX, &tm_v, bar, 64 * c, w.it.row0, w.it.h * t.v.mul_h, w.it.b * t.v.mul_b);
+            } else {
+              tma_load_4d(dst + c * G::RBOX, &tm_q, bar, 64 * c, w.it.row0, w.it.h * t.q.mul_h, w.it.b * t.q.mul_b);
+              tma_load_4d(dst + G::RTILE + c * G::RBOX, &tm_g, bar, 64 * c, w.it.row0, w.it.h * t.g.mul_h, w.it.b * t.g.mul_b);
+            }
+          }
+        }
+        int c0, h;
+        columns<DC, KEYS>(a, w.it, w.j, c0, h);
+        if (!mbar_wait(smem_u32(&hdr->empty[s]), sp ^ 1u, abort_flag, status, 22, t.wait_limit)) break;
+        const uint32_t bar = smem_u32(&hdr->full[s]), dst = scol + s * 2 * G::CTILE;
+        mbar_expect_tx(bar, 2 * G::CTILE + (KEYS ? 2 * CT * 4 : 0));
+        for (int c = 0; c < DC; ++c) {
+          if (KEYS) {
+            tma_load_4d(dst + c * G::CBOX, &tm_q, bar, 64 * c, c0, h * t.q.mul_h, w.it.b * t.q.mul_b);
+            tma_load_4d(dst + G::CTILE + c * G::CBOX, &tm_g, bar, 64 * c, c0, h * t.g.mul_h, w.it.b * t.g.mul_b);
+          } else {
+            tma_load_4d(dst + c * G::CBOX, &tm_k, bar, 64 * c, c0, h / a.group * t.k.mul_h, w.it.b * t.k.mul_b);
+            tma_load_4d(dst + G::CTILE + c * G::CBOX, &tm_v, bar, 64 * c, c0, h / a.group * t.v.mul_h, w.it.b * t.v.mul_b);
+          }
+        }
+        if (KEYS) {
+          const int64_t at = ((int64_t)w.it.b * a.H + h) * g.pitch + c0;
+          bulk_load(sstat + s * 2 * CT * 4, g.nl + at, CT * 4, bar);
+          bulk_load(sstat + s * 2 * CT * 4 + CT * 4, g.nd + at, CT * 4, bar);
+        }
+        if (++s == G::NS) { s = 0; sp ^= 1u; }
+      }
+      if (*abort_flag)      // copies in flight get time to land before the block leaves its shared memory
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+  } else if (warp == EW_WARPS) {
+    // ------------------------------------------------------------ MMAs (all lanes loop, one issues: see elect_one)
+    const int dsteps = (a.D + 15) / 16;
+    const uint32_t id_acc = at_idesc(dsteps * 16, true);
+    const uint32_t u_srow = warp_uniform(srow), u_scol = warp_uniform(scol), u_tmem = warp_uniform(tmem);
+    uint32_t s = 0, sp = 0, n_s = 0, n_m = 0, ms = 0;
+    Walk<DC, KEYS> w(g), m(g);
+    bool ok = true;
+    auto scores = [&]() {
+      const uint32_t f = w.seq & 1;
+      if (w.j == 0 && !mbar_wait_warp(smem_u32(&hdr->row_full[f]), w.seq >> 1 & 1, abort_flag, status, 23, t.wait_limit)) return false;
+      if (!mbar_wait_warp(smem_u32(&hdr->full[s]), sp, abort_flag, status, 24, t.wait_limit)) return false;
+      if (n_s > 0 && !mbar_wait_warp(smem_u32(&hdr->s_free), (n_s - 1) & 1, abort_flag, status, 25, t.wait_limit)) return false;
+      tc_fence_after();
+      int c0, h;
+      const int n = warp_uniform((columns<DC, KEYS>(a, w.it, w.j, c0, h) + 15) / 16 * 16);
+      const bool last = w.j + 1 == w.it.n;
+      if (elect_one()) {
+        const uint32_t rows = u_srow + f * 2 * G::RTILE, cols = u_scol + s * 2 * G::CTILE, id = at_idesc(0, false) | ((uint32_t)(n >> 3) << 17);
+        mma_rows(u_tmem, rows, G::RBOX, cols, G::CBOX, dsteps, id);
+        mma_rows(u_tmem + G::DP, rows + G::RTILE, G::RBOX, cols + G::CTILE, G::CBOX, dsteps, id);
+        tc_commit(smem_u32(&hdr->s_full));
+        if (last) tc_commit(smem_u32(&hdr->row_empty[f]));
+      }
+      __syncwarp();
+      if (++s == G::NS) { s = 0; sp ^= 1u; }
+      ++n_s;
+      w.next(g);
+      return true;
+    };
+    if (w.more(g)) ok = scores();
+    for (; ok && m.more(g); m.next(g)) {
+      if (w.more(g)) ok = scores();
+      ok = ok && mbar_wait_warp(smem_u32(&hdr->p_full), n_m & 1, abort_flag, status, 26, t.wait_limit);
+      if (ok && m.j == 0 && m.seq > 0) ok = mbar_wait_warp(smem_u32(&hdr->acc_free), (m.seq - 1) & 1, abort_flag, status, 27, t.wait_limit);
+      if (!ok) break;
+      tc_fence_after();
+      int c0, h;
+      const int steps = warp_uniform((columns<DC, KEYS>(a, m.it, m.j, c0, h) + 15) / 16);
+      if (elect_one()) {
+        const uint32_t cols = u_scol + ms * 2 * G::CTILE;
+        if (KEYS) mma_mix(u_tmem + G::ACC2, u_tmem + G::P, cols + G::CTILE, G::CBOX, steps, id_acc, m.j > 0);
+        mma_mix(u_tmem + G::ACC1, u_tmem + G::DS, cols, G::CBOX, steps, id_acc, m.j > 0);
+        tc_commit(smem_u32(&hdr->empty[ms]));
+        tc_commit(smem_u32(&hdr->mixed));
+      }
+      __syncwarp();
+      if (++ms == G::NS) ms = 0;
+      ++n_m;
+    }
+    if (*abort_flag && elect_one()) {      // no MMA may still be reading shared memory or writing tensor memory
+      tc_commit(smem_u32(&hdr->drain));
+      for (uint32_t it = 0; it < (1u << 20); ++it)
+        if (mbar_try_wait(smem_u32(&hdr->drain), 0)) break;
+    }
+  } else {
+    // ------------------------------------------------------------ elements: thread = row, half the columns
+    const int r = (warp & 3) * 32 + lane, half = warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c = a.scale_log2;
+    uint32_t n = 0, slot = 0, sphase = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
+      const Item it = item_at<DC, KEYS>(g, i);
+      const int row = it.row0 + r;
+      const bool idle = it.row0 + (warp & 3) * 32 >= (KEYS ? it.end : a.Lq);
+      const uint8_t* mask = a.mask ? a.mask + (int64_t)it.b * a.Lk : nullptr;
+      float nl = 0.f, nd = 0.f;
+      bool row_ok = true;
+      if (KEYS) {
+        row_ok = row < it.end && (!mask || __ldg(mask + row));
+      } else if (row < g.pitch) {
+        const int64_t at = ((int64_t)it.b * a.H + it.h) * g.pitch + row;
+        nl = __ldg(g.nl + at); nd = __ldg(g.nd + at);
+      }
+      for (int j = 0; j < it.n; ++j, ++n) {
+        int c0, h;
+        const int cols = columns<DC, KEYS>(a, it, j, c0, h);
+        const int first = half * HALF;
+        uint32_t bits[HALF / 32];
+        bool whole = true;
+        if (!KEYS) {
+#pragma unroll
+          for (int e = 0; e < HALF / 32; ++e) { bits[e] = key_bits(a, mask, c0 + first + 32 * e, it.end, lane); whole = whole && bits[e] == 0xffffffffu; }
+        }
+        ok = mbar_wait_warp(smem_u32(&hdr->s_full), n & 1, abort_flag, status, 28, t.wait_limit);
+        if (ok && KEYS) ok = mbar_wait_warp(smem_u32(&hdr->full[slot]), sphase, abort_flag, status, 29, t.wait_limit);     // (done: the scores needed it too)
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t pw[HALF / 2], dw[HALF / 2];
+        const float* st = reinterpret_cast<const float*>(smem_raw + (sstat - raw) + slot * 2 * CT * 4) + first;
+#pragma unroll
+        for (int e = 0; e < HALF; e += 32) {          // 32 columns at a time: all of them at once would not fit the registers
+          float s[32], d[32];
+          const bool work = !idle && first + e < cols;
+          if (work) {
+            tc_ld32(lanes + first + e, reinterpret_cast<uint32_t*>(s));
+            tc_ld32(lanes + G::DP + first + e, reinterpret_cast<uint32_t*>(d));
+            tc_ld_wait();
+          }
+          if (e + 32 == HALF) {                       // the last columns are in registers: the next scores may come
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&hdr->s_free));
+          }
+          if (!work) continue;
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            float4 l4, d4;
+            if (KEYS) {
+              l4 = *reinterpret_cast<const float4*>(st + e + k);
+              d4 = *reinterpret_cast<const float4*>(st + CT + e + k);
+            } else {
+              l4 = make_float4(nl, nl, nl, nl); d4 = make_float4(nd, nd, nd, nd);
+            }
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const int x = k + 2 * z;
+              const float2 ex = fma2(make_float2(s[x], s[x + 1]), make_float2(c, c), z ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y));
+              const float2 p = make_float2(ex2(ex.x), ex2(ex.y));
+              float2 ds = mul2(p, add2(make_float2(d[x], d[x + 1]), z ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y)));
+              if (!KEYS && !whole) {
+                ds.x = bits[e >> 5] >> x & 1u ? ds.x : 0.f;
+                ds.y = bits[e >> 5] >> (x + 1) & 1u ? ds.y : 0.f;
+              }
+              if (KEYS) pw[(e + x) >> 1] = pack_bf16(p.x, p.y);
+              dw[(e + x) >> 1] = pack_bf16(ds.x, ds.y);
+            }
+          }
+        }
+        if (KEYS && !row_ok) {
+#pragma unroll
+          for (int e = 0; e < HALF / 2; ++e) pw[e] = dw[e] = 0u;
+        }
+        if (n > 0) {          // the previous P and dS have been read
+          ok = mbar_wait_warp(smem_u32(&hdr->mixed), (n - 1) & 1, abort_flag, status, 30, t.wait_limit);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        if (!idle) {
+          if (first < cols) {
+            if constexpr (HALF == 64) {
+              if (KEYS) tc_st32(lanes + G::P + first / 2, pw);
+              tc_st32(lanes + G::DS + first / 2, dw);
+            } else {
+              if (KEYS) tc_st16(lanes + G::P + first / 2, pw);
+              tc_st16(lanes + G::DS + first / 2, dw);
+            }
+          }
+        }
+        if (!KEYS && !whole) {          // rows of K that must not be read; the scores are done with the tile
+          const int k = lane + 32 * (warp & 3);         // four warps share the half's keys
+          if (k < HALF) {
+            uint32_t word = bits[0];
+#pragma unroll
+            for (int e = 1; e < HALF / 32; ++e) word = (k >> 5) == e ? bits[e] : word;
+            if (!(word >> (k & 31) & 1u)) {
+              unsigned char* p = smem_raw + (scol - raw) + slot * 2 * G::CTILE + (first + k) * 128;
+#pragma unroll
+              for (int e = 0; e < DC * 8; ++e) *reinterpret_cast<uint4*>(p + (e >> 3) * G::CBOX + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_async_smem();
+        }
+        tc_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&hdr->p_full));
+        if (++slot == (uint32_t)G::NS) { slot = 0; sphase ^= 1u; }
+      }
+      if (!ok) break;
+      if (it.n > 0) {
+        ok = mbar_wait_warp(smem_u32(&hdr->mixed), (n - 1) & 1, abort_flag, status, 31, t.wait_limit);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      // results: dk by the first four warps and dv by the others; dq by halves of its channels
+      constexpr int SPAN = KEYS ? DC * 64 : DC * 32;
+      const uint32_t from = KEYS ? (half ? G::ACC2 : G::ACC1) : G::ACC1 + half * SPAN;
+      const int ch0 = KEYS ? 0 : half * SPAN, rows = KEYS ? a.Lk : a.Lq, heads = KEYS ? a.Hkv : a.H;
+      const float f = KEYS && half ? 1.f : a.scale;
+      const bool zero = it.n == 0 || (KEYS && !row_ok);
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(KEYS ? (half ? a.dv : a.dk) : a.dq) + (((int64_t)it.b * rows + row) * heads + it.h) * a.D;
+#pragma unroll 1
+      for (int e = 0; e < SPAN; e += 32) {
+        float v[32];
+        if (it.n > 0) {
+          tc_ld32(lanes + from + e, reinterpret_cast<uint32_t*>(v));
+          tc_ld_wait();
+          if (e + 32 == SPAN) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&hdr->acc_free));
+          }
+        }
+        if (row < rows) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            if (ch0 + e + k < a.D) {
+              uint32_t w[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) w[z] = zero ? 0u : pack_bf16(v[k + 2 * z] * f, v[k + 2 * z + 1] * f);
+              *reinterpret_cast<uint4*>(out + ch0 + e + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == EW_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// -lse and -delta = -<dy, o> of every row, in rows of `pitch`: sixteen lanes a row, 8 channels each.
+__global__ void __launch_bounds__(256) attn_row_stats_kernel(const AttnArgs a, float* nl, float* nd, int pitch) {
+  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);          // b, row, h: the heads of a row lie together
+  const int lane = threadIdx.x & 15;
+  if (i >= (int64_t)a.B * pitch * a.H) return;
+  const int h = (int)(i % a.H);
+  const int64_t bl = i / a.H, b = bl / pitch;
+  const int l = (int)(bl - b * pitch);
+  float s = 0.f;
+  if (l < a.Lq && lane * 8 < a.D) {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.o) + ((b * a.Lq + l) * a.H + h) * a.D) + lane);
+    const uint4 y = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.dy) + b * a.g_sb + l * a.g_sl + h * a.g_sh) + lane);
+    const __nv_bfloat162 *u = reinterpret_cast<const __nv_bfloat162*>(&x), *v = reinterpret_cast<const __nv_bfloat162*>(&y);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 p = __bfloat1622float2(u[k]), q = __bfloat1622float2(v[k]);
+      s = fmaf(p.x, q.x, s); s = fmaf(p.y, q.y, s);
+    }
+  }
+  for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+  if (lane == 0) {
+    const int64_t at = (b * a.H + h) * pitch + l;
+    nl[at] = l < a.Lq ? -__ldg(a.lse + (b * a.H + h) * a.Lq + l) : -AT_INF;
+    nd[at] = -s;
+  }
+}
+
+template <int DC, bool KEYS>
+int launch(const AttnArgs& a, GradArgs g, cudaStream_t st) {
+  using G = Grad<DC>;
+  CUtensorMap tq, tk, tv, tg;
+  const int q_rows = KEYS ? G::CT : AT_M, k_rows = KEYS ? AT_M : G::CT;
+  int rc = fovi::encode_rows(&tq, &g.t.q, a.q, a.q_sb, a.q_sl, a.q_sh, a.B, a.Lq, a.H, a.D, q_rows);
+  if (!rc) rc = fovi::encode_rows(&tg, &g.t.g, a.dy, a.g_sb, a.g_sl, a.g_sh, a.B, a.Lq, a.H, a.D, q_rows);
+  if (!rc) rc = fovi::encode_rows(&tk, &g.t.k, a.k, a.k_sb, a.k_sl, a.k_sh, a.B, a.Lk, a.Hkv, a.D, k_rows);
+  if (!rc) rc = fovi::encode_rows(&tv, &g.t.v, a.v, a.v_sb, a.v_sl, a.v_sh, a.B, a.Lk, a.Hkv, a.D, k_rows);
+  if (rc) return rc;
+  g.tiles = ((KEYS ? a.Lk : a.Lq) + AT_M - 1) / AT_M;
+  const int64_t items = (int64_t)g.tiles * (KEYS ? a.Hkv : a.H) * a.B;
+  if (items > INT_MAX - 65536) return FOVI_ERR_UNSUPPORTED;
+  g.items = (int)items;
+  const int grid = std::min(g.items, fovi::sm_count());
+  FOVI_CUDA(cudaFuncSetAttribute(attn_tc_grad_kernel<DC, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::SMEM));
+  FOVI_CUDA(fovi::launch_pdl(attn_tc_grad_kernel<DC, KEYS>, grid, GR_THREADS, G::SMEM, st, tq, tk, tv, tg, g));
+  return fovi::after_launch("attn_tc_grad_kernel");
+}
+
+}  // namespace
+
+int64_t fovi::attention_tc_backward_bytes(int B, int Lq, int H) { return (int64_t)B * H * ((Lq + AT_M - 1) / AT_M * AT_M) * 8; }
+
+int fovi::launch_attention_tc_backward(const AttnArgs& a, void* work, cudaStream_t st, bool selftest) {
+  GradArgs g = {};
+  g.t.a = a;
+  g.t.wait_limit = selftest ? 4096u : WAIT_LIMIT;
+  g.t.skip_loads = selftest;
+  int rc = attention_tc_status(&g.t.status);
+  if (rc) return rc;
+  g.pitch = (a.Lq + AT_M - 1) / AT_M * AT_M;
+  const int64_t rows = (int64_t)a.B * a.H * g.pitch, blocks = (rows + 15) / 16;
+  if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;
+  float* nl = static_cast<float*>(work);
+  g.nl = nl; g.nd = nl + rows;
+  attn_row_stats_kernel<<<(int)blocks, 256, 0, st>>>(a, nl, nl + rows, g.pitch);
+  rc = after_launch("attn_row_stats_kernel");
+  if (!rc && a.dk) rc = a.D <= 64 ? launch<1, true>(a, g, st) : launch<2, true>(a, g, st);
+  if (!rc && a.dq) rc = a.D <= 64 ? launch<1, false>(a, g, st) : launch<2, false>(a, g, st);
+  return rc;
+}

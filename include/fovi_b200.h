@@ -497,6 +497,10 @@ int fovi_attention_check(void* stream);
 /* Diagnostic: the tensor-core forward kernel with its loads withheld and a short wait limit, so that its first wait gives up; o is left unwritten or undefined. */
 int fovi_attention_forward_selftest_wait_timeout(const void* q, const void* k, const void* v, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides,
                                                  float scale, void* o, void* stream);
+/* The same of the tensor-core backward kernels that are asked for (dq, or dk and dv, not NULL). */
+int fovi_attention_backward_selftest_wait_timeout(const void* q, const void* k, const void* v, const void* o, const void* dy, int B, int Lq, int Lk, int H, int Hkv, int D,
+                                                  const int64_t* strides, float scale, const float* lse, void* dq, void* dk, void* dv, void* work, int64_t work_bytes,
+                                                  void* stream);
 
 #ifdef __cplusplus
 }
