@@ -4,6 +4,8 @@
 //   dw = sum over rows of dy * xh,   db = sum over rows of dy
 // Sums and statistics are float32; results are rounded once, to their tensor's type.  The variance is taken about the row's own mean (two passes over
 // values that are already on the chip), so a large common offset does not cost digits.
+#include <algorithm>
+
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -80,23 +82,335 @@ __global__ void __launch_bounds__(STRIP_COLS) layer_norm_dw_kernel(const TX* x, 
   part[((size_t)blockIdx.y * 2 + 1) * C + c] = sb;
 }
 
-// The parts of every column added in the order of the strips: the same bits every time.
-__global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* part, int strips, int C, float* dw, float* db) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= C) return;
-  float sw = 0.f, sb = 0.f;
-  for (int s = 0; s < strips; ++s) {
-    sw += __ldg(part + ((size_t)s * 2) * C + c);
-    sb += __ldg(part + ((size_t)s * 2 + 1) * C + c);
-  }
-  if (dw) dw[c] = sw;
-  if (db) db[c] = sb;
+// The parts of dw and db added in a fixed order, the same bits every time: a block takes 32 of the 2C columns, 32 warps every 32nd part.
+__global__ void __launch_bounds__(1024) layer_norm_join_kernel(const float* part, int parts, int C, float* dw, float* db) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < 2 * C)
+    for (int p = w; p < parts; p += 32) s += part[(size_t)p * 2 * C + c];
+  red[w][lane] = s;
+  __syncthreads();
+  if (w || c >= 2 * C) return;
+  s = 0.f;
+  for (int i = 0; i < 32; ++i) s += red[i][lane];
+  float* to = c < C ? dw : db;
+  if (to) to[c < C ? c : c - C] = s;
 }
 
+// ------------------------------------------------------------------------------------------------------------ rows in registers
+// A row is held in registers by a team of threads, a warp or (rows too long for one) a block, each with CH pieces of VEC values; the next row's loads are issued before this row's
+// sums, so that every warp has two rows in flight.  One pass over memory in both directions: the backward kernel reads x and dy once, writes dx, and keeps every column's
+// part of dw and db in registers over all rows of its team.
+template <typename T, int VEC> struct Piece { uint32_t w[sizeof(T) * VEC / 4]; };
+template <> struct Piece<__nv_bfloat16, 1> { unsigned short w[1]; };
+
+template <typename T, int VEC> __device__ __forceinline__ Piece<T, VEC> load_piece(const T* p) {
+  Piece<T, VEC> r;
+  constexpr int B = sizeof(T) * VEC;
+  if constexpr (B == 16) *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
+  else if constexpr (B == 8) *reinterpret_cast<uint2*>(&r) = __ldg(reinterpret_cast<const uint2*>(p));
+  else if constexpr (B == 4) r.w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  else r.w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+  return r;
+}
+template <typename T, int VEC> __device__ __forceinline__ void widen(const Piece<T, VEC>& r, float* v) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(r.w[i]);
+  } else if constexpr (VEC == 1) {
+    v[0] = __uint_as_float((uint32_t)r.w[0] << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) { v[2 * i] = __uint_as_float(r.w[i] << 16); v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u); }
+  }
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_piece(T* p, const float* v) {
+  constexpr int B = sizeof(T) * VEC;
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else p[0] = v[0];
+  } else if constexpr (VEC == 1) {
+    p[0] = __float2bfloat16_rn(v[0]);
+  } else {
+    uint32_t w[VEC / 2];
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    if constexpr (B == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Where a thread's pieces lie, and which rows its team takes.
+template <int VEC, bool BLOCK> struct Team {
+  int first, pitch, warp, warps;
+  int64_t row, step;
+  __device__ __forceinline__ Team() {
+    warp = threadIdx.x >> 5; warps = blockDim.x >> 5;
+    const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31;
+    first = lane * VEC;
+    pitch = (BLOCK ? blockDim.x : 32) * VEC;
+    row = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * warps + warp;
+    step = BLOCK ? gridDim.x : (int64_t)gridDim.x * warps;
+  }
+};
+
+template <typename TX, typename TY, int VEC, int CH, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) layer_norm_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64_t stride, const float* __restrict__ w,
+                                                                             const float* __restrict__ b, float eps, TY* __restrict__ y, float2* __restrict__ stats) {
+  __shared__ float2 part[2][32];
+  const Team<VEC, BLOCK> t;
+  float wv[CH * VEC], bv[CH * VEC];
+#pragma unroll
+  for (int k = 0; k < CH; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = t.first + k * t.pitch + i;
+      wv[k * VEC + i] = w && c < C ? __ldg(w + c) : 1.f;
+      bv[k * VEC + i] = b && c < C ? __ldg(b + c) : 0.f;
+    }
+  Piece<TX, VEC> next[CH];
+  auto fetch = [&](int64_t r) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (t.first + k * t.pitch < C) next[k] = load_piece<TX, VEC>(x + r * stride + t.first + k * t.pitch);
+  };
+  if (t.row < rows) fetch(t.row);
+  int flip = 0;
+  for (int64_t r = t.row; r < rows; r += t.step, flip ^= 1) {
+    float v[CH * VEC];
+    float s = 0.f, n = 0.f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const bool in = t.first + k * t.pitch < C;
+      if (in) { widen<TX, VEC>(next[k], v + k * VEC); n += VEC; }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { v[k * VEC + i] = in ? v[k * VEC + i] : 0.f; s += v[k * VEC + i]; }
+    }
+    if (r + t.step < rows) fetch(r + t.step);
+    // mean and sum of squares about it: of the warp's values, then (block) of all warps' by the parallel form of the same
+    const float count = BLOCK ? warp_sum(n) : (float)C;
+    float mean = warp_sum(s) / fmaxf(count, 1.f), q = 0.f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (t.first + k * t.pitch < C) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) { const float d = v[k * VEC + i] - mean; q = fmaf(d, d, q); }
+      }
+    q = warp_sum(q);
+    if (BLOCK) {
+      if ((threadIdx.x & 31) == 0) part[flip][t.warp] = make_float2(mean, q);
+      __syncthreads();                     // (two sets of parts: a warp that is ahead writes the other one)
+      // every warp's count follows from C; warps hold pieces in turn, so it is that of the pieces that fall on them
+      float all = 0.f;
+      q = 0.f;
+      float total = 0.f;
+      for (int i = 0; i < t.warps; ++i) {
+        float ni = 0.f;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) ni += (float)min(max(C - (i * 32 * VEC + k * t.pitch), 0), 32 * VEC);
+        const float2 p = part[flip][i];
+        total = fmaf(ni, p.x, total);
+        all += ni;
+      }
+      mean = total / all;
+      for (int i = 0; i < t.warps; ++i) {
+        float ni = 0.f;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) ni += (float)min(max(C - (i * 32 * VEC + k * t.pitch), 0), 32 * VEC);
+        const float2 p = part[flip][i];
+        const float d = p.x - mean;
+        q += ni > 0.f ? fmaf(ni * d, d, p.y) : 0.f;
+      }
+    }
+    const float rstd = 1.f / sqrtf(q / C + eps);
+    if (stats && (BLOCK ? threadIdx.x : threadIdx.x & 31) == 0) stats[r] = make_float2(mean, rstd);
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (t.first + k * t.pitch < C) {
+        float o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = fmaf((v[k * VEC + i] - mean) * rstd, wv[k * VEC + i], bv[k * VEC + i]);
+        store_piece<TY, VEC>(y + r * C + t.first + k * t.pitch, o);
+      }
+  }
+}
+
+template <typename TX, typename TY, int VEC, int CH, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256, BLOCK ? 1 : 2)
+layer_norm_grad_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64_t stride, const TY* __restrict__ dy, int64_t dy_stride, const float* __restrict__ w,
+                            const float2* __restrict__ stats, TX* __restrict__ dx, float* __restrict__ part) {
+  constexpr int E = CH * VEC;
+  __shared__ float2 sums[2][32];
+  extern __shared__ float joined[];        // warp teams: their parts, [2][C]
+  const Team<VEC, BLOCK> t;
+  float wv[E], aw[E], ab[E];
+#pragma unroll
+  for (int k = 0; k < CH; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = t.first + k * t.pitch + i;
+      wv[k * VEC + i] = w && c < C ? __ldg(w + c) : 1.f;
+      aw[k * VEC + i] = ab[k * VEC + i] = 0.f;
+    }
+  Piece<TX, VEC> nx[CH];
+  Piece<TY, VEC> ng[CH];
+  float2 ns = make_float2(0.f, 0.f);
+  auto fetch = [&](int64_t r) {
+    ns = __ldg(stats + r);
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (t.first + k * t.pitch < C) {
+        nx[k] = load_piece<TX, VEC>(x + r * stride + t.first + k * t.pitch);
+        ng[k] = load_piece<TY, VEC>(dy + r * dy_stride + t.first + k * t.pitch);
+      }
+  };
+  if (t.row < rows) fetch(t.row);
+  const float inv = 1.f / C;
+  int flip = 0;
+  for (int64_t r = t.row; r < rows; r += t.step, flip ^= 1) {
+    const float2 st = ns;
+    float xh[E], g[E], sg = 0.f, sx = 0.f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (t.first + k * t.pitch < C) {
+        widen<TX, VEC>(nx[k], xh + k * VEC);
+        widen<TY, VEC>(ng[k], g + k * VEC);
+#pragma unroll
+        for (int i = k * VEC; i < (k + 1) * VEC; ++i) {
+          xh[i] = (xh[i] - st.x) * st.y;
+          aw[i] = fmaf(g[i], xh[i], aw[i]);
+          ab[i] += g[i];
+          g[i] *= wv[i];
+          sg += g[i];
+          sx = fmaf(g[i], xh[i], sx);
+        }
+      }
+    if (r + t.step < rows) fetch(r + t.step);
+    sg = warp_sum(sg);
+    sx = warp_sum(sx);
+    if (BLOCK) {
+      if ((threadIdx.x & 31) == 0) sums[flip][t.warp] = make_float2(sg, sx);
+      __syncthreads();
+      sg = sx = 0.f;
+      for (int i = 0; i < t.warps; ++i) { const float2 p = sums[flip][i]; sg += p.x; sx += p.y; }
+    }
+    sg *= inv;
+    sx *= inv;
+    if (dx) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+        if (t.first + k * t.pitch < C) {
+          float o[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) o[i] = st.y * (g[k * VEC + i] - sg - xh[k * VEC + i] * sx);
+          store_piece<TX, VEC>(dx + r * C + t.first + k * t.pitch, o);
+        }
+    }
+  }
+  if (!part) return;
+  float* mine = part + (size_t)blockIdx.x * 2 * C;
+  if (!BLOCK) {            // the warps' parts one after another: a fixed order
+    for (int u = 0; u < t.warps; ++u) {
+      if (t.warp == u) {
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const int c = t.first + k * t.pitch + i;
+            if (c < C) {
+              joined[c] = (u ? joined[c] : 0.f) + aw[k * VEC + i];
+              joined[C + c] = (u ? joined[C + c] : 0.f) + ab[k * VEC + i];
+            }
+          }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * C; c += blockDim.x) mine[c] = joined[c];
+  } else {
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int c = t.first + k * t.pitch + i;
+        if (c < C) { mine[c] = aw[k * VEC + i]; mine[C + c] = ab[k * VEC + i]; }
+      }
+  }
+}
+
+// How a row is held: pieces of `vec` values, `ch` of them a thread, teams of `threads` (0: the kernels above, which read a row several times).
+struct Shape { int vec, ch, threads; bool block; };
+Shape shape_of(const void* x, int64_t x_stride, int xs, const void* y, int64_t y_stride, int ys, int C) {
+  auto fits = [&](int v) {
+    return C % v == 0 && x_stride % v == 0 && y_stride % v == 0 && (reinterpret_cast<uintptr_t>(x) % (v * xs)) == 0 && (reinterpret_cast<uintptr_t>(y) % (v * ys)) == 0;
+  };
+  const bool wide = xs == 4 || ys == 4;                       // VEC 8 is for bf16 on both sides: 16 bytes
+  const int vec = !wide && C >= 512 && fits(8) ? 8 : fits(4) ? 4 : 1;
+  // A warp holds up to 24 values a thread of bf16, 12 of float32 or one by one; beyond, its registers would leave too few warps on an SM.
+  int ch = (C + 32 * vec - 1) / (32 * vec);
+  if (vec == 1) ch = (ch + 3) / 4 * 4;
+  if (ch * vec <= (wide || vec == 1 ? 12 : 24)) return {vec, ch, 32, false};
+  const int per = vec == 8 ? 1 : vec == 4 ? 2 : 8;             // a block: 8 values a thread
+  const int threads = ((C + per * vec - 1) / (per * vec) + 31) / 32 * 32;
+  if (threads <= 1024) return {vec, per, threads, true};
+  return {0, 0, 0, false};
+}
+
+constexpr int GRAD_BLOCKS = 592;         // most parts of dw and db
+int grad_blocks(const Shape& s, int64_t rows) {
+  const int64_t want = s.block ? rows : (rows + 7) / 8, most = s.block ? std::max(148, std::min(GRAD_BLOCKS, 148 * 640 / s.threads)) : 296;
+  return (int)std::min<int64_t>(want, most);
+}
+
+template <typename TX, typename TY> struct Run {
+  const void* x; int64_t rows; int C; int64_t stride; const float* w; const float* b; float eps; void* y; float* stats;
+  const void* dy; int64_t dy_stride; void* dx; float* part; cudaStream_t st;
+  template <int VEC, int CH, bool BLOCK> int go(const Shape& s, bool backward) const {
+    const int threads = BLOCK ? s.threads : 256;
+    if (!backward) {
+      const int64_t want = BLOCK ? rows : (rows + 7) / 8, most = BLOCK ? 148 * std::max(1, 2048 / s.threads) : 148 * 6;
+      layer_norm_rows_kernel<TX, TY, VEC, CH, BLOCK><<<(int)std::min(want, most), threads, 0, st>>>((const TX*)x, rows, C, stride, w, b, eps, (TY*)y, (float2*)stats);
+      return fovi::after_launch("layer_norm_rows_kernel");
+    }
+    layer_norm_grad_rows_kernel<TX, TY, VEC, CH, BLOCK><<<grad_blocks(s, rows), threads, BLOCK ? 0 : 2 * C * sizeof(float), st>>>(
+        (const TX*)x, rows, C, stride, (const TY*)dy, dy_stride, w, (const float2*)stats, (TX*)dx, part);
+    return fovi::after_launch("layer_norm_grad_rows_kernel");
+  }
+  template <int VEC, int MOST, int STEP = 1, int CH = STEP> int warp(const Shape& s, bool backward) const {
+    if constexpr (CH * VEC <= MOST) return s.ch == CH ? go<VEC, CH, false>(s, backward) : warp<VEC, MOST, STEP, CH + STEP>(s, backward);
+    return FOVI_ERR_UNSUPPORTED;
+  }
+  int operator()(const Shape& s, bool backward) const {
+    if (s.block) {
+      if constexpr (sizeof(TX) == 2 && sizeof(TY) == 2) {
+        if (s.vec == 8) return go<8, 1, true>(s, backward);
+      }
+      return s.vec == 4 ? go<4, 2, true>(s, backward) : go<1, 8, true>(s, backward);
+    }
+    if constexpr (sizeof(TX) == 2 && sizeof(TY) == 2) {
+      if (s.vec == 8) return warp<8, 24>(s, backward);
+      if (s.vec == 4) return warp<4, 24>(s, backward);
+    }
+    return s.vec == 4 ? warp<4, 12>(s, backward) : warp<1, 12, 4>(s, backward);
+  }
+};
+
+// ------------------------------------------------------------------------------------------------------------ host
 int strips_of(int64_t rows) { return (int)(rows < 512 ? (rows + 15) / 16 : 64); }
 
 template <typename TX, typename TY>
 int forward(const void* x, int64_t rows, int C, int64_t stride, const float* w, const float* b, float eps, void* y, float* stats, cudaStream_t st) {
+  const Shape s = shape_of(x, stride, sizeof(TX), y, C, sizeof(TY), C);
+  if (s.threads) return Run<TX, TY>{x, rows, C, stride, w, b, eps, y, stats, nullptr, 0, nullptr, nullptr, st}(s, false);
   const int grid = (int)(rows < 148 * 8 ? rows : 148 * 8);
   layer_norm_kernel<TX, TY><<<grid, GEN_THREADS, 0, st>>>((const TX*)x, rows, C, stride, w, b, eps, (TY*)y, (float2*)stats);
   return fovi::after_launch("layer_norm_kernel");
@@ -105,29 +419,35 @@ int forward(const void* x, int64_t rows, int C, int64_t stride, const float* w, 
 template <typename TX, typename TY>
 int backward(const void* x, int64_t rows, int C, int64_t stride, const void* dy, int64_t dy_stride, const float* w, const float* stats, void* dx, float* dw, float* db,
              float* work, cudaStream_t st) {
-  if (dx) {
-    const int grid = (int)(rows < 148 * 8 ? rows : 148 * 8);
-    layer_norm_dx_kernel<TX, TY><<<grid, GEN_THREADS, 0, st>>>((const TX*)x, rows, C, stride, (const TY*)dy, dy_stride, w, (const float2*)stats, (TX*)dx);
-    const int rc = fovi::after_launch("layer_norm_dx_kernel");
-    if (rc) return rc;
-  }
-  if (dw || db) {
-    const int strips = strips_of(rows);
+  Shape s = shape_of(x, stride, sizeof(TX), dy, dy_stride, sizeof(TY), C);
+  if (s.threads && dx && (reinterpret_cast<uintptr_t>(dx) % (s.vec * sizeof(TX)))) s.threads = 0;
+  int strips = strips_of(rows);
+  if (s.threads) {
+    const int rc = Run<TX, TY>{x, rows, C, stride, w, nullptr, 0.f, nullptr, const_cast<float*>(stats), dy, dy_stride, dx, dw || db ? work : nullptr, st}(s, true);
+    if (rc || !(dw || db)) return rc;
+    strips = grad_blocks(s, rows);
+  } else {
+    if (dx) {
+      const int grid = (int)(rows < 148 * 8 ? rows : 148 * 8);
+      layer_norm_dx_kernel<TX, TY><<<grid, GEN_THREADS, 0, st>>>((const TX*)x, rows, C, stride, (const TY*)dy, dy_stride, w, (const float2*)stats, (TX*)dx);
+      const int rc = fovi::after_launch("layer_norm_dx_kernel");
+      if (rc) return rc;
+    }
+    if (!dw && !db) return FOVI_OK;
     const dim3 grid((C + STRIP_COLS - 1) / STRIP_COLS, strips);
     layer_norm_dw_kernel<TX, TY><<<grid, STRIP_COLS, 0, st>>>((const TX*)x, rows, C, stride, (const TY*)dy, dy_stride, (const float2*)stats, work, strips);
-    int rc = fovi::after_launch("layer_norm_dw_kernel");
+    const int rc = fovi::after_launch("layer_norm_dw_kernel");
     if (rc) return rc;
-    layer_norm_join_kernel<<<(C + 255) / 256, 256, 0, st>>>(work, strips, C, dw, db);
-    return fovi::after_launch("layer_norm_join_kernel");
   }
-  return FOVI_OK;
+  layer_norm_join_kernel<<<(2 * C + 31) / 32, 1024, 0, st>>>(work, strips, C, dw, db);
+  return fovi::after_launch("layer_norm_join_kernel");
 }
 
 }  // namespace
 
 extern "C" int64_t fovi_layer_norm_workspace_bytes(int64_t rows, int C) {
   if (rows < 0 || C < 1) return -1;
-  return (int64_t)strips_of(rows) * 2 * C * 4;
+  return std::max<int64_t>(std::min<int64_t>(rows, GRAD_BLOCKS), strips_of(rows)) * 2 * C * 4;
 }
 
 extern "C" int fovi_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int C, int64_t x_stride, const float* weight, const float* bias, float eps, void* y,
