@@ -47,7 +47,7 @@ def build_native(force=False):
     src, stamp = os.path.join(CSRC, "bind.cpp"), os.path.splitext(NATIVE)[0] + ".stamp"
     torch, version = _torch_version()
     made_for = f"torch {version}, python {sys.version}"
-    newest = max(os.path.getmtime(f) for f in (src, os.path.join(HERE, "..", "include", "fovi_b200.h"), os.path.abspath(__file__)))
+    newest = max(os.path.getmtime(f) for f in (src, os.path.join(CSRC, "bind_tokens.h"), os.path.join(HERE, "..", "include", "fovi_b200.h"), os.path.abspath(__file__)))
     plain = os.path.join(os.path.dirname(NATIVE), "_native.so")          # a name that any interpreter would import
     if plain != NATIVE and os.path.exists(plain):
         os.remove(plain)

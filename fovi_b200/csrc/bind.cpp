@@ -301,6 +301,12 @@ BODY(block_backward, 10)
   return tuple;
 END
 
+}  // namespace
+
+#include "bind_tokens.h"
+
+namespace {
+
 // {name of the C ABI's function: its address}
 PyObject* connect(PyObject*, PyObject* dict) {
   const struct { const char* name; void** at; } want[] = {
@@ -309,7 +315,11 @@ PyObject* connect(PyObject*, PyObject* dict) {
       {"fovi_knnconv_pack_weights_transposed", (void**)&abi.pack_weights_t}, {"fovi_knndw_run", (void**)&abi.dw_run},
       {"fovi_weight_grad_unpack", (void**)&abi.unpack}, {"fovi_points_to_channels", (void**)&abi.to_channels},
       {"fovi_relu_pool_forward", (void**)&abi.relu_pool}, {"fovi_norm_block_workspace_bytes", (void**)&abi.norm_work},
-      {"fovi_norm_block_backward", (void**)&abi.norm_back}};
+      {"fovi_norm_block_backward", (void**)&abi.norm_back}, {"fovi_status_string", (void**)&tok.status}, {"fovi_last_cuda_error", (void**)&tok.cuda_error},
+      {"fovi_layer_norm_forward", (void**)&tok.norm}, {"fovi_layer_norm_workspace_bytes", (void**)&tok.norm_work},
+      {"fovi_layer_norm_backward", (void**)&tok.norm_back}, {"fovi_rotary", (void**)&tok.rotary},
+      {"fovi_attention_workspace_bytes", (void**)&tok.attend_work}, {"fovi_attention_forward", (void**)&tok.attend},
+      {"fovi_attention_backward", (void**)&tok.attend_back}};
   for (const auto& w : want) {
     PyObject* a = PyDict_GetItemString(dict, w.name);
     if (!a) { PyErr_Format(PyExc_KeyError, "%s", w.name); return nullptr; }
@@ -321,7 +331,7 @@ PyObject* connect(PyObject*, PyObject* dict) {
 
 #define FAST(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(sample), FAST(conv_forward), FAST(conv_forward_f32), FAST(pack_points), FAST(pack_slabs), FAST(weight_grad), FAST(block_forward),
-                         FAST(block_backward), {"connect", connect, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         FAST(block_backward), FAST(layer_norm), FAST(rotary), FAST(attention), {"connect", connect, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -47,6 +47,11 @@ class _LayerNormFunction(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     """Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias with the biased variance.  x [..., C] float32 or bf16; weight, bias [C] or
     None; the result has x's type, or `out_dtype`.  Statistics, sums and the parameters' gradients are float32; those gradients are the same bits every time."""
+    if ops._native is not None and out_dtype is None and x.is_cuda:
+        dev = ops._current_device()
+        got = ops._native.layer_norm(x, weight, bias, eps, dev, ops._raw_stream(dev))
+        if got is not None:
+            return ops._checked(got, "fovi_layer_norm_forward")
     if _wants_grad(x, weight, bias):
         return _LayerNormFunction.apply(x, weight, bias, eps, out_dtype)
     return ops.layer_norm(x, weight, bias, eps, out_dtype)
@@ -76,6 +81,11 @@ def rotary(x, positions, frequencies, pairs_per_axis, prefix=0, pairing="halves"
     ("pairs"); channels from 2P on pass.  Differentiable with respect to x; positions and frequencies carry no gradient."""
     if pairing not in _PAIRINGS:
         raise ValueError(f"pairing is {pairing!r}: 'halves' or 'pairs'")
+    if ops._native is not None and x.is_cuda:
+        dev = ops._current_device()
+        got = ops._native.rotary(x, positions, frequencies, pairs_per_axis, prefix, _PAIRINGS[pairing], dev, ops._raw_stream(dev))
+        if got is not None:
+            return ops._checked(got, "fovi_rotary")
     if _wants_grad(positions, frequencies):
         raise NotImplementedError("rotary: positions and frequencies carry no gradient; detach them")
     if _wants_grad(x):
@@ -104,6 +114,11 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
     Float32 or bf16, any strides (slices of a packed projection, expanded tensors); Hkv divides H, and head h reads state head h // (H // Hkv); D up to 128; scale 1 / sqrt(D) by default.
     key_lengths [B]: states at and behind it are not read; key_mask [B, Lk]: nor those where it is False.  What k and v hold there has no effect, not-a-number
     included, and their gradients are zero; a query without any state gives zeros.  Gradients are the same bits every time."""
+    if ops._native is not None and q.is_cuda:
+        dev = ops._current_device()
+        got = ops._native.attention(q, k, v, key_lengths, key_mask, scale, dev, ops._raw_stream(dev))
+        if got is not None:
+            return ops._checked(got, "fovi_attention_forward")
     if _wants_grad(q, k, v):
         return _AttentionFunction.apply(q, k, v, key_lengths, key_mask, scale)
     return ops.attention(q, k, v, key_lengths, key_mask, scale)

@@ -8,6 +8,15 @@ pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True, params=["native", "python"])
+def launch_path(request, monkeypatch):
+    """Every test with the native launch path (csrc/bind_tokens.h) and with the Python one."""
+    from fovi_b200 import ops
+    assert ops._native is not None
+    if request.param == "python":
+        monkeypatch.setattr(ops, "_native", None)
+
+
 def _inputs(rows, C, dtype, seed, offset=0.5):
     g = torch.Generator(device="cuda").manual_seed(seed)
     x = (torch.randn(rows, C, generator=g, device="cuda") + offset).to(dtype)

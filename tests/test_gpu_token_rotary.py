@@ -10,6 +10,15 @@ pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True, params=["native", "python"])
+def launch_path(request, monkeypatch):
+    """Every test with the native launch path (csrc/bind_tokens.h) and with the Python one."""
+    from fovi_b200 import ops
+    assert ops._native is not None
+    if request.param == "python":
+        monkeypatch.setattr(ops, "_native", None)
+
+
 def _inputs(B, L, H, D, pairs, prefix, shared, dtype, seed, reach=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     x = torch.randn(B, L, H, D, generator=g, device="cuda").to(dtype)
