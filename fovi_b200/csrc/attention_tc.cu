@@ -1,13 +1,13 @@
 // Cross attention on the tensor cores: bf16 q, k, v of up to 128 channels a head (a multiple of 8), 16-byte aligned rows.
 //
-// Forward.  One CTA per (128 queries, head, sample), two CTAs per SM; keys in tiles of KT = 128 (64 above 64 channels).  Per tile
-//   S = Q K^T     SS MMA, M = 128, N = KT, into tensor memory
-//   P = 2^(scale log2(e) (S - m))     four warps, a thread per query: its row of S in registers, its maximum and sum in two more; P goes back to tensor memory as bf16
+// Forward.  One CTA per (128 queries, head, sample), two CTAs per SM; keys in tiles of 64.  Per tile
+//   S = Q K^T     SS MMA, M = 128, N = 64, into one of two places in tensor memory
+//   P = 2^(scale log2(e) (S - m))     four warps, a thread per query: its row of S in registers, its maximum and sum in two more; P goes back over S as bf16
 //   O += P V      TS MMA: P from tensor memory, the tile of V read MN-major, so nothing is transposed
-// A TMA warp keeps the rings of K and V tiles full, an MMA warp issues both products.  S is given back as soon as its row is in registers, so the next
-// S is computed while this one's exponentials are; the other CTA of the SM fills what gaps remain.  The reference value m of a row only moves when its maximum has risen
+// A TMA warp keeps the rings of K and V tiles full, an MMA warp issues both products.  While the exponentials of one tile are computed the scores of the next are; the other CTA of
+// the SM fills what gaps remain.  The reference value m of a row only moves when its maximum has risen
 // by more than 8 (in base 2): P then stays below 2^8, bf16's relative rounding is the same at any size, and the pass over O that a move costs is rare.
-// Tensor memory (256 columns): S [0, KT), P [KT, 3 KT / 2), O behind.
+// Tensor memory (256 columns): S and P [0, 64) and [64, 128), O behind.
 // Masked keys: their scores are -inf by a select and their rows of V are set to zero in shared memory, so what they hold has no effect.  A warp whose
 // 32 queries lie behind the last one skips the arithmetic.
 #include <cuda_bf16.h>
@@ -24,16 +24,17 @@ __device__ int g_status;           // wait site at which a kernel gave up, see f
 constexpr int AT_THREADS = 192;
 constexpr float AT_INF = __builtin_huge_valf();
 
+constexpr int KT = 64;             // keys of a tile
+
 template <int DC> struct Fwd {                     // DC: 64-channel boxes of a row
-  static constexpr int KT = DC == 1 ? 128 : 64;    // keys of a tile
-  static constexpr int NK = DC == 1 ? 3 : 2, NV = 2;
+  static constexpr int NK = DC == 1 ? 4 : 2, NV = NK;
   static constexpr uint32_t BOX = KT * 128u, TILE = DC * BOX, QBOX = AT_M * 128u, QTILE = DC * QBOX;
   static constexpr uint32_t SMEM = 1024 + 1024 + QTILE + (NK + NV) * TILE;
-  static constexpr uint32_t P_COL = KT, O_COL = DC == 1 ? 192 : 128;
+  static constexpr uint32_t O_COL = 2 * KT;
 };
 
 struct FwdHeader {
-  uint64_t q_full, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full, s_free, p_full, o_full, drain;
+  uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full, o_full, drain;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -42,7 +43,6 @@ template <int DC>
 __global__ void __launch_bounds__(AT_THREADS, 2)
 attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnTcArgs t) {
   using F = Fwd<DC>;
-  constexpr int KT = F::KT;
   const AttnArgs& a = t.a;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -53,9 +53,12 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&hdr->q_full), 1);
-    for (int i = 0; i < 3; ++i) { mbar_init(smem_u32(&hdr->k_full[i]), 1); mbar_init(smem_u32(&hdr->k_empty[i]), 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->v_full[i]), 1); mbar_init(smem_u32(&hdr->v_empty[i]), 1); }
-    mbar_init(smem_u32(&hdr->s_full), 1); mbar_init(smem_u32(&hdr->s_free), 4); mbar_init(smem_u32(&hdr->p_full), 4); mbar_init(smem_u32(&hdr->o_full), 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&hdr->k_full[i]), 1); mbar_init(smem_u32(&hdr->k_empty[i]), 1);
+      mbar_init(smem_u32(&hdr->v_full[i]), 1); mbar_init(smem_u32(&hdr->v_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&hdr->s_full[i]), 1);
+    mbar_init(smem_u32(&hdr->p_full), 4); mbar_init(smem_u32(&hdr->o_full), 1);
     mbar_init(smem_u32(&hdr->drain), 1);
     hdr->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -105,31 +108,32 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     bool ok = tiles == 0 || mbar_wait_warp(smem_u32(&hdr->q_full), 0, abort_flag, t.status, 3, t.wait_limit);
     auto scores = [&](int j) {
       if (!mbar_wait_warp(smem_u32(&hdr->k_full[ks]), kp, abort_flag, t.status, 4, t.wait_limit)) return false;
-      if (j > 0 && !mbar_wait_warp(smem_u32(&hdr->s_free), (j - 1) & 1, abort_flag, t.status, 5, t.wait_limit)) return false;
+      if (j > 1 && !mbar_wait_warp(smem_u32(&hdr->o_full), j & 1, abort_flag, t.status, 5, t.wait_limit)) return false;      // P of tile j - 2, in the same columns, is read
       tc_fence_after();
       if (elect_one()) {
-        mma_rows(u_tmem, u_sq, F::QBOX, u_sk + ks * F::TILE, F::BOX, dsteps, id_s);
+        mma_rows(u_tmem + (j & 1) * KT, u_sq, F::QBOX, u_sk + ks * F::TILE, F::BOX, dsteps, id_s);
         tc_commit(smem_u32(&hdr->k_empty[ks]));
-        tc_commit(smem_u32(&hdr->s_full));
+        tc_commit(smem_u32(&hdr->s_full[j & 1]));
       }
       __syncwarp();
       if (++ks == F::NK) { ks = 0; kp ^= 1u; }
       return true;
     };
     if (ok && tiles > 0) ok = scores(0);
+    if (ok && tiles > 1) ok = scores(1);
     for (int j = 0; j < tiles && ok; ++j) {
-      if (j + 1 < tiles) ok = scores(j + 1);
-      ok = ok && mbar_wait_warp(smem_u32(&hdr->v_full[vs]), vp, abort_flag, t.status, 6, t.wait_limit);
+      ok = mbar_wait_warp(smem_u32(&hdr->v_full[vs]), vp, abort_flag, t.status, 6, t.wait_limit);
       ok = ok && mbar_wait_warp(smem_u32(&hdr->p_full), j & 1, abort_flag, t.status, 7, t.wait_limit);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        mma_mix(u_tmem + F::O_COL, u_tmem + F::P_COL, u_sv + vs * F::TILE, F::BOX, KT / 16, id_o, j > 0);
+        mma_mix(u_tmem + F::O_COL, u_tmem + (j & 1) * KT, u_sv + vs * F::TILE, F::BOX, KT / 16, id_o, j > 0);
         tc_commit(smem_u32(&hdr->v_empty[vs]));
         tc_commit(smem_u32(&hdr->o_full));
       }
       __syncwarp();
       if (++vs == F::NV) { vs = 0; vp ^= 1u; }
+      if (j + 2 < tiles) ok = scores(j + 2);
     }
     if (*abort_flag && elect_one()) {      // no MMA may still be reading shared memory or writing tensor memory
       tc_commit(smem_u32(&hdr->drain));
@@ -151,34 +155,32 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       bool whole = true;
 #pragma unroll
       for (int i = 0; i < KT / 32; ++i) { bits[i] = key_bits(a, mask, j * KT + 32 * i, end, lane); whole = whole && bits[i] == 0xffffffffu; }
-      ok = mbar_wait_warp(smem_u32(&hdr->s_full), j & 1, abort_flag, t.status, 8, t.wait_limit);
+      ok = mbar_wait_warp(smem_u32(&hdr->s_full[j & 1]), j >> 1 & 1, abort_flag, t.status, 8, t.wait_limit);
       if (!ok) break;
       tc_fence_after();
-      float x[KT];
-      if (!idle) {
-#pragma unroll
-        for (int i = 0; i < KT; i += 32) tc_ld32(lanes + i, reinterpret_cast<uint32_t*>(x) + i);
-        tc_ld_wait();
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&hdr->s_free));
-      float m_new = m, f = 1.f;
       bool move = false;
+      float f = 1.f;
       if (!idle) {
+        const uint32_t at = lanes + (j & 1) * KT;
+        float x[KT];
+#pragma unroll
+        for (int i = 0; i < KT; i += 32) tc_ld32(at + i, reinterpret_cast<uint32_t*>(x) + i);
+        tc_ld_wait();
+        tc_loaded<KT>(reinterpret_cast<uint32_t*>(x));
         if (!whole) {
 #pragma unroll
           for (int i = 0; i < KT; ++i) x[i] = bits[i >> 5] >> (i & 31) & 1u ? x[i] : -AT_INF;
         }
-        float top[4] = {x[0], x[1], x[2], x[3]};
+        float top[4] = {m, x[0], x[1], x[2]};
+        top[0] = fmaxf(top[0], x[3]);
 #pragma unroll
         for (int i = 4; i < KT; i += 4) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[i + e]);
+          if (i & 4) { top[0] = max3(top[0], x[i], x[i + 1]); top[1] = max3(top[1], x[i + 2], x[i + 3]); }
+          else { top[2] = max3(top[2], x[i], x[i + 1]); top[3] = max3(top[3], x[i + 2], x[i + 3]); }
         }
-        m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        const float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         move = (m_new - m) * c > 8.f;
-        if (move) { f = ex2((m - m_new) * c); m = m_new; l.x *= f; l.y *= f; }
+        if (move) { f = ex2((m - m_new) * c); m = m_new; l = mul2(l, make_float2(f, f)); }
         const float mc = m == -AT_INF ? 0.f : m * c;      // no key yet: every exponent is -inf
 #pragma unroll
         for (int i = 0; i < KT; i += 2) {
@@ -187,26 +189,26 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           l = add2(l, p);
           x[i >> 1] = __uint_as_float(pack_bf16(p.x, p.y));
         }
+        tc_st32(at, reinterpret_cast<uint32_t*>(x));       // over S, which is in registers
       }
-      if (j > 0) {                      // the product with the previous P is done: P and O are this thread's
+      if (j > 0) {
+        // The product with the previous P is done: O is this thread's.  Every warp waits here in every tile: one that ran ahead would meet barriers a phase behind
+        // the one that it means, which look the same as those a phase ahead.
         ok = mbar_wait_warp(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit);
         if (!ok) break;
-        tc_fence_after();
         if (__any_sync(0xffffffffu, move)) {
+          tc_fence_after();
 #pragma unroll
           for (int o = 0; o < DC * 64; o += 32) {
             uint32_t r[32];
             tc_ld32(lanes + F::O_COL + o, r);
             tc_ld_wait();
+            tc_loaded<32>(r);
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
             tc_st32(lanes + F::O_COL + o, r);
           }
         }
-      }
-      if (!idle) {
-#pragma unroll
-        for (int i = 0; i < KT / 2; i += 32) tc_st32(lanes + F::P_COL + i, reinterpret_cast<uint32_t*>(x) + i);
       }
       if (!whole) {                     // rows of V that must not be read: a zero weight times what they hold need not be zero
         ok = mbar_wait_warp(smem_u32(&hdr->v_full[j % F::NV]), (j / F::NV) & 1, abort_flag, t.status, 10, t.wait_limit);
@@ -240,7 +242,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll
       for (int o = 0; o < DC * 64; o += 32) {
         uint32_t r[32];
-        if (tiles > 0) { tc_ld32(lanes + F::O_COL + o, r); tc_ld_wait(); }
+        if (tiles > 0) { tc_ld32(lanes + F::O_COL + o, r); tc_ld_wait(); tc_loaded<32>(r); }
         if (row < a.Lq) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
@@ -282,8 +284,8 @@ int forward(const AttnArgs& a, cudaStream_t st, bool selftest) {
   t.skip_loads = selftest;
   int rc = fovi::attention_tc_status(&t.status);
   if (!rc) rc = fovi::encode_rows(&tq, &t.q, a.q, a.q_sb, a.q_sl, a.q_sh, a.B, a.Lq, a.H, a.D, AT_M);
-  if (!rc) rc = fovi::encode_rows(&tk, &t.k, a.k, a.k_sb, a.k_sl, a.k_sh, a.B, a.Lk, a.Hkv, a.D, F::KT);
-  if (!rc) rc = fovi::encode_rows(&tv, &t.v, a.v, a.v_sb, a.v_sl, a.v_sh, a.B, a.Lk, a.Hkv, a.D, F::KT);
+  if (!rc) rc = fovi::encode_rows(&tk, &t.k, a.k, a.k_sb, a.k_sl, a.k_sh, a.B, a.Lk, a.Hkv, a.D, KT);
+  if (!rc) rc = fovi::encode_rows(&tv, &t.v, a.v, a.v_sb, a.v_sl, a.v_sh, a.B, a.Lk, a.Hkv, a.D, KT);
   if (rc) return rc;
   const int64_t blocks = (int64_t)((a.Lq + AT_M - 1) / AT_M) * a.H * a.B;
   if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;

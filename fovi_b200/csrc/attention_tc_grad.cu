@@ -266,6 +266,8 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             tc_ld32(lanes + first + e, reinterpret_cast<uint32_t*>(s));
             tc_ld32(lanes + G::DP + first + e, reinterpret_cast<uint32_t*>(d));
             tc_ld_wait();
+            tc_loaded<32>(reinterpret_cast<uint32_t*>(s));
+            tc_loaded<32>(reinterpret_cast<uint32_t*>(d));
           }
           if (e + 32 == HALF) {                       // the last columns are in registers: the next scores may come
             tc_fence_before();
@@ -356,6 +358,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         if (it.n > 0) {
           tc_ld32(lanes + from + e, reinterpret_cast<uint32_t*>(v));
           tc_ld_wait();
+          tc_loaded<32>(reinterpret_cast<uint32_t*>(v));
           if (e + 32 == SPAN) {
             tc_fence_before();
             __syncwarp();

@@ -33,6 +33,7 @@ def _check(q, k, v, dy, **mask):
         oracle.near(g, want)
     with torch.no_grad():
         assert torch.equal(tokens.cross_attention(q, k, v, **mask), o)
+    tokens.check()
     return got
 
 
@@ -48,6 +49,19 @@ SHAPES = [  # B, Lq, Lk, H, Hkv, D
 @pytest.mark.parametrize("shape", SHAPES)
 def test_forward_and_gradients(shape, dtype):
     _check(*_inputs(*shape, dtype, sum(shape)))
+
+
+def test_many_blocks_of_few_queries():
+    """Warps without a query do no arithmetic and would run ahead of the one that does; several blocks follow one another on every SM."""
+    from fovi_b200 import tokens
+    for B, Lq, Lk, D in ((64, 1, 2056, 64), (40, 33, 700, 128), (64, 70, 1030, 64)):
+        q, k, v, _ = _inputs(B, Lq, Lk, 20, 20, D, BF, Lk)
+        for kw in ({}, dict(key_lengths=torch.randint(0, Lk + 1, (B,), device="cuda", dtype=torch.int32)), dict(key_mask=torch.rand(B, Lk, device="cuda") < 0.7)):
+            got = tokens.cross_attention(q, k, v, **kw)
+            tokens.check()
+            for b in range(0, B, 8):
+                part = {n: t[b:b + 8] for n, t in kw.items()}
+                oracle.near(got[b:b + 8], oracle.attention(q[b:b + 8], k[b:b + 8], v[b:b + 8], **part))
 
 
 @pytest.mark.autograd
