@@ -346,7 +346,8 @@ void gradients(AttnArgs& a, const void* o, const void* dy, const int64_t* s, con
 extern "C" int64_t fovi_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, int backward) {
   const int64_t none = 0;
   if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, &none, 0)) return -1;
-  return backward ? fovi::attention_tc_backward_bytes(B, Lq, H) : 0;          // the plain kernels need a part of it
+  if (backward) return fovi::attention_tc_backward_bytes(B, Lq, H);          // (the plain kernels need a part of it)
+  return dtype == FOVI_BF16 && D % 8 == 0 && D <= fovi::ATT_MAX_DIM && Lk > 0 ? fovi::attention_tc_forward_bytes(B, Lq, Lk, H, D) : 0;
 }
 
 extern "C" int fovi_attention_forward(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides,
@@ -361,7 +362,7 @@ extern "C" int fovi_attention_forward(const void* q, const void* k, const void* 
   AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
   a.out = o; a.lse = lse;
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  if (fovi::attention_tc_takes(a, dtype, false)) return fovi::launch_attention_tc_forward(a, st, false);
+  if (fovi::attention_tc_takes(a, dtype, false)) return fovi::launch_attention_tc_forward(a, need > 0 ? work : nullptr, st, false);
   if (dtype == FOVI_BF16) return D <= 64 ? forward<__nv_bfloat16, 64>(a, st) : forward<__nv_bfloat16, 128>(a, st);
   return D <= 64 ? forward<float, 64>(a, st) : forward<float, 128>(a, st);
 }
@@ -398,7 +399,7 @@ extern "C" int fovi_attention_forward_selftest_wait_timeout(const void* q, const
   AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, nullptr, nullptr, scale);
   a.out = o;
   if (!fovi::attention_tc_takes(a, FOVI_BF16, false)) return FOVI_ERR_UNSUPPORTED;
-  return fovi::launch_attention_tc_forward(a, reinterpret_cast<cudaStream_t>(stream), true);
+  return fovi::launch_attention_tc_forward(a, nullptr, reinterpret_cast<cudaStream_t>(stream), true);
 }
 
 extern "C" int fovi_attention_backward_selftest_wait_timeout(const void* q, const void* k, const void* v, const void* o, const void* dy, int B, int Lq, int Lk, int H, int Hkv,

@@ -1,13 +1,15 @@
 // Cross attention on the tensor cores: bf16 q, k, v of up to 128 channels a head (a multiple of 8), 16-byte aligned rows.
 //
-// Forward.  One CTA per (128 queries, head, sample), two CTAs per SM; keys in tiles of 64.  Per tile
-//   S = Q K^T     SS MMA, M = 128, N = 64, into one of two places in tensor memory
-//   P = 2^(scale log2(e) (S - m))     four warps, a thread per query: its row of S in registers, its maximum and sum in two more; P goes back over S as bf16
+// Forward.  One CTA per (128 queries, head, sample), three per SM (two above 64 channels); keys in tiles of 64.  Per tile
+//   S = Q K^T     SS MMA, M = 128, N = 64, into tensor memory
+//   P = 2^(scale log2(e) (S - m))     four warps, a thread per query: its row of S in registers, its running maximum and sum too; P goes to tensor memory as bf16
 //   O += P V      TS MMA: P from tensor memory, the tile of V read MN-major, so nothing is transposed
-// A TMA warp keeps the rings of K and V tiles full, an MMA warp issues both products.  While the exponentials of one tile are computed the scores of the next are; the other CTA of
-// the SM fills what gaps remain.  The reference value m of a row only moves when its maximum has risen
+// A fifth warp issues the tensor copies and both products.  S is given back as soon as its row is in registers, so the next tile's scores are computed while this one's exponentials
+// are.  What bounds it are the exponentials (16 a clock and SM: 512 clocks a tile) and, as long as a warp's tile takes 1400 clocks in all (barriers, tensor memory and the
+// maximum the rest), how many warps a scheduler has to choose from: three, with 128 registers each.  (A block's registers are given out evenly over the four schedulers: with two
+// issuing warps, six in all, a third block would leave a thread 96.)
+// The reference value m of a row only moves when its maximum has risen
 // by more than 8 (in base 2): P then stays below 2^8, bf16's relative rounding is the same at any size, and the pass over O that a move costs is rare.
-// Tensor memory (256 columns): S and P [0, 64) and [64, 128), O behind.
 // Masked keys: their scores are -inf by a select and their rows of V are set to zero in shared memory, so what they hold has no effect.  A warp whose
 // 32 queries lie behind the last one skips the arithmetic.
 #include <cuda_bf16.h>
@@ -21,26 +23,29 @@ using fovi::key_end;
 namespace {
 
 __device__ int g_status;           // wait site at which a kernel gave up, see fovi_attention_check: one word per device
-constexpr int AT_THREADS = 192;
+constexpr int AT_THREADS = 160;
 constexpr float AT_INF = __builtin_huge_valf();
 
 constexpr int KT = 64;             // keys of a tile
 
 template <int DC> struct Fwd {                     // DC: 64-channel boxes of a row
-  static constexpr int NK = DC == 1 ? 4 : 2, NV = NK;
+  static constexpr int CTAS = DC == 1 ? 3 : 2;     // per SM
+  static constexpr int NP = DC == 1 ? 1 : 2;       // places for P
+  static constexpr int NK = DC == 1 ? 3 : 2, NV = NK;
   static constexpr uint32_t BOX = KT * 128u, TILE = DC * BOX, QBOX = AT_M * 128u, QTILE = DC * QBOX;
   static constexpr uint32_t SMEM = 1024 + 1024 + QTILE + (NK + NV) * TILE;
-  static constexpr uint32_t O_COL = 2 * KT;
+  // Tensor memory comes in powers of two.  One box: S and O in 128 columns and P in 32 of its own, so that three CTAs fit 512.
+  static constexpr uint32_t COLS = DC == 1 ? 128 : 256, O_COL = DC == 1 ? 64 : 128, P_COLS = DC == 1 ? 32 : 0, P_COL = 64;
 };
 
 struct FwdHeader {
-  uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full, o_full, drain;
-  uint32_t tmem_base;
+  uint64_t q_full, k_full[3], v_full[3], s_full, s_free, p_full[2], o_full, done, drain;
+  uint32_t tmem_base, tmem_p;
   int abort_flag;
 };
 
 template <int DC>
-__global__ void __launch_bounds__(AT_THREADS, 2)
+__global__ void __launch_bounds__(AT_THREADS, Fwd<DC>::CTAS)
 attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnTcArgs t) {
   using F = Fwd<DC>;
   const AttnArgs& a = t.a;
@@ -53,161 +58,179 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&hdr->q_full), 1);
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(smem_u32(&hdr->k_full[i]), 1); mbar_init(smem_u32(&hdr->k_empty[i]), 1);
-      mbar_init(smem_u32(&hdr->v_full[i]), 1); mbar_init(smem_u32(&hdr->v_empty[i]), 1);
-    }
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&hdr->s_full[i]), 1);
-    mbar_init(smem_u32(&hdr->p_full), 4); mbar_init(smem_u32(&hdr->o_full), 1);
-    mbar_init(smem_u32(&hdr->drain), 1);
+    for (int i = 0; i < 3; ++i) { mbar_init(smem_u32(&hdr->k_full[i]), 1); mbar_init(smem_u32(&hdr->v_full[i]), 1); }
+    mbar_init(smem_u32(&hdr->s_full), 1); mbar_init(smem_u32(&hdr->s_free), 4);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&hdr->p_full[i]), 4);
+    mbar_init(smem_u32(&hdr->o_full), 1); mbar_init(smem_u32(&hdr->done), 1); mbar_init(smem_u32(&hdr->drain), 1);
     hdr->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 4) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hdr->tmem_base)), "r"(256u) : "memory");
+  if (warp == 4) {         // the small piece first: blocks that wait for the large one then hold next to nothing of what the others wait for
+    if (F::P_COLS)
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hdr->tmem_p)), "r"(32u) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hdr->tmem_base)), "r"(F::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int n_qt = (a.Lq + AT_M - 1) / AT_M;
-  const int q0 = (int)(blockIdx.x % n_qt) * AT_M, h = blockIdx.x / n_qt % a.H, b = blockIdx.x / n_qt / a.H, hk = h / a.group;
-  const int end = key_end(a, b), tiles = (end + KT - 1) / KT;
+  const int n_qt = (a.Lq + AT_M - 1) / AT_M, split = blockIdx.x % t.splits, block = blockIdx.x / t.splits;
+  const int q0 = block % n_qt * AT_M, h = block / n_qt % a.H, b = block / n_qt / a.H, hk = h / a.group;
+  const int end = key_end(a, b), share = ((end + KT - 1) / KT + t.splits - 1) / t.splits, first = split * share;       // tiles [first, first + tiles) of the keys
+  const int tiles = min(max((end + KT - 1) / KT - first, 0), share);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = hdr->tmem_base;
+  const uint32_t tmem = hdr->tmem_base, tmem_p = F::P_COLS ? hdr->tmem_p : tmem + F::P_COL;
 
-  if (warp == 5) {
-    // ------------------------------------------------------------ tensor copies
-    if (lane == 0 && tiles > 0 && !t.skip_loads) {
-      const uint32_t qf = smem_u32(&hdr->q_full);
-      mbar_expect_tx(qf, F::QTILE);
-      for (int c = 0; c < DC; ++c) tma_load_4d(sq + c * F::QBOX, &tm_q, qf, 64 * c, q0, h * t.q.mul_h, b * t.q.mul_b);
-      uint32_t ks = 0, kp = 0, vs = 0, vp = 0;
-      for (int j = 0; j < tiles; ++j) {
-        if (!mbar_wait(smem_u32(&hdr->k_empty[ks]), kp ^ 1u, abort_flag, t.status, 1, t.wait_limit)) break;
-        const uint32_t kf = smem_u32(&hdr->k_full[ks]);
-        mbar_expect_tx(kf, F::TILE);
-        for (int c = 0; c < DC; ++c) tma_load_4d(sk + ks * F::TILE + c * F::BOX, &tm_k, kf, 64 * c, j * KT, hk * t.k.mul_h, b * t.k.mul_b);
-        if (++ks == F::NK) { ks = 0; kp ^= 1u; }
-        if (!mbar_wait(smem_u32(&hdr->v_empty[vs]), vp ^ 1u, abort_flag, t.status, 2, t.wait_limit)) break;
-        const uint32_t vf = smem_u32(&hdr->v_full[vs]);
-        mbar_expect_tx(vf, F::TILE);
-        for (int c = 0; c < DC; ++c) tma_load_4d(sv + vs * F::TILE + c * F::BOX, &tm_v, vf, 64 * c, j * KT, hk * t.v.mul_h, b * t.v.mul_b);
-        if (++vs == F::NV) { vs = 0; vp ^= 1u; }
-      }
-      if (*abort_flag)      // copies in flight get time to land before the block leaves its shared memory
-        for (int i = 0; i < 64; ++i) __nanosleep(1000);
-    }
-  } else if (warp == 4) {
-    // ------------------------------------------------------------ MMAs (all lanes loop, one issues: see elect_one)
+  if (warp == 4) {
+    // ------------------------------------------------------------ copies and MMAs (all lanes loop, one issues: see elect_one)
     const int dsteps = (a.D + 15) / 16;
     const uint32_t id_s = at_idesc(KT, false), id_o = at_idesc(dsteps * 16, true);
-    const uint32_t u_sq = warp_uniform(sq), u_sk = warp_uniform(sk), u_sv = warp_uniform(sv), u_tmem = warp_uniform(tmem);
-    uint32_t ks = 0, kp = 0, vs = 0, vp = 0;
-    bool ok = tiles == 0 || mbar_wait_warp(smem_u32(&hdr->q_full), 0, abort_flag, t.status, 3, t.wait_limit);
+    const uint32_t u_sq = warp_uniform(sq), u_sk = warp_uniform(sk), u_sv = warp_uniform(sv), u_tmem = warp_uniform(tmem), u_p = warp_uniform(tmem_p);
+    auto load_k = [&](int j) {
+      const uint32_t bar = smem_u32(&hdr->k_full[j % F::NK]);
+      mbar_expect_tx(bar, F::TILE);
+      for (int c = 0; c < DC; ++c) tma_load_4d(u_sk + j % F::NK * F::TILE + c * F::BOX, &tm_k, bar, 64 * c, (first + j) * KT, hk * t.k.mul_h, b * t.k.mul_b);
+    };
+    auto load_v = [&](int j) {
+      const uint32_t bar = smem_u32(&hdr->v_full[j % F::NV]);
+      mbar_expect_tx(bar, F::TILE);
+      for (int c = 0; c < DC; ++c) tma_load_4d(u_sv + j % F::NV * F::TILE + c * F::BOX, &tm_v, bar, 64 * c, (first + j) * KT, hk * t.v.mul_h, b * t.v.mul_b);
+    };
     auto scores = [&](int j) {
-      if (!mbar_wait_warp(smem_u32(&hdr->k_full[ks]), kp, abort_flag, t.status, 4, t.wait_limit)) return false;
-      if (j > 1 && !mbar_wait_warp(smem_u32(&hdr->o_full), j & 1, abort_flag, t.status, 5, t.wait_limit)) return false;      // P of tile j - 2, in the same columns, is read
+      if (!mbar_wait_warp(smem_u32(&hdr->k_full[j % F::NK]), j / F::NK & 1, abort_flag, t.status, 4, t.wait_limit)) return false;
+      if (j > 0 && !mbar_wait_warp(smem_u32(&hdr->s_free), (j - 1) & 1, abort_flag, t.status, 5, t.wait_limit)) return false;
       tc_fence_after();
       if (elect_one()) {
-        mma_rows(u_tmem + (j & 1) * KT, u_sq, F::QBOX, u_sk + ks * F::TILE, F::BOX, dsteps, id_s);
-        tc_commit(smem_u32(&hdr->k_empty[ks]));
-        tc_commit(smem_u32(&hdr->s_full[j & 1]));
+        mma_rows(u_tmem, u_sq, F::QBOX, u_sk + j % F::NK * F::TILE, F::BOX, dsteps, id_s);
+        tc_commit(smem_u32(&hdr->s_full));      // and with it the product of tile j - 2, which this thread issued before
+        if (j > 0 && j - 1 + F::NK < tiles) load_k(j - 1 + F::NK);      // the scores of tile j - 1 were read: its K is done with
       }
       __syncwarp();
-      if (++ks == F::NK) { ks = 0; kp ^= 1u; }
       return true;
     };
-    if (ok && tiles > 0) ok = scores(0);
-    if (ok && tiles > 1) ok = scores(1);
+    bool ok = true;
+    if (tiles > 0) {
+      if (!t.skip_loads && elect_one()) {
+        const uint32_t qf = smem_u32(&hdr->q_full);
+        mbar_expect_tx(qf, F::QTILE);
+        for (int c = 0; c < DC; ++c) tma_load_4d(u_sq + c * F::QBOX, &tm_q, qf, 64 * c, q0, h * t.q.mul_h, b * t.q.mul_b);
+        for (int j = 0; j < F::NK && j < tiles; ++j) { load_k(j); load_v(j); }
+      }
+      __syncwarp();
+      ok = mbar_wait_warp(smem_u32(&hdr->q_full), 0, abort_flag, t.status, 3, t.wait_limit) && scores(0);
+    }
     for (int j = 0; j < tiles && ok; ++j) {
-      ok = mbar_wait_warp(smem_u32(&hdr->v_full[vs]), vp, abort_flag, t.status, 6, t.wait_limit);
-      ok = ok && mbar_wait_warp(smem_u32(&hdr->p_full), j & 1, abort_flag, t.status, 7, t.wait_limit);
+      if (j + 1 < tiles) ok = scores(j + 1);
+      ok = ok && mbar_wait_warp(smem_u32(&hdr->v_full[j % F::NV]), j / F::NV & 1, abort_flag, t.status, 6, t.wait_limit);
+      ok = ok && mbar_wait_warp(smem_u32(&hdr->p_full[j & 1]), j >> 1 & 1, abort_flag, t.status, 7, t.wait_limit);
+      // (waited for in front of the next product: behind it this phase of the barrier could not be told from the one after the next)
+      const bool more_v = j > 0 && j - 1 + F::NV < tiles;
+      if (more_v) ok = ok && mbar_wait_warp(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 2, t.wait_limit);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        mma_mix(u_tmem + F::O_COL, u_tmem + (j & 1) * KT, u_sv + vs * F::TILE, F::BOX, KT / 16, id_o, j > 0);
-        tc_commit(smem_u32(&hdr->v_empty[vs]));
+        mma_mix(u_tmem + F::O_COL, u_p + (F::NP == 2 ? (j & 1) * (KT / 2) : 0), u_sv + j % F::NV * F::TILE, F::BOX, KT / 16, id_o, j > 0);
         tc_commit(smem_u32(&hdr->o_full));
+        if (j + 1 == tiles) tc_commit(smem_u32(&hdr->done));
+        if (more_v) load_v(j - 1 + F::NV);                 // the product before this one is done, and its V with it
       }
       __syncwarp();
-      if (++vs == F::NV) { vs = 0; vp ^= 1u; }
-      if (j + 2 < tiles) ok = scores(j + 2);
     }
-    if (*abort_flag && elect_one()) {      // no MMA may still be reading shared memory or writing tensor memory
-      tc_commit(smem_u32(&hdr->drain));
-      for (uint32_t it = 0; it < (1u << 20); ++it)
-        if (mbar_try_wait(smem_u32(&hdr->drain), 0)) break;
+    if (*abort_flag) {
+      if (elect_one()) {                   // no MMA may still be reading shared memory or writing tensor memory
+        tc_commit(smem_u32(&hdr->drain));
+        for (uint32_t it = 0; it < (1u << 20); ++it)
+          if (mbar_try_wait(smem_u32(&hdr->drain), 0)) break;
+      }
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);      // copies in flight get time to land before the block leaves its shared memory
     }
   } else {
     // ------------------------------------------------------------ softmax: thread = query
     const int row = q0 + threadIdx.x;
     const bool idle = q0 + warp * 32 >= a.Lq;          // no query in this warp
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16), lanes_p = tmem_p + ((uint32_t)(warp * 32) << 16);
     const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.Lk : nullptr;
     const float c = a.scale_log2;
     float m = -AT_INF;                 // the row's reference value, in units of S
-    float2 l = make_float2(0.f, 0.f);
+    float2 l[4] = {};                  // its sum, in eight parts: additions that do not wait for one another
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       uint32_t bits[KT / 32];
-      bool whole = true;
+      const int key0 = (first + j) * KT;
+      bool whole = !mask && key0 + KT <= end;
+      if (!whole) {
+        whole = true;
 #pragma unroll
-      for (int i = 0; i < KT / 32; ++i) { bits[i] = key_bits(a, mask, j * KT + 32 * i, end, lane); whole = whole && bits[i] == 0xffffffffu; }
-      ok = mbar_wait_warp(smem_u32(&hdr->s_full[j & 1]), j >> 1 & 1, abort_flag, t.status, 8, t.wait_limit);
-      if (!ok) break;
+        for (int i = 0; i < KT / 32; ++i) { bits[i] = key_bits(a, mask, key0 + 32 * i, end, lane); whole = whole && bits[i] == 0xffffffffu; }
+      }
+      ok = mbar_wait(smem_u32(&hdr->s_full), j & 1, abort_flag, t.status, 8, t.wait_limit);
+      __syncwarp();
       tc_fence_after();
-      bool move = false;
-      float f = 1.f;
+      float x[KT];
       if (!idle) {
-        const uint32_t at = lanes + (j & 1) * KT;
-        float x[KT];
 #pragma unroll
-        for (int i = 0; i < KT; i += 32) tc_ld32(at + i, reinterpret_cast<uint32_t*>(x) + i);
+        for (int i = 0; i < KT; i += 32) tc_ld32(lanes + i, reinterpret_cast<uint32_t*>(x) + i);
         tc_ld_wait();
         tc_loaded<KT>(reinterpret_cast<uint32_t*>(x));
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&hdr->s_free));
+      bool move = false;
+      float m_new = m;
+      if (!idle) {
         if (!whole) {
 #pragma unroll
           for (int i = 0; i < KT; ++i) x[i] = bits[i >> 5] >> (i & 31) & 1u ? x[i] : -AT_INF;
         }
-        float top[4] = {m, x[0], x[1], x[2]};
-        top[0] = fmaxf(top[0], x[3]);
+        float top[4] = {m, m, m, m};
 #pragma unroll
-        for (int i = 4; i < KT; i += 4) {
-          if (i & 4) { top[0] = max3(top[0], x[i], x[i + 1]); top[1] = max3(top[1], x[i + 2], x[i + 3]); }
-          else { top[2] = max3(top[2], x[i], x[i + 1]); top[3] = max3(top[3], x[i + 2], x[i + 3]); }
+        for (int i = 0; i < KT; i += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], x[i + 2 * e], x[i + 2 * e + 1]);
         }
-        const float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         move = (m_new - m) * c > 8.f;
-        if (move) { f = ex2((m - m_new) * c); m = m_new; l = mul2(l, make_float2(f, f)); }
+      }
+      // The place for P.  One: the product before this one has to be done, and every warp waits for it in every tile.  Two: this tile's scores say that the product before the last is
+      // done and that every warp has arrived for it; a warp can be ahead of another by a tile, never by the two that would let it arrive twice at the barriers, which come in pairs.
+      if (F::NP == 1 && j > 0) ok = ok && mbar_wait(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit);
+      if (__any_sync(0xffffffffu, move || !ok)) {
+        const float f = move ? ex2((m - m_new) * c) : 1.f;
+        if (move) m = m_new;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l[e] = mul2(l[e], make_float2(f, f));
+        if (F::NP == 2 && j > 0) ok = ok && mbar_wait(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (j > 0) {                    // the product with the previous P is done: O is this thread's
+          tc_fence_after();
+#pragma unroll 1
+          for (int o = 0; o < DC * 64; o += 16) {
+            uint32_t r[16];
+            tc_ld16(lanes + F::O_COL + o, r);
+            tc_ld_wait();
+            tc_loaded<16>(r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+            tc_st16(lanes + F::O_COL + o, r);
+          }
+        }
+      }
+      if (!idle) {
         const float mc = m == -AT_INF ? 0.f : m * c;      // no key yet: every exponent is -inf
 #pragma unroll
-        for (int i = 0; i < KT; i += 2) {
-          const float2 e = fma2(make_float2(x[i], x[i + 1]), make_float2(c, c), make_float2(-mc, -mc));
-          const float2 p = make_float2(ex2(e.x), ex2(e.y));
-          l = add2(l, p);
-          x[i >> 1] = __uint_as_float(pack_bf16(p.x, p.y));
-        }
-        tc_st32(at, reinterpret_cast<uint32_t*>(x));       // over S, which is in registers
-      }
-      if (j > 0) {
-        // The product with the previous P is done: O is this thread's.  Every warp waits here in every tile: one that ran ahead would meet barriers a phase behind
-        // the one that it means, which look the same as those a phase ahead.
-        ok = mbar_wait_warp(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit);
-        if (!ok) break;
-        if (__any_sync(0xffffffffu, move)) {
-          tc_fence_after();
+        for (int p = 0; p < KT; p += 32) {
+          uint32_t w[16];
 #pragma unroll
-          for (int o = 0; o < DC * 64; o += 32) {
-            uint32_t r[32];
-            tc_ld32(lanes + F::O_COL + o, r);
-            tc_ld_wait();
-            tc_loaded<32>(r);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-            tc_st32(lanes + F::O_COL + o, r);
+          for (int i = p; i < p + 32; i += 2) {
+            const float2 e = fma2(make_float2(x[i], x[i + 1]), make_float2(c, c), make_float2(-mc, -mc));
+            const float2 y = make_float2(ex2(e.x), ex2(e.y));
+            l[i / 2 % 4] = add2(l[i / 2 % 4], y);
+            w[(i - p) >> 1] = pack_bf16(y.x, y.y);
           }
+          tc_st16(lanes_p + (F::NP == 2 ? (j & 1) * (KT / 2) : 0) + p / 2, w);
         }
       }
       if (!whole) {                     // rows of V that must not be read: a zero weight times what they hold need not be zero
@@ -229,16 +252,19 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       tc_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&hdr->p_full));
+      if (lane == 0) mbar_arrive(smem_u32(&hdr->p_full[j & 1]));
     }
-    if (ok && tiles > 0) ok = mbar_wait_warp(smem_u32(&hdr->o_full), (tiles - 1) & 1, abort_flag, t.status, 11, t.wait_limit);
+    if (ok && tiles > 0) ok = mbar_wait_warp(smem_u32(&hdr->done), 0, abort_flag, t.status, 11, t.wait_limit);
     if (ok && !idle) {
       tc_fence_after();
       const bool none = m == -AT_INF;
-      const float sum = l.x + l.y, inv = none ? 0.f : 1.f / sum;
+      const float2 l2 = add2(add2(l[0], l[1]), add2(l[2], l[3]));
+      const float sum = l2.x + l2.y, inv = none ? 0.f : 1.f / sum;
       // `none` also holds for a row of scores that are all not a number; its sum is not a number then, and so is its result
       const bool zero = none && !(sum != sum);
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (((int64_t)b * a.Lq + row) * a.H + h) * a.D;
+      const int64_t at = ((int64_t)b * a.Lq + row) * a.H + h, rows = (int64_t)a.B * a.Lq * a.H;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + at * a.D;
+      float* part = t.part_o + (split * rows + at) * a.D;
 #pragma unroll
       for (int o = 0; o < DC * 64; o += 32) {
         uint32_t r[32];
@@ -247,6 +273,16 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             if (o + 8 * g < a.D) {
+              if (t.splits > 1) {            // a part of the keys: float32, for the join
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  float u[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) u[e] = zero ? 0.f : none ? sum : __uint_as_float(r[8 * g + 4 * i + e]) * inv;
+                  *reinterpret_cast<float4*>(part + o + 8 * g + 4 * i) = make_float4(u[0], u[1], u[2], u[3]);
+                }
+                continue;
+              }
               uint32_t w[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -259,13 +295,52 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         __syncwarp();
       }
-      if (a.lse && row < a.Lq) a.lse[((int64_t)b * a.H + h) * a.Lq + row] = zero ? AT_INF : m * c + log2f(sum);
+      const float lse = zero ? AT_INF : m * c + log2f(sum);
+      if (row < a.Lq) {
+        if (t.splits > 1) t.part_lse[split * rows + at] = lse;
+        else if (a.lse) a.lse[((int64_t)b * a.H + h) * a.Lq + row] = lse;
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+  if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F::COLS) : "memory");
+  if (warp == 4 && F::P_COLS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_p), "r"(32u) : "memory");
+}
+
+// The parts of a row over the splits of its keys, weighted with the parts' sums, added in their order.  A thread for four channels.
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnTcArgs t) {
+  const AttnArgs& a = t.a;
+  const int per = a.D / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.B * a.Lq * a.H, row = i / per;
+  if (row >= rows) return;
+  const int d = (int)(i - row * per) * 4;
+  float top = -AT_INF;                    // a part without a key has +inf in place of its logarithm
+  for (int s = 0; s < t.splits; ++s) {
+    const float v = __ldg(t.part_lse + s * rows + row);
+    top = v == AT_INF ? top : v != v ? v : fmaxf(top, v);
+  }
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int s = 0; s < t.splits; ++s) {
+    const float v = __ldg(t.part_lse + s * rows + row);
+    if (v == AT_INF) continue;
+    const float w = exp2f(v - top);
+    const float4 p = __ldg(reinterpret_cast<const float4*>(t.part_o + (s * rows + row) * a.D + d));
+    o.x = fmaf(w, p.x, o.x); o.y = fmaf(w, p.y, o.y); o.z = fmaf(w, p.z, o.z); o.w = fmaf(w, p.w, o.w);
+    sum += w;
+  }
+  const bool none = top == -AT_INF;
+  const float inv = none ? 0.f : 1.f / sum;
+  uint2 w;
+  w.x = pack_bf16(o.x * inv, o.y * inv); w.y = pack_bf16(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + row * a.D + d) = w;
+  if (a.lse && d == 0) {
+    const int h = (int)(row % a.H);
+    const int64_t bl = row / a.H, b = bl / a.Lq;
+    a.lse[(b * a.H + h) * a.Lq + (bl - b * a.Lq)] = none ? AT_INF : top + log2f(sum);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
@@ -274,11 +349,28 @@ bool rows_ok(const void* p, int64_t sb, int64_t sl, int64_t sh, int B, int L, in
          sl < (int64_t)1 << 38 && sh < (int64_t)1 << 38 && sb < (int64_t)1 << 38;
 }
 
+// Into how many parts the keys of a row tile are cut, so that the blocks fill the SMs: the number for which the rounds of blocks, each as long as its tiles and about six more for a block's
+// beginning and end, are shortest.  More than one part also costs the join, a launch and a pass over the parts: about eight tiles.
+int splits_of(int B, int Lq, int Lk, int H, int D) {
+  const int64_t blocks = (int64_t)((Lq + AT_M - 1) / AT_M) * H * B, slots = (int64_t)fovi::sm_count() * (D <= 64 ? Fwd<1>::CTAS : Fwd<2>::CTAS);
+  const int tiles = (Lk + KT - 1) / KT;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= 32 && s <= tiles; ++s) {
+    const int64_t time = (blocks * s + slots - 1) / slots * ((tiles + s - 1) / s + 6) + (s > 1 ? 8 : 0);
+    if (time < least) { least = time; best = s; }
+  }
+  return best;
+}
+
 template <int DC>
-int forward(const AttnArgs& a, cudaStream_t st, bool selftest) {
+int forward(const AttnArgs& a, void* work, cudaStream_t st, bool selftest) {
   using F = Fwd<DC>;
   CUtensorMap tq, tk, tv;
   AttnTcArgs t = {};
+  t.splits = work ? splits_of(a.B, a.Lq, a.Lk, a.H, a.D) : 1;
+  t.part_o = static_cast<float*>(work);
+  t.part_lse = t.part_o + (int64_t)t.splits * a.B * a.Lq * a.H * a.D;
   t.a = a;
   t.wait_limit = selftest ? 4096u : WAIT_LIMIT;
   t.skip_loads = selftest;
@@ -287,11 +379,14 @@ int forward(const AttnArgs& a, cudaStream_t st, bool selftest) {
   if (!rc) rc = fovi::encode_rows(&tk, &t.k, a.k, a.k_sb, a.k_sl, a.k_sh, a.B, a.Lk, a.Hkv, a.D, KT);
   if (!rc) rc = fovi::encode_rows(&tv, &t.v, a.v, a.v_sb, a.v_sl, a.v_sh, a.B, a.Lk, a.Hkv, a.D, KT);
   if (rc) return rc;
-  const int64_t blocks = (int64_t)((a.Lq + AT_M - 1) / AT_M) * a.H * a.B;
-  if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;
+  const int64_t blocks = (int64_t)((a.Lq + AT_M - 1) / AT_M) * a.H * a.B * t.splits, join = ((int64_t)a.B * a.Lq * a.H * (a.D / 4) + 255) / 256;
+  if (blocks > INT_MAX || join > INT_MAX) return FOVI_ERR_UNSUPPORTED;
   FOVI_CUDA(cudaFuncSetAttribute(attn_tc_forward_kernel<DC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::SMEM));
   FOVI_CUDA(fovi::launch_pdl(attn_tc_forward_kernel<DC>, (int)blocks, AT_THREADS, F::SMEM, st, tq, tk, tv, t));
-  return fovi::after_launch("attn_tc_forward_kernel");
+  rc = fovi::after_launch("attn_tc_forward_kernel");
+  if (rc || t.splits == 1) return rc;
+  attn_join_kernel<<<(int)join, 256, 0, st>>>(t);
+  return fovi::after_launch("attn_join_kernel");
 }
 
 }  // namespace
@@ -314,8 +409,13 @@ bool fovi::attention_tc_takes(const AttnArgs& a, int dtype, bool backward) {
                    : !(reinterpret_cast<uintptr_t>(a.out) & 15u));
 }
 
-int fovi::launch_attention_tc_forward(const AttnArgs& a, cudaStream_t st, bool selftest) {
-  return a.D <= 64 ? forward<1>(a, st, selftest) : forward<2>(a, st, selftest);
+int64_t fovi::attention_tc_forward_bytes(int B, int Lq, int Lk, int H, int D) {
+  const int s = splits_of(B, Lq, Lk, H, D);
+  return s == 1 ? 0 : (int64_t)s * B * Lq * H * (D + 1) * 4;
+}
+
+int fovi::launch_attention_tc_forward(const AttnArgs& a, void* work, cudaStream_t st, bool selftest) {
+  return a.D <= 64 ? forward<1>(a, work, st, selftest) : forward<2>(a, work, st, selftest);
 }
 
 int fovi::attention_tc_status(int** word) {

@@ -9,13 +9,16 @@ struct TcView { int mul_h, mul_b; };
 struct AttnTcArgs {
   AttnArgs a;
   TcView q, k, v, g;
+  int splits;              // forward: parts of a row tile's keys, and what each found
+  float *part_o, *part_lse;
   int* status;             // wait site at which a kernel gave up
   uint32_t wait_limit;
   int skip_loads;          // self-test: the loads are withheld, so the first wait must give up
 };
 
 bool attention_tc_takes(const AttnArgs& a, int dtype, bool backward);
-int launch_attention_tc_forward(const AttnArgs& a, cudaStream_t st, bool selftest);
+int64_t attention_tc_forward_bytes(int B, int Lq, int Lk, int H, int D);
+int launch_attention_tc_forward(const AttnArgs& a, void* work, cudaStream_t st, bool selftest);      // work null: no splits
 int64_t attention_tc_backward_bytes(int B, int Lq, int H);
 int launch_attention_tc_backward(const AttnArgs& a, void* work, cudaStream_t st, bool selftest);
 int attention_tc_check(cudaStream_t st);
