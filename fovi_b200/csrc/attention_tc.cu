@@ -98,11 +98,11 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       for (int c = 0; c < DC; ++c) tma_load_4d(u_sv + j % F::NV * F::TILE + c * F::BOX, &tm_v, bar, 64 * c, (first + j) * KT, hk * t.v.mul_h, b * t.v.mul_b);
     };
     auto scores = [&](int j) {
-      if (!mbar_wait_warp(smem_u32(&hdr->k_full[j % F::NK]), j / F::NK & 1, abort_flag, t.status, 4, t.wait_limit)) return false;
-      if (j > 0 && !mbar_wait_warp(smem_u32(&hdr->s_free), (j - 1) & 1, abort_flag, t.status, 5, t.wait_limit)) return false;
+      if (!at_wait(smem_u32(&hdr->k_full[j % F::NK]), j / F::NK & 1, abort_flag, t.status, 4, t.wait_limit)) return false;
+      if (j > 0 && !at_wait(smem_u32(&hdr->s_free), (j - 1) & 1, abort_flag, t.status, 5, t.wait_limit)) return false;
       tc_fence_after();
+      mma_rows<DC>(u_tmem, u_sq, F::QBOX, u_sk + warp_uniform(j % F::NK) * F::TILE, F::BOX, id_s);
       if (elect_one()) {
-        mma_rows(u_tmem, u_sq, F::QBOX, u_sk + j % F::NK * F::TILE, F::BOX, dsteps, id_s);
         tc_commit(smem_u32(&hdr->s_full));      // and with it the product of tile j - 2, which this thread issued before
         if (j > 0 && j - 1 + F::NK < tiles) load_k(j - 1 + F::NK);      // the scores of tile j - 1 were read: its K is done with
       }
@@ -118,19 +118,19 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         for (int j = 0; j < F::NK && j < tiles; ++j) { load_k(j); load_v(j); }
       }
       __syncwarp();
-      ok = mbar_wait_warp(smem_u32(&hdr->q_full), 0, abort_flag, t.status, 3, t.wait_limit) && scores(0);
+      ok = at_wait(smem_u32(&hdr->q_full), 0, abort_flag, t.status, 3, t.wait_limit) && scores(0);
     }
     for (int j = 0; j < tiles && ok; ++j) {
       if (j + 1 < tiles) ok = scores(j + 1);
-      ok = ok && mbar_wait_warp(smem_u32(&hdr->v_full[j % F::NV]), j / F::NV & 1, abort_flag, t.status, 6, t.wait_limit);
-      ok = ok && mbar_wait_warp(smem_u32(&hdr->p_full[j & 1]), j >> 1 & 1, abort_flag, t.status, 7, t.wait_limit);
+      ok = ok && at_wait(smem_u32(&hdr->v_full[j % F::NV]), j / F::NV & 1, abort_flag, t.status, 6, t.wait_limit);
+      ok = ok && at_wait(smem_u32(&hdr->p_full[j & 1]), j >> 1 & 1, abort_flag, t.status, 7, t.wait_limit);
       // (waited for in front of the next product: behind it this phase of the barrier could not be told from the one after the next)
       const bool more_v = j > 0 && j - 1 + F::NV < tiles;
-      if (more_v) ok = ok && mbar_wait_warp(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 2, t.wait_limit);
+      if (more_v) ok = ok && at_wait(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 2, t.wait_limit);
       if (!ok) break;
       tc_fence_after();
+      mma_mix(u_tmem + F::O_COL, u_p + (F::NP == 2 ? (j & 1) * (KT / 2) : 0), u_sv + warp_uniform(j % F::NV) * F::TILE, F::BOX, KT / 16, id_o, j > 0);
       if (elect_one()) {
-        mma_mix(u_tmem + F::O_COL, u_p + (F::NP == 2 ? (j & 1) * (KT / 2) : 0), u_sv + j % F::NV * F::TILE, F::BOX, KT / 16, id_o, j > 0);
         tc_commit(smem_u32(&hdr->o_full));
         if (j + 1 == tiles) tc_commit(smem_u32(&hdr->done));
         if (more_v) load_v(j - 1 + F::NV);                 // the product before this one is done, and its V with it
@@ -164,8 +164,8 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll
         for (int i = 0; i < KT / 32; ++i) { bits[i] = key_bits(a, mask, key0 + 32 * i, end, lane); whole = whole && bits[i] == 0xffffffffu; }
       }
-      ok = mbar_wait(smem_u32(&hdr->s_full), j & 1, abort_flag, t.status, 8, t.wait_limit);
-      __syncwarp();
+      ok = at_wait(smem_u32(&hdr->s_full), j & 1, abort_flag, t.status, 8, t.wait_limit);
+      if (!ok) break;
       tc_fence_after();
       float x[KT];
       if (!idle) {
@@ -195,15 +195,13 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       // The place for P.  One: the product before this one has to be done, and every warp waits for it in every tile.  Two: this tile's scores say that the product before the last is
       // done and that every warp has arrived for it; a warp can be ahead of another by a tile, never by the two that would let it arrive twice at the barriers, which come in pairs.
-      if (F::NP == 1 && j > 0) ok = ok && mbar_wait(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit);
-      if (__any_sync(0xffffffffu, move || !ok)) {
+      if (F::NP == 1 && j > 0 && !at_wait(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit)) { ok = false; break; }
+      if (__any_sync(0xffffffffu, move)) {
         const float f = move ? ex2((m - m_new) * c) : 1.f;
         if (move) m = m_new;
 #pragma unroll
         for (int e = 0; e < 4; ++e) l[e] = mul2(l[e], make_float2(f, f));
-        if (F::NP == 2 && j > 0) ok = ok && mbar_wait(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (F::NP == 2 && j > 0 && !at_wait(smem_u32(&hdr->o_full), (j - 1) & 1, abort_flag, t.status, 9, t.wait_limit)) { ok = false; break; }
         if (j > 0) {                    // the product with the previous P is done: O is this thread's
           tc_fence_after();
 #pragma unroll 1
@@ -234,7 +232,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
       if (!whole) {                     // rows of V that must not be read: a zero weight times what they hold need not be zero
-        ok = mbar_wait_warp(smem_u32(&hdr->v_full[j % F::NV]), (j / F::NV) & 1, abort_flag, t.status, 10, t.wait_limit);
+        ok = at_wait(smem_u32(&hdr->v_full[j % F::NV]), (j / F::NV) & 1, abort_flag, t.status, 10, t.wait_limit);
         if (!ok) break;
         if (threadIdx.x < KT) {
           const int r = threadIdx.x;
@@ -254,7 +252,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&hdr->p_full[j & 1]));
     }
-    if (ok && tiles > 0) ok = mbar_wait_warp(smem_u32(&hdr->done), 0, abort_flag, t.status, 11, t.wait_limit);
+    if (ok && tiles > 0) ok = at_wait(smem_u32(&hdr->done), 0, abort_flag, t.status, 11, t.wait_limit);
     if (ok && !idle) {
       tc_fence_after();
       const bool none = m == -AT_INF;

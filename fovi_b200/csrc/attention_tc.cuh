@@ -37,6 +37,17 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
 }
 
+// The other way; what lies outside the tensor is left out.
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+               ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+// Ends the group of this thread's stores and waits until they have read shared memory.
+__device__ __forceinline__ void bulk_commit_and_read() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
 // A from tensor memory (bf16, two per column), B from shared memory.
 __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -109,16 +120,39 @@ __device__ __forceinline__ constexpr uint32_t at_idesc(int n, bool b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(AT_M >> 4) << 24);
 }
 
-// D[128, N] (+)= A[128 rows, channels] B[N rows, channels]^T: both tiles K-major, `steps` slices of 16 channels in boxes of 64 that are a_box, b_box bytes apart.
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a_smem, uint32_t a_box, uint32_t b_smem, uint32_t b_box, int steps, uint32_t idesc) {
-  const uint64_t desc = smem_desc(0, 16u, 1024u, 2u);
-  for (int k = 0; k < steps; ++k)
-    tc_mma_bf16(d, desc + ((a_smem + (k >> 2) * a_box) >> 4) + (k & 3) * 2, desc + ((b_smem + (k >> 2) * b_box) >> 4) + (k & 3) * 2, idesc, k ? 1u : 0u);
+// Bounded wait of a converged warp (see mbar_wait).  All lanes ask and leave together: a barrier that is done costs about 90 clocks, where lanes that leave a loop one by one cost 240,
+// and these kernels pass four to six such barriers a tile.
+__device__ __forceinline__ bool at_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code, uint32_t limit) {
+  for (uint32_t it = 0; it < limit; ++it) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((it & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag)) return false;
+  }
+  *abort_flag = 1;
+  atomicCAS(status, 0, code);
+  return false;
 }
-// D[128, channels] (+)= A[128, rows] B[rows, channels]: A in tensor memory, B the same kind of tile read MN-major, `steps` slices of 16 rows.
+
+// The products, issued by one lane of a warp that is together.  Operands' descriptors are made by the whole warp and the loops have a fixed number of turns, so that they stay in uniform
+// registers, where the instruction takes them from: from a loop of one thread an MMA of N = 64 took 75 clocks to issue instead of 32 to 48.
+// D[128, N] = A[128 rows, channels] B[N rows, channels]^T: both tiles K-major, in boxes of 64 channels that are a_box, b_box bytes apart; then `done` is told.
+template <int DC> __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a_smem, uint32_t a_box, uint32_t b_smem, uint32_t b_box, uint32_t idesc) {
+  const uint64_t desc = smem_desc(0, 16u, 1024u, 2u), da = desc + (a_smem >> 4), db = desc + (b_smem >> 4);
+  if (elect_one()) {
+#pragma unroll
+    for (int k = 0; k < 4 * DC; ++k)
+      tc_mma_bf16(d, da + (k >> 2) * (a_box >> 4) + (k & 3) * 2, db + (k >> 2) * (b_box >> 4) + (k & 3) * 2, idesc, k ? 1u : 0u);
+  }
+  __syncwarp();
+}
+// D[128, channels] (+)= A[128, 64 rows] B[64 rows, channels]: A in tensor memory, B the same kind of tile read MN-major; of its four slices of 16 rows the first `steps`.
 __device__ __forceinline__ void mma_mix(uint32_t d, uint32_t a_tmem, uint32_t b_smem, uint32_t b_box, int steps, uint32_t idesc, bool accumulate) {
   const uint64_t desc = smem_desc(0, b_box, 1024u, 2u) + (b_smem >> 4);
-  for (int k = 0; k < steps; ++k) tc_mma_bf16_ts(d, a_tmem + k * 8, desc + k * 128, idesc, accumulate || k ? 1u : 0u);
+  if (elect_one()) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < steps) tc_mma_bf16_ts(d, a_tmem + k * 8, desc + k * 128, idesc, accumulate || k ? 1u : 0u);
+  }
+  __syncwarp();
 }
 
 // Bits of the 32 keys from `key`: which may be read.  `all` when there is no mask: only the sample's end counts.

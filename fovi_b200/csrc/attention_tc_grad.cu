@@ -7,8 +7,11 @@
 //   P, dS                              eight warps, a thread per row and half the columns: registers, then back to tensor memory as bf16
 //   acc1 += dS C1 (dq, dk),  acc2 += P C2 (dv)          TS MMAs, the column tiles read MN-major: nothing is transposed, nothing goes through shared memory
 // Each gradient is summed by one CTA in a fixed order: no atomics, the same bits every time, no float32 buffer of dq, for 7 products instead of 5.
-// One CTA per SM with all 512 columns of tensor memory, over many row tiles (persistent): the next tile's S and dP are computed while this one's elements are worked on,
-// and the next row tile's operands arrive meanwhile.  A last tile of fewer columns costs only its own (N and the steps over its columns follow).
+// One CTA per SM with all 512 columns of tensor memory, over many row tiles (persistent).  Beside the eight warps one issues the scores, one the products, one the copies in and one the
+// copies out: a single MMA warp spent 2000 clocks a tile on its barriers and on issuing, one after the other, where the tensor cores have 800 to 1100 of work.  The next tile's scores are
+// computed while this one's elements are worked on, and the next row tile's operands arrive meanwhile.  Results go through the row tile's own operand buffers, which the scores are done
+// with, and out as tensor copies: stored from registers, 16 bytes of a row per thread, they took half the time of dk and dv (716 us with, 400 without them, 4 x 111 heads, 256 over 4096).
+// A last tile of fewer columns costs only its own (N and the steps over its columns follow).
 // Rows of K whose key is masked are set to zero in shared memory in front of dS K; for dk and dv a masked key is a row, whose results are zeros by a select.
 #include <cuda_bf16.h>
 
@@ -20,7 +23,8 @@ using fovi::key_end;
 
 namespace {
 
-constexpr int EW_WARPS = 8, GR_THREADS = (EW_WARPS + 2) * 32;
+constexpr int EW_WARPS = 8, GR_THREADS = (EW_WARPS + 4) * 32;        // then the warps of the scores, the products, the copies in, the copies out
+constexpr int SCORES = EW_WARPS, PRODUCTS = EW_WARPS + 1, LOADS = EW_WARPS + 2, STORES = EW_WARPS + 3;
 constexpr float AT_INF = __builtin_huge_valf();
 
 template <int DC> struct Grad {
@@ -33,7 +37,7 @@ template <int DC> struct Grad {
 };
 
 struct GradHeader {
-  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_free, drain;
+  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_full, acc_free, staged, drain;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -91,7 +95,7 @@ __device__ __forceinline__ int columns(const AttnArgs& a, const Item& it, int j,
 template <int DC, bool KEYS>
 __global__ void __launch_bounds__(GR_THREADS, 1)
 attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                    const __grid_constant__ CUtensorMap tm_g, const GradArgs g) {
+                    const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_1, const __grid_constant__ CUtensorMap tm_2, const GradArgs g) {
   using G = Grad<DC>;
   constexpr int CT = G::CT, HALF = G::HALF;
   const AttnTcArgs& t = g.t;
@@ -109,11 +113,12 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->row_full[i]), 1); mbar_init(smem_u32(&hdr->row_empty[i]), 1); }
     for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&hdr->full[i]), 1); mbar_init(smem_u32(&hdr->empty[i]), 1); }
     mbar_init(smem_u32(&hdr->s_full), 1); mbar_init(smem_u32(&hdr->s_free), EW_WARPS); mbar_init(smem_u32(&hdr->p_full), EW_WARPS);
-    mbar_init(smem_u32(&hdr->mixed), 1); mbar_init(smem_u32(&hdr->acc_free), EW_WARPS); mbar_init(smem_u32(&hdr->drain), 1);
+    mbar_init(smem_u32(&hdr->mixed), 1); mbar_init(smem_u32(&hdr->acc_full), 1); mbar_init(smem_u32(&hdr->acc_free), EW_WARPS);
+    mbar_init(smem_u32(&hdr->staged), EW_WARPS); mbar_init(smem_u32(&hdr->drain), 1);
     hdr->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == EW_WARPS) {
+  if (warp == SCORES) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hdr->tmem_base)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -124,8 +129,8 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   tc_fence_after();
   const uint32_t tmem = hdr->tmem_base;
 
-  if (warp == EW_WARPS + 1) {
-    // ------------------------------------------------------------ copies
+  if (warp == LOADS) {
+    // ------------------------------------------------------------ copies in
     if (lane == 0 && !t.skip_loads) {
       uint32_t s = 0, sp = 0;
       for (Walk<DC, KEYS> w(g); w.more(g); w.next(g)) {
@@ -167,67 +172,84 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       if (*abort_flag)      // copies in flight get time to land before the block leaves its shared memory
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
-  } else if (warp == EW_WARPS) {
-    // ------------------------------------------------------------ MMAs (all lanes loop, one issues: see elect_one)
-    const int dsteps = (a.D + 15) / 16;
-    const uint32_t id_acc = at_idesc(dsteps * 16, true);
+  } else if (warp == SCORES) {
+    // ------------------------------------------------------------ S and dP (the MMA warps loop with all lanes, one issues: see elect_one)
     const uint32_t u_srow = warp_uniform(srow), u_scol = warp_uniform(scol), u_tmem = warp_uniform(tmem);
-    uint32_t s = 0, sp = 0, n_s = 0, n_m = 0, ms = 0;
-    Walk<DC, KEYS> w(g), m(g);
-    bool ok = true;
-    auto scores = [&]() {
+    uint32_t s = 0, sp = 0, n = 0;
+    for (Walk<DC, KEYS> w(g); w.more(g); w.next(g), ++n) {
       const uint32_t f = w.seq & 1;
-      if (w.j == 0 && !mbar_wait_warp(smem_u32(&hdr->row_full[f]), w.seq >> 1 & 1, abort_flag, status, 23, t.wait_limit)) return false;
-      if (!mbar_wait_warp(smem_u32(&hdr->full[s]), sp, abort_flag, status, 24, t.wait_limit)) return false;
-      if (n_s > 0 && !mbar_wait_warp(smem_u32(&hdr->s_free), (n_s - 1) & 1, abort_flag, status, 25, t.wait_limit)) return false;
+      if (w.j == 0 && !at_wait(smem_u32(&hdr->row_full[f]), w.seq >> 1 & 1, abort_flag, status, 23, t.wait_limit)) break;
+      if (!at_wait(smem_u32(&hdr->full[s]), sp, abort_flag, status, 24, t.wait_limit)) break;
+      if (n > 0 && !at_wait(smem_u32(&hdr->s_free), (n - 1) & 1, abort_flag, status, 25, t.wait_limit)) break;
       tc_fence_after();
       int c0, h;
-      const int n = warp_uniform((columns<DC, KEYS>(a, w.it, w.j, c0, h) + 15) / 16 * 16);
-      const bool last = w.j + 1 == w.it.n;
-      if (elect_one()) {
-        const uint32_t rows = u_srow + f * 2 * G::RTILE, cols = u_scol + s * 2 * G::CTILE, id = at_idesc(0, false) | ((uint32_t)(n >> 3) << 17);
-        mma_rows(u_tmem, rows, G::RBOX, cols, G::CBOX, dsteps, id);
-        mma_rows(u_tmem + G::DP, rows + G::RTILE, G::RBOX, cols + G::CTILE, G::CBOX, dsteps, id);
-        tc_commit(smem_u32(&hdr->s_full));
-        if (last) tc_commit(smem_u32(&hdr->row_empty[f]));
-      }
+      const int cols = warp_uniform((columns<DC, KEYS>(a, w.it, w.j, c0, h) + 15) / 16 * 16);
+      const uint32_t rows = warp_uniform(u_srow + f * 2 * G::RTILE), tile = warp_uniform(u_scol + s * 2 * G::CTILE), id = at_idesc(0, false) | ((uint32_t)(cols >> 3) << 17);
+      mma_rows<DC>(u_tmem, rows, G::RBOX, tile, G::CBOX, id);
+      mma_rows<DC>(u_tmem + G::DP, rows + G::RTILE, G::RBOX, tile + G::CTILE, G::CBOX, id);
+      if (elect_one()) tc_commit(smem_u32(&hdr->s_full));
       __syncwarp();
       if (++s == G::NS) { s = 0; sp ^= 1u; }
-      ++n_s;
-      w.next(g);
-      return true;
-    };
-    if (w.more(g)) ok = scores();
-    for (; ok && m.more(g); m.next(g)) {
-      if (w.more(g)) ok = scores();
-      ok = ok && mbar_wait_warp(smem_u32(&hdr->p_full), n_m & 1, abort_flag, status, 26, t.wait_limit);
-      if (ok && m.j == 0 && m.seq > 0) ok = mbar_wait_warp(smem_u32(&hdr->acc_free), (m.seq - 1) & 1, abort_flag, status, 27, t.wait_limit);
-      if (!ok) break;
-      tc_fence_after();
-      int c0, h;
-      const int steps = warp_uniform((columns<DC, KEYS>(a, m.it, m.j, c0, h) + 15) / 16);
-      if (elect_one()) {
-        const uint32_t cols = u_scol + ms * 2 * G::CTILE;
-        if (KEYS) mma_mix(u_tmem + G::ACC2, u_tmem + G::P, cols + G::CTILE, G::CBOX, steps, id_acc, m.j > 0);
-        mma_mix(u_tmem + G::ACC1, u_tmem + G::DS, cols, G::CBOX, steps, id_acc, m.j > 0);
-        tc_commit(smem_u32(&hdr->empty[ms]));
-        tc_commit(smem_u32(&hdr->mixed));
-      }
-      __syncwarp();
-      if (++ms == G::NS) ms = 0;
-      ++n_m;
     }
     if (*abort_flag && elect_one()) {      // no MMA may still be reading shared memory or writing tensor memory
       tc_commit(smem_u32(&hdr->drain));
       for (uint32_t it = 0; it < (1u << 20); ++it)
         if (mbar_try_wait(smem_u32(&hdr->drain), 0)) break;
     }
+  } else if (warp == PRODUCTS) {
+    // ------------------------------------------------------------ the accumulators
+    const uint32_t id_acc = at_idesc((a.D + 15) / 16 * 16, true);
+    const uint32_t u_scol = warp_uniform(scol), u_tmem = warp_uniform(tmem);
+    uint32_t s = 0, sp = 0, n = 0;
+    for (Walk<DC, KEYS> w(g); w.more(g); w.next(g), ++n) {
+      if (!at_wait(smem_u32(&hdr->full[s]), sp, abort_flag, status, 26, t.wait_limit)) break;
+      if (w.j == 0 && w.seq > 0 && !at_wait(smem_u32(&hdr->acc_free), (w.seq - 1) & 1, abort_flag, status, 27, t.wait_limit)) break;
+      if (!at_wait(smem_u32(&hdr->p_full), n & 1, abort_flag, status, 32, t.wait_limit)) break;
+      tc_fence_after();
+      int c0, h;
+      const int steps = warp_uniform((columns<DC, KEYS>(a, w.it, w.j, c0, h) + 15) / 16);
+      const uint32_t tile = warp_uniform(u_scol + s * 2 * G::CTILE);
+      const bool more = warp_uniform(w.j) > 0;
+#pragma unroll
+      for (int q = 0; q < CT / 64; ++q) {         // 64 columns at a time
+        if (KEYS) mma_mix(u_tmem + G::ACC2, u_tmem + G::P + q * 32, tile + G::CTILE + q * 8192, G::CBOX, steps - 4 * q, id_acc, more || q);
+        mma_mix(u_tmem + G::ACC1, u_tmem + G::DS + q * 32, tile + q * 8192, G::CBOX, steps - 4 * q, id_acc, more || q);
+      }
+      if (elect_one()) {
+        tc_commit(smem_u32(&hdr->empty[s]));
+        tc_commit(smem_u32(&hdr->mixed));
+        if (w.j + 1 == w.it.n) tc_commit(smem_u32(&hdr->acc_full));
+      }
+      __syncwarp();
+      if (++s == G::NS) { s = 0; sp ^= 1u; }
+    }
+    if (*abort_flag && elect_one()) {
+      tc_commit(smem_u32(&hdr->drain));
+      for (uint32_t it = 0; it < (1u << 20); ++it)
+        if (mbar_try_wait(smem_u32(&hdr->drain), 0)) break;
+    }
+  } else if (warp == STORES) {
+    // ------------------------------------------------------------ copies out
+    for (Walk<DC, KEYS> w(g); w.more(g); w.next(g)) {
+      if (w.j) continue;
+      const uint32_t f = w.seq & 1, from = srow + f * 2 * G::RTILE;
+      if (!at_wait(smem_u32(&hdr->staged), w.seq & 1, abort_flag, status, 33, t.wait_limit)) break;
+      if (elect_one()) {
+        for (int c = 0; c < DC; ++c) {
+          tma_store_4d(&tm_1, from + c * G::RBOX, 64 * c, w.it.row0, w.it.h, w.it.b);
+          if (KEYS) tma_store_4d(&tm_2, from + G::RTILE + c * G::RBOX, 64 * c, w.it.row0, w.it.h, w.it.b);
+        }
+        bulk_commit_and_read();                // the buffers may be filled again
+        mbar_arrive(smem_u32(&hdr->row_empty[f]));
+      }
+      __syncwarp();
+    }
   } else {
     // ------------------------------------------------------------ elements: thread = row, half the columns
     const int r = (warp & 3) * 32 + lane, half = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c = a.scale_log2;
-    uint32_t n = 0, slot = 0, sphase = 0;
+    uint32_t n = 0, slot = 0, sphase = 0, seq = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
       const Item it = item_at<DC, KEYS>(g, i);
@@ -247,13 +269,14 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int cols = columns<DC, KEYS>(a, it, j, c0, h);
         const int first = half * HALF;
         uint32_t bits[HALF / 32];
-        bool whole = true;
-        if (!KEYS) {
+        bool whole = KEYS || (!mask && cols == CT);
+        if (!whole) {
+          whole = true;
 #pragma unroll
           for (int e = 0; e < HALF / 32; ++e) { bits[e] = key_bits(a, mask, c0 + first + 32 * e, it.end, lane); whole = whole && bits[e] == 0xffffffffu; }
         }
-        ok = mbar_wait_warp(smem_u32(&hdr->s_full), n & 1, abort_flag, status, 28, t.wait_limit);
-        if (ok && KEYS) ok = mbar_wait_warp(smem_u32(&hdr->full[slot]), sphase, abort_flag, status, 29, t.wait_limit);     // (done: the scores needed it too)
+        ok = at_wait(smem_u32(&hdr->s_full), n & 1, abort_flag, status, 28, t.wait_limit);
+        if (ok && KEYS) ok = at_wait(smem_u32(&hdr->full[slot]), sphase, abort_flag, status, 29, t.wait_limit);     // (done: the scores needed it too)
         if (!ok) break;
         tc_fence_after();
         uint32_t pw[HALF / 2], dw[HALF / 2];
@@ -304,7 +327,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           for (int e = 0; e < HALF / 2; ++e) pw[e] = dw[e] = 0u;
         }
         if (n > 0) {          // the previous P and dS have been read
-          ok = mbar_wait_warp(smem_u32(&hdr->mixed), (n - 1) & 1, abort_flag, status, 30, t.wait_limit);
+          ok = at_wait(smem_u32(&hdr->mixed), (n - 1) & 1, abort_flag, status, 30, t.wait_limit);
           if (!ok) break;
           tc_fence_after();
         }
@@ -340,55 +363,66 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         if (++slot == (uint32_t)G::NS) { slot = 0; sphase ^= 1u; }
       }
       if (!ok) break;
-      if (it.n > 0) {
-        ok = mbar_wait_warp(smem_u32(&hdr->mixed), (n - 1) & 1, abort_flag, status, 31, t.wait_limit);
-        if (!ok) break;
-        tc_fence_after();
-      }
-      // results: dk by the first four warps and dv by the others; dq by halves of its channels
+      // Results: dk by the first four warps and dv by the others, dq by halves of its channels, into the row tile's operand buffers (128-byte swizzle).
       constexpr int SPAN = KEYS ? DC * 64 : DC * 32;
+      const int ch0 = KEYS ? 0 : half * SPAN;
+      if (it.n == 0) {                 // no key in reach: zeros, and no buffer that is this row tile's
+        const int rows = KEYS ? a.Lk : a.Lq, heads = KEYS ? a.Hkv : a.H, per = a.D / 8;
+        for (int e = threadIdx.x; e < AT_M * per; e += EW_WARPS * 32) {
+          const int z = it.row0 + e / per;
+          const int64_t at = (((int64_t)it.b * rows + z) * heads + it.h) * a.D + e % per * 8;
+          if (z < rows) {
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(KEYS ? a.dk : a.dq) + at) = make_uint4(0, 0, 0, 0);
+            if (KEYS) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.dv) + at) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        __syncwarp();
+        continue;
+      }
+      ok = at_wait(smem_u32(&hdr->acc_full), seq & 1, abort_flag, status, 31, t.wait_limit);
+      if (!ok) break;
+      tc_fence_after();
       const uint32_t from = KEYS ? (half ? G::ACC2 : G::ACC1) : G::ACC1 + half * SPAN;
-      const int ch0 = KEYS ? 0 : half * SPAN, rows = KEYS ? a.Lk : a.Lq, heads = KEYS ? a.Hkv : a.H;
       const float f = KEYS && half ? 1.f : a.scale;
-      const bool zero = it.n == 0 || (KEYS && !row_ok);
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(KEYS ? (half ? a.dv : a.dk) : a.dq) + (((int64_t)it.b * rows + row) * heads + it.h) * a.D;
+      unsigned char* stage = smem_raw + (srow - raw) + (seq & 1) * 2 * G::RTILE + (KEYS ? half * G::RTILE : 0) + r * 128;
+      const bool zero = KEYS && !row_ok;
 #pragma unroll 1
       for (int e = 0; e < SPAN; e += 32) {
         float v[32];
-        if (it.n > 0) {
-          tc_ld32(lanes + from + e, reinterpret_cast<uint32_t*>(v));
-          tc_ld_wait();
-          tc_loaded<32>(reinterpret_cast<uint32_t*>(v));
-          if (e + 32 == SPAN) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&hdr->acc_free));
-          }
+        tc_ld32(lanes + from + e, reinterpret_cast<uint32_t*>(v));
+        tc_ld_wait();
+        tc_loaded<32>(reinterpret_cast<uint32_t*>(v));
+        if (e + 32 == SPAN) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&hdr->acc_free));
         }
-        if (row < rows) {
+        const int ch = ch0 + e;
 #pragma unroll
-          for (int k = 0; k < 32; k += 8)
-            if (ch0 + e + k < a.D) {
-              uint32_t w[4];
+        for (int k = 0; k < 32; k += 8) {
+          uint32_t w[4];
 #pragma unroll
-              for (int z = 0; z < 4; ++z) w[z] = zero ? 0u : pack_bf16(v[k + 2 * z] * f, v[k + 2 * z + 1] * f);
-              *reinterpret_cast<uint4*>(out + ch0 + e + k) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+          for (int z = 0; z < 4; ++z) w[z] = zero ? 0u : pack_bf16(v[k + 2 * z] * f, v[k + 2 * z + 1] * f);
+          *reinterpret_cast<uint4*>(stage + (ch >> 6) * G::RBOX + ((((ch & 63) + k) >> 3 ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        __syncwarp();
       }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&hdr->staged));
+      ++seq;
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == EW_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (warp == SCORES) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// -lse and -delta = -<dy, o> of every row, in rows of `pitch`: sixteen lanes a row, 8 channels each.
+// -lse and -delta = -<dy, o> of every row, in rows of `pitch`: LANES lanes a row, 8 channels each.
+template <int LANES>
 __global__ void __launch_bounds__(256) attn_row_stats_kernel(const AttnArgs a, float* nl, float* nd, int pitch) {
-  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);          // b, row, h: the heads of a row lie together
-  const int lane = threadIdx.x & 15;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;       // b, row, h: the heads of a row lie together
+  const int lane = threadIdx.x % LANES;
   if (i >= (int64_t)a.B * pitch * a.H) return;
   const int h = (int)(i % a.H);
   const int64_t bl = i / a.H, b = bl / pitch;
@@ -404,7 +438,8 @@ __global__ void __launch_bounds__(256) attn_row_stats_kernel(const AttnArgs a, f
       s = fmaf(p.x, q.x, s); s = fmaf(p.y, q.y, s);
     }
   }
-  for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+  const uint32_t team = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << (threadIdx.x % 32 / LANES * LANES);      // (the last warp's other rows may not be there)
+  for (int w = LANES / 2; w > 0; w >>= 1) s += __shfl_xor_sync(team, s, w);
   if (lane == 0) {
     const int64_t at = (b * a.H + h) * pitch + l;
     nl[at] = l < a.Lq ? -__ldg(a.lse + (b * a.H + h) * a.Lq + l) : -AT_INF;
@@ -415,12 +450,16 @@ __global__ void __launch_bounds__(256) attn_row_stats_kernel(const AttnArgs a, f
 template <int DC, bool KEYS>
 int launch(const AttnArgs& a, GradArgs g, cudaStream_t st) {
   using G = Grad<DC>;
-  CUtensorMap tq, tk, tv, tg;
+  CUtensorMap tq, tk, tv, tg, t1, t2;
   const int q_rows = KEYS ? G::CT : AT_M, k_rows = KEYS ? AT_M : G::CT;
   int rc = fovi::encode_rows(&tq, &g.t.q, a.q, a.q_sb, a.q_sl, a.q_sh, a.B, a.Lq, a.H, a.D, q_rows);
   if (!rc) rc = fovi::encode_rows(&tg, &g.t.g, a.dy, a.g_sb, a.g_sl, a.g_sh, a.B, a.Lq, a.H, a.D, q_rows);
   if (!rc) rc = fovi::encode_rows(&tk, &g.t.k, a.k, a.k_sb, a.k_sl, a.k_sh, a.B, a.Lk, a.Hkv, a.D, k_rows);
   if (!rc) rc = fovi::encode_rows(&tv, &g.t.v, a.v, a.v_sb, a.v_sl, a.v_sh, a.B, a.Lk, a.Hkv, a.D, k_rows);
+  const int64_t L = KEYS ? a.Lk : a.Lq, heads = KEYS ? a.Hkv : a.H;
+  fovi::TcView whole;
+  if (!rc) rc = fovi::encode_rows(&t1, &whole, KEYS ? a.dk : a.dq, L * heads * a.D, heads * a.D, a.D, a.B, (int)L, (int)heads, a.D, AT_M);
+  if (!rc) rc = fovi::encode_rows(&t2, &whole, KEYS ? a.dv : a.dq, L * heads * a.D, heads * a.D, a.D, a.B, (int)L, (int)heads, a.D, AT_M);
   if (rc) return rc;
   g.tiles = ((KEYS ? a.Lk : a.Lq) + AT_M - 1) / AT_M;
   const int64_t items = (int64_t)g.tiles * (KEYS ? a.Hkv : a.H) * a.B;
@@ -428,7 +467,7 @@ int launch(const AttnArgs& a, GradArgs g, cudaStream_t st) {
   g.items = (int)items;
   const int grid = std::min(g.items, fovi::sm_count());
   FOVI_CUDA(cudaFuncSetAttribute(attn_tc_grad_kernel<DC, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::SMEM));
-  FOVI_CUDA(fovi::launch_pdl(attn_tc_grad_kernel<DC, KEYS>, grid, GR_THREADS, G::SMEM, st, tq, tk, tv, tg, g));
+  FOVI_CUDA(fovi::launch_pdl(attn_tc_grad_kernel<DC, KEYS>, grid, GR_THREADS, G::SMEM, st, tq, tk, tv, tg, t1, t2, g));
   return fovi::after_launch("attn_tc_grad_kernel");
 }
 
@@ -444,11 +483,12 @@ int fovi::launch_attention_tc_backward(const AttnArgs& a, void* work, cudaStream
   int rc = attention_tc_status(&g.t.status);
   if (rc) return rc;
   g.pitch = (a.Lq + AT_M - 1) / AT_M * AT_M;
-  const int64_t rows = (int64_t)a.B * a.H * g.pitch, blocks = (rows + 15) / 16;
+  const int64_t rows = (int64_t)a.B * a.H * g.pitch, blocks = (rows * (a.D <= 64 ? 8 : 16) + 255) / 256;
   if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;
   float* nl = static_cast<float*>(work);
   g.nl = nl; g.nd = nl + rows;
-  attn_row_stats_kernel<<<(int)blocks, 256, 0, st>>>(a, nl, nl + rows, g.pitch);
+  if (a.D <= 64) attn_row_stats_kernel<8><<<(int)blocks, 256, 0, st>>>(a, nl, nl + rows, g.pitch);
+  else attn_row_stats_kernel<16><<<(int)blocks, 256, 0, st>>>(a, nl, nl + rows, g.pitch);
   rc = after_launch("attn_row_stats_kernel");
   if (!rc && a.dk) rc = a.D <= 64 ? launch<1, true>(a, g, st) : launch<2, true>(a, g, st);
   if (!rc && a.dq) rc = a.D <= 64 ? launch<1, false>(a, g, st) : launch<2, false>(a, g, st);
