@@ -9,6 +9,7 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "pairs.cuh"
 
 namespace {
 
@@ -164,112 +165,133 @@ template <int VEC, bool BLOCK> struct Team {
   }
 };
 
+// Threads of the largest block: single values take more instructions and more registers.
+template <int VEC> constexpr int BLOCK_MOST = VEC == 1 ? 512 : 1024;
+
+// Values two by two, for the instructions that take two.
+template <int E> struct Pairs {
+  static_assert(E % 2 == 0, "an even number of values a thread");
+  float2 v[E / 2];
+  __device__ __forceinline__ float* at(int i) { return reinterpret_cast<float*>(v) + i; }
+};
+
 template <typename TX, typename TY, int VEC, int CH, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) layer_norm_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64_t stride, const float* __restrict__ w,
+__global__ void __launch_bounds__(BLOCK ? BLOCK_MOST<VEC> : 256, !BLOCK && sizeof(TX) == 2 && CH * VEC <= 12 ? 4 : 0)
+layer_norm_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64_t stride, const float* __restrict__ w,
                                                                              const float* __restrict__ b, float eps, TY* __restrict__ y, float2* __restrict__ stats) {
+  constexpr int E = CH * VEC, H = VEC > 1 ? VEC / 2 : 1;       // pairs of a piece; single values pair up over two pieces
+  constexpr int STEP = VEC > 1 ? 1 : 2;                        // pieces of a step
   __shared__ float2 part[2][32];
   const Team<VEC, BLOCK> t;
-  float wv[CH * VEC], bv[CH * VEC];
+  Pairs<E> wv, bv;
+  Piece<TX, VEC> next[CH] = {};                                // pieces behind the row's end stay zeros
+  int pieces = 0;
 #pragma unroll
-  for (int k = 0; k < CH; ++k)
+  for (int k = 0; k < CH; ++k) {
+    pieces += t.first + k * t.pitch < C;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int c = t.first + k * t.pitch + i;
-      wv[k * VEC + i] = w && c < C ? __ldg(w + c) : 1.f;
-      bv[k * VEC + i] = b && c < C ? __ldg(b + c) : 0.f;
+      *wv.at(k * VEC + i) = w && c < C ? __ldg(w + c) : 1.f;
+      *bv.at(k * VEC + i) = b && c < C ? __ldg(b + c) : 0.f;
     }
-  Piece<TX, VEC> next[CH];
+  }
   auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < CH; ++k)
-      if (t.first + k * t.pitch < C) next[k] = load_piece<TX, VEC>(x + r * stride + t.first + k * t.pitch);
+      if (k < pieces) next[k] = load_piece<TX, VEC>(x + r * stride + t.first + k * t.pitch);
   };
   if (t.row < rows) fetch(t.row);
+  const float n = BLOCK ? warp_sum((float)(pieces * VEC)) : (float)C, inv_n = 1.f / fmaxf(n, 1.f), inv = 1.f / C;
   int flip = 0;
   for (int64_t r = t.row; r < rows; r += t.step, flip ^= 1) {
-    float v[CH * VEC];
-    float s = 0.f, n = 0.f;
+    Pairs<E> v;
+    float2 s2 = both(0.f);
 #pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const bool in = t.first + k * t.pitch < C;
-      if (in) { widen<TX, VEC>(next[k], v + k * VEC); n += VEC; }
+    for (int k = 0; k < CH; ++k) widen<TX, VEC>(next[k], v.at(k * VEC));
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) { v[k * VEC + i] = in ? v[k * VEC + i] : 0.f; s += v[k * VEC + i]; }
-    }
+    for (int i = 0; i < E / 2; ++i) s2 = add2(s2, v.v[i]);
     if (r + t.step < rows) fetch(r + t.step);
     // mean and sum of squares about it: of the warp's values, then (block) of all warps' by the parallel form of the same
-    const float count = BLOCK ? warp_sum(n) : (float)C;
-    float mean = warp_sum(s) / fmaxf(count, 1.f), q = 0.f;
+    float mean = warp_sum(s2.x + s2.y) * inv_n;
+    s2 = both(0.f);
 #pragma unroll
-    for (int k = 0; k < CH; ++k)
-      if (t.first + k * t.pitch < C) {
+    for (int k = 0; k < CH; k += STEP) {
+      if (k < pieces) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) { const float d = v[k * VEC + i] - mean; q = fmaf(d, d, q); }
-      }
-    q = warp_sum(q);
-    if (BLOCK) {
-      if ((threadIdx.x & 31) == 0) part[flip][t.warp] = make_float2(mean, q);
-      __syncthreads();                     // (two sets of parts: a warp that is ahead writes the other one)
-      // every warp's count follows from C; warps hold pieces in turn, so it is that of the pieces that fall on them
-      float all = 0.f;
-      q = 0.f;
-      float total = 0.f;
-      for (int i = 0; i < t.warps; ++i) {
-        float ni = 0.f;
-#pragma unroll
-        for (int k = 0; k < CH; ++k) ni += (float)min(max(C - (i * 32 * VEC + k * t.pitch), 0), 32 * VEC);
-        const float2 p = part[flip][i];
-        total = fmaf(ni, p.x, total);
-        all += ni;
-      }
-      mean = total / all;
-      for (int i = 0; i < t.warps; ++i) {
-        float ni = 0.f;
-#pragma unroll
-        for (int k = 0; k < CH; ++k) ni += (float)min(max(C - (i * 32 * VEC + k * t.pitch), 0), 32 * VEC);
-        const float2 p = part[flip][i];
-        const float d = p.x - mean;
-        q += ni > 0.f ? fmaf(ni * d, d, p.y) : 0.f;
+        for (int i = k * VEC / 2; i < k * VEC / 2 + H; ++i) {
+          v.v[i] = add2(v.v[i], both(-mean));
+          if (STEP == 2 && k + 1 >= pieces) v.v[i].y = 0.f;
+          s2 = fma2(v.v[i], v.v[i], s2);
+        }
       }
     }
-    const float rstd = 1.f / sqrtf(q / C + eps);
+    float q = warp_sum(s2.x + s2.y), shift = 0.f;
+    if (BLOCK) {          // a lane per warp: its mean, its sum of squares; how many values it holds follows from the row's length
+      if ((threadIdx.x & 31) == 0) part[flip][t.warp] = make_float2(mean, q);
+      __syncthreads();    // (two sets of parts: a warp that is ahead writes the other one)
+      const int lane = threadIdx.x & 31;
+      const float2 p = lane < t.warps ? part[flip][lane] : make_float2(0.f, 0.f);
+      float held = 0.f;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) held += (float)min(max(C - (lane * 32 * VEC + k * t.pitch), 0), 32 * VEC);
+      if (lane >= t.warps) held = 0.f;
+      const float all = warp_sum(held * p.x) * inv, d = p.x - all;
+      q = warp_sum(held > 0.f ? fmaf(held * d, d, p.y) : 0.f);
+      shift = mean - all;
+      mean = all;
+    }
+    const float rstd = rsqrtf(fmaf(q, inv, eps));
     if (stats && (BLOCK ? threadIdx.x : threadIdx.x & 31) == 0) stats[r] = make_float2(mean, rstd);
 #pragma unroll
-    for (int k = 0; k < CH; ++k)
-      if (t.first + k * t.pitch < C) {
-        float o[VEC];
+    for (int k = 0; k < CH; k += STEP) {
+      if (k < pieces) {
+        Pairs<VEC * STEP> o;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = fmaf((v[k * VEC + i] - mean) * rstd, wv[k * VEC + i], bv[k * VEC + i]);
-        store_piece<TY, VEC>(y + r * C + t.first + k * t.pitch, o);
+        for (int i = 0; i < H; ++i) {
+          const int e = k * VEC / 2 + i;
+          o.v[i] = fma2(mul2(BLOCK ? add2(v.v[e], both(shift)) : v.v[e], both(rstd)), wv.v[e], bv.v[e]);
+        }
+        store_piece<TY, VEC>(y + r * C + t.first + k * t.pitch, o.at(0));
+        if (STEP == 2 && k + 1 < pieces) store_piece<TY, VEC>(y + r * C + t.first + (k + 1) * t.pitch, o.at(1));
       }
+    }
   }
 }
 
 template <typename TX, typename TY, int VEC, int CH, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256, BLOCK ? 1 : 2)
+__global__ void __launch_bounds__(BLOCK ? BLOCK_MOST<VEC> : 256, BLOCK ? 1 : CH * VEC <= 8 ? 3 : 2)
 layer_norm_grad_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64_t stride, const TY* __restrict__ dy, int64_t dy_stride, const float* __restrict__ w,
                             const float2* __restrict__ stats, TX* __restrict__ dx, float* __restrict__ part) {
-  constexpr int E = CH * VEC;
+  constexpr int E = CH * VEC, H = VEC > 1 ? VEC / 2 : 1, STEP = VEC > 1 ? 1 : 2;
   __shared__ float2 sums[2][32];
-  extern __shared__ float joined[];        // warp teams: their parts, [2][C]
+  extern __shared__ float joined[];        // warp teams: the weights (in shared memory: their registers are a third block's), then the warps' parts, [2][C]
   const Team<VEC, BLOCK> t;
-  float wv[E], aw[E], ab[E];
+  Pairs<BLOCK ? E : 2> wv;
+  Pairs<E> aw, ab;
+  Piece<TX, VEC> nx[CH] = {};
+  Piece<TY, VEC> ng[CH] = {};
+  int pieces = 0;
 #pragma unroll
-  for (int k = 0; k < CH; ++k)
+  for (int k = 0; k < CH; ++k) {
+    pieces += t.first + k * t.pitch < C;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int c = t.first + k * t.pitch + i;
-      wv[k * VEC + i] = w && c < C ? __ldg(w + c) : 1.f;
-      aw[k * VEC + i] = ab[k * VEC + i] = 0.f;
+      if (BLOCK) *wv.at(BLOCK ? k * VEC + i : 0) = w && c < C ? __ldg(w + c) : 1.f;
+      *aw.at(k * VEC + i) = *ab.at(k * VEC + i) = 0.f;
     }
-  Piece<TX, VEC> nx[CH];
-  Piece<TY, VEC> ng[CH];
+  }
+  if (!BLOCK) {
+    for (int c = threadIdx.x; c < C; c += blockDim.x) joined[c] = w ? __ldg(w + c) : 1.f;
+    __syncthreads();
+  }
   float2 ns = make_float2(0.f, 0.f);
   auto fetch = [&](int64_t r) {
     ns = __ldg(stats + r);
 #pragma unroll
     for (int k = 0; k < CH; ++k)
-      if (t.first + k * t.pitch < C) {
+      if (k < pieces) {
         nx[k] = load_piece<TX, VEC>(x + r * stride + t.first + k * t.pitch);
         ng[k] = load_piece<TY, VEC>(dy + r * dy_stride + t.first + k * t.pitch);
       }
@@ -278,48 +300,61 @@ layer_norm_grad_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64
   const float inv = 1.f / C;
   int flip = 0;
   for (int64_t r = t.row; r < rows; r += t.step, flip ^= 1) {
-    const float2 st = ns;
-    float xh[E], g[E], sg = 0.f, sx = 0.f;
+    const float rstd = ns.y;
+    Pairs<E> xh, g;
+    float2 sg = both(0.f), sx = both(0.f);
 #pragma unroll
-    for (int k = 0; k < CH; ++k)
-      if (t.first + k * t.pitch < C) {
-        widen<TX, VEC>(nx[k], xh + k * VEC);
-        widen<TY, VEC>(ng[k], g + k * VEC);
+    for (int k = 0; k < CH; ++k) { widen<TX, VEC>(nx[k], xh.at(k * VEC)); widen<TY, VEC>(ng[k], g.at(k * VEC)); }
 #pragma unroll
-        for (int i = k * VEC; i < (k + 1) * VEC; ++i) {
-          xh[i] = (xh[i] - st.x) * st.y;
-          aw[i] = fmaf(g[i], xh[i], aw[i]);
-          ab[i] += g[i];
-          g[i] *= wv[i];
-          sg += g[i];
-          sx = fmaf(g[i], xh[i], sx);
+    for (int k = 0; k < CH; k += STEP) {
+      if (k < pieces) {                     // (a single value without a second: its gradient is zero, and so is all that it adds)
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          const int e = k * VEC / 2 + i;
+          float2 we;
+          if (BLOCK) we = wv.v[BLOCK ? e : 0];
+          else if (VEC > 1) we = *reinterpret_cast<const float2*>(joined + t.first + k * t.pitch + 2 * i);
+          else we = make_float2(joined[t.first + k * t.pitch], k + 1 < pieces ? joined[t.first + (k + 1) * t.pitch] : 0.f);
+          xh.v[e] = mul2(add2(xh.v[e], both(-ns.x)), both(rstd));
+          aw.v[e] = fma2(g.v[e], xh.v[e], aw.v[e]);
+          ab.v[e] = add2(ab.v[e], g.v[e]);
+          g.v[e] = mul2(g.v[e], we);
+          sg = add2(sg, g.v[e]);
+          sx = fma2(g.v[e], xh.v[e], sx);
         }
       }
-    if (r + t.step < rows) fetch(r + t.step);
-    sg = warp_sum(sg);
-    sx = warp_sum(sx);
-    if (BLOCK) {
-      if ((threadIdx.x & 31) == 0) sums[flip][t.warp] = make_float2(sg, sx);
-      __syncthreads();
-      sg = sx = 0.f;
-      for (int i = 0; i < t.warps; ++i) { const float2 p = sums[flip][i]; sg += p.x; sx += p.y; }
     }
-    sg *= inv;
-    sx *= inv;
+    if (r + t.step < rows) fetch(r + t.step);
+    float mg = warp_sum(sg.x + sg.y), mx = warp_sum(sx.x + sx.y);
+    if (BLOCK) {
+      if ((threadIdx.x & 31) == 0) sums[flip][t.warp] = make_float2(mg, mx);
+      __syncthreads();
+      const float2 p = (int)(threadIdx.x & 31) < t.warps ? sums[flip][threadIdx.x & 31] : make_float2(0.f, 0.f);
+      mg = warp_sum(p.x);
+      mx = warp_sum(p.y);
+    }
+    mg *= inv;
+    mx *= inv;
     if (dx) {
 #pragma unroll
-      for (int k = 0; k < CH; ++k)
-        if (t.first + k * t.pitch < C) {
-          float o[VEC];
+      for (int k = 0; k < CH; k += STEP) {
+        if (k < pieces) {
+          Pairs<VEC * STEP> o;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o[i] = st.y * (g[k * VEC + i] - sg - xh[k * VEC + i] * sx);
-          store_piece<TX, VEC>(dx + r * C + t.first + k * t.pitch, o);
+          for (int i = 0; i < H; ++i) {
+            const int e = k * VEC / 2 + i;
+            o.v[i] = mul2(fma2(xh.v[e], both(-mx), add2(g.v[e], both(-mg))), both(rstd));
+          }
+          store_piece<TX, VEC>(dx + r * C + t.first + k * t.pitch, o.at(0));
+          if (STEP == 2 && k + 1 < pieces) store_piece<TX, VEC>(dx + r * C + t.first + (k + 1) * t.pitch, o.at(1));
         }
+      }
     }
   }
   if (!part) return;
   float* mine = part + (size_t)blockIdx.x * 2 * C;
-  if (!BLOCK) {            // the warps' parts one after another: a fixed order
+  if (!BLOCK) __syncthreads();             // the weights have been read
+  if (!BLOCK) {                            // the warps' parts one after another: a fixed order
     for (int u = 0; u < t.warps; ++u) {
       if (t.warp == u) {
 #pragma unroll
@@ -328,8 +363,8 @@ layer_norm_grad_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64
           for (int i = 0; i < VEC; ++i) {
             const int c = t.first + k * t.pitch + i;
             if (c < C) {
-              joined[c] = (u ? joined[c] : 0.f) + aw[k * VEC + i];
-              joined[C + c] = (u ? joined[C + c] : 0.f) + ab[k * VEC + i];
+              joined[c] = (u ? joined[c] : 0.f) + *aw.at(k * VEC + i);
+              joined[C + c] = (u ? joined[C + c] : 0.f) + *ab.at(k * VEC + i);
             }
           }
       }
@@ -342,7 +377,7 @@ layer_norm_grad_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const int c = t.first + k * t.pitch + i;
-        if (c < C) { mine[c] = aw[k * VEC + i]; mine[C + c] = ab[k * VEC + i]; }
+        if (c < C) { mine[c] = *aw.at(k * VEC + i); mine[C + c] = *ab.at(k * VEC + i); }
       }
   }
 }
@@ -361,13 +396,13 @@ Shape shape_of(const void* x, int64_t x_stride, int xs, const void* y, int64_t y
   if (ch * vec <= (wide || vec == 1 ? 12 : 24)) return {vec, ch, 32, false};
   const int per = vec == 8 ? 1 : vec == 4 ? 2 : 8;             // a block: 8 values a thread
   const int threads = ((C + per * vec - 1) / (per * vec) + 31) / 32 * 32;
-  if (threads <= 1024) return {vec, per, threads, true};
+  if (threads <= (vec == 1 ? BLOCK_MOST<1> : BLOCK_MOST<4>)) return {vec, per, threads, true};
   return {0, 0, 0, false};
 }
 
 constexpr int GRAD_BLOCKS = 592;         // most parts of dw and db
 int grad_blocks(const Shape& s, int64_t rows) {
-  const int64_t want = s.block ? rows : (rows + 7) / 8, most = s.block ? std::max(148, std::min(GRAD_BLOCKS, 148 * 640 / s.threads)) : 296;
+  const int64_t want = s.block ? rows : (rows + 7) / 8, most = s.block ? std::max(148, std::min(GRAD_BLOCKS, 148 * 640 / s.threads)) : s.ch * s.vec <= 8 ? 444 : 296;
   return (int)std::min<int64_t>(want, most);
 }
 
@@ -377,13 +412,21 @@ template <typename TX, typename TY> struct Run {
   template <int VEC, int CH, bool BLOCK> int go(const Shape& s, bool backward) const {
     const int threads = BLOCK ? s.threads : 256;
     if (!backward) {
-      const int64_t want = BLOCK ? rows : (rows + 7) / 8, most = BLOCK ? 148 * std::max(1, 2048 / s.threads) : 148 * 6;
-      layer_norm_rows_kernel<TX, TY, VEC, CH, BLOCK><<<(int)std::min(want, most), threads, 0, st>>>((const TX*)x, rows, C, stride, w, b, eps, (TY*)y, (float2*)stats);
+      auto k = layer_norm_rows_kernel<TX, TY, VEC, CH, BLOCK>;
+      const int64_t want = BLOCK ? rows : (rows + 7) / 8;
+      k<<<(int)std::min(want, resident<VEC, CH, BLOCK>(k, threads)), threads, 0, st>>>((const TX*)x, rows, C, stride, w, b, eps, (TY*)y, (float2*)stats);
       return fovi::after_launch("layer_norm_rows_kernel");
     }
-    layer_norm_grad_rows_kernel<TX, TY, VEC, CH, BLOCK><<<grad_blocks(s, rows), threads, BLOCK ? 0 : 2 * C * sizeof(float), st>>>(
-        (const TX*)x, rows, C, stride, (const TY*)dy, dy_stride, w, (const float2*)stats, (TX*)dx, part);
+    auto k = layer_norm_grad_rows_kernel<TX, TY, VEC, CH, BLOCK>;
+    k<<<grad_blocks(s, rows), threads, BLOCK ? 0 : 2 * C * sizeof(float), st>>>((const TX*)x, rows, C, stride, (const TY*)dy, dy_stride, w, (const float2*)stats, (TX*)dx, part);
     return fovi::after_launch("layer_norm_grad_rows_kernel");
+  }
+  // As many blocks as are on the SMs at once: every team then takes the same number of rows.
+  template <int VEC, int CH, bool BLOCK, typename Kernel> static int64_t resident(Kernel k, int threads) {
+    static int per_sm[33] = {};
+    int& n = per_sm[threads / 32];
+    if (!n && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, threads, 0) != cudaSuccess || n < 1)) n = 1;
+    return (int64_t)fovi::sm_count() * n;
   }
   template <int VEC, int MOST, int STEP = 1, int CH = STEP> int warp(const Shape& s, bool backward) const {
     if constexpr (CH * VEC <= MOST) return s.ch == CH ? go<VEC, CH, false>(s, backward) : warp<VEC, MOST, STEP, CH + STEP>(s, backward);
