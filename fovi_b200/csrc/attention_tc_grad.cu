@@ -473,7 +473,9 @@ int launch(const AttnArgs& a, GradArgs g, cudaStream_t st) {
 
 }  // namespace
 
-int64_t fovi::attention_tc_backward_bytes(int B, int Lq, int H) { return (int64_t)B * H * ((Lq + AT_M - 1) / AT_M * AT_M) * 8; }
+// Statistics of a row of queries: Lq rounded up to 16, as far as an MMA reads a last tile; copies of a whole tile may read up to 128 values more.
+static int64_t stats_pitch(int Lq) { return ((int64_t)Lq + 15) / 16 * 16; }
+int64_t fovi::attention_tc_backward_bytes(int B, int Lq, int H) { return (int64_t)B * H * stats_pitch(Lq) * 8 + 128 * 4; }
 
 int fovi::launch_attention_tc_backward(const AttnArgs& a, void* work, cudaStream_t st, bool selftest) {
   GradArgs g = {};
@@ -482,7 +484,7 @@ int fovi::launch_attention_tc_backward(const AttnArgs& a, void* work, cudaStream
   g.t.skip_loads = selftest;
   int rc = attention_tc_status(&g.t.status);
   if (rc) return rc;
-  g.pitch = (a.Lq + AT_M - 1) / AT_M * AT_M;
+  g.pitch = (int)stats_pitch(a.Lq);
   const int64_t rows = (int64_t)a.B * a.H * g.pitch, blocks = (rows * (a.D <= 64 ? 8 : 16) + 255) / 256;
   if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;
   float* nl = static_cast<float*>(work);
