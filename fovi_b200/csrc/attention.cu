@@ -26,61 +26,113 @@ __device__ __forceinline__ bool key_ok(const AttnArgs& a, int b, int key, int en
   return key < end && (!a.mask || __ldg(a.mask + (int64_t)b * a.Lk + key));
 }
 
-// Rows [r0, r0 + 64) of one head as float32, zeros behind n and D, and where `ok` says no.
+// A thread's part of a tile: rows [r0, r0 + 64) of one head as float32, zeros behind `n` and D.  It is fetched while the tile before it is worked on.  With `vec` the rows are whole pieces of
+// 16 bytes on 16-byte boundaries.
 template <typename E, int DP>
-__device__ __forceinline__ void load_tile(float* dst, const E* src, int64_t sl, int r0, int n, int D, const unsigned char* ok = nullptr) {
-  for (int i = threadIdx.x; i < T * DP; i += THREADS) {
-    const int r = i / DP, d = i - r * DP;
-    dst[r * PITCH<DP> + d] = r0 + r < n && d < D && (!ok || ok[r]) ? ld_as_float(src + (int64_t)(r0 + r) * sl + d) : 0.f;
+struct Part {
+  static constexpr int V = 16 / sizeof(E), N = T * DP / (V * THREADS), ROW = DP / V;      // pieces of V channels
+  float x[N][V];
+  __device__ __forceinline__ void fetch(const E* src, int64_t sl, int r0, int n, int D, bool vec) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = threadIdx.x + k * THREADS, r = i / ROW, c = i % ROW * V;
+      const E* p = src + (int64_t)(r0 + r) * sl + c;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[k][e] = 0.f;
+      if (r0 + r >= n) continue;
+      if (vec) {
+        if (c >= D) continue;
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[k][e] = V == 4 ? __uint_as_float(u[e % 4]) : __uint_as_float(e & 1 ? u[e / 2 % 4] & 0xffff0000u : u[e / 2 % 4] << 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c + e < D) x[k][e] = ld_as_float(p + e);
+      }
+    }
   }
-}
+  __device__ __forceinline__ void store(float* dst, const unsigned char* ok = nullptr) const {      // zeros in the rows where `ok` says no
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = threadIdx.x + k * THREADS, r = i / ROW, c = i % ROW * V;
+      const bool in = !ok || ok[r];
+#pragma unroll
+      for (int e = 0; e < V; e += 4)
+        *reinterpret_cast<float4*>(dst + r * PITCH<DP> + c + e) = in ? make_float4(x[k][e], x[k][e + 1], x[k][e + 2], x[k][e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+};
 
-// acc[i][j] = <A row ty + 16 i, B row tx + 16 j>
+// Rounds of 16 rows that `n` rows take, four at most.
+__device__ __forceinline__ int rounds(int n) { return min(4, (n + 15) / 16); }
+
+// acc[i][j] = <A row ty + 16 i, B row tx + 16 j>; of a last tile only the first ni, nj rounds of rows, zeros beyond
 template <int DP>
-__device__ __forceinline__ void dot_tile(const float* A, const float* B, float (&acc)[4][4]) {
+__device__ __forceinline__ void dot_tile(const float* A, const float* B, float (&acc)[4][4], int ni, int nj) {
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  auto step = [&](int d, int i, int j, const float4& x, const float4& y) {
+    acc[i][j] = fmaf(x.x, y.x, acc[i][j]); acc[i][j] = fmaf(x.y, y.y, acc[i][j]);
+    acc[i][j] = fmaf(x.z, y.z, acc[i][j]); acc[i][j] = fmaf(x.w, y.w, acc[i][j]);
+  };
+  if (ni + nj == 8) {
 #pragma unroll 4
-  for (int d = 0; d < DP; d += 4) {
-    float4 x[4], y[4];
+    for (int d = 0; d < DP; d += 4) {
+      float4 x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = *reinterpret_cast<const float4*>(A + (ty + 16 * i) * PITCH<DP> + d);
+        y[i] = *reinterpret_cast<const float4*>(B + (tx + 16 * i) * PITCH<DP> + d);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) step(d, i, j, x[i], y[j]);
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[i] = *reinterpret_cast<const float4*>(A + (ty + 16 * i) * PITCH<DP> + d);
-      y[i] = *reinterpret_cast<const float4*>(B + (tx + 16 * i) * PITCH<DP> + d);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
+      if (i >= ni) break;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]); acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
-        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]); acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+        if (j >= nj) break;
+#pragma unroll 8
+        for (int d = 0; d < DP; d += 4)
+          step(d, i, j, *reinterpret_cast<const float4*>(A + (ty + 16 * i) * PITCH<DP> + d), *reinterpret_cast<const float4*>(B + (tx + 16 * j) * PITCH<DP> + d));
       }
+    }
   }
 }
 
-// acc[i][c] += sum over r of P[ty + 16 i][r] * V[r][channel c of this thread], channels 64 jj + 4 tx .. + 3
+// acc[i][c] += sum over r of P[ty + 16 i][r] * V[r][channel c of this thread], channels 64 jj + 4 tx .. + 3; the first ni rounds of rows, 16 nr values of r
 template <int DP>
-__device__ __forceinline__ void mix_tile(const float* P, const float* V, float (&acc)[4][DP / 16]) {
+__device__ __forceinline__ void mix_tile(const float* P, const float* V, float (&acc)[4][DP / 16], int ni, int nr) {
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
 #pragma unroll 2
-  for (int r = 0; r < T; r += 4) {
-    float p[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(p[i]) = *reinterpret_cast<const float4*>(P + (ty + 16 * i) * PP + r);
+  for (int r = 0; r < 16 * nr; r += 4) {
+    float4 v[4][DP / 64];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int jj = 0; jj < DP / 64; ++jj) {
-        const float4 v = *reinterpret_cast<const float4*>(V + (r + q) * PITCH<DP> + 64 * jj + 4 * tx);
+      for (int jj = 0; jj < DP / 64; ++jj) v[q][jj] = *reinterpret_cast<const float4*>(V + (r + q) * PITCH<DP> + 64 * jj + 4 * tx);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[i][4 * jj] = fmaf(p[i][q], v.x, acc[i][4 * jj]); acc[i][4 * jj + 1] = fmaf(p[i][q], v.y, acc[i][4 * jj + 1]);
-          acc[i][4 * jj + 2] = fmaf(p[i][q], v.z, acc[i][4 * jj + 2]); acc[i][4 * jj + 3] = fmaf(p[i][q], v.w, acc[i][4 * jj + 3]);
+    for (int i = 0; i < 4; ++i) {
+      if (i >= ni) break;
+      float p[4];
+      *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(P + (ty + 16 * i) * PP + r);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int jj = 0; jj < DP / 64; ++jj) {
+          acc[i][4 * jj] = fmaf(p[q], v[q][jj].x, acc[i][4 * jj]); acc[i][4 * jj + 1] = fmaf(p[q], v[q][jj].y, acc[i][4 * jj + 1]);
+          acc[i][4 * jj + 2] = fmaf(p[q], v[q][jj].z, acc[i][4 * jj + 2]); acc[i][4 * jj + 3] = fmaf(p[q], v[q][jj].w, acc[i][4 * jj + 3]);
         }
-      }
+    }
   }
 }
 
@@ -120,7 +172,12 @@ __global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a)
   const int qt = blockIdx.x % n_qt, h = blockIdx.x / n_qt % a.H, b = blockIdx.x / n_qt / a.H, end = key_end(a, b);
   const E* k = (const E*)a.k + b * a.k_sb + (h / a.group) * a.k_sh;
   const E* v = (const E*)a.v + b * a.v_sb + (h / a.group) * a.v_sh;
-  load_tile<E, DP>(Q, (const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, qt * T, a.Lq, a.D);
+  const int ni = rounds(a.Lq - qt * T);
+  Part<E, DP> nk, nv;
+  nv.fetch((const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, qt * T, a.Lq, a.D, a.vec);
+  nv.store(Q);
+  nk.fetch(k, a.k_sl, 0, end, a.D, a.vec);
+  nv.fetch(v, a.v_sl, 0, end, a.D, a.vec);
   float m[4], l[4], acc[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -129,14 +186,19 @@ __global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a)
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
   for (int k0 = 0; k0 < end; k0 += T) {
+    const int nj = rounds(end - k0);
     __syncthreads();
     if (threadIdx.x < T) ok[threadIdx.x] = key_ok(a, b, k0 + threadIdx.x, end);
+    if (a.mask) __syncthreads();
+    nk.store(K, a.mask ? ok : nullptr);
+    nv.store(V, a.mask ? ok : nullptr);
     __syncthreads();
-    load_tile<E, DP>(K, k, a.k_sl, k0, a.Lk, a.D, ok);
-    load_tile<E, DP>(V, v, a.v_sl, k0, a.Lk, a.D, ok);
-    __syncthreads();
+    if (k0 + T < end) {
+      nk.fetch(k, a.k_sl, k0 + T, end, a.D, a.vec);
+      nv.fetch(v, a.v_sl, k0 + T, end, a.D, a.vec);
+    }
     float s[4][4];
-    dot_tile<DP>(Q, K, s);
+    dot_tile<DP>(Q, K, s, ni, nj);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float top = -INF;
@@ -160,7 +222,7 @@ __global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a)
       for (int c = 0; c < DP / 16; ++c) acc[i][c] *= f;
     }
     __syncthreads();
-    mix_tile<DP>(P, V, acc);
+    mix_tile<DP>(P, V, acc, ni, nj);
   }
   float inv[4];
 #pragma unroll
@@ -199,8 +261,14 @@ __global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
   const int qt = blockIdx.x % n_qt, h = blockIdx.x / n_qt % a.H, b = blockIdx.x / n_qt / a.H, end = key_end(a, b);
   const E* k = (const E*)a.k + b * a.k_sb + (h / a.group) * a.k_sh;
   const E* v = (const E*)a.v + b * a.v_sb + (h / a.group) * a.v_sh;
-  load_tile<E, DP>(Q, (const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, qt * T, a.Lq, a.D);
-  load_tile<E, DP>(G, (const E*)a.dy + b * a.g_sb + h * a.g_sh, a.g_sl, qt * T, a.Lq, a.D);
+  const int ni = rounds(a.Lq - qt * T);
+  Part<E, DP> nk, nv;
+  nk.fetch((const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, qt * T, a.Lq, a.D, a.vec);
+  nv.fetch((const E*)a.dy + b * a.g_sb + h * a.g_sh, a.g_sl, qt * T, a.Lq, a.D, a.vec);
+  nk.store(Q);
+  nv.store(G);
+  nk.fetch(k, a.k_sl, 0, end, a.D, a.vec);
+  nv.fetch(v, a.v_sl, 0, end, a.D, a.vec);
   float lse[4], delta[4], acc[4][DP / 16], f[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -213,15 +281,20 @@ __global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
   for (int k0 = 0; k0 < end; k0 += T) {
+    const int nj = rounds(end - k0);
     __syncthreads();
     if (threadIdx.x < T) ok[threadIdx.x] = key_ok(a, b, k0 + threadIdx.x, end);
+    if (a.mask) __syncthreads();
+    nk.store(K, a.mask ? ok : nullptr);
+    nv.store(V, a.mask ? ok : nullptr);
     __syncthreads();
-    load_tile<E, DP>(K, k, a.k_sl, k0, a.Lk, a.D, ok);
-    load_tile<E, DP>(V, v, a.v_sl, k0, a.Lk, a.D, ok);
-    __syncthreads();
+    if (k0 + T < end) {
+      nk.fetch(k, a.k_sl, k0 + T, end, a.D, a.vec);
+      nv.fetch(v, a.v_sl, k0 + T, end, a.D, a.vec);
+    }
     float s[4][4], dp[4][4];
-    dot_tile<DP>(Q, K, s);
-    dot_tile<DP>(G, V, dp);
+    dot_tile<DP>(Q, K, s, ni, nj);
+    dot_tile<DP>(G, V, dp, ni, nj);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -230,7 +303,7 @@ __global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
         P[(ty + 16 * i) * PP + tx + 16 * j] = ok[tx + 16 * j] ? p * (dp[i][j] - delta[i]) : 0.f;
       }
     __syncthreads();
-    mix_tile<DP>(P, K, acc);
+    mix_tile<DP>(P, K, acc, ni, nj);
   }
   store_tile<E, DP>((E*)a.dq + ((int64_t)b * a.Lq * a.H + h) * a.D, (int64_t)a.H * a.D, qt * T, a.Lq, a.D, acc, f);
 }
@@ -253,18 +326,29 @@ __global__ void __launch_bounds__(THREADS) attn_dkv_kernel(const AttnArgs a) {
   }
   if (threadIdx.x < T) ok[threadIdx.x] = key_ok(a, b, kt * T + threadIdx.x, end);
   __syncthreads();
-  load_tile<E, DP>(K, (const E*)a.k + b * a.k_sb + hk * a.k_sh, a.k_sl, kt * T, a.Lk, a.D, ok);
-  load_tile<E, DP>(V, (const E*)a.v + b * a.v_sb + hk * a.v_sh, a.v_sl, kt * T, a.Lk, a.D, ok);
-  const int first = kt * T < end ? hk * a.group : (hk + 1) * a.group;         // a tile behind the sample's length has gradients of zero
-  for (int h = first; h < (hk + 1) * a.group; ++h)
-    for (int q0 = 0; q0 < a.Lq; q0 += T) {
+  const int ni = rounds(min(end, a.Lk) - kt * T);
+  Part<E, DP> nq, ng;
+  nq.fetch((const E*)a.k + b * a.k_sb + hk * a.k_sh, a.k_sl, kt * T, end, a.D, a.vec);
+  ng.fetch((const E*)a.v + b * a.v_sb + hk * a.v_sh, a.v_sl, kt * T, end, a.D, a.vec);
+  nq.store(K, ok);
+  ng.store(V, ok);
+  const int n_qt = (a.Lq + T - 1) / T, steps = kt * T < end ? a.group * n_qt : 0;         // a tile behind the sample's length has gradients of zero
+  auto fetch = [&](int i) {
+    const int h = hk * a.group + i / n_qt, q0 = i % n_qt * T;
+    nq.fetch((const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, q0, a.Lq, a.D, a.vec);
+    ng.fetch((const E*)a.dy + b * a.g_sb + h * a.g_sh, a.g_sl, q0, a.Lq, a.D, a.vec);
+  };
+  if (steps) fetch(0);
+  for (int i0 = 0; i0 < steps; ++i0) {
+      const int h = hk * a.group + i0 / n_qt, q0 = i0 % n_qt * T, nj = rounds(a.Lq - q0);
       __syncthreads();
-      load_tile<E, DP>(Q, (const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, q0, a.Lq, a.D);
-      load_tile<E, DP>(G, (const E*)a.dy + b * a.g_sb + h * a.g_sh, a.g_sl, q0, a.Lq, a.D);
+      nq.store(Q);
+      ng.store(G);
       __syncthreads();
+      if (i0 + 1 < steps) fetch(i0 + 1);
       float s[4][4], dp[4][4];
-      dot_tile<DP>(K, Q, s);
-      dot_tile<DP>(V, G, dp);
+      dot_tile<DP>(K, Q, s, ni, nj);
+      dot_tile<DP>(V, G, dp, ni, nj);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = q0 + tx + 16 * j;
@@ -279,8 +363,8 @@ __global__ void __launch_bounds__(THREADS) attn_dkv_kernel(const AttnArgs a) {
         }
       }
       __syncthreads();
-      mix_tile<DP>(P, G, dv);
-      mix_tile<DP>(S, Q, dk);
+      mix_tile<DP>(P, G, dv, ni, nj);
+      mix_tile<DP>(S, Q, dk, ni, nj);
     }
   // a masked key's weights are zeros, but zero times a query that is not a number is none: its gradients are set to zero
 #pragma unroll
@@ -327,18 +411,25 @@ bool shape_ok(int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int
   return true;
 }
 
-AttnArgs arguments(const void* q, const void* k, const void* v, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* s, const int32_t* lengths,
+AttnArgs arguments(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* s, const int32_t* lengths,
                    const uint8_t* mask, float scale) {
   AttnArgs a = {};
   a.q = q; a.k = k; a.v = v; a.lengths = lengths; a.mask = mask;
   a.q_sb = s[0]; a.q_sl = s[1]; a.q_sh = s[2]; a.k_sb = s[3]; a.k_sl = s[4]; a.k_sh = s[5]; a.v_sb = s[6]; a.v_sl = s[7]; a.v_sh = s[8];
   a.B = B; a.Lq = Lq; a.Lk = Lk; a.H = H; a.Hkv = Hkv; a.D = D; a.group = H / Hkv;
+  const int size = (int)fovi::dtype_size(dtype);
+  auto whole = [&](const void* p, const int64_t* s) {
+    return !((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(s[0] * size) | (uintptr_t)(s[1] * size) | (uintptr_t)(s[2] * size)) & 15u);
+  };
+  a.vec = D * size % 16 == 0 && whole(q, s) && whole(k, s + 3) && whole(v, s + 6);
   a.scale = scale; a.scale_log2 = scale * 1.44269504088896340736f;
   return a;
 }
-void gradients(AttnArgs& a, const void* o, const void* dy, const int64_t* s, const float* lse, void* dq, void* dk, void* dv, void* work) {
+void gradients(AttnArgs& a, int dtype, const void* o, const void* dy, const int64_t* s, const float* lse, void* dq, void* dk, void* dv, void* work) {
   a.o = o; a.dy = dy; a.lse = const_cast<float*>(lse); a.dq = dq; a.dk = a.Lk > 0 ? dk : nullptr; a.dv = dv; a.delta = static_cast<float*>(work);
   a.g_sb = s[9]; a.g_sl = s[10]; a.g_sh = s[11];
+  const int size = (int)fovi::dtype_size(dtype);
+  a.vec = a.vec && !((reinterpret_cast<uintptr_t>(dy) | (uintptr_t)(s[9] * size) | (uintptr_t)(s[10] * size) | (uintptr_t)(s[11] * size)) & 15u);
 }
 
 }  // namespace
@@ -359,7 +450,7 @@ extern "C" int fovi_attention_forward(const void* q, const void* k, const void* 
   if (!q || !o || (Lk > 0 && (!k || !v))) return FOVI_ERR_INVALID_ARGUMENT;
   const int64_t need = fovi_attention_workspace_bytes(dtype, B, Lq, Lk, H, Hkv, D, 0);
   if (need > 0 && (!work || work_bytes < need)) return FOVI_ERR_INVALID_ARGUMENT;
-  AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
+  AttnArgs a = arguments(q, k, v, dtype, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
   a.out = o; a.lse = lse;
   auto st = reinterpret_cast<cudaStream_t>(stream);
   if (fovi::attention_tc_takes(a, dtype, false)) return fovi::launch_attention_tc_forward(a, need > 0 ? work : nullptr, st, false);
@@ -384,8 +475,8 @@ extern "C" int fovi_attention_backward(const void* q, const void* k, const void*
   if (!q || !o || !dy || !lse || (Lk > 0 && (!k || !v))) return FOVI_ERR_INVALID_ARGUMENT;
   const int64_t need = fovi_attention_workspace_bytes(dtype, B, Lq, Lk, H, Hkv, D, 1);
   if (need > 0 && (!work || work_bytes < need)) return FOVI_ERR_INVALID_ARGUMENT;
-  AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
-  gradients(a, o, dy, strides, lse, dq, dk, dv, work);
+  AttnArgs a = arguments(q, k, v, dtype, B, Lq, Lk, H, Hkv, D, strides, key_lengths, key_mask, scale);
+  gradients(a, dtype, o, dy, strides, lse, dq, dk, dv, work);
   if (fovi::attention_tc_takes(a, dtype, true)) return fovi::launch_attention_tc_backward(a, work, st, false);
   if (dtype == FOVI_BF16) return D <= 64 ? backward<__nv_bfloat16, 64>(a, st) : backward<__nv_bfloat16, 128>(a, st);
   return D <= 64 ? backward<float, 64>(a, st) : backward<float, 128>(a, st);
@@ -396,7 +487,7 @@ extern "C" int fovi_attention_check(void* stream) { return fovi::attention_tc_ch
 extern "C" int fovi_attention_forward_selftest_wait_timeout(const void* q, const void* k, const void* v, int B, int Lq, int Lk, int H, int Hkv, int D,
                                                             const int64_t* strides, float scale, void* o, void* stream) {
   if (!shape_ok(FOVI_BF16, B, Lq, Lk, H, Hkv, D, strides, 9) || !q || !k || !v || !o || (int64_t)B * Lq * Lk == 0) return FOVI_ERR_INVALID_ARGUMENT;
-  AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, nullptr, nullptr, scale);
+  AttnArgs a = arguments(q, k, v, FOVI_BF16, B, Lq, Lk, H, Hkv, D, strides, nullptr, nullptr, scale);
   a.out = o;
   if (!fovi::attention_tc_takes(a, FOVI_BF16, false)) return FOVI_ERR_UNSUPPORTED;
   return fovi::launch_attention_tc_forward(a, nullptr, reinterpret_cast<cudaStream_t>(stream), true);
@@ -408,8 +499,8 @@ extern "C" int fovi_attention_backward_selftest_wait_timeout(const void* q, cons
   if (!shape_ok(FOVI_BF16, B, Lq, Lk, H, Hkv, D, strides, 12) || !q || !k || !v || !o || !dy || !lse || !dk != !dv || (int64_t)B * Lq * Lk == 0 || !work ||
       work_bytes < fovi_attention_workspace_bytes(FOVI_BF16, B, Lq, Lk, H, Hkv, D, 1))
     return FOVI_ERR_INVALID_ARGUMENT;
-  AttnArgs a = arguments(q, k, v, B, Lq, Lk, H, Hkv, D, strides, nullptr, nullptr, scale);
-  gradients(a, o, dy, strides, lse, dq, dk, dv, work);
+  AttnArgs a = arguments(q, k, v, FOVI_BF16, B, Lq, Lk, H, Hkv, D, strides, nullptr, nullptr, scale);
+  gradients(a, FOVI_BF16, o, dy, strides, lse, dq, dk, dv, work);
   if (!fovi::attention_tc_takes(a, FOVI_BF16, true)) return FOVI_ERR_UNSUPPORTED;
   return fovi::launch_attention_tc_backward(a, work, reinterpret_cast<cudaStream_t>(stream), true);
 }

@@ -17,7 +17,7 @@ struct AttnArgs {
   const int32_t* lengths;                   // [B] or null: keys at and behind lengths[b] are masked
   const uint8_t* mask;                      // [B, Lk] or null: keys whose byte is 0 are masked
   int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, g_sb, g_sl, g_sh;
-  int B, Lq, Lk, H, Hkv, D, group;
+  int B, Lq, Lk, H, Hkv, D, group, vec;     // vec: rows of whole 16-byte pieces on 16-byte boundaries
   float scale, scale_log2;                  // scale_log2 = scale * log2(e): the softmax is taken in base 2
 };
 
