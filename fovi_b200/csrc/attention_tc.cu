@@ -7,7 +7,10 @@
 // A fifth warp issues the tensor copies and both products.  S is given back as soon as its row is in registers, so the next tile's scores are computed while this one's exponentials
 // are.  What bounds it are the exponentials (16 a clock and SM: 512 clocks a tile) and, as long as a warp's tile takes 1400 clocks in all (barriers, tensor memory and the
 // maximum the rest), how many warps a scheduler has to choose from: three, with 128 registers each.  (A block's registers are given out evenly over the four schedulers: with two
-// issuing warps, six in all, a third block would leave a thread 96.)
+// issuing warps, six in all, a third block would leave a thread 96.)  One exponential of eight is worked out on the multiply-add units (243 -> 230 us at 257 queries over 1028 keys,
+// 256 x 6 heads; one of four: 233).  Measured: 256 queries over 4096 keys, 4 x 111 heads of 64 channels: 167 us, 712 TFLOP/s, 65 % of the exponential unit's rate; 4 x 74 heads of 128
+// channels: 182 us, 874 TFLOP/s; one query over 2056 keys, 64 x 20 heads: 110 us, 6.1 TB/s.
+// Few row tiles: their keys are cut into parts, one block each, joined by a second kernel (see splits_of).
 // The reference value m of a row only moves when its maximum has risen
 // by more than 8 (in base 2): P then stays below 2^8, bf16's relative rounding is the same at any size, and the pass over O that a move costs is rare.
 // Masked keys: their scores are -inf by a select and their rows of V are set to zero in shared memory, so what they hold has no effect.  A warp whose
@@ -25,6 +28,17 @@ namespace {
 __device__ int g_status;           // wait site at which a kernel gave up, see fovi_attention_check: one word per device
 constexpr int AT_THREADS = 160;
 constexpr float AT_INF = __builtin_huge_valf();
+
+// 2^x of two numbers x <= 8 on the multiply-add units: x = n + f with n whole and |f| <= 1/2 (Cody and Waite's reduction; n by adding 1.5 * 2^23), 2^f by a polynomial of degree 3 fitted
+// with Remez' exchange (relative error 7.5e-5, a fiftieth of bf16's rounding), times 2^n.  Below -126 it stays 2^-126; not a number stays that.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+  asm("max.NaN.f32 %0, %0, %2;\n max.NaN.f32 %1, %1, %2;" : "+f"(x.x), "+f"(x.y) : "f"(-126.f));
+  const float2 t = add2(x, both(12582912.f)), f = fma2(add2(t, both(-12582912.f)), both(-1.f), x);
+  float2 p = fma2(both(0.0551716685295105f), f, both(0.2426111251115799f));
+  p = fma2(p, f, both(0.6932609677314758f));
+  p = fma2(p, f, both(0.9999280571937561f));
+  return mul2(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
+}
 
 constexpr int KT = 64;             // keys of a tile
 
@@ -224,7 +238,7 @@ attn_tc_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll
           for (int i = p; i < p + 32; i += 2) {
             const float2 e = fma2(make_float2(x[i], x[i + 1]), make_float2(c, c), make_float2(-mc, -mc));
-            const float2 y = make_float2(ex2(e.x), ex2(e.y));
+            const float2 y = i / 2 % 8 == 3 ? ex2_fma(e) : make_float2(ex2(e.x), ex2(e.y));      // one pair of eight beside the exponential unit
             l[i / 2 % 4] = add2(l[i / 2 % 4], y);
             w[(i - p) >> 1] = pack_bf16(y.x, y.y);
           }
