@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
     const int64_t at = ((int64_t)b * a.H + h) * a.Lq + r;
     lse[i] = r < a.Lq ? __ldg(a.lse + at) : INF;
     delta[i] = r < a.Lq ? a.delta[at] : 0.f;
-    f[i] = a.scale;
+    f[i] = end == 1 ? 0.f : a.scale;       // one key: its weight is one whatever its score
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(THREADS) attn_dkv_kernel(const AttnArgs a) {
   float dk[4][DP / 16], dv[4][DP / 16], f[4], one[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f[i] = a.scale; one[i] = 1.f;
+    f[i] = end == 1 ? 0.f : a.scale; one[i] = 1.f;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
   }

@@ -5,8 +5,10 @@
 // (the keys; the queries of all heads that read the state head).  Per tile
 //   S = R1 C1^T, dP = R2 C2^T          SS MMAs, M = 128, N = CT, into tensor memory; for dk and dv these are the transposed scores, rows = keys
 //   P, dS                              eight warps, a thread per row and half the columns: registers, then back to tensor memory as bf16
-//   acc1 += dS C1 (dq, dk),  acc2 += P C2 (dv)          TS MMAs, the column tiles read MN-major: nothing is transposed, nothing goes through shared memory
-// Each gradient is summed by one CTA in a fixed order: no atomics, the same bits every time, no float32 buffer of dq, for 7 products instead of 5.
+//   acc1 += dS C1 (dq, dk),  acc2 += P C2 (dv; P C1 for dq)          TS MMAs, the column tiles read MN-major: nothing is transposed, nothing goes through shared memory
+// Each gradient is summed by one CTA in a fixed order: no atomics, the same bits every time, no float32 buffer of dq, for 8 products instead of 5.
+// The eighth, sum p k, is for delta: taken from the rounded result it is off by some 0.2 % of a dp's size, the same for all of a row's keys, which where a row's weight lies on few keys
+// was a tenth to a fifth of dq's and dk's whole error.  The row's sum of ds says how far it is off.
 // One CTA per SM with all 512 columns of tensor memory, over many row tiles (persistent).  Beside the eight warps one issues the scores, one the products, one the copies in and one the
 // copies out: a single MMA warp spent 2000 clocks a tile on its barriers and on issuing, one after the other, where the tensor cores have 800 to 1100 of work.  The next tile's scores are
 // computed while this one's elements are worked on, and the next row tile's operands arrive meanwhile.  Results go through the row tile's own operand buffers, which the scores are done
@@ -37,7 +39,7 @@ template <int DC> struct Grad {
 };
 
 struct GradHeader {
-  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_full, acc_free, staged, drain;
+  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_full, acc_free, summed, staged, drain;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -45,6 +47,7 @@ struct GradHeader {
 struct GradArgs {
   AttnTcArgs t;
   const float *nl, *nd;        // [B, H, pitch]: -lse and -delta, -inf and 0 behind the last query
+  float* nd_out;               // dq: -delta without its error
   int pitch, items, tiles;     // tiles: row tiles of a head
 };
 
@@ -114,7 +117,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&hdr->full[i]), 1); mbar_init(smem_u32(&hdr->empty[i]), 1); }
     mbar_init(smem_u32(&hdr->s_full), 1); mbar_init(smem_u32(&hdr->s_free), EW_WARPS); mbar_init(smem_u32(&hdr->p_full), EW_WARPS);
     mbar_init(smem_u32(&hdr->mixed), 1); mbar_init(smem_u32(&hdr->acc_full), 1); mbar_init(smem_u32(&hdr->acc_free), EW_WARPS);
-    mbar_init(smem_u32(&hdr->staged), EW_WARPS); mbar_init(smem_u32(&hdr->drain), 1);
+    mbar_init(smem_u32(&hdr->summed), EW_WARPS); mbar_init(smem_u32(&hdr->staged), EW_WARPS); mbar_init(smem_u32(&hdr->drain), 1);
     hdr->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -212,7 +215,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const bool more = warp_uniform(w.j) > 0;
 #pragma unroll
       for (int q = 0; q < CT / 64; ++q) {         // 64 columns at a time
-        if (KEYS) mma_mix(u_tmem + G::ACC2, u_tmem + G::P + q * 32, tile + G::CTILE + q * 8192, G::CBOX, steps - 4 * q, id_acc, more || q);
+        mma_mix(u_tmem + G::ACC2, u_tmem + G::P + q * 32, tile + (KEYS ? G::CTILE : 0u) + q * 8192, G::CBOX, steps - 4 * q, id_acc, more || q);
         mma_mix(u_tmem + G::ACC1, u_tmem + G::DS + q * 32, tile + q * 8192, G::CBOX, steps - 4 * q, id_acc, more || q);
       }
       if (elect_one()) {
@@ -264,6 +267,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int64_t at = ((int64_t)it.b * a.H + it.h) * g.pitch + row;
         nl = __ldg(g.nl + at); nd = __ldg(g.nd + at);
       }
+      float2 rest[2] = {};                   // dq: the sum of the row's ds, of this thread's columns
       for (int j = 0; j < it.n; ++j, ++n) {
         int c0, h;
         const int cols = columns<DC, KEYS>(a, it, j, c0, h);
@@ -279,7 +283,6 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         if (ok && KEYS) ok = at_wait(smem_u32(&hdr->full[slot]), sphase, abort_flag, status, 29, t.wait_limit);     // (done: the scores needed it too)
         if (!ok) break;
         tc_fence_after();
-        uint32_t pw[HALF / 2], dw[HALF / 2];
         const float* st = reinterpret_cast<const float*>(smem_raw + (sstat - raw) + slot * 2 * CT * 4) + first;
 #pragma unroll
         for (int e = 0; e < HALF; e += 32) {          // 32 columns at a time: all of them at once would not fit the registers
@@ -297,51 +300,45 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&hdr->s_free));
           }
-          if (!work) continue;
+          uint32_t pw[16], dw[16];
+          if (work) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            float4 l4, d4;
-            if (KEYS) {
-              l4 = *reinterpret_cast<const float4*>(st + e + k);
-              d4 = *reinterpret_cast<const float4*>(st + CT + e + k);
-            } else {
-              l4 = make_float4(nl, nl, nl, nl); d4 = make_float4(nd, nd, nd, nd);
-            }
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const int x = k + 2 * z;
-              const float2 ex = fma2(make_float2(s[x], s[x + 1]), make_float2(c, c), z ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y));
-              const float2 p = make_float2(ex2(ex.x), ex2(ex.y));
-              float2 ds = mul2(p, add2(make_float2(d[x], d[x + 1]), z ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y)));
-              if (!KEYS && !whole) {
-                ds.x = bits[e >> 5] >> x & 1u ? ds.x : 0.f;
-                ds.y = bits[e >> 5] >> (x + 1) & 1u ? ds.y : 0.f;
+            for (int k = 0; k < 32; k += 4) {
+              float4 l4, d4;
+              if (KEYS) {
+                l4 = *reinterpret_cast<const float4*>(st + e + k);
+                d4 = *reinterpret_cast<const float4*>(st + CT + e + k);
+              } else {
+                l4 = make_float4(nl, nl, nl, nl); d4 = make_float4(nd, nd, nd, nd);
               }
-              if (KEYS) pw[(e + x) >> 1] = pack_bf16(p.x, p.y);
-              dw[(e + x) >> 1] = pack_bf16(ds.x, ds.y);
-            }
-          }
-        }
-        if (KEYS && !row_ok) {
 #pragma unroll
-          for (int e = 0; e < HALF / 2; ++e) pw[e] = dw[e] = 0u;
-        }
-        if (n > 0) {          // the previous P and dS have been read
-          ok = at_wait(smem_u32(&hdr->mixed), (n - 1) & 1, abort_flag, status, 30, t.wait_limit);
-          if (!ok) break;
-          tc_fence_after();
-        }
-        if (!idle) {
-          if (first < cols) {
-            if constexpr (HALF == 64) {
-              if (KEYS) tc_st32(lanes + G::P + first / 2, pw);
-              tc_st32(lanes + G::DS + first / 2, dw);
-            } else {
-              if (KEYS) tc_st16(lanes + G::P + first / 2, pw);
-              tc_st16(lanes + G::DS + first / 2, dw);
+              for (int z = 0; z < 2; ++z) {
+                const int x = k + 2 * z;
+                const float2 ex = fma2(make_float2(s[x], s[x + 1]), make_float2(c, c), z ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y));
+                float2 p = make_float2(ex2(ex.x), ex2(ex.y));
+                float2 ds = mul2(p, add2(make_float2(d[x], d[x + 1]), z ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y)));
+                if (!KEYS && !whole) {
+                  const bool in0 = bits[e >> 5] >> x & 1u, in1 = bits[e >> 5] >> (x + 1) & 1u;
+                  p.x = in0 ? p.x : 0.f; p.y = in1 ? p.y : 0.f;
+                  ds.x = in0 ? ds.x : 0.f; ds.y = in1 ? ds.y : 0.f;
+                }
+                if (!KEYS) rest[z] = add2(rest[z], ds);
+                pw[x >> 1] = KEYS && !row_ok ? 0u : pack_bf16(p.x, p.y);
+                dw[x >> 1] = KEYS && !row_ok ? 0u : pack_bf16(ds.x, ds.y);
+              }
             }
           }
+          if (e == 0 && n > 0) {          // the previous P and dS have been read
+            ok = at_wait(smem_u32(&hdr->mixed), (n - 1) & 1, abort_flag, status, 30, t.wait_limit);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          if (work) {
+            tc_st16(lanes + G::P + (first + e) / 2, pw);
+            tc_st16(lanes + G::DS + (first + e) / 2, dw);
+          }
         }
+        if (!ok) break;
         if (!KEYS && !whole) {          // rows of K that must not be read; the scores are done with the tile
           const int k = lane + 32 * (warp & 3);         // four warps share the half's keys
           if (k < HALF) {
@@ -383,19 +380,39 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       if (!ok) break;
       tc_fence_after();
       const uint32_t from = KEYS ? (half ? G::ACC2 : G::ACC1) : G::ACC1 + half * SPAN;
-      const float f = KEYS && half ? 1.f : a.scale;
+      float corr = 0.f;
+      if (!KEYS) {
+        // Over a row ds sums to zero.  What it sums to is the error of delta, which comes from a result that was rounded, with weights that were rounded: it is taken out, times sum p k, here,
+        // and out of delta itself for dk and dv.  The row's two threads join their columns' sums (in the room of the statistics, which this kernel has none of).
+        float* joined = reinterpret_cast<float*>(smem_raw + (sstat - raw));
+        static_assert(2 * AT_M <= G::NS * 2 * CT, "room for the sums");
+        joined[half * AT_M + r] = (rest[0].x + rest[0].y) + (rest[1].x + rest[1].y);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&hdr->summed));
+        ok = at_wait(smem_u32(&hdr->summed), seq & 1, abort_flag, status, 34, t.wait_limit);
+        if (!ok) break;
+        corr = joined[r] + joined[AT_M + r];
+        if (half == 0 && row < a.Lq) g.nd_out[((int64_t)it.b * a.H + it.h) * g.pitch + row] = nd - corr;
+      }
+      const float f = KEYS && half ? 1.f : it.end == 1 ? 0.f : a.scale;      // one key: its weight is one whatever its score
       unsigned char* stage = smem_raw + (srow - raw) + (seq & 1) * 2 * G::RTILE + (KEYS ? half * G::RTILE : 0) + r * 128;
       const bool zero = KEYS && !row_ok;
 #pragma unroll 1
       for (int e = 0; e < SPAN; e += 32) {
-        float v[32];
+        float v[32], m[KEYS ? 1 : 32];
         tc_ld32(lanes + from + e, reinterpret_cast<uint32_t*>(v));
+        if (!KEYS) tc_ld32(lanes + from + e + (G::ACC2 - G::ACC1), reinterpret_cast<uint32_t*>(m));
         tc_ld_wait();
         tc_loaded<32>(reinterpret_cast<uint32_t*>(v));
+        if (!KEYS) tc_loaded<KEYS ? 0 : 32>(reinterpret_cast<uint32_t*>(m));
         if (e + 32 == SPAN) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&hdr->acc_free));
+        }
+        if (!KEYS) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = fmaf(-corr, m[KEYS ? 0 : k], v[k]);
         }
         const int ch = ch0 + e;
 #pragma unroll
@@ -488,11 +505,11 @@ int fovi::launch_attention_tc_backward(const AttnArgs& a, void* work, cudaStream
   const int64_t rows = (int64_t)a.B * a.H * g.pitch, blocks = (rows * (a.D <= 64 ? 8 : 16) + 255) / 256;
   if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;
   float* nl = static_cast<float*>(work);
-  g.nl = nl; g.nd = nl + rows;
+  g.nl = nl; g.nd = g.nd_out = nl + rows;
   if (a.D <= 64) attn_row_stats_kernel<8><<<(int)blocks, 256, 0, st>>>(a, nl, nl + rows, g.pitch);
   else attn_row_stats_kernel<16><<<(int)blocks, 256, 0, st>>>(a, nl, nl + rows, g.pitch);
   rc = after_launch("attn_row_stats_kernel");
-  if (!rc && a.dk) rc = a.D <= 64 ? launch<1, true>(a, g, st) : launch<2, true>(a, g, st);
   if (!rc && a.dq) rc = a.D <= 64 ? launch<1, false>(a, g, st) : launch<2, false>(a, g, st);
+  if (!rc && a.dk) rc = a.D <= 64 ? launch<1, true>(a, g, st) : launch<2, true>(a, g, st);      // behind dq: it has mended delta
   return rc;
 }

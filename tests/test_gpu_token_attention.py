@@ -164,6 +164,29 @@ def test_rising_scores(dtype):
 
 
 @pytest.mark.autograd
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Lk", [1, 90])
+def test_one_key_has_weight_one(Lk, D, dtype):
+    """Its gradients with respect to the score's sides are zeros, not what roundings leave of them."""
+    q, k, v, dy = _inputs(3, 70, Lk, 2, 2, D, dtype, 8)
+    o, gq, gk, gv = _check(q, k, v, dy, key_lengths=torch.ones(3, dtype=torch.int32, device="cuda"))
+    assert torch.equal(o, v[:, :1].expand_as(o)) and not gq.any() and not gk.any() and not gv[:, 1:].any()
+
+
+@pytest.mark.autograd
+def test_delta_of_few_keys():
+    """bf16: where a row's weight lies on a key or two, the rounding of the result is not to be seen in dq and dk: their error is that of two roundings to bf16 of independent values, as where
+    it lies on many.  (2^-9 / sqrt(3) of the value at most, each, in the root mean square; 1.1 for what is not rounded there.)"""
+    from fovi_b200 import ops
+    for Lk in (2, 3, 6, 40):
+        q, k, v, dy = _inputs(4, 200, Lk, 4, 4, 64, BF, Lk)
+        o, lse = ops.attention(q, k, v, want_lse=True)
+        for got, (want, _) in zip(ops.attention_backward(q, k, v, o, dy, lse)[:2], oracle.attention(q, k, v, dy=dy)[1:3]):
+            assert (got.double() - want).norm() <= 1.1 * 2 ** 0.5 * 2.0 ** -8 / 3 ** 0.5 * want.norm()
+
+
+@pytest.mark.autograd
 def test_no_keys_no_queries_no_samples():
     from fovi_b200 import tokens
     for B, Lq, Lk in ((2, 5, 0), (2, 0, 5), (0, 5, 5)):
