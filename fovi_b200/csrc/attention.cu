@@ -20,6 +20,14 @@ constexpr int THREADS = 256;
 constexpr int PP = T + 4;                // pitch of a tile of scores
 constexpr float INF = __builtin_huge_valf();
 
+// Keys of split `split`: the splits share out the sample's keys in whole tiles.
+struct Range { int first, end; };
+__device__ __forceinline__ Range keys_of(const AttnArgs& a, int end, int split, int tile) {
+  const int share = ((end + tile - 1) / tile + a.splits - 1) / a.splits * tile;
+  const int64_t first = (int64_t)split * share;
+  return {(int)min(first, (int64_t)end), (int)min(first + share, (int64_t)end)};
+}
+
 template <int DP> constexpr int PITCH = DP + 4;        // rows 4 floats apart modulo 32 banks: eight threads' float4 reads of one column do not collide
 
 __device__ __forceinline__ bool key_ok(const AttnArgs& a, int b, int key, int end) {
@@ -168,16 +176,18 @@ __global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a)
   float* Q = reinterpret_cast<float*>(smem4);
   float *K = Q + T * PITCH<DP>, *V = K + T * PITCH<DP>, *P = V + T * PITCH<DP>;
   __shared__ unsigned char ok[T];
-  const int n_qt = (a.Lq + T - 1) / T, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  const int qt = blockIdx.x % n_qt, h = blockIdx.x / n_qt % a.H, b = blockIdx.x / n_qt / a.H, end = key_end(a, b);
+  const int n_qt = (a.Lq + T - 1) / T, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, split = blockIdx.x % a.splits, block = blockIdx.x / a.splits;
+  const int qt = block % n_qt, h = block / n_qt % a.H, b = block / n_qt / a.H;
+  const Range range = keys_of(a, key_end(a, b), split, T);
+  const int end = range.end;
   const E* k = (const E*)a.k + b * a.k_sb + (h / a.group) * a.k_sh;
   const E* v = (const E*)a.v + b * a.v_sb + (h / a.group) * a.v_sh;
   const int ni = rounds(a.Lq - qt * T);
   Part<E, DP> nk, nv;
   nv.fetch((const E*)a.q + b * a.q_sb + h * a.q_sh, a.q_sl, qt * T, a.Lq, a.D, a.vec);
   nv.store(Q);
-  nk.fetch(k, a.k_sl, 0, end, a.D, a.vec);
-  nv.fetch(v, a.v_sl, 0, end, a.D, a.vec);
+  nk.fetch(k, a.k_sl, range.first, end, a.D, a.vec);
+  nv.fetch(v, a.v_sl, range.first, end, a.D, a.vec);
   float m[4], l[4], acc[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -185,7 +195,7 @@ __global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a)
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
-  for (int k0 = 0; k0 < end; k0 += T) {
+  for (int k0 = range.first; k0 < end; k0 += T) {
     const int nj = rounds(end - k0);
     __syncthreads();
     if (threadIdx.x < T) ok[threadIdx.x] = key_ok(a, b, k0 + threadIdx.x, end);
@@ -229,9 +239,134 @@ __global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a)
   for (int i = 0; i < 4; ++i) {
     inv[i] = m[i] == -INF ? 0.f : 1.f / l[i];
     const int r = qt * T + ty + 16 * i;
-    if (a.lse && tx == 0 && r < a.Lq) a.lse[((int64_t)b * a.H + h) * a.Lq + r] = m[i] == -INF ? INF : m[i] + log2f(l[i]);
+    const float lse = m[i] == -INF ? INF : m[i] + log2f(l[i]);
+    if (tx == 0 && r < a.Lq) {
+      if (a.splits > 1) a.part_lse[(((int64_t)split * a.B + b) * a.Lq + r) * a.H + h] = lse;
+      else if (a.lse) a.lse[((int64_t)b * a.H + h) * a.Lq + r] = lse;
+    }
   }
-  store_tile<E, DP>((E*)a.out + ((int64_t)b * a.Lq * a.H + h) * a.D, (int64_t)a.H * a.D, qt * T, a.Lq, a.D, acc, inv);
+  const int64_t at = ((int64_t)b * a.Lq * a.H + h) * a.D, pitch = (int64_t)a.H * a.D;
+  if (a.splits > 1) store_tile<float, DP>(a.part_o + (int64_t)split * a.B * a.Lq * pitch + at, pitch, qt * T, a.Lq, a.D, acc, inv);
+  else store_tile<E, DP>((E*)a.out + at, pitch, qt * T, a.Lq, a.D, acc, inv);
+}
+
+// A block per query (few of them: a tile would stand nearly empty): DP / 4 lanes hold a key's channels, four each, and take every 8th (4th above 64 channels) key of the block's, four at a
+// time so that their loads are on the way together.  Memory bounds it: keys and values are read once per query, of the same sample and head one after another.
+constexpr int FEW = 8, FEW_THREADS = 128, FEW_KEYS = 4;
+
+template <typename E>
+__device__ __forceinline__ float4 load4(const E* p, int c, int D, bool vec) {
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (vec && c < D) {
+    if constexpr (sizeof(E) == 4) {
+      return __ldg(reinterpret_cast<const float4*>(p + c));
+    } else {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(p + c));
+      return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < D) x[e] = ld_as_float(p + c + e);
+  return make_float4(x[0], x[1], x[2], x[3]);
+}
+
+template <typename E, int DP>
+__global__ void __launch_bounds__(FEW_THREADS) attn_few_kernel(const AttnArgs a) {
+  constexpr int LANES = DP / 4, GROUPS = FEW_THREADS / LANES;
+  __shared__ float part[GROUPS][DP + 2];
+  const int split = blockIdx.x % a.splits, block = blockIdx.x / a.splits;
+  const int q = block % a.Lq, h = block / a.Lq % a.H, b = block / a.Lq / a.H, group = threadIdx.x / LANES, c = threadIdx.x % LANES * 4;
+  const Range range = keys_of(a, key_end(a, b), split, FEW_KEYS * GROUPS);
+  const E* k = (const E*)a.k + b * a.k_sb + (h / a.group) * a.k_sh;
+  const E* v = (const E*)a.v + b * a.v_sb + (h / a.group) * a.v_sh;
+  const float4 x = load4((const E*)a.q + b * a.q_sb + (int64_t)q * a.q_sl + h * a.q_sh, c, a.D, a.vec);
+  float m = -INF, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = range.first + group; k0 - group < range.end; k0 += FEW_KEYS * GROUPS) {       // (all lanes of a warp the same number of times)
+    float s[FEW_KEYS];
+    float4 y[FEW_KEYS], z[FEW_KEYS];
+    bool in[FEW_KEYS];
+#pragma unroll
+    for (int u = 0; u < FEW_KEYS; ++u) {
+      const int key = k0 + u * GROUPS;
+      in[u] = key_ok(a, b, key, range.end);
+      y[u] = z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in[u]) {
+        y[u] = load4(k + (int64_t)key * a.k_sl, c, a.D, a.vec);
+        z[u] = load4(v + (int64_t)key * a.v_sl, c, a.D, a.vec);
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < FEW_KEYS; ++u) {
+      s[u] = fmaf(x.w, y[u].w, fmaf(x.z, y[u].z, fmaf(x.y, y[u].y, x.x * y[u].x)));
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], o);
+      s[u] = in[u] ? s[u] * a.scale_log2 : -INF;
+      top = fmaxf(top, s[u]);
+    }
+    const float base = top == -INF ? 0.f : top, f = exp2f(m - base);
+    m = top;
+    l *= f;
+    acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll
+    for (int u = 0; u < FEW_KEYS; ++u) {
+      const float p = exp2f(s[u] - base);
+      l += p;
+      acc.x = fmaf(p, z[u].x, acc.x); acc.y = fmaf(p, z[u].y, acc.y); acc.z = fmaf(p, z[u].z, acc.z); acc.w = fmaf(p, z[u].w, acc.w);
+    }
+  }
+  *reinterpret_cast<float2*>(&part[group][c]) = make_float2(acc.x, acc.y);
+  *reinterpret_cast<float2*>(&part[group][c + 2]) = make_float2(acc.z, acc.w);
+  if (c == 0) { part[group][DP] = m; part[group][DP + 1] = l; }
+  __syncthreads();
+  if (threadIdx.x >= a.D) return;
+  float top = -INF, sum = 0.f, o = 0.f;
+  for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, part[g][DP]);
+  const float base = top == -INF ? 0.f : top;
+  for (int g = 0; g < GROUPS; ++g) {
+    const float f = exp2f(part[g][DP] - base);
+    sum = fmaf(f, part[g][DP + 1], sum);
+    o = fmaf(f, part[g][threadIdx.x], o);
+  }
+  // (no key: the sum is zero; scores that are not a number: so is it)
+  const bool none = top == -INF && !(sum != sum);
+  const float res = none ? 0.f : o / sum, lse = none ? INF : base + log2f(sum);
+  const int64_t row = ((int64_t)b * a.Lq + q) * a.H + h, rows = (int64_t)a.B * a.Lq * a.H;
+  if (a.splits > 1) {
+    a.part_o[(split * rows + row) * a.D + threadIdx.x] = res;
+    if (threadIdx.x == 0) a.part_lse[split * rows + row] = lse;
+  } else {
+    ((E*)a.out)[row * a.D + threadIdx.x] = from_float<E>(res);
+    if (a.lse && threadIdx.x == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + q] = lse;
+  }
+}
+
+// The parts of a row over the splits of its keys, weighted with the parts' sums, added in their order.  A thread per channel.
+template <typename E>
+__global__ void __launch_bounds__(256) attn_join_parts_kernel(const AttnArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.B * a.Lq * a.H, row = i / a.D;
+  if (row >= rows) return;
+  float top = -INF, sum = 0.f, o = 0.f;                    // a part without a key has +inf in place of its logarithm
+  for (int s = 0; s < a.splits; ++s) {
+    const float v = __ldg(a.part_lse + s * rows + row);
+    top = v == INF ? top : v != v ? v : fmaxf(top, v);
+  }
+  for (int s = 0; s < a.splits; ++s) {
+    const float v = __ldg(a.part_lse + s * rows + row);
+    if (v == INF) continue;
+    const float w = exp2f(v - top);
+    o = fmaf(w, __ldg(a.part_o + s * rows * a.D + i), o);
+    sum += w;
+  }
+  const bool none = top == -INF;
+  ((E*)a.out)[i] = from_float<E>(none ? 0.f : o / sum);
+  if (a.lse && i - row * a.D == 0) {
+    const int h = (int)(row % a.H);
+    const int64_t bl = row / a.H, b = bl / a.Lq;
+    a.lse[(b * a.H + h) * a.Lq + (bl - b * a.Lq)] = none ? INF : top + log2f(sum);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
@@ -391,9 +526,37 @@ int launch(Kernel kernel, int64_t blocks, size_t smem, cudaStream_t st, const At
   return fovi::after_launch(name);
 }
 
+// Parts of a row's keys, so that the blocks fill the SMs: the number for which the rounds of blocks are shortest, each as long as its tiles and a beginning and an end of about two;
+// joining the parts is about two more.  Few queries: 16 blocks an SM, as long as a part keeps 128 keys; else two an SM (one above 64 channels).
+int splits_of(int B, int Lq, int Lk, int H, int D) {
+  const bool few = Lq <= FEW;
+  const int64_t blocks = (int64_t)B * H * (few ? Lq : (Lq + T - 1) / T), slots = (int64_t)fovi::sm_count() * (few ? 16 : D <= 64 ? 2 : 1);
+  const int tile = few ? 128 : T, tiles = (Lk + tile - 1) / tile;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= 32 && s <= tiles; ++s) {
+    const int64_t time = (blocks * s + slots - 1) / slots * ((tiles + s - 1) / s + 2) + (s > 1 ? 2 : 0);
+    if (time < least) { least = time; best = s; }
+  }
+  return best;
+}
+
 template <typename E, int DP>
-int forward(const AttnArgs& a, cudaStream_t st) {
-  return launch(attn_forward_kernel<E, DP>, (int64_t)((a.Lq + T - 1) / T) * a.H * a.B, FWD_SMEM<DP>, st, a, "attn_forward_kernel");
+int forward(AttnArgs a, void* work, cudaStream_t st) {
+  a.splits = work ? splits_of(a.B, a.Lq, a.Lk, a.H, a.D) : 1;
+  a.part_o = static_cast<float*>(work);
+  a.part_lse = a.part_o + (int64_t)a.splits * a.B * a.Lq * a.H * a.D;
+  int rc;
+  if (a.Lq <= FEW) {
+    const int64_t blocks = (int64_t)a.B * a.H * a.Lq * a.splits;
+    if (blocks > INT_MAX) return FOVI_ERR_UNSUPPORTED;
+    attn_few_kernel<E, DP><<<(int)blocks, FEW_THREADS, 0, st>>>(a);
+    rc = fovi::after_launch("attn_few_kernel");
+  } else {
+    rc = launch(attn_forward_kernel<E, DP>, (int64_t)((a.Lq + T - 1) / T) * a.H * a.B * a.splits, FWD_SMEM<DP>, st, a, "attn_forward_kernel");
+  }
+  if (rc || a.splits == 1) return rc;
+  return launch(attn_join_parts_kernel<E>, ((int64_t)a.B * a.Lq * a.H * a.D + 255) / 256, 0, st, a, "attn_join_parts_kernel");
 }
 
 template <typename E, int DP>
@@ -438,7 +601,10 @@ extern "C" int64_t fovi_attention_workspace_bytes(int dtype, int B, int Lq, int 
   const int64_t none = 0;
   if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, &none, 0)) return -1;
   if (backward) return fovi::attention_tc_backward_bytes(B, Lq, H);          // (the plain kernels need a part of it)
-  return dtype == FOVI_BF16 && D % 8 == 0 && D <= fovi::ATT_MAX_DIM && Lk > 0 ? fovi::attention_tc_forward_bytes(B, Lq, Lk, H, D) : 0;
+  if (Lk < 1 || D > fovi::ATT_MAX_DIM) return 0;
+  const int s = splits_of(B, Lq, Lk, H, D);                       // of the plain kernels, which any call may come to
+  const int64_t plain = s == 1 ? 0 : (int64_t)s * B * Lq * H * (D + 1) * 4;
+  return dtype == FOVI_BF16 && D % 8 == 0 ? std::max(plain, fovi::attention_tc_forward_bytes(B, Lq, Lk, H, D)) : plain;
 }
 
 extern "C" int fovi_attention_forward(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides,
@@ -454,8 +620,9 @@ extern "C" int fovi_attention_forward(const void* q, const void* k, const void* 
   a.out = o; a.lse = lse;
   auto st = reinterpret_cast<cudaStream_t>(stream);
   if (fovi::attention_tc_takes(a, dtype, false)) return fovi::launch_attention_tc_forward(a, need > 0 ? work : nullptr, st, false);
-  if (dtype == FOVI_BF16) return D <= 64 ? forward<__nv_bfloat16, 64>(a, st) : forward<__nv_bfloat16, 128>(a, st);
-  return D <= 64 ? forward<float, 64>(a, st) : forward<float, 128>(a, st);
+  void* room = need > 0 ? work : nullptr;
+  if (dtype == FOVI_BF16) return D <= 64 ? forward<__nv_bfloat16, 64>(a, room, st) : forward<__nv_bfloat16, 128>(a, room, st);
+  return D <= 64 ? forward<float, 64>(a, room, st) : forward<float, 128>(a, room, st);
 }
 
 extern "C" int fovi_attention_backward(const void* q, const void* k, const void* v, const void* o, const void* dy, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D,
