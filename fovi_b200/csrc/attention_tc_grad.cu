@@ -10,7 +10,12 @@
 // The eighth, sum p k, is for delta: taken from the rounded result it is off by some 0.2 % of a dp's size, the same for all of a row's keys, which where a row's weight lies on few keys
 // was a tenth to a fifth of dq's and dk's whole error.  The row's sum of ds says how far it is off.
 // One CTA per SM with all 512 columns of tensor memory, over many row tiles (persistent).  Beside the eight warps one issues the scores, one the products, one the copies in and one the
-// copies out: a single MMA warp spent 2000 clocks a tile on its barriers and on issuing, one after the other, where the tensor cores have 800 to 1100 of work.  The next tile's scores are
+// copies out: a single MMA warp spent 2000 clocks a tile on its barriers and on issuing, one after the other, where the tensor cores have 800 to 1100 of work.
+// Measured with the rows' statistics (us; 257 queries over 1028 keys, 256 x 6 heads of 64 channels; 256 over 4096, 4 x 111 heads): dq 391 and 236, dk and dv 444 and 363.  Time stamps
+// of one warp of dq at a tile of 128 x 128 (period 2000 clocks; taken before masks became a step of their own): elements 1360, waits for the scores 180 and for the last products 200,
+// stores 140; the exponential unit needs 1024 for the two warps of a scheduler.
+// A mask is applied to a whole chunk of scores in front of the arithmetic, and only where one is: selects at each p and ds cost every tile (ALU pipe 50 %, now 20; dq 405 and 243 us).
+// 16 columns at a time, the next on their way, was slower (dq 211 -> 236 us, 4 x 111 heads, an earlier form).  The next tile's scores are
 // computed while this one's elements are worked on, and the next row tile's operands arrive meanwhile.  Results go through the row tile's own operand buffers, which the scores are done
 // with, and out as tensor copies: stored from registers, 16 bytes of a row per thread, they took half the time of dk and dv (716 us with, 400 without them, 4 x 111 heads, 256 over 4096).
 // A last tile of fewer columns costs only its own (N and the steps over its columns follow).
@@ -267,6 +272,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int64_t at = ((int64_t)it.b * a.H + it.h) * g.pitch + row;
         nl = __ldg(g.nl + at); nd = __ldg(g.nd + at);
       }
+      const float none = c > 0.f ? -INFINITY : c < 0.f ? INFINITY : 0.f;      // the score whose exponential is 0
       float2 rest[2] = {};                   // dq: the sum of the row's ds, of this thread's columns
       for (int j = 0; j < it.n; ++j, ++n) {
         int c0, h;
@@ -301,6 +307,11 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if (lane == 0) mbar_arrive(smem_u32(&hdr->s_free));
           }
           uint32_t pw[16], dw[16];
+          if (work && !KEYS && !whole) {    // masked keys: p = 0 (scale 0: a finite p, which meets zeroed rows of K only) and ds = 0
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!(bits[e >> 5] >> k & 1u)) { s[k] = none; d[k] = -nd; }
+          }
           if (work) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
@@ -317,11 +328,6 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 const float2 ex = fma2(make_float2(s[x], s[x + 1]), make_float2(c, c), z ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y));
                 float2 p = make_float2(ex2(ex.x), ex2(ex.y));
                 float2 ds = mul2(p, add2(make_float2(d[x], d[x + 1]), z ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y)));
-                if (!KEYS && !whole) {
-                  const bool in0 = bits[e >> 5] >> x & 1u, in1 = bits[e >> 5] >> (x + 1) & 1u;
-                  p.x = in0 ? p.x : 0.f; p.y = in1 ? p.y : 0.f;
-                  ds.x = in0 ? ds.x : 0.f; ds.y = in1 ? ds.y : 0.f;
-                }
                 if (!KEYS) rest[z] = add2(rest[z], ds);
                 pw[x >> 1] = KEYS && !row_ok ? 0u : pack_bf16(p.x, p.y);
                 dw[x >> 1] = KEYS && !row_ok ? 0u : pack_bf16(ds.x, ds.y);

@@ -154,6 +154,25 @@ def test_scales(scale, dtype):
 
 @pytest.mark.autograd
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale", [0.0, -0.3, -4.0])
+def test_scales_with_masks(scale, dtype):
+    """A masked score has to lose whatever the scale's sign, and without a scale; what the masked states hold stays out."""
+    q, k, v, dy = _inputs(3, 66, 290, 2, 1, 64, dtype, 23)
+    mask = torch.rand(3, 290, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda") < 0.6
+    mask[1] = False
+    kw = dict(key_mask=mask, key_lengths=torch.tensor([290, 290, 129], dtype=torch.int32, device="cuda"), scale=scale)
+    want = _check(q, k, v, dy, **kw)
+    from fovi_b200 import tokens
+    gone = ~mask | (torch.arange(290, device="cuda") >= kw["key_lengths"][:, None])
+    k, v = (t.masked_fill(gone[:, :, None, None], float("nan")).requires_grad_(True) for t in (k, v))
+    q = q.requires_grad_(True)
+    o = tokens.cross_attention(q, k, v, **kw)
+    for g, w in zip((o,) + torch.autograd.grad(o, (q, k, v), dy), want):
+        assert torch.equal(g, w)
+
+
+@pytest.mark.autograd
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_rising_scores(dtype):
     """Keys whose scores rise by hundreds from tile to tile, so that the running maximum moves in every one; and fall."""
     q, k, v, dy = _inputs(1, 40, 700, 1, 1, 64, dtype, 3)
