@@ -3,6 +3,8 @@
 //   s = scale * q k^T (masked keys: -inf),  p = softmax(s),  o = p v;  a row without a key gives 0
 //   delta = rowsum(dy * o),  ds = p * (dy v^T - delta),  dq = scale * ds k,  dk = scale * ds^T q,  dv = p^T dy, the last two summed over the heads that
 //   share a state head
+// What bounds it are the multiply-adds and the shared-memory reads that feed them: 512 queries over 1024 keys, 8 x 20 heads of 64 channels: forward 722 us (30 TFLOP/s), dq
+// 1099 (29), dk and dv 1412 (30).  Two blocks an SM up to 64 channels, for a few spilled registers: with one block of 150 registers the forward pass took 936 us.
 // Tiles of 64 x 64 scores, 16 x 16 threads with 4 x 4 each, operands in shared memory as float32.  The forward pass goes over the keys once with the running
 // maximum and sum of every row; the backward pass recomputes p from the row's logarithm of the sum.  dq goes by query tiles and dk, dv by key tiles,
 // each by one CTA in a fixed order: no atomics, the same bits every time.  Masked keys are read as zeros, whatever they hold.
@@ -76,44 +78,45 @@ struct Part {
 // Rounds of 16 rows that `n` rows take, four at most.
 __device__ __forceinline__ int rounds(int n) { return min(4, (n + 15) / 16); }
 
-// acc[i][j] = <A row ty + 16 i, B row tx + 16 j>; of a last tile only the first ni, nj rounds of rows, zeros beyond
-template <int DP>
-__device__ __forceinline__ void dot_tile(const float* A, const float* B, float (&acc)[4][4], int ni, int nj) {
+// acc[i][j] = <A row ty + 16 i, B row tx + 16 j>, of NI and NJ rounds of rows; zeros beyond
+template <int DP, int NI, int NJ>
+__device__ __forceinline__ void dot_rounds(const float* A, const float* B, float (&acc)[4][4]) {
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  auto step = [&](int d, int i, int j, const float4& x, const float4& y) {
-    acc[i][j] = fmaf(x.x, y.x, acc[i][j]); acc[i][j] = fmaf(x.y, y.y, acc[i][j]);
-    acc[i][j] = fmaf(x.z, y.z, acc[i][j]); acc[i][j] = fmaf(x.w, y.w, acc[i][j]);
-  };
-  if (ni + nj == 8) {
 #pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
-      float4 x[4], y[4];
+  for (int d = 0; d < DP; d += 4) {
+    float4 x[NI], y[NJ];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = *reinterpret_cast<const float4*>(A + (ty + 16 * i) * PITCH<DP> + d);
-        y[i] = *reinterpret_cast<const float4*>(B + (tx + 16 * i) * PITCH<DP> + d);
+    for (int i = 0; i < NI; ++i) x[i] = *reinterpret_cast<const float4*>(A + (ty + 16 * i) * PITCH<DP> + d);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) y[j] = *reinterpret_cast<const float4*>(B + (tx + 16 * j) * PITCH<DP> + d);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]); acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]); acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) step(d, i, j, x[i], y[j]);
-    }
+  }
+}
+
+// The same of a last tile's first ni, nj rounds, each taken as one, two or four (rows behind a tile's end are zeros).  One product at a
+// time reads eight times as much shared memory a product: 23 queries over 621 keys, 17 x 12 heads of 128 channels, forward, dq, dk and dv: 198, 373, 324 us, so 146, 231, 211.
+template <int DP>
+__device__ __forceinline__ void dot_tile(const float* A, const float* B, float (&acc)[4][4], int ni, int nj) {
+  if (ni > 2) {
+    if (nj > 2) dot_rounds<DP, 4, 4>(A, B, acc);
+    else if (nj == 2) dot_rounds<DP, 4, 2>(A, B, acc);
+    else dot_rounds<DP, 4, 1>(A, B, acc);
+  } else if (ni == 2) {
+    if (nj > 2) dot_rounds<DP, 2, 4>(A, B, acc);
+    else dot_rounds<DP, 2, 2>(A, B, acc);
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i >= ni) break;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j >= nj) break;
-#pragma unroll 8
-        for (int d = 0; d < DP; d += 4)
-          step(d, i, j, *reinterpret_cast<const float4*>(A + (ty + 16 * i) * PITCH<DP> + d), *reinterpret_cast<const float4*>(B + (tx + 16 * j) * PITCH<DP> + d));
-      }
-    }
+    if (nj > 2) dot_rounds<DP, 1, 4>(A, B, acc);
+    else dot_rounds<DP, 1, 2>(A, B, acc);
   }
 }
 
@@ -171,7 +174,7 @@ __device__ __forceinline__ void store_tile(E* dst, int64_t pitch, int r0, int n,
 
 // ------------------------------------------------------------------------------------------------------------ forward: a CTA per (64 queries, head, sample)
 template <typename E, int DP>
-__global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(THREADS, DP <= 64 ? 2 : 1) attn_forward_kernel(const AttnArgs a) {
   extern __shared__ float4 smem4[];
   float* Q = reinterpret_cast<float*>(smem4);
   float *K = Q + T * PITCH<DP>, *V = K + T * PITCH<DP>, *P = V + T * PITCH<DP>;
@@ -251,7 +254,8 @@ __global__ void __launch_bounds__(THREADS) attn_forward_kernel(const AttnArgs a)
 }
 
 // A block per query (few of them: a tile would stand nearly empty): DP / 4 lanes hold a key's channels, four each, and take every 8th (4th above 64 channels) key of the block's, four at a
-// time so that their loads are on the way together.  Memory bounds it: keys and values are read once per query, of the same sample and head one after another.
+// time so that their loads are on the way together.  Memory bounds it: keys and values are read once per query, of the same sample and head one after another.  One query over 2056 keys,
+// 64 x 20 heads, float32: 202 us, 6.7 TB/s (as a tile of 64: 1056).  Eight queries over 700, 8 x 12 heads: 40 us, as much as sixteen take as a tile (39): the rule's bound.
 constexpr int FEW = 8, FEW_THREADS = 128, FEW_KEYS = 4;
 
 template <typename E>
@@ -387,13 +391,15 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
 
 // A CTA per (64 queries, head, sample): dq.
 template <typename E, int DP>
-__global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(THREADS, DP <= 64 ? 2 : 1) attn_dq_kernel(const AttnArgs a) {
   extern __shared__ float4 smem4[];
   float* Q = reinterpret_cast<float*>(smem4);
   float *G = Q + T * PITCH<DP>, *K = G + T * PITCH<DP>, *V = K + T * PITCH<DP>, *P = V + T * PITCH<DP>;
   __shared__ unsigned char ok[T];
-  const int n_qt = (a.Lq + T - 1) / T, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  const int qt = blockIdx.x % n_qt, h = blockIdx.x / n_qt % a.H, b = blockIdx.x / n_qt / a.H, end = key_end(a, b);
+  const int n_qt = (a.Lq + T - 1) / T, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, split = blockIdx.x % a.splits, block = blockIdx.x / a.splits;
+  const int qt = block % n_qt, h = block / n_qt % a.H, b = block / n_qt / a.H, keys = key_end(a, b);
+  const Range range = keys_of(a, keys, split, T);
+  const int end = range.end;
   const E* k = (const E*)a.k + b * a.k_sb + (h / a.group) * a.k_sh;
   const E* v = (const E*)a.v + b * a.v_sb + (h / a.group) * a.v_sh;
   const int ni = rounds(a.Lq - qt * T);
@@ -402,8 +408,8 @@ __global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
   nv.fetch((const E*)a.dy + b * a.g_sb + h * a.g_sh, a.g_sl, qt * T, a.Lq, a.D, a.vec);
   nk.store(Q);
   nv.store(G);
-  nk.fetch(k, a.k_sl, 0, end, a.D, a.vec);
-  nv.fetch(v, a.v_sl, 0, end, a.D, a.vec);
+  nk.fetch(k, a.k_sl, range.first, end, a.D, a.vec);
+  nv.fetch(v, a.v_sl, range.first, end, a.D, a.vec);
   float lse[4], delta[4], acc[4][DP / 16], f[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -411,11 +417,11 @@ __global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
     const int64_t at = ((int64_t)b * a.H + h) * a.Lq + r;
     lse[i] = r < a.Lq ? __ldg(a.lse + at) : INF;
     delta[i] = r < a.Lq ? a.delta[at] : 0.f;
-    f[i] = end == 1 ? 0.f : a.scale;       // one key: its weight is one whatever its score
+    f[i] = keys == 1 ? 0.f : a.scale;       // one key: its weight is one whatever its score
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
-  for (int k0 = 0; k0 < end; k0 += T) {
+  for (int k0 = range.first; k0 < end; k0 += T) {
     const int nj = rounds(end - k0);
     __syncthreads();
     if (threadIdx.x < T) ok[threadIdx.x] = key_ok(a, b, k0 + threadIdx.x, end);
@@ -440,12 +446,24 @@ __global__ void __launch_bounds__(THREADS) attn_dq_kernel(const AttnArgs a) {
     __syncthreads();
     mix_tile<DP>(P, K, acc, ni, nj);
   }
-  store_tile<E, DP>((E*)a.dq + ((int64_t)b * a.Lq * a.H + h) * a.D, (int64_t)a.H * a.D, qt * T, a.Lq, a.D, acc, f);
+  const int64_t at = ((int64_t)b * a.Lq * a.H + h) * a.D, pitch = (int64_t)a.H * a.D;
+  if (a.splits > 1) store_tile<float, DP>(a.part_o + (int64_t)split * a.B * a.Lq * pitch + at, pitch, qt * T, a.Lq, a.D, acc, f);
+  else store_tile<E, DP>((E*)a.dq + at, pitch, qt * T, a.Lq, a.D, acc, f);
+}
+
+// dq's parts over the splits of the keys, added in their order.  A thread per channel.
+template <typename E>
+__global__ void __launch_bounds__(256) attn_sum_parts_kernel(const AttnArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.B * a.Lq * a.H * a.D;
+  if (i >= n) return;
+  float sum = 0.f;
+  for (int s = 0; s < a.splits; ++s) sum += __ldg(a.part_o + s * n + i);
+  ((E*)a.dq)[i] = from_float<E>(sum);
 }
 
 // A CTA per (64 keys, state head, sample): dk and dv, over all queries of all heads that read the state head.
 template <typename E, int DP>
-__global__ void __launch_bounds__(THREADS) attn_dkv_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(THREADS, DP <= 64 ? 2 : 1) attn_dkv_kernel(const AttnArgs a) {
   extern __shared__ float4 smem4[];
   float* K = reinterpret_cast<float*>(smem4);
   float *V = K + T * PITCH<DP>, *Q = V + T * PITCH<DP>, *G = Q + T * PITCH<DP>, *P = G + T * PITCH<DP>, *S = P + T * PP;
@@ -526,10 +544,9 @@ int launch(Kernel kernel, int64_t blocks, size_t smem, cudaStream_t st, const At
   return fovi::after_launch(name);
 }
 
-// Parts of a row's keys, so that the blocks fill the SMs: the number for which the rounds of blocks are shortest, each as long as its tiles and a beginning and an end of about two;
+// Parts of a row's keys (forward, and dq; 8 queries over 3000, 2 x 16 heads: dq 258 us in one part, 71 so; 100 over 900, 4 x 8: 128 and 71), so that the blocks fill the SMs: the number for which the rounds of blocks are shortest, each as long as its tiles and a beginning and an end of about two;
 // joining the parts is about two more.  Few queries: 16 blocks an SM, as long as a part keeps 128 keys; else two an SM (one above 64 channels).
-int splits_of(int B, int Lq, int Lk, int H, int D) {
-  const bool few = Lq <= FEW;
+int splits_of(int B, int Lq, int Lk, int H, int D, bool few) {
   const int64_t blocks = (int64_t)B * H * (few ? Lq : (Lq + T - 1) / T), slots = (int64_t)fovi::sm_count() * (few ? 16 : D <= 64 ? 2 : 1);
   const int tile = few ? 128 : T, tiles = (Lk + tile - 1) / tile;
   int best = 1;
@@ -541,9 +558,13 @@ int splits_of(int B, int Lq, int Lk, int H, int D) {
   return best;
 }
 
+// The backward workspace: delta, and behind it, on a 16-byte boundary, dq's parts.  bf16 has none: here it is what the tensor cores do not take, and their workspace need not grow for it.
+int64_t delta_floats(int B, int Lq, int H) { return fovi::attention_tc_backward_bytes(B, Lq, H) / 16 * 4 + 4; }
+int dq_splits(int B, int Lq, int Lk, int H, int D, bool f32) { return f32 && Lk > 0 ? splits_of(B, Lq, Lk, H, D, false) : 1; }
+
 template <typename E, int DP>
 int forward(AttnArgs a, void* work, cudaStream_t st) {
-  a.splits = work ? splits_of(a.B, a.Lq, a.Lk, a.H, a.D) : 1;
+  a.splits = work ? splits_of(a.B, a.Lq, a.Lk, a.H, a.D, a.Lq <= FEW) : 1;
   a.part_o = static_cast<float*>(work);
   a.part_lse = a.part_o + (int64_t)a.splits * a.B * a.Lq * a.H * a.D;
   int rc;
@@ -560,9 +581,12 @@ int forward(AttnArgs a, void* work, cudaStream_t st) {
 }
 
 template <typename E, int DP>
-int backward(const AttnArgs& a, cudaStream_t st) {
+int backward(AttnArgs a, cudaStream_t st) {
+  a.splits = dq_splits(a.B, a.Lq, a.Lk, a.H, a.D, sizeof(E) == 4);
+  a.part_o = a.delta + delta_floats(a.B, a.Lq, a.H);
   int rc = launch(attn_delta_kernel<E>, ((int64_t)a.B * a.Lq * a.H + 7) / 8, 0, st, a, "attn_delta_kernel");
-  if (!rc && a.dq) rc = launch(attn_dq_kernel<E, DP>, (int64_t)((a.Lq + T - 1) / T) * a.H * a.B, DQ_SMEM<DP>, st, a, "attn_dq_kernel");
+  if (!rc && a.dq) rc = launch(attn_dq_kernel<E, DP>, (int64_t)((a.Lq + T - 1) / T) * a.H * a.B * a.splits, DQ_SMEM<DP>, st, a, "attn_dq_kernel");
+  if (!rc && a.dq && a.splits > 1) rc = launch(attn_sum_parts_kernel<E>, ((int64_t)a.B * a.Lq * a.H * a.D + 255) / 256, 0, st, a, "attn_sum_parts_kernel");
   if (!rc && a.dk) rc = launch(attn_dkv_kernel<E, DP>, (int64_t)((a.Lk + T - 1) / T) * a.Hkv * a.B, DKV_SMEM<DP>, st, a, "attn_dkv_kernel");
   return rc;
 }
@@ -600,9 +624,12 @@ void gradients(AttnArgs& a, int dtype, const void* o, const void* dy, const int6
 extern "C" int64_t fovi_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, int backward) {
   const int64_t none = 0;
   if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, &none, 0)) return -1;
-  if (backward) return fovi::attention_tc_backward_bytes(B, Lq, H);          // (the plain kernels need a part of it)
+  if (backward) {
+    const int s = D > fovi::ATT_MAX_DIM || (int64_t)B * Lq == 0 ? 1 : dq_splits(B, Lq, Lk, H, D, dtype != FOVI_BF16);
+    return s == 1 ? fovi::attention_tc_backward_bytes(B, Lq, H) : (delta_floats(B, Lq, H) + (int64_t)s * B * Lq * H * D) * 4;      // (of the first, delta is a part)
+  }
   if (Lk < 1 || D > fovi::ATT_MAX_DIM) return 0;
-  const int s = splits_of(B, Lq, Lk, H, D);                       // of the plain kernels, which any call may come to
+  const int s = splits_of(B, Lq, Lk, H, D, Lq <= FEW);                       // of the plain kernels, which any call may come to
   const int64_t plain = s == 1 ? 0 : (int64_t)s * B * Lq * H * (D + 1) * 4;
   return dtype == FOVI_BF16 && D % 8 == 0 ? std::max(plain, fovi::attention_tc_forward_bytes(B, Lq, Lk, H, D)) : plain;
 }

@@ -18,7 +18,7 @@ struct AttnArgs {
   const uint8_t* mask;                      // [B, Lk] or null: keys whose byte is 0 are masked
   int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, g_sb, g_sl, g_sh;
   int B, Lq, Lk, H, Hkv, D, group, vec;     // vec: rows of whole 16-byte pieces on 16-byte boundaries
-  int splits;                               // forward: parts of a row's keys, each to part_o [splits][B, Lq, H, D] and part_lse [splits][B, Lq, H]
+  int splits;                               // parts of a row's keys, each to part_o [splits][B, Lq, H, D] and (forward) part_lse [splits][B, Lq, H]
   float *part_o, *part_lse;
   float scale, scale_log2;                  // scale_log2 = scale * log2(e): the softmax is taken in base 2
 };
