@@ -8,7 +8,7 @@
 // are.  What bounds it are the exponentials (16 a clock and SM: 512 clocks a tile) and, as long as a warp's tile takes 1400 clocks in all (barriers, tensor memory and the
 // maximum the rest), how many warps a scheduler has to choose from: three, with 128 registers each.  (A block's registers are given out evenly over the four schedulers: with two
 // issuing warps, six in all, a third block would leave a thread 96.)  One exponential of eight is worked out on the multiply-add units (243 -> 230 us at 257 queries over 1028 keys,
-// 256 x 6 heads; one of four: 233).  Measured: 256 queries over 4096 keys, 4 x 111 heads of 64 channels: 167 us, 712 TFLOP/s, 65 % of the exponential unit's rate; 4 x 74 heads of 128
+// 256 x 6 heads; one of four: 233).  Measured: 256 queries over 4096 keys, 4 x 111 heads of 64 channels: 167 to 171 us, 700 TFLOP/s, 61 to 65 % of the exponential unit's rate; 4 x 74 heads of 128
 // channels: 182 us, 874 TFLOP/s; one query over 2056 keys, 64 x 20 heads: 110 us, 6.1 TB/s.
 // Few row tiles: their keys are cut into parts, one block each, joined by a second kernel (see splits_of).
 // The reference value m of a row only moves when its maximum has risen

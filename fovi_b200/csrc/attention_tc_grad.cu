@@ -11,15 +11,15 @@
 // was a tenth to a fifth of dq's and dk's whole error.  The row's sum of ds says how far it is off.
 // One CTA per SM with all 512 columns of tensor memory, over many row tiles (persistent).  Beside the eight warps one issues the scores, one the products, one the copies in and one the
 // copies out: a single MMA warp spent 2000 clocks a tile on its barriers and on issuing, one after the other, where the tensor cores have 800 to 1100 of work.
+// The next tile's scores are computed while this one's elements are worked on, and the next row tile's operands arrive meanwhile.  Results go through the row tile's own operand buffers, which the scores are done
+// with, and out as tensor copies: stored from registers, 16 bytes of a row per thread, they took half the time of dk and dv (716 us with, 400 without them, 4 x 111 heads, 256 over 4096).
+// A last tile of fewer columns costs only its own (N and the steps over its columns follow).
+// Rows of K whose key is masked are set to zero in shared memory in front of dS K; for dk and dv a masked key is a row, whose results are zeros by a select.
 // Measured with the rows' statistics (us; 257 queries over 1028 keys, 256 x 6 heads of 64 channels; 256 over 4096, 4 x 111 heads): dq 391 and 236, dk and dv 444 and 363.  Time stamps
 // of one warp of dq at a tile of 128 x 128 (period 2000 clocks; taken before masks became a step of their own): elements 1360, waits for the scores 180 and for the last products 200,
 // stores 140; the exponential unit needs 1024 for the two warps of a scheduler.
 // A mask is applied to a whole chunk of scores in front of the arithmetic, and only where one is: selects at each p and ds cost every tile (ALU pipe 50 %, now 20; dq 405 and 243 us).
-// 16 columns at a time, the next on their way, was slower (dq 211 -> 236 us, 4 x 111 heads, an earlier form).  The next tile's scores are
-// computed while this one's elements are worked on, and the next row tile's operands arrive meanwhile.  Results go through the row tile's own operand buffers, which the scores are done
-// with, and out as tensor copies: stored from registers, 16 bytes of a row per thread, they took half the time of dk and dv (716 us with, 400 without them, 4 x 111 heads, 256 over 4096).
-// A last tile of fewer columns costs only its own (N and the steps over its columns follow).
-// Rows of K whose key is masked are set to zero in shared memory in front of dS K; for dk and dv a masked key is a row, whose results are zeros by a select.
+// 16 columns at a time, the next on their way, was slower (dq 211 -> 236 us, 4 x 111 heads, an earlier form).
 #include <cuda_bf16.h>
 
 #include "attention_tc.cuh"
