@@ -23,10 +23,12 @@
 #include <cuda_bf16.h>
 
 #include "attention_tc.cuh"
+#include "row_turns.cuh"
 
 using fovi::AttnArgs;
 using fovi::AttnTcArgs;
 using fovi::key_end;
+using fovi::RowTurn;
 
 namespace {
 
@@ -44,7 +46,7 @@ template <int DC> struct Grad {
 };
 
 struct GradHeader {
-  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_full, acc_free, summed, staged, drain;
+  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_full, acc_free, summed, staged[2], drain;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -72,9 +74,10 @@ __device__ __forceinline__ Item item_at(const GradArgs& g, int i) {
 // (row tile, column tile) pairs in the order in which every role meets them; row tiles without columns are passed over.
 template <int DC, bool KEYS>
 struct Walk {
-  int i, j, seq;               // seq: how many row tiles with columns came before
+  int i, j;
+  RowTurn row;                 // counts the row tiles with columns
   Item it;
-  __device__ __forceinline__ explicit Walk(const GradArgs& g) : i(blockIdx.x), j(0), seq(0) { settle(g); }
+  __device__ __forceinline__ explicit Walk(const GradArgs& g) : i(blockIdx.x), j(0) { settle(g); }
   __device__ __forceinline__ void settle(const GradArgs& g) {
     for (; i < g.items; i += gridDim.x) {
       it = item_at<DC, KEYS>(g, i);
@@ -84,7 +87,10 @@ struct Walk {
   __device__ __forceinline__ bool more(const GradArgs& g) const { return i < g.items; }
   __device__ __forceinline__ void next(const GradArgs& g) {
     if (++j < it.n) return;
-    j = 0; ++seq; i += gridDim.x;
+    next_row(g);
+  }
+  __device__ __forceinline__ void next_row(const GradArgs& g) {
+    j = 0; row.next(); i += gridDim.x;
     settle(g);
   }
 };
@@ -118,11 +124,11 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->row_full[i]), 1); mbar_init(smem_u32(&hdr->row_empty[i]), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->row_full[i]), 1); mbar_init(smem_u32(&hdr->row_empty[i]), 1); mbar_init(smem_u32(&hdr->staged[i]), EW_WARPS); }
     for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&hdr->full[i]), 1); mbar_init(smem_u32(&hdr->empty[i]), 1); }
     mbar_init(smem_u32(&hdr->s_full), 1); mbar_init(smem_u32(&hdr->s_free), EW_WARPS); mbar_init(smem_u32(&hdr->p_full), EW_WARPS);
     mbar_init(smem_u32(&hdr->mixed), 1); mbar_init(smem_u32(&hdr->acc_full), 1); mbar_init(smem_u32(&hdr->acc_free), EW_WARPS);
-    mbar_init(smem_u32(&hdr->summed), EW_WARPS); mbar_init(smem_u32(&hdr->staged), EW_WARPS); mbar_init(smem_u32(&hdr->drain), 1);
+    mbar_init(smem_u32(&hdr->summed), EW_WARPS); mbar_init(smem_u32(&hdr->drain), 1);
     hdr->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -143,7 +149,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       uint32_t s = 0, sp = 0;
       for (Walk<DC, KEYS> w(g); w.more(g); w.next(g)) {
         if (w.j == 0) {
-          const uint32_t f = w.seq & 1, fp = w.seq >> 1 & 1, bar = smem_u32(&hdr->row_full[f]), dst = srow + f * 2 * G::RTILE;
+          const uint32_t f = w.row.buffer(), fp = w.row.parity(), bar = smem_u32(&hdr->row_full[f]), dst = srow + f * 2 * G::RTILE;
           if (!mbar_wait(smem_u32(&hdr->row_empty[f]), fp ^ 1u, abort_flag, status, 21, t.wait_limit)) break;
           mbar_expect_tx(bar, 2 * G::RTILE);
           for (int c = 0; c < DC; ++c) {
@@ -185,8 +191,8 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const uint32_t u_srow = warp_uniform(srow), u_scol = warp_uniform(scol), u_tmem = warp_uniform(tmem);
     uint32_t s = 0, sp = 0, n = 0;
     for (Walk<DC, KEYS> w(g); w.more(g); w.next(g), ++n) {
-      const uint32_t f = w.seq & 1;
-      if (w.j == 0 && !at_wait(smem_u32(&hdr->row_full[f]), w.seq >> 1 & 1, abort_flag, status, 23, t.wait_limit)) break;
+      const uint32_t f = w.row.buffer();
+      if (w.j == 0 && !at_wait(smem_u32(&hdr->row_full[f]), w.row.parity(), abort_flag, status, 23, t.wait_limit)) break;
       if (!at_wait(smem_u32(&hdr->full[s]), sp, abort_flag, status, 24, t.wait_limit)) break;
       if (n > 0 && !at_wait(smem_u32(&hdr->s_free), (n - 1) & 1, abort_flag, status, 25, t.wait_limit)) break;
       tc_fence_after();
@@ -211,7 +217,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     uint32_t s = 0, sp = 0, n = 0;
     for (Walk<DC, KEYS> w(g); w.more(g); w.next(g), ++n) {
       if (!at_wait(smem_u32(&hdr->full[s]), sp, abort_flag, status, 26, t.wait_limit)) break;
-      if (w.j == 0 && w.seq > 0 && !at_wait(smem_u32(&hdr->acc_free), (w.seq - 1) & 1, abort_flag, status, 27, t.wait_limit)) break;
+      if (w.j == 0 && w.row.seq > 0 && !at_wait(smem_u32(&hdr->acc_free), (w.row.seq - 1) & 1, abort_flag, status, 27, t.wait_limit)) break;
       if (!at_wait(smem_u32(&hdr->p_full), n & 1, abort_flag, status, 32, t.wait_limit)) break;
       tc_fence_after();
       int c0, h;
@@ -238,10 +244,9 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
   } else if (warp == STORES) {
     // ------------------------------------------------------------ copies out
-    for (Walk<DC, KEYS> w(g); w.more(g); w.next(g)) {
-      if (w.j) continue;
-      const uint32_t f = w.seq & 1, from = srow + f * 2 * G::RTILE;
-      if (!at_wait(smem_u32(&hdr->staged), w.seq & 1, abort_flag, status, 33, t.wait_limit)) break;
+    for (Walk<DC, KEYS> w(g); w.more(g); w.next_row(g)) {
+      const uint32_t f = w.row.buffer(), from = srow + f * 2 * G::RTILE;
+      if (!at_wait(smem_u32(&hdr->staged[f]), w.row.parity(), abort_flag, status, 33, t.wait_limit)) break;
       if (elect_one()) {
         for (int c = 0; c < DC; ++c) {
           tma_store_4d(&tm_1, from + c * G::RBOX, 64 * c, w.it.row0, w.it.h, w.it.b);
@@ -257,7 +262,8 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int r = (warp & 3) * 32 + lane, half = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c = a.scale_log2;
-    uint32_t n = 0, slot = 0, sphase = 0, seq = 0;
+    uint32_t n = 0, slot = 0, sphase = 0;
+    RowTurn turn;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < g.items; i += gridDim.x) {
       const Item it = item_at<DC, KEYS>(g, i);
@@ -382,7 +388,7 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         __syncwarp();
         continue;
       }
-      ok = at_wait(smem_u32(&hdr->acc_full), seq & 1, abort_flag, status, 31, t.wait_limit);
+      ok = at_wait(smem_u32(&hdr->acc_full), turn.seq & 1, abort_flag, status, 31, t.wait_limit);
       if (!ok) break;
       tc_fence_after();
       const uint32_t from = KEYS ? (half ? G::ACC2 : G::ACC1) : G::ACC1 + half * SPAN;
@@ -395,13 +401,13 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         joined[half * AT_M + r] = (rest[0].x + rest[0].y) + (rest[1].x + rest[1].y);
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&hdr->summed));
-        ok = at_wait(smem_u32(&hdr->summed), seq & 1, abort_flag, status, 34, t.wait_limit);
+        ok = at_wait(smem_u32(&hdr->summed), turn.seq & 1, abort_flag, status, 34, t.wait_limit);
         if (!ok) break;
         corr = joined[r] + joined[AT_M + r];
         if (half == 0 && row < a.Lq) g.nd_out[((int64_t)it.b * a.H + it.h) * g.pitch + row] = nd - corr;
       }
       const float f = KEYS && half ? 1.f : it.end == 1 ? 0.f : a.scale;      // one key: its weight is one whatever its score
-      unsigned char* stage = smem_raw + (srow - raw) + (seq & 1) * 2 * G::RTILE + (KEYS ? half * G::RTILE : 0) + r * 128;
+      unsigned char* stage = smem_raw + (srow - raw) + turn.buffer() * 2 * G::RTILE + (KEYS ? half * G::RTILE : 0) + r * 128;
       const bool zero = KEYS && !row_ok;
 #pragma unroll 1
       for (int e = 0; e < SPAN; e += 32) {
@@ -431,8 +437,8 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&hdr->staged));
-      ++seq;
+      if (lane == 0) mbar_arrive(smem_u32(&hdr->staged[turn.buffer()]));
+      turn.next();
     }
   }
   tc_fence_before();
