@@ -46,7 +46,7 @@ template <int DC> struct Grad {
 };
 
 struct GradHeader {
-  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_full, acc_free, summed, staged[2], drain;
+  uint64_t row_full[2], row_empty[2], full[4], empty[4], s_full, s_free, p_full, mixed, acc_full, acc_free, summed, staged[2], drain[2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -124,11 +124,11 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->row_full[i]), 1); mbar_init(smem_u32(&hdr->row_empty[i]), 1); mbar_init(smem_u32(&hdr->staged[i]), EW_WARPS); }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->row_full[i]), 1); mbar_init(smem_u32(&hdr->row_empty[i]), 1); mbar_init(smem_u32(&hdr->staged[i]), EW_WARPS); mbar_init(smem_u32(&hdr->drain[i]), 1); }
     for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&hdr->full[i]), 1); mbar_init(smem_u32(&hdr->empty[i]), 1); }
     mbar_init(smem_u32(&hdr->s_full), 1); mbar_init(smem_u32(&hdr->s_free), EW_WARPS); mbar_init(smem_u32(&hdr->p_full), EW_WARPS);
     mbar_init(smem_u32(&hdr->mixed), 1); mbar_init(smem_u32(&hdr->acc_full), 1); mbar_init(smem_u32(&hdr->acc_free), EW_WARPS);
-    mbar_init(smem_u32(&hdr->summed), EW_WARPS); mbar_init(smem_u32(&hdr->drain), 1);
+    mbar_init(smem_u32(&hdr->summed), EW_WARPS);
     hdr->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -205,10 +205,12 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       __syncwarp();
       if (++s == G::NS) { s = 0; sp ^= 1u; }
     }
-    if (*abort_flag && elect_one()) {      // no MMA may still be reading shared memory or writing tensor memory
-      tc_commit(smem_u32(&hdr->drain));
+    // No MMA may still be reading shared memory or writing tensor memory when the block leaves.  A commit covers its own warp's MMAs only, so each of the two warps has a barrier for this:
+    // on one for both, the first to arrive would let the other go with MMAs in flight, and two arrivals before a look would look like none.
+    if (*abort_flag && elect_one()) {
+      tc_commit(smem_u32(&hdr->drain[0]));
       for (uint32_t it = 0; it < (1u << 20); ++it)
-        if (mbar_try_wait(smem_u32(&hdr->drain), 0)) break;
+        if (mbar_try_wait(smem_u32(&hdr->drain[0]), 0)) break;
     }
   } else if (warp == PRODUCTS) {
     // ------------------------------------------------------------ the accumulators
@@ -238,9 +240,9 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       if (++s == G::NS) { s = 0; sp ^= 1u; }
     }
     if (*abort_flag && elect_one()) {
-      tc_commit(smem_u32(&hdr->drain));
+      tc_commit(smem_u32(&hdr->drain[1]));
       for (uint32_t it = 0; it < (1u << 20); ++it)
-        if (mbar_try_wait(smem_u32(&hdr->drain), 0)) break;
+        if (mbar_try_wait(smem_u32(&hdr->drain[1]), 0)) break;
     }
   } else if (warp == STORES) {
     // ------------------------------------------------------------ copies out
