@@ -240,9 +240,11 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 2 : 1) attn_forward_kernel
   float inv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    inv[i] = m[i] == -INF ? 0.f : 1.f / l[i];
+    // (no key: the sum is zero; scores that are all not a number leave no maximum either, but a sum that is none, and so are the result and its logarithm)
+    const bool none = m[i] == -INF && !(l[i] != l[i]);
+    inv[i] = none ? 0.f : 1.f / l[i];
     const int r = qt * T + ty + 16 * i;
-    const float lse = m[i] == -INF ? INF : m[i] + log2f(l[i]);
+    const float lse = none ? INF : m[i] + log2f(l[i]);
     if (tx == 0 && r < a.Lq) {
       if (a.splits > 1) a.part_lse[(((int64_t)split * a.B + b) * a.Lq + r) * a.H + h] = lse;
       else if (a.lse) a.lse[((int64_t)b * a.H + h) * a.Lq + r] = lse;
