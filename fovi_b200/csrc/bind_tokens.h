@@ -55,6 +55,8 @@ bool real_type(const at::Tensor& t) { return t.scalar_type() == at::kFloat || t.
 bool needs_graph(const at::Tensor& a, const at::Tensor* b = nullptr, const at::Tensor* c = nullptr) {
   return at::GradMode::is_enabled() && (a.requires_grad() || (b && b->requires_grad()) || (c && c->requires_grad()));
 }
+// A tensor with a tangent: the Python path names the derivative that is not built, where this one would lose it.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
 at::Tensor or_none(const at::Tensor* t) { return t ? *t : at::Tensor(); }
 
 // ------------------------------------------------------------------------------------------------------------ layer norm
@@ -104,6 +106,7 @@ BODY(layer_norm, 6)
   if (PyErr_Occurred()) return nullptr;
   if (!(eps >= 0)) GENERAL;
   const at::Tensor *w = wp ? plain(v[1], dev) : nullptr, *b = bp ? plain(v[2], dev) : nullptr;
+  if (has_tangent(*x) || (w && has_tangent(*w)) || (b && has_tangent(*b))) GENERAL;
   at::Tensor y;
   int rcode;
   {
@@ -184,7 +187,8 @@ BODY(rotary, 8)
   if (PyErr_Occurred()) return nullptr;
   const int64_t B = x->size(0), L = x->size(1);
   if (prefix < 0 || prefix > L || 2 * P > x->size(3) || f->numel() != P || pos->size(-1) != t.axes || pos->size(-2) != L - prefix || (pos->dim() == 3 && pos->size(0) != B) ||
-      B > INT32_MAX || L > INT32_MAX || x->size(2) > INT32_MAX || x->size(3) > INT32_MAX || needs_graph(*pos, f))
+      B > INT32_MAX || L > INT32_MAX || x->size(2) > INT32_MAX || x->size(3) > INT32_MAX || needs_graph(*pos, f) || has_tangent(*x) ||
+      has_tangent(*pos) || has_tangent(*f))
     GENERAL;
   t.prefix = (int)prefix; t.interleaved = (int)inter;
   at::Tensor y;
@@ -264,7 +268,9 @@ BODY(attention, 8)
       s->sizes() != k->sizes() || k->size(0) != q->size(0) || k->size(3) != q->size(3) || q->numel() == 0 || k->numel() == 0)
     GENERAL;
   const int64_t B = q->size(0), Lq = q->size(1), H = q->size(2), D = q->size(3), Lk = k->size(1), Hkv = k->size(2);
-  if (H % Hkv || D > 128 || B > INT32_MAX || Lq > INT32_MAX || Lk > INT32_MAX || H > INT32_MAX || !rows_plain(*q) || !rows_plain(*k) || !rows_plain(*s)) GENERAL;
+  if (H % Hkv || D > 128 || B > INT32_MAX || Lq > INT32_MAX || Lk > INT32_MAX || H > INT32_MAX || !rows_plain(*q) || !rows_plain(*k) || !rows_plain(*s) ||
+      has_tangent(*q) || has_tangent(*k) || has_tangent(*s))
+    GENERAL;
   if (v[3] != Py_None && (!(len = plain(v[3], dev)) || len->scalar_type() != at::kInt || len->dim() != 1 || len->size(0) != B || !len->is_contiguous())) GENERAL;
   if (v[4] != Py_None &&
       (!(mask = plain(v[4], dev)) || mask->scalar_type() != at::kBool || mask->dim() != 2 || mask->size(0) != B || mask->size(1) != Lk || !mask->is_contiguous()))

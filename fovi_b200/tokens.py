@@ -15,6 +15,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -24,6 +25,12 @@ __all__ = ["layer_norm", "rotary", "cross_attention", "TokenNorm", "AxialRotary"
 
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _no_tangents(name, *tensors):
+    """Forward-mode derivatives are not built: a tensor that carries one is refused, where the kernels would give a result without it, whose derivative reads as zero."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: forward-mode derivatives are not built; use backward-mode ones, or pass tensors without a tangent")
 
 
 # ------------------------------------------------------------------------------------------------------------ functions
@@ -52,6 +59,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
         got = ops._native.layer_norm(x, weight, bias, eps, dev, ops._raw_stream(dev))
         if got is not None:
             return ops._checked(got, "fovi_layer_norm_forward")
+    _no_tangents("layer_norm", x, weight, bias)
     if _wants_grad(x, weight, bias):
         return _LayerNormFunction.apply(x, weight, bias, eps, out_dtype)
     return ops.layer_norm(x, weight, bias, eps, out_dtype)
@@ -86,6 +94,7 @@ def rotary(x, positions, frequencies, pairs_per_axis, prefix=0, pairing="halves"
         got = ops._native.rotary(x, positions, frequencies, pairs_per_axis, prefix, _PAIRINGS[pairing], dev, ops._raw_stream(dev))
         if got is not None:
             return ops._checked(got, "fovi_rotary")
+    _no_tangents("rotary", x, positions, frequencies)
     if _wants_grad(positions, frequencies):
         raise NotImplementedError("rotary: positions and frequencies carry no gradient; detach them")
     if _wants_grad(x):
@@ -119,6 +128,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
         got = ops._native.attention(q, k, v, key_lengths, key_mask, scale, dev, ops._raw_stream(dev))
         if got is not None:
             return ops._checked(got, "fovi_attention_forward")
+    _no_tangents("cross_attention", q, k, v)
     if _wants_grad(q, k, v):
         return _AttentionFunction.apply(q, k, v, key_lengths, key_mask, scale)
     return ops.attention(q, k, v, key_lengths, key_mask, scale)
