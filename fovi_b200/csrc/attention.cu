@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 2 : 1) attn_dkv_kernel(con
       for (int c = 0; c < DP / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
     }
   const int64_t at = ((int64_t)b * a.Lk * a.Hkv + hk) * a.D, pitch = (int64_t)a.Hkv * a.D;
-  store_tile<E, DP>((E*)a.dk + at, pitch, kt * T, a.Lk, a.D, dk, f);
+  if (a.dk) store_tile<E, DP>((E*)a.dk + at, pitch, kt * T, a.Lk, a.D, dk, f);
   store_tile<E, DP>((E*)a.dv + at, pitch, kt * T, a.Lk, a.D, dv, one);
 }
 
@@ -589,7 +589,7 @@ int backward(AttnArgs a, cudaStream_t st) {
   int rc = launch(attn_delta_kernel<E>, ((int64_t)a.B * a.Lq * a.H + 7) / 8, 0, st, a, "attn_delta_kernel");
   if (!rc && a.dq) rc = launch(attn_dq_kernel<E, DP>, (int64_t)((a.Lq + T - 1) / T) * a.H * a.B * a.splits, DQ_SMEM<DP>, st, a, "attn_dq_kernel");
   if (!rc && a.dq && a.splits > 1) rc = launch(attn_sum_parts_kernel<E>, ((int64_t)a.B * a.Lq * a.H * a.D + 255) / 256, 0, st, a, "attn_sum_parts_kernel");
-  if (!rc && a.dk) rc = launch(attn_dkv_kernel<E, DP>, (int64_t)((a.Lk + T - 1) / T) * a.Hkv * a.B, DKV_SMEM<DP>, st, a, "attn_dkv_kernel");
+  if (!rc && a.dv) rc = launch(attn_dkv_kernel<E, DP>, (int64_t)((a.Lk + T - 1) / T) * a.Hkv * a.B, DKV_SMEM<DP>, st, a, "attn_dkv_kernel");
   return rc;
 }
 
@@ -615,7 +615,7 @@ AttnArgs arguments(const void* q, const void* k, const void* v, int dtype, int B
   return a;
 }
 void gradients(AttnArgs& a, int dtype, const void* o, const void* dy, const int64_t* s, const float* lse, void* dq, void* dk, void* dv, void* work) {
-  a.o = o; a.dy = dy; a.lse = const_cast<float*>(lse); a.dq = dq; a.dk = a.Lk > 0 ? dk : nullptr; a.dv = dv; a.delta = static_cast<float*>(work);
+  a.o = o; a.dy = dy; a.lse = const_cast<float*>(lse); a.dq = dq; a.dk = a.Lk > 0 ? dk : nullptr; a.dv = a.Lk > 0 ? dv : nullptr; a.delta = static_cast<float*>(work);
   a.g_sb = s[9]; a.g_sl = s[10]; a.g_sh = s[11];
   const int size = (int)fovi::dtype_size(dtype);
   a.vec = a.vec && !((reinterpret_cast<uintptr_t>(dy) | (uintptr_t)(s[9] * size) | (uintptr_t)(s[10] * size) | (uintptr_t)(s[11] * size)) & 15u);
@@ -657,15 +657,13 @@ extern "C" int fovi_attention_forward(const void* q, const void* k, const void* 
 extern "C" int fovi_attention_backward(const void* q, const void* k, const void* v, const void* o, const void* dy, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D,
                                        const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, float scale, const float* lse, void* dq, void* dk,
                                        void* dv, void* work, int64_t work_bytes, void* stream) {
-  if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, strides, 12) || !dk != !dv) return FOVI_ERR_INVALID_ARGUMENT;
+  if (!shape_ok(dtype, B, Lq, Lk, H, Hkv, D, strides, 12) || (dk && !dv)) return FOVI_ERR_INVALID_ARGUMENT;
   if (D > fovi::ATT_MAX_DIM) return FOVI_ERR_UNSUPPORTED;
   auto st = reinterpret_cast<cudaStream_t>(stream);
   if ((int64_t)B * Lq == 0) {       // no query: no gradient reaches the states
     const size_t bytes = (size_t)B * Lk * Hkv * D * fovi::dtype_size(dtype);
-    if (dk && bytes) {
-      FOVI_CUDA(cudaMemsetAsync(dk, 0, bytes, st));
-      FOVI_CUDA(cudaMemsetAsync(dv, 0, bytes, st));
-    }
+    if (dk && bytes) FOVI_CUDA(cudaMemsetAsync(dk, 0, bytes, st));
+    if (dv && bytes) FOVI_CUDA(cudaMemsetAsync(dv, 0, bytes, st));
     return FOVI_OK;
   }
   if (!q || !o || !dy || !lse || (Lk > 0 && (!k || !v))) return FOVI_ERR_INVALID_ARGUMENT;

@@ -241,19 +241,18 @@ struct AttentionNode : Node {
       const at::Tensor g = rows_plain(in[0]) ? in[0] : in[0].clone(at::MemoryFormat::Contiguous);
       const int dev = qv.get_device(), type = code_of(qv.scalar_type());
       const int B = (int)qv.size(0), Lq = (int)qv.size(1), H = (int)qv.size(2), D = (int)qv.size(3), Lk = (int)kv.size(1), Hkv = (int)kv.size(2);
-      const bool states = task_should_compute_output(1) || task_should_compute_output(2);
       if (task_should_compute_output(0)) out[0] = fresh(qv.sizes(), qv.scalar_type(), dev);
-      at::Tensor dk, dv;
-      if (states) { dk = fresh(kv.sizes(), kv.scalar_type(), dev); dv = fresh(kv.sizes(), kv.scalar_type(), dev); }
+      at::Tensor dv;
+      if (task_should_compute_output(1)) out[1] = fresh(kv.sizes(), kv.scalar_type(), dev);
+      if (out[1].defined() || task_should_compute_output(2)) dv = fresh(kv.sizes(), kv.scalar_type(), dev);
       const int64_t bytes = tok.attend_work(type, B, Lq, Lk, H, Hkv, D, 1);
       const at::Tensor work = fresh({bytes}, at::kByte, dev);
       int64_t s[12];
       put_strides(s, qv); put_strides(s + 3, kv); put_strides(s + 6, vv); put_strides(s + 9, g);
       launched(tok.attend_back(qv.const_data_ptr(), kv.const_data_ptr(), vv.const_data_ptr(), ov.const_data_ptr(), g.const_data_ptr(), type, B, Lq, Lk, H, Hkv, D, s,
                                len.defined() ? len.const_data_ptr<int32_t>() : nullptr, mk.defined() ? (const uint8_t*)mk.const_data_ptr() : nullptr, scale,
-                               lse.const_data_ptr<float>(), out_ptr(out[0]), out_ptr(dk), out_ptr(dv), work.mutable_data_ptr(), bytes, stream_of(qv)),
+                               lse.const_data_ptr<float>(), out_ptr(out[0]), out_ptr(out[1]), out_ptr(dv), work.mutable_data_ptr(), bytes, stream_of(qv)),
                "fovi_attention_backward");
-      if (task_should_compute_output(1)) out[1] = dk;
       if (task_should_compute_output(2)) out[2] = dv;
     }
     once(out, {in[0], qv, kv, vv}, "cross_attention");

@@ -968,8 +968,8 @@ def attention(q, k, v, key_lengths=None, key_mask=None, scale=None, want_lse=Fal
 
 
 def attention_backward(q, k, v, o, grad, lse, key_lengths=None, key_mask=None, scale=None, need=(True, True, True)):
-    """Gradients of attention with respect to (q, k, v), contiguous, from its result, its lse and the gradient of its result.  need: which are wanted (those of k and v are made
-    together)."""
+    """Gradients of attention with respect to (q, k, v), contiguous, from its result, its lse and the gradient of its result.  need: which are wanted; each has the same
+    bits whichever they are.  (v's is made where k's is.)"""
     q, k, v, lengths, mask, dims, scale = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
     B, Lq, Lk, H, Hkv, D = dims
     _same_device(q, o, grad, lse)
@@ -980,7 +980,7 @@ def attention_backward(q, k, v, o, grad, lse, key_lengths=None, key_mask=None, s
         grad = grad.to(q.dtype)
     grad = _rows_for_copies(grad)
     dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev) if need[0] else None
-    dk, dv = (torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev) if need[1] or need[2] else None for _ in range(2))
+    dk, dv = (torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev) if m else None for m in (need[1], need[1] or need[2]))
     size = lib.fovi_attention_workspace_bytes(dt, *dims, 1)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
     with _on(dev):
@@ -989,7 +989,7 @@ def attention_backward(q, k, v, o, grad, lse, key_lengths=None, key_mask=None, s
                                           None if lengths is None else _ptr(lengths), None if mask is None else _ptr(mask), scale, _ptr(lse),
                                           None if dq is None else _ptr(dq), None if dk is None else _ptr(dk), None if dv is None else _ptr(dv),
                                           None if work is None else _ptr(work), size, _stream()), "fovi_attention_backward")
-    return dq, dk if need[1] else None, dv if need[2] else None
+    return dq, dk, dv if need[2] else None
 
 
 def attention_check():

@@ -122,7 +122,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
 
     Float32 or bf16, any strides (slices of a packed projection, expanded tensors); Hkv divides H, and head h reads state head h // (H // Hkv); D up to 128; scale 1 / sqrt(D) by default.
     key_lengths [B]: states at and behind it are not read; key_mask [B, Lk]: nor those where it is False.  What k and v hold there has no effect, not-a-number
-    included, and their gradients are zero; a query without any state gives zeros.  Gradients are the same bits every time."""
+    included, and their gradients are zero; a query without any state gives zeros.  Gradients are the same bits every time, whichever of them are asked for."""
     if ops._native is not None and q.is_cuda:
         dev = ops._current_device()
         got = ops._native.attention(q, k, v, key_lengths, key_mask, scale, dev, ops._raw_stream(dev))

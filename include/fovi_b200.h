@@ -486,8 +486,8 @@ int fovi_rotary(const void* x, int dtype, int B, int L, int H, int D, const int6
 int64_t fovi_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, int backward);
 int fovi_attention_forward(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D, const int64_t* strides,
                            const int32_t* key_lengths, const uint8_t* key_mask, float scale, void* o, float* lse, void* work, int64_t work_bytes, void* stream);
-/* The gradients dq (like o), dk and dv (contiguous [B, Lk, Hkv, D], both or neither), summed over the heads that share a state head; strides: [12], dy last.  dq, or dk and
- * dv, may be NULL.  Fixed order of all sums: the same bits every time. */
+/* The gradients dq (like o), dk and dv (contiguous [B, Lk, Hkv, D]), summed over the heads that share a state head; strides: [12], dy last.  Each may be NULL (dv only where dk is).
+ * Fixed order of all sums: the same bits every time, whichever gradients are asked for. */
 int fovi_attention_backward(const void* q, const void* k, const void* v, const void* o, const void* dy, int dtype, int B, int Lq, int Lk, int H, int Hkv, int D,
                             const int64_t* strides, const int32_t* key_lengths, const uint8_t* key_mask, float scale, const float* lse, void* dq, void* dk, void* dv,
                             void* work, int64_t work_bytes, void* stream);
