@@ -938,7 +938,7 @@ def _attention_inputs(q, k, v, key_lengths, key_mask, scale):
         if key_lengths.shape != (B,) or key_lengths.is_floating_point() or key_lengths.dtype == torch.bool:
             raise ValueError(f"key_lengths: whole numbers, one for each of {B} samples")
         if key_lengths.dtype != torch.int32 or not key_lengths.is_contiguous():
-            key_lengths = key_lengths.clamp(0, Lk).to(torch.int32).contiguous()
+            key_lengths = key_lengths.to(torch.int64).clamp(0, Lk).to(torch.int32).contiguous()      # (Lk may pass a short type's largest number)
     if key_mask is not None:
         if key_mask.dtype != torch.bool or key_mask.shape != (B, Lk):
             raise ValueError(f"key_mask: truth values (true: the key is read) of the shape {(B, Lk)}")
