@@ -63,6 +63,7 @@ at::Tensor or_none(const at::Tensor* t) { return t ? *t : at::Tensor(); }
 struct LayerNormNode : Node {
   SavedVariable x, w;
   at::Tensor stats;
+  at::DimVector shape[2];                // of the weight and the bias: C values, in whatever shape
   std::string name() const override { return "FoviLayerNormBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -81,7 +82,7 @@ struct LayerNormNode : Node {
       const int dev = xv.get_device();
       if (task_should_compute_output(0)) out[0] = fresh(xv.sizes(), xv.scalar_type(), dev);
       for (int i = 1; i < 3; ++i)
-        if (task_should_compute_output(i)) out[i] = fresh({C}, at::kFloat, dev);
+        if (task_should_compute_output(i)) out[i] = fresh(shape[i - 1], at::kFloat, dev);
       const bool sums = out[1].defined() || out[2].defined();
       const int64_t bytes = sums ? tok.norm_work(rows, (int)C) : 0;
       const at::Tensor work = sums ? fresh({bytes}, at::kByte, dev) : at::Tensor();
@@ -125,6 +126,8 @@ BODY(layer_norm, 6)
       node->set_next_edges(torch::autograd::collect_next_edges(*x, or_none(w), or_none(b)));
       node->x = SavedVariable(*x, false);
       node->w = SavedVariable(or_none(w), false);
+      if (w) node->shape[0] = w->sizes();
+      if (b) node->shape[1] = b->sizes();
       node->stats = stats;
       torch::autograd::set_history(y, node);
     }

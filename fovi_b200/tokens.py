@@ -39,7 +39,7 @@ class _LayerNormFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, out_dtype):
         y, stats = ops.layer_norm(x, weight, bias, eps, out_dtype, want_stats=True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.types = tuple(None if t is None else t.dtype for t in (weight, bias))
+        ctx.like = tuple(None if t is None else (t.dtype, t.shape) for t in (weight, bias))
         return y
 
     @staticmethod
@@ -47,7 +47,7 @@ class _LayerNormFunction(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight, stats = ctx.saved_tensors
         dx, dw, db = ops.layer_norm_backward(x, grad, weight, stats, ctx.needs_input_grad[:3])
-        dw, db = (None if g is None else g if g.dtype is t else g.to(t) for g, t in zip((dw, db), ctx.types))
+        dw, db = (None if g is None else g.to(like[0]).view(like[1]) for g, like in zip((dw, db), ctx.like))
         return dx, dw, db, None, None
 
 
