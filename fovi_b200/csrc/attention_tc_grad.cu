@@ -281,7 +281,6 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int64_t at = ((int64_t)it.b * a.H + it.h) * g.pitch + row;
         nl = __ldg(g.nl + at); nd = __ldg(g.nd + at);
       }
-      const float none = c > 0.f ? -INFINITY : c < 0.f ? INFINITY : 0.f;      // the score whose exponential is 0
       float2 rest[2] = {};                   // dq: the sum of the row's ds, of this thread's columns
       for (int j = 0; j < it.n; ++j, ++n) {
         int c0, h;
@@ -316,10 +315,10 @@ attn_tc_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if (lane == 0) mbar_arrive(smem_u32(&hdr->s_free));
           }
           uint32_t pw[16], dw[16];
-          if (work && !KEYS && !whole) {    // masked keys: p = 0 (scale 0: a finite p, which meets zeroed rows of K only) and ds = 0
+          if (work && !KEYS && !whole) {    // masked keys: p = 0 (the scale is positive here, see attention_tc_takes) and ds = 0
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (!(bits[e >> 5] >> k & 1u)) { s[k] = none; d[k] = -nd; }
+              if (!(bits[e >> 5] >> k & 1u)) { s[k] = -AT_INF; d[k] = -nd; }
           }
           if (work) {
 #pragma unroll
