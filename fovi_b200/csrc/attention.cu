@@ -280,7 +280,7 @@ __device__ __forceinline__ float4 load4(const E* p, int c, int D, bool vec) {
 template <typename E, int DP>
 __global__ void __launch_bounds__(FEW_THREADS) attn_few_kernel(const AttnArgs a) {
   constexpr int LANES = DP / 4, GROUPS = FEW_THREADS / LANES;
-  __shared__ float part[GROUPS][DP + 2];
+  __shared__ __align__(8) float part[GROUPS][DP + 2];
   const int split = blockIdx.x % a.splits, block = blockIdx.x / a.splits;
   const int q = block % a.Lq, h = block / a.Lq % a.H, b = block / a.Lq / a.H, group = threadIdx.x / LANES, c = threadIdx.x % LANES * 4;
   const Range range = keys_of(a, key_end(a, b), split, FEW_KEYS * GROUPS);

@@ -267,7 +267,8 @@ layer_norm_grad_rows_kernel(const TX* __restrict__ x, int64_t rows, int C, int64
                             const float2* __restrict__ stats, TX* __restrict__ dx, float* __restrict__ part) {
   constexpr int E = CH * VEC, H = VEC > 1 ? VEC / 2 : 1, STEP = VEC > 1 ? 1 : 2;
   __shared__ float2 sums[2][32];
-  extern __shared__ float joined[];        // warp teams: the weights (in shared memory: their registers are a third block's), then the warps' parts, [2][C]
+  extern __shared__ float4 joined4[];        // warp teams: the weights (in shared memory: their registers are a third block's), then the warps' parts, [2][C]
+  float* joined = reinterpret_cast<float*>(joined4);
   const Team<VEC, BLOCK> t;
   Pairs<BLOCK ? E : 2> wv;
   Pairs<E> aw, ab;
