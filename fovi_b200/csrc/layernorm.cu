@@ -391,7 +391,9 @@ Shape shape_of(const void* x, int64_t x_stride, int xs, const void* y, int64_t y
   auto fits = [&](int v) {
     return C % v == 0 && x_stride % v == 0 && y_stride % v == 0 && (reinterpret_cast<uintptr_t>(x) % (v * xs)) == 0 && (reinterpret_cast<uintptr_t>(y) % (v * ys)) == 0;
   };
-  const bool wide = xs == 4 || ys == 4;                       // VEC 8 is for bf16 on both sides: 16 bytes
+  // VEC 8 is for bf16 on both sides, 16 bytes, from 512 channels on: below, lanes stay idle (forward at 384 channels 84 us in place of 75, backward 142 of 135); at 512 and 768 the two are
+  // equal to 2 %, and from 1024 on 16 bytes are the faster ones (backward at 1280 channels 158 us in place of 185).
+  const bool wide = xs == 4 || ys == 4;
   const int vec = !wide && C >= 512 && fits(8) ? 8 : fits(4) ? 4 : 1;
   // A warp holds up to 24 values a thread of bf16, 12 of float32 or one by one; beyond, its registers would leave too few warps on an SM.
   int ch = (C + 32 * vec - 1) / (32 * vec);
@@ -403,10 +405,14 @@ Shape shape_of(const void* x, int64_t x_stride, int xs, const void* y, int64_t y
   return {0, 0, 0, false};
 }
 
-constexpr int GRAD_BLOCKS = 592;         // most parts of dw and db
+// Blocks of the backward kernel, a part of dw and db each: as many as the SMs hold at once by its registers, three an SM for teams of a warp with up to 8 values a thread and two beyond, about
+// 640 threads an SM for teams of a block.  Half as many, this many, twice as many (us): 263168 x 384 bf16 207, 135, 146; 80000 x 1280 bf16 249, 159, 169; 200000 x 384 float32 196, 152, 163;
+// 100000 x 1024 bf16, whose blocks of 128 threads the limit of 592 cuts short, 299, 183, 131.
+constexpr int GRAD_BLOCKS = 592;         // most parts: four for each of 148 SMs
 int grad_blocks(const Shape& s, int64_t rows) {
-  const int64_t want = s.block ? rows : (rows + 7) / 8, most = s.block ? std::max(148, std::min(GRAD_BLOCKS, 148 * 640 / s.threads)) : s.ch * s.vec <= 8 ? 444 : 296;
-  return (int)std::min<int64_t>(want, most);
+  const int64_t want = s.block ? rows : (rows + 7) / 8, sms = fovi::sm_count();
+  const int64_t most = s.block ? std::max(sms, sms * 640 / s.threads) : s.ch * s.vec <= 8 ? 3 * sms : 2 * sms;
+  return (int)std::min({want, most, (int64_t)GRAD_BLOCKS});
 }
 
 template <typename TX, typename TY> struct Run {
@@ -457,7 +463,7 @@ template <typename TX, typename TY>
 int forward(const void* x, int64_t rows, int C, int64_t stride, const float* w, const float* b, float eps, void* y, float* stats, cudaStream_t st) {
   const Shape s = shape_of(x, stride, sizeof(TX), y, C, sizeof(TY), C);
   if (s.threads) return Run<TX, TY>{x, rows, C, stride, w, b, eps, y, stats, nullptr, 0, nullptr, nullptr, st}(s, false);
-  const int grid = (int)(rows < 148 * 8 ? rows : 148 * 8);
+  const int grid = (int)std::min<int64_t>(rows, fovi::sm_count() * 8);
   layer_norm_kernel<TX, TY><<<grid, GEN_THREADS, 0, st>>>((const TX*)x, rows, C, stride, w, b, eps, (TY*)y, (float2*)stats);
   return fovi::after_launch("layer_norm_kernel");
 }
@@ -474,7 +480,7 @@ int backward(const void* x, int64_t rows, int C, int64_t stride, const void* dy,
     strips = grad_blocks(s, rows);
   } else {
     if (dx) {
-      const int grid = (int)(rows < 148 * 8 ? rows : 148 * 8);
+      const int grid = (int)std::min<int64_t>(rows, fovi::sm_count() * 8);
       layer_norm_dx_kernel<TX, TY><<<grid, GEN_THREADS, 0, st>>>((const TX*)x, rows, C, stride, (const TY*)dy, dy_stride, w, (const float2*)stats, (TX*)dx);
       const int rc = fovi::after_launch("layer_norm_dx_kernel");
       if (rc) return rc;
