@@ -71,7 +71,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const T* x, T* y, const Rot
 
 // Rows on 16-byte boundaries, whole pieces of V channels (16 bytes).  A block takes `tokens` tokens: their cosines and sines once, into shared memory, then all heads
 // piece by piece, "halves" with the two pieces that turn together in one thread.  A thread's first PIECES pieces are on their way while the angles are worked out.
-// What bounds it is memory: one read and one write.  With launches (us): 256 x 257 x 6 x 64 bf16, two axes: 25 (4.0 TB/s; a thread per pair over all heads: 50);
+// What bounds it is a block's chain (places, barrier, loads, angles, barrier, stores), which it goes through once and which only the SM's other blocks cover, next to its instructions: issue slots
+// 68 % and shared memory 65 % taken, no one kind of stall above a quarter of a warp's time (first size below).  With launches (us): 256 x 257 x 6 x 64 bf16, two axes: 25 (4.0 TB/s; a thread per pair over all heads: 50);
 // 7 x 1029 x 20 x 64 float32, three axes: 18 to 19 (3.8 to 4.2 TB/s; 19 as well); 64 x 500 x 12 x 128 bf16: 40 (4.9 TB/s; 72).
 struct Tile { int tokens, per, row; uint32_t by_per, by_row, by_pairs; };      // pieces of a head and of a token; 2^32 / d rounded up, for divisions of small numbers
 
