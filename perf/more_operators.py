@@ -163,7 +163,9 @@ def _run_own(s):
     if case["op"] == "ffn":
         y = tokens.gated_feed_forward(s["x"], s["gate_weight"], s["up_weight"], s["down_weight"], s["gate_bias"], s["up_bias"], s["down_bias"],
                                       activation=case["activation"])
-        outs, grads = (y,), (s.get("grad"),)
+        if not case["train"]:
+            return y
+        outs, grads = (y,), (s["grad"],)
     elif case["form"] == "int8":
         q, scale, *stream = tokens.rms_norm_int8(s["x"], s["weight"], eps=EPS, residual=s["residual"])
         values = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
