@@ -91,6 +91,16 @@ SIGNATURES = {
     "fovi_attention_backward": (C.c_int, [_P] * 5 + [C.c_int] * 7 + [C.POINTER(C.c_int64), _P, _P, C.c_float] + [_P] * 5 + [C.c_int64, _P]),
     "fovi_attention_check": (C.c_int, [_P]),
     "fovi_attention_forward_selftest_wait_timeout": (C.c_int, [_P, _P, _P] + [C.c_int] * 6 + [C.POINTER(C.c_int64), C.c_float, _P, _P]),
+    "fovi_rms_norm_forward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int64, _P, C.c_float, _P, _P, _P, C.c_int64, _P, _P, _P]),
+    "fovi_rms_norm_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int]),
+    "fovi_rms_norm_backward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "fovi_quantize_rows": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int64, _P, _P]),
+    "fovi_linear_int8": (C.c_int, [_P, C.c_int64, C.c_int, C.c_int64, _P, _P, C.c_int, C.c_int64, _P, _P, _P, C.c_int, _P]),
+    "fovi_gated_ffn_saved_bytes": (C.c_int64, [C.c_int, C.c_int64, C.c_int]),
+    "fovi_gated_ffn_workspace_bytes": (C.c_int64, [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "fovi_gated_ffn_forward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int64] + [_P, C.c_int64] * 3 + [_P] * 3 + [C.c_int, _P, _P, _P, C.c_int64, _P]),
+    "fovi_gated_ffn_backward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int64] + [_P, C.c_int64] * 3 + [C.c_int, _P, _P, C.c_int64] + [_P] * 8
+                                + [C.c_int64, _P]),
     "fovi_attention_backward_selftest_wait_timeout": (C.c_int, [_P] * 5 + [C.c_int] * 6 + [C.POINTER(C.c_int64), C.c_float] + [_P] * 5 + [C.c_int64, _P]),
 }
 

@@ -57,6 +57,11 @@ def _ptr(t):
     return t.data_ptr()
 
 
+def _opt(t):
+    """An optional tensor's address."""
+    return None if t is None else t.data_ptr()
+
+
 class _Here:
     def __enter__(self):
         pass
@@ -867,6 +872,182 @@ def layer_norm_backward(x, grad, weight, stats, need=(True, True, True)):
                                            None if dx is None else _ptr(dx), None if dw is None else _ptr(dw), None if db is None else _ptr(db),
                                            None if work is None else _ptr(work), size, _stream()), "fovi_layer_norm_backward")
     return dx, dw, db
+
+
+def _rms_inputs(x, weight, eps, residual):
+    """Checked arguments of a root-mean-square norm: weight in float32, rows of x and of the residual, their number and length."""
+    _same_device(x, weight, residual)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"rms norm needs a last axis of at least one value, got the shape {tuple(x.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"eps is {eps}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"the residual is {residual.dtype} of the shape {tuple(residual.shape)}, x {x.dtype} of {tuple(x.shape)}; the same are wanted")
+    c = x.shape[-1]
+    xr, n, stride = _rows(x, c)
+    rr, _, r_stride = (None, 0, 0) if residual is None else _rows(residual, c)
+    return _f32_param(weight, c, "weight"), xr, stride, rr, r_stride, n, c
+
+
+def rms_norm(x, weight=None, eps=1e-6, residual=None, want_rstd=False):
+    """Root-mean-square norm over the last axis of x [..., C] (float32 or bf16), or of total = x + residual rounded to their type; weight [C].  Returns (y, total or None,
+    float32 [rows] 1/rms for rms_norm_backward or None), y and total contiguous, of x's type."""
+    w, xr, stride, rr, r_stride, n, c = _rms_inputs(x, weight, eps, residual)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    total = None if rr is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rstd = torch.empty(n, dtype=torch.float32, device=x.device) if want_rstd else None
+    with _on(x.device):
+        check(lib.fovi_rms_norm_forward(_ptr(xr), _dt(x.dtype), n, c, stride, _opt(rr), r_stride, _opt(w), eps, _opt(total), _ptr(y), None, 0, None, _opt(rstd), _stream()),
+              "fovi_rms_norm_forward")
+    return y, total, rstd
+
+
+def rms_norm_backward(t, grad, grad_total, weight, rstd, need=(True, True)):
+    """Gradients of rms_norm with respect to (x, weight), x's being the residual's too, from t (x, or total), the gradients of the result and of total (or None) and rstd; None
+    where `need` says no.  The weight's is float32 [C], summed in a fixed order."""
+    _same_device(t, grad, grad_total, weight, rstd)
+    c = t.shape[-1]
+    if grad.shape != t.shape or (grad_total is not None and grad_total.shape != t.shape):
+        raise ValueError(f"the gradient has the shape {tuple(grad.shape)}, the result {tuple(t.shape)}")
+    if rstd.dtype != torch.float32 or not rstd.is_contiguous() or rstd.numel() * c != t.numel():
+        raise ValueError("rstd is not what rms_norm gave for x")
+    w = _f32_param(weight, c, "weight")
+    tr, n, stride = _rows(t, c)
+    gr, _, g_stride = _rows(grad.to(t.dtype), c)
+    sr, _, s_stride = (None, 0, 0) if grad_total is None else _rows(grad_total.to(t.dtype), c)
+    dev = t.device
+    dx = torch.empty(t.shape, dtype=t.dtype, device=dev) if need[0] else None
+    dw = torch.empty(c, dtype=torch.float32, device=dev) if need[1] else None
+    size = lib.fovi_rms_norm_workspace_bytes(n, c) if need[1] else 0
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    with _on(dev):
+        check(lib.fovi_rms_norm_backward(_ptr(tr), _dt(t.dtype), n, c, stride, _ptr(gr), g_stride, _opt(sr), s_stride, _opt(w), _ptr(rstd), _opt(dx), _opt(dw), _opt(work), size,
+                                         _stream()), "fovi_rms_norm_backward")
+    return dx, dw
+
+
+def _eight_bits(shape, device):
+    """An int8 tensor whose rows start on 16-byte boundaries, as the tensor copies want them."""
+    c = shape[-1]
+    return torch.empty(tuple(shape[:-1]) + (-(-c // 16) * 16,), dtype=torch.int8, device=device)[..., :c]
+
+
+def rms_norm_int8(x, weight=None, eps=1e-6, residual=None):
+    """rms_norm with its result in 8 bits: (q int8 [..., C], scale float32 [...], total or None), y = q * scale."""
+    w, xr, stride, rr, r_stride, n, c = _rms_inputs(x, weight, eps, residual)
+    q, scale = _eight_bits(x.shape, x.device), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    total = None if rr is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        check(lib.fovi_rms_norm_forward(_ptr(xr), _dt(x.dtype), n, c, stride, _opt(rr), r_stride, _opt(w), eps, _opt(total), None, _ptr(q), -(-c // 16) * 16, _ptr(scale), None,
+                                        _stream()), "fovi_rms_norm_forward")
+    return q, scale, total
+
+
+def quantize(x):
+    """Rows x [..., C] (float32 or bf16) in 8 bits: (q int8 [..., C], scale float32 [...]), x = q * scale to half a step."""
+    _need_cuda(x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize needs a last axis of at least one value, got the shape {tuple(x.shape)}")
+    c = x.shape[-1]
+    xr, n, stride = _rows(x, c)
+    q, scale = _eight_bits(x.shape, x.device), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        check(lib.fovi_quantize_rows(_ptr(xr), _dt(x.dtype), n, c, stride, _ptr(q), -(-c // 16) * 16, _ptr(scale), _stream()), "fovi_quantize_rows")
+    return q, scale
+
+
+def _copy_rows(t, c, plain=False):
+    """t [..., C] as (rows on 16-byte boundaries for the tensor copies, their number, the stride); a copy where its memory does not give that.  plain: boundaries do not matter."""
+    t2, n, stride = _rows(t, c)
+    per = 16 // t.element_size()
+    if plain or (t2.data_ptr() % 16 == 0 and (n <= 1 or (stride % per == 0 and stride > 0))):
+        return t2, n, max(stride, -(-c // per) * per) if n <= 1 else stride
+    buffer = torch.empty((n, -(-c // per) * per), dtype=t.dtype, device=t.device)
+    buffer[:, :c] = t2.view(n, c) if t2.is_contiguous() else t2
+    return buffer, n, buffer.shape[1]
+
+
+def linear_int8(q, scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
+    """scale * weight_scale * (q weight^T) + bias: q int8 [..., K] with scale float32 [...], weight int8 [N, K] with weight_scale float32 [N], bias [N].  Exact integer sums;
+    the result is contiguous [..., N] in `out_dtype` (float32 or bf16)."""
+    _same_device(q, scale, weight, weight_scale, bias)
+    if q.dtype != torch.int8 or weight.dtype != torch.int8 or scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
+        raise TypeError(f"q and weight are {q.dtype} and {weight.dtype}, their scales {scale.dtype} and {weight_scale.dtype}; int8 and float32 are wanted")
+    if q.dim() < 1 or weight.dim() != 2 or q.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or not 1 <= q.shape[-1] < 131072:
+        raise ValueError(f"q {tuple(q.shape)}, weight {tuple(weight.shape)}: [..., K] and [N, K] are wanted, K from 1 to 131071")
+    if scale.shape != q.shape[:-1] or weight_scale.shape != weight.shape[:1]:
+        raise ValueError(f"scale {tuple(scale.shape)}, weight_scale {tuple(weight_scale.shape)}: one for each of {tuple(q.shape[:-1])} rows and {weight.shape[0]} channels")
+    (n, k), dt = weight.shape, _dt(out_dtype)
+    b = _f32_param(bias, n, "bias")
+    qr, m, q_stride = _copy_rows(q, k)
+    wr, _, w_stride = _copy_rows(weight, k)
+    scale, weight_scale = scale.contiguous(), weight_scale.contiguous()
+    y = torch.empty(q.shape[:-1] + (n,), dtype=out_dtype, device=q.device)
+    with _on(q.device):
+        check(lib.fovi_linear_int8(_ptr(qr), m, k, q_stride, _ptr(scale), _ptr(wr), n, w_stride, _ptr(weight_scale), _opt(b), _ptr(y), dt, _stream()), "fovi_linear_int8")
+    return y
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _ffn_inputs(x, gate_weight, up_weight, down_weight, biases, activation):
+    """Checked arguments of a gated feed-forward block: (rows of x, of the three weights with their strides), biases, (tokens, C, F, O)."""
+    _same_device(x, gate_weight, up_weight, down_weight, *biases)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation is {activation!r}: 'silu' or 'gelu'")
+    if gate_weight.dim() != 2 or up_weight.shape != gate_weight.shape or down_weight.dim() != 2 or down_weight.shape[1] != gate_weight.shape[0] or x.dim() < 1 \
+            or x.shape[-1] != gate_weight.shape[1] or 0 in gate_weight.shape or 0 in down_weight.shape:
+        raise ValueError(f"x {tuple(x.shape)}, gate, up and down weights {tuple(gate_weight.shape)}, {tuple(up_weight.shape)}, {tuple(down_weight.shape)}: [..., C], [F, C], [F, C], [O, F] "
+                         "are wanted")
+    (F, c), o = gate_weight.shape, down_weight.shape[0]
+    for t, n, name in zip(biases, (F, F, o), ("gate", "up", "down")):
+        if t is not None and t.shape != (n,):
+            raise ValueError(f"the {name} bias has the shape {tuple(t.shape)}, {(n,)} is wanted")
+    if any(t is not None and t.dtype != x.dtype for t in (gate_weight, up_weight, down_weight, *biases)):
+        raise TypeError(f"x is {x.dtype}; weights and biases of the same type are wanted")
+    plain = x.dtype == torch.float32
+    xr, m, xs = _copy_rows(x, c, plain)
+    rows = [(xr, xs)] + [_copy_rows(w, w.shape[1], plain)[::2] for w in (gate_weight, up_weight, down_weight)]
+    return rows, [None if t is None else t.contiguous() for t in biases], (m, c, F, o)
+
+
+def gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=None, down_bias=None, activation="silu", want_saved=False):
+    """(act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd: x [..., C], Wg, Wu [F, C], Wd [O, F], float32 or bf16, all of one type.  Returns (y [..., O] contiguous, what
+    gated_feed_forward_backward takes or None)."""
+    dt = _dt(x.dtype)
+    rows, biases, (m, c, F, o) = _ffn_inputs(x, gate_weight, up_weight, down_weight, (gate_bias, up_bias, down_bias), activation)
+    dev = x.device
+    y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=dev)
+    saved = torch.empty(lib.fovi_gated_ffn_saved_bytes(dt, m, F), dtype=torch.uint8, device=dev) if want_saved else None
+    size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, 0)
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        check(lib.fovi_gated_ffn_forward(_ptr(rows[0][0]), dt, m, c, F, o, rows[0][1], *(a for w, s in rows[1:] for a in (_ptr(w), s)), *(_opt(b) for b in biases),
+                                         ACTIVATIONS[activation], _ptr(y), _opt(saved), _ptr(work), size, _stream()), "fovi_gated_ffn_forward")
+    return y, saved
+
+
+def gated_feed_forward_backward(x, gate_weight, up_weight, down_weight, saved, grad, activation="silu", need=(True,) * 7):
+    """Gradients of gated_feed_forward with respect to (x, the three weights, the three biases), contiguous, of x's type, from what it saved and the gradient of its result;
+    None where `need` says no."""
+    dt = _dt(x.dtype)
+    rows, _, (m, c, F, o) = _ffn_inputs(x, gate_weight, up_weight, down_weight, (None,) * 3, activation)
+    _same_device(x, saved, grad)
+    if grad.shape != x.shape[:-1] + (o,):
+        raise ValueError(f"the gradient has the shape {tuple(grad.shape)}, the result {tuple(x.shape[:-1] + (o,))}")
+    if saved.dtype != torch.uint8 or saved.numel() != lib.fovi_gated_ffn_saved_bytes(dt, m, F):
+        raise ValueError("saved is not what gated_feed_forward gave for x")
+    gr, _, gs = _copy_rows(grad.to(x.dtype), o, x.dtype == torch.float32)
+    dev = x.device
+    shapes = (x.shape, gate_weight.shape, up_weight.shape, down_weight.shape, (F,), (F,), (o,))
+    out = tuple(torch.empty(s, dtype=x.dtype, device=dev) if n else None for s, n in zip(shapes, need))
+    size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, 1)
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        check(lib.fovi_gated_ffn_backward(_ptr(rows[0][0]), dt, m, c, F, o, rows[0][1], *(a for w, s in rows[1:] for a in (_ptr(w), s)), ACTIVATIONS[activation], _ptr(saved),
+                                          _ptr(gr), gs, *(_opt(t) for t in out), _ptr(work), size, _stream()), "fovi_gated_ffn_backward")
+    return out
 
 
 @functools.lru_cache(maxsize=256)

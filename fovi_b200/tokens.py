@@ -1,11 +1,13 @@
-"""Operators on tokens, for what stands behind a foveated patch embedding: layer norm, rotary positions with several axes, and cross attention to an encoder's
-states of another length, each with its gradients, on the library's own kernels.
+"""Operators on tokens, for what stands behind a foveated patch embedding: layer norm, rotary positions with several axes, cross attention to an encoder's
+states of another length, root-mean-square norm with the residual's addition, and the gated feed-forward block, each with its gradients; and for serving tokens and weights in 8 bits
+and their product.  All on the library's own kernels.
 
 In the reference they are torch calls inside its vision transformers (fovi/arch/vit.py:351-381: attention; fovi/arch/knnvit.py:420-464: rotary positions from the
 tokens' sensor coordinates).  Here
 
-* ``layer_norm`` / ``rotary`` / ``cross_attention`` are differentiable functions of tensors,
-* ``TokenNorm`` / ``AxialRotary`` / ``CrossAttention`` the modules around them, and
+* ``layer_norm`` / ``rotary`` / ``cross_attention`` / ``rms_norm`` / ``gated_feed_forward`` are differentiable functions of tensors,
+* ``TokenNorm`` / ``AxialRotary`` / ``CrossAttention`` / ``TokenRMSNorm`` / ``GatedFeedForward`` the modules around them,
+* ``rms_norm_int8`` / ``quantize`` / ``linear_int8`` serve in 8 bits, without gradients, and ``Linear8`` is a linear layer in that form, and
 * ``FixationReader`` runs them together: the tokens of all fixations of an image become states with a place (time, height, width) of their own, and a set of learned queries
   reads them out.
 
@@ -20,7 +22,8 @@ from torch.autograd.function import once_differentiable
 
 from . import ops
 
-__all__ = ["layer_norm", "rotary", "cross_attention", "TokenNorm", "AxialRotary", "CrossAttention", "FixationReader", "check"]
+__all__ = ["layer_norm", "rotary", "cross_attention", "rms_norm", "rms_norm_int8", "quantize", "linear_int8", "gated_feed_forward", "TokenNorm", "AxialRotary", "CrossAttention",
+           "TokenRMSNorm", "GatedFeedForward", "Linear8", "FixationReader", "check"]
 
 
 def _wants_grad(*tensors):
@@ -134,6 +137,93 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
     return ops.attention(q, k, v, key_lengths, key_mask, scale)
 
 
+class _RmsNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps, residual):
+        y, total, rstd = ops.rms_norm(x, weight, eps, residual, want_rstd=True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if total is None else total, weight, rstd)
+        ctx.like = None if weight is None else (weight.dtype, weight.shape)
+        return y if total is None else (y, total)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, grad_total=None):
+        t, weight, rstd = ctx.saved_tensors
+        x_needs, w_needs, _, r_needs = ctx.needs_input_grad
+        if grad is None:                                 # the norm's result was not used: the sum alone
+            return (grad_total if x_needs else None), None, None, (grad_total if r_needs else None)
+        dx, dw = ops.rms_norm_backward(t, grad, grad_total, weight, rstd, (x_needs or r_needs, w_needs))
+        return (dx if x_needs else None), (None if dw is None else dw.to(ctx.like[0]).view(ctx.like[1])), None, (dx if r_needs else None)
+
+
+def rms_norm(x, weight=None, eps=1e-6, residual=None):
+    """Root-mean-square norm over the last axis: y = t / sqrt(mean(t^2) + eps) * weight of t = x, or with `residual` (x's shape and type) of t = x + residual as their type holds it:
+    then (y, t) is returned, the same values as from the addition and the norm one after the other.  x [..., C] float32 or bf16; weight [C] or None.  Statistics, sums and the
+    weight's gradient are float32; gradients are the same bits every time."""
+    _no_tangents("rms_norm", x, weight, residual)
+    if _wants_grad(x, weight, residual):
+        return _RmsNormFunction.apply(x, weight, eps, residual)
+    y, total, _ = ops.rms_norm(x, weight, eps, residual)
+    return y if total is None else (y, total)
+
+
+def _no_gradient(name, *tensors):
+    if _wants_grad(*tensors):
+        raise NotImplementedError(f"{name}: what is held in 8 bits carries no gradient; call it under torch.no_grad(), or detach its tensors")
+
+
+def rms_norm_int8(x, weight=None, eps=1e-6, residual=None):
+    """rms_norm with its result in 8 bits for linear_int8: (q, scale), or (q, scale, t) with `residual`; y = q * scale to half a step.  q int8 [..., C], values of -127 .. 127 rounded
+    from the unrounded y; scale float32 [...], max |y| / 127 of the row (at least the smallest normal number).  A row that holds infinity or not-a-number has one of them as its scale.
+    No gradient."""
+    _no_tangents("rms_norm_int8", x, weight, residual)
+    _no_gradient("rms_norm_int8", x, weight, residual)
+    q, scale, total = ops.rms_norm_int8(x, weight, eps, residual)
+    return (q, scale) if total is None else (q, scale, total)
+
+
+def quantize(x):
+    """Rows of x [..., C] (float32 or bf16) in 8 bits with a scale each, as rms_norm_int8 gives them: tokens for linear_int8, or a weight [N, K] with a scale for each
+    output channel.  No gradient."""
+    _no_tangents("quantize", x)
+    _no_gradient("quantize", x)
+    return ops.quantize(x)
+
+
+def linear_int8(q, scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
+    """y = scale * weight_scale * (q weight^T) + bias: q int8 [..., K] with scale float32 [...], weight int8 [N, K] with weight_scale float32 [N], both as ``quantize`` gives them (or
+    any other int8 tensors), bias [N] or None; K up to 131071.  The sums are exact; the result [..., N] is float32 or bf16.  No gradient."""
+    _no_tangents("linear_int8", scale, weight_scale, bias)
+    _no_gradient("linear_int8", scale, weight_scale, bias)
+    return ops.linear_int8(q, scale, weight, weight_scale, bias, out_dtype)
+
+
+class _FeedForwardFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias, activation):
+        y, saved = ops.gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias, activation, want_saved=True)
+        ctx.save_for_backward(x, gate_weight, up_weight, down_weight, saved)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        return ops.gated_feed_forward_backward(*ctx.saved_tensors, grad, ctx.activation, ctx.needs_input_grad[:7]) + (None,)
+
+
+def gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=None, down_bias=None, activation="silu"):
+    """The gated feed-forward block of a transformer: (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd.  x [..., C], weights as torch's Linear has them (Wg, Wu [F, C], Wd [O, F]),
+    biases [F], [F], [O] or None, all float32 or all bf16; activation "silu" or "gelu" (with the error function).  Differentiable in all tensors.  Sums are float32; with bf16 the
+    hidden values, and in the backward pass their gradients, are rounded to bf16 between the products.  Gradients are the same bits every time, whichever are asked for."""
+    leaves = (x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias)
+    _no_tangents("gated_feed_forward", *leaves)
+    if _wants_grad(*leaves):
+        return _FeedForwardFunction.apply(*leaves, activation)
+    return ops.gated_feed_forward(*leaves, activation)[0]
+
+
 def check():
     """Synchronise the current stream and raise if an attention launch on the current device since the last check, forward or backward, gave up on a bounded wait."""
     ops.attention_check()
@@ -205,6 +295,59 @@ class CrossAttention(nn.Module):
         if positions is not None:
             q = self.rotary(q, positions, prefix)
         return self.out(cross_attention(q, *kv, key_lengths=key_lengths, key_mask=key_mask).flatten(2))
+
+
+class TokenRMSNorm(nn.Module):
+    """Root-mean-square norm with a weight (torch's RMSNorm by parameters and state dict).  Called with a residual it returns (norm of the sum, sum)."""
+
+    def __init__(self, dim, eps=1e-6, device="cuda", dtype=None):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim, device=device, dtype=dtype))
+
+    def forward(self, x, residual=None):
+        return rms_norm(x, self.weight, self.eps, residual)
+
+
+class GatedFeedForward(nn.Module):
+    """A block's gated feed-forward half: `gate`, `up` and `down` are torch's Linear by parameters and state dict; their values are taken in x's type."""
+
+    def __init__(self, dim, hidden, activation="silu", bias=True, device="cuda", dtype=None):
+        super().__init__()
+        if activation not in ops.ACTIVATIONS:
+            raise ValueError(f"activation is {activation!r}: 'silu' or 'gelu'")
+        kw = dict(bias=bias, device=device, dtype=dtype)
+        self.activation = activation
+        self.gate, self.up, self.down = nn.Linear(dim, hidden, **kw), nn.Linear(dim, hidden, **kw), nn.Linear(hidden, dim, **kw)
+
+    def forward(self, x):
+        layers = (self.gate, self.up, self.down)
+        return gated_feed_forward(x, *(m.weight.to(x.dtype) for m in layers), *(None if m.bias is None else m.bias.to(x.dtype) for m in layers), activation=self.activation)
+
+
+class Linear8(nn.Module):
+    """A linear layer for serving in 8 bits, made from torch's Linear: its weight with a scale for each output channel, its input with one for each token.  Called with a tensor, which it
+    quantises, or with the (q, scale) of rms_norm_int8 or quantize.  The result has `out_dtype`."""
+
+    def __init__(self, linear, out_dtype=torch.bfloat16):
+        super().__init__()
+        self.out_dtype = out_dtype
+        q, scale = quantize(linear.weight.detach())
+        self.register_buffer("weight", q)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().to(torch.float32, copy=True))
+
+    def _apply(self, fn, recurse=True):      # scales and bias stay float32 when the model is cast
+        kept = self.weight_scale, self.bias
+        super()._apply(fn, recurse)
+        for name, t in zip(("weight_scale", "bias"), kept):
+            if t is not None and getattr(self, name).dtype != torch.float32:
+                setattr(self, name, t.to(getattr(self, name).device))
+        return self
+
+    def forward(self, x, scale=None):
+        q, scale = quantize(x) if scale is None else (x, scale)
+        return linear_int8(q, scale, self.weight, self.weight_scale, self.bias, self.out_dtype)
 
 
 class FixationReader(nn.Module):

@@ -502,6 +502,41 @@ int fovi_attention_backward_selftest_wait_timeout(const void* q, const void* k, 
                                                   const int64_t* strides, float scale, const float* lse, void* dq, void* dk, void* dv, void* work, int64_t work_bytes,
                                                   void* stream);
 
+/* Root-mean-square norm over the last axis of `rows` rows of C elements (dtype; x_stride elements apart), of x or, with residual (same type, rows residual_stride
+ * apart), of total = x + residual rounded to their type, which is written (contiguous; NULL where residual is):  y = t / sqrt(mean(t^2) + eps) * weight.
+ * weight: DEVICE float32 [C] or NULL.  Either y (contiguous, same type), or q and scale: the result in 8 bits, y = q * scale, scale = max(max |y| / 127, smallest normal
+ * number) of the row, q rounded from the unrounded y; rows of q q_stride bytes apart.  A row that holds infinity or not-a-number has one of them as its scale.
+ * rstd: float32 [rows], 1 / sqrt(mean(t^2) + eps), or NULL. */
+int fovi_rms_norm_forward(const void* x, int dtype, int64_t rows, int C, int64_t x_stride, const void* residual, int64_t residual_stride, const float* weight, float eps,
+                          void* total, void* y, int8_t* q, int64_t q_stride, float* scale, float* rstd, void* stream);
+/* Its gradients from t (x, or total), dy (rows dy_stride apart), the gradient dt of total itself (or NULL) and the forward's rstd, all of one type: dx (contiguous; the residual's
+ * gradient too) and dweight (float32 [C]); each may be NULL.  work: fovi_rms_norm_workspace_bytes bytes, where dweight is wanted.  The same bits every time. */
+int64_t fovi_rms_norm_workspace_bytes(int64_t rows, int C);
+int fovi_rms_norm_backward(const void* t, int dtype, int64_t rows, int C, int64_t t_stride, const void* dy, int64_t dy_stride, const void* dt, int64_t dt_stride,
+                           const float* weight, const float* rstd, void* dx, float* dweight, void* work, int64_t work_bytes, void* stream);
+/* Rows in 8 bits with a scale each, as above, without a norm. */
+int fovi_quantize_rows(const void* x, int dtype, int64_t rows, int C, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, void* stream);
+
+/* y[m, n] = scale[m] * weight_scale[n] * sum over k of q[m, k] * weight[n, k] + bias[n]: q [tokens, K], weight [N, K] 8-bit integers (rows q_stride, weight_stride bytes
+ * apart), exact 32-bit sums (K < 131072); scale [tokens], weight_scale [N], bias [N] or NULL float32; y contiguous [tokens, N] float32 or bf16. */
+int fovi_linear_int8(const int8_t* q, int64_t tokens, int K, int64_t q_stride, const float* scale, const int8_t* weight, int N, int64_t weight_stride,
+                     const float* weight_scale, const float* bias, void* y, int y_dtype, void* stream);
+
+/* Gated feed-forward block: g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) * u, y = h Wd^T + bd; x [tokens, C], Wg, Wu [F, C], Wd [O, F], biases [F], [F], [O] (contiguous) or NULL,
+ * y contiguous [tokens, O], all of one type; strides: elements from one row to the next.  activation 0: act(g) = g / (1 + exp(-g)), 1: g times the normal distribution
+ * function.  saved: fovi_gated_ffn_saved_bytes bytes for the backward pass, or NULL (then work holds fovi_gated_ffn_workspace_bytes(.., 0) bytes).
+ * Backward: each gradient may be NULL; all are of the block's type, contiguous, and have the same bits every time, whichever are asked for.
+ * work: fovi_gated_ffn_workspace_bytes(.., 1) bytes. */
+int64_t fovi_gated_ffn_saved_bytes(int dtype, int64_t tokens, int F);
+int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int backward);
+int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
+                           const void* up_weight, int64_t up_stride, const void* down_weight, int64_t down_stride, const void* gate_bias, const void* up_bias,
+                           const void* down_bias, int activation, void* y, void* saved, void* work, int64_t work_bytes, void* stream);
+int fovi_gated_ffn_backward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
+                            const void* up_weight, int64_t up_stride, const void* down_weight, int64_t down_stride, int activation, const void* saved, const void* dy,
+                            int64_t dy_stride, void* dx, void* dgate_weight, void* dup_weight, void* ddown_weight, void* dgate_bias, void* dup_bias, void* ddown_bias,
+                            void* work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
