@@ -96,6 +96,8 @@ SIGNATURES = {
     "fovi_rms_norm_backward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P, _P, _P, _P, C.c_int64, _P]),
     "fovi_quantize_rows": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int64, _P, C.c_int64, _P, _P]),
     "fovi_linear_int8": (C.c_int, [_P, C.c_int64, C.c_int, C.c_int64, _P, _P, C.c_int, C.c_int64, _P, _P, _P, C.c_int, _P]),
+    "fovi_linear_int8_selftest_wait_timeout": (C.c_int, [_P, C.c_int64, C.c_int, C.c_int64, _P, _P, C.c_int, C.c_int64, _P, _P, _P, C.c_int, _P]),
+    "fovi_product_check": (C.c_int, [_P]),
     "fovi_gated_ffn_saved_bytes": (C.c_int64, [C.c_int, C.c_int64, C.c_int]),
     "fovi_gated_ffn_workspace_bytes": (C.c_int64, [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int]),
     "fovi_gated_ffn_forward": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int64] + [_P, C.c_int64] * 3 + [_P] * 3 + [C.c_int, _P, _P, _P, C.c_int64, _P]),

@@ -4,15 +4,15 @@
 //   dh = dy Wd,  dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h,  and column sums of dg, du, dy for the biases.
 #include <algorithm>
 
-#include "product.cuh"
 #include "product_simt.cuh"
+#include "product_tc.cuh"
 
 using fovi::Hidden;
 using fovi::Operand;
+using fovi::TcMatrix;
+using fovi::TcTask;
 
 namespace {
-
-template <typename T> __device__ __forceinline__ float bias_at(const void* b, int n) { return b ? ld_as_float(static_cast<const T*>(b) + n) : 0.f; }
 
 // act(g) and act'(g)
 __device__ __forceinline__ float2 activate(float g, int act) {
@@ -24,50 +24,34 @@ __device__ __forceinline__ float2 activate(float g, int act) {
   return make_float2(g * p, fmaf(g * 0.39894228040143268f, expf(-0.5f * g * g), p));
 }
 
-template <typename T> struct GateUp {       // g and u -> h
-  Hidden to; const void *bg, *bu; int act;
+struct GateUp {       // g and u -> h
+  Hidden to; const float *bg, *bu; int act;
   __device__ __forceinline__ void operator()(int64_t m, int n, float g, float u) const {
-    g += bias_at<T>(bg, n);
-    u += bias_at<T>(bu, n);
+    g += bg ? __ldg(bg + n) : 0.f;
+    u += bu ? __ldg(bu + n) : 0.f;
     const int64_t at = m * to.pitch + n;
     if (to.g) {
-      if (sizeof(T) == 4) {
-        static_cast<float*>(to.g)[at] = g;
-        static_cast<float*>(to.u)[at] = u;
-      } else {
-        const uint32_t gb = __float_as_uint(g), ub = __float_as_uint(u);
-        static_cast<uint16_t*>(to.g)[at] = gb >> 16;
-        static_cast<uint16_t*>(to.u)[at] = ub >> 16;
-        to.g_low[at] = gb >> 8;
-        to.u_low[at] = ub >> 8;
-      }
+      static_cast<float*>(to.g)[at] = g;
+      static_cast<float*>(to.u)[at] = u;
     }
-    static_cast<T*>(to.h)[at] = from_float<T>(activate(g, act).x * u);
+    static_cast<float*>(to.h)[at] = activate(g, act).x * u;
   }
 };
-template <typename T> struct HiddenGrad {   // dh -> dg, du
-  Hidden from; T *dg, *du; int act;
+struct HiddenGrad {   // dh -> dg, du
+  Hidden from; float *dg, *du; int act;
   __device__ __forceinline__ void operator()(int64_t m, int n, float dh, float) const {
     const int64_t at = m * from.pitch + n;
-    float g, u;
-    if (sizeof(T) == 4) {
-      g = static_cast<const float*>(from.g)[at];
-      u = static_cast<const float*>(from.u)[at];
-    } else {
-      g = upper24(static_cast<const uint16_t*>(from.g)[at], from.g_low[at]);
-      u = upper24(static_cast<const uint16_t*>(from.u)[at], from.u_low[at]);
-    }
-    const float2 s = activate(g, act);
-    dg[at] = from_float<T>(dh * u * s.y);
-    du[at] = from_float<T>(dh * s.x);
+    const float2 s = activate(static_cast<const float*>(from.g)[at], act);
+    dg[at] = dh * static_cast<const float*>(from.u)[at] * s.y;
+    du[at] = dh * s.x;
   }
 };
-template <typename T> struct Store {
-  T* y; int64_t pitch; const void* bias;
-  __device__ __forceinline__ void operator()(int64_t m, int n, float v, float) const { y[m * pitch + n] = from_float<T>(v + bias_at<T>(bias, n)); }
+struct Store {
+  float* y; int64_t pitch; const float* bias;
+  __device__ __forceinline__ void operator()(int64_t m, int n, float v, float) const { y[m * pitch + n] = v + (bias ? __ldg(bias + n) : 0.f); }
 };
 
-// Column sums of [rows, n] in a fixed order: parts of 64 rows' strips, then their sum.
+// Column sums of [rows, n] in a fixed order: parts of strips of rows, then the parts of a column.
 template <typename T>
 __global__ void __launch_bounds__(128) column_parts_kernel(const T* x, int64_t rows, int n, int64_t pitch, int strips, float* part) {
   const int c = blockIdx.x * 128 + threadIdx.x;
@@ -77,12 +61,12 @@ __global__ void __launch_bounds__(128) column_parts_kernel(const T* x, int64_t r
   part[(size_t)blockIdx.y * n + c] = s;
 }
 template <typename T>
-__global__ void __launch_bounds__(1024) column_join_kernel(const float* part, int parts, int n, T* out) {
+__global__ void __launch_bounds__(1024) column_join_kernel(const float* part, int parts, int n, int64_t pitch, T* out) {
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
   if (c < n)
-    for (int p = w; p < parts; p += 32) s += part[(size_t)p * n + c];
+    for (int p = w; p < parts; p += 32) s += part[p * pitch + c];
   red[w][lane] = s;
   __syncthreads();
   if (w || c >= n) return;
@@ -91,13 +75,15 @@ __global__ void __launch_bounds__(1024) column_join_kernel(const float* part, in
   out[c] = from_float<T>(s);
 }
 constexpr int STRIPS = 64;
+template <typename T> int column_join(const float* part, int parts, int n, int64_t pitch, void* out, cudaStream_t st) {
+  column_join_kernel<T><<<(n + 31) / 32, 1024, 0, st>>>(part, parts, n, pitch, static_cast<T*>(out));
+  return fovi::after_launch("column_join_kernel");
+}
 template <typename T> int column_sums(const void* x, int64_t rows, int n, int64_t pitch, float* part, void* out, cudaStream_t st) {
   const int strips = (int)std::min<int64_t>(STRIPS, rows);
   column_parts_kernel<T><<<dim3((n + 127) / 128, strips), 128, 0, st>>>(static_cast<const T*>(x), rows, n, pitch, strips, part);
   const int rc = fovi::after_launch("column_parts_kernel");
-  if (rc) return rc;
-  column_join_kernel<T><<<(n + 31) / 32, 1024, 0, st>>>(part, strips, n, static_cast<T*>(out));
-  return fovi::after_launch("column_join_kernel");
+  return rc ? rc : column_join<T>(part, strips, n, n, out, st);
 }
 
 int64_t pitch_of(int F) { return ((int64_t)F + 31) / 32 * 32; }
@@ -122,25 +108,33 @@ struct Block {
   int64_t M, xs, gs, us, ds; int C, F, O, act;
 };
 
-template <typename T> int forward(const Block& b, void* y, const Hidden& hid, cudaStream_t st) {
+int forward_f32(const Block& b, void* y, const Hidden& hid, cudaStream_t st) {
   SimtArgs p{};
   p.m = b.M; p.n = b.F; p.k[0] = b.C; p.segments = 1;
   p.a[0] = Operand{b.x, b.xs, 1};
   p.b[0] = Operand{b.wg, b.gs, 1};
   p.b2 = Operand{b.wu, b.us, 1};
-  int rc = product_simt<T, true>(p, GateUp<T>{hid, b.bg, b.bu, b.act}, st);
+  int rc = product_simt<float, true>(p, GateUp{hid, static_cast<const float*>(b.bg), static_cast<const float*>(b.bu), b.act}, st);
   if (rc) return rc;
   p.n = b.O; p.k[0] = b.F;
   p.a[0] = Operand{hid.h, hid.pitch, 1};
   p.b[0] = Operand{b.wd, b.ds, 1};
-  return product_simt<T, false>(p, Store<T>{static_cast<T*>(y), b.O, b.bd}, st);
+  return product_simt<float, false>(p, Store{static_cast<float*>(y), b.O, static_cast<const float*>(b.bd)}, st);
+}
+
+// The parts of a workspace, each on a boundary of 256 bytes.
+int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int forward_bf16(const Block& b, void* y, const Hidden& hid, void* work, cudaStream_t st) {
+  const TcMatrix x{b.x, b.M, b.C, b.xs}, wg{b.wg, b.F, b.C, b.gs}, wu{b.wu, b.F, b.C, b.us}, wd{b.wd, b.O, b.F, b.ds}, h{hid.h, b.M, b.F, hid.pitch};
+  const int rc = fovi::tc_gated(x, wg, wu, b.bg, b.bu, b.act, hid, st);
+  return rc ? rc : fovi::tc_linear(h, wd, nullptr, nullptr, false, (int)b.M, b.O, b.bd, y, work, st);
 }
 
 struct Grads { const void* dy; int64_t dys; void *dx, *dwg, *dwu, *dwd, *dbg, *dbu, *dbd; };
 
-template <typename T> int backward(const Block& b, const Hidden& hid, const Grads& g, char* work, cudaStream_t st) {
-  T *dg = reinterpret_cast<T*>(work), *du = dg + b.M * hid.pitch;
-  float* part = reinterpret_cast<float*>(du + b.M * hid.pitch);
+int backward_f32(const Block& b, const Hidden& hid, const Grads& g, char* work, cudaStream_t st) {
+  float *dg = reinterpret_cast<float*>(work), *du = dg + b.M * hid.pitch, *part = du + b.M * hid.pitch;
   int rc;
   SimtArgs p{};
   p.segments = 1;
@@ -148,13 +142,13 @@ template <typename T> int backward(const Block& b, const Hidden& hid, const Grad
     p.m = b.M; p.n = b.F; p.k[0] = b.O;
     p.a[0] = Operand{g.dy, g.dys, 1};
     p.b[0] = Operand{b.wd, 1, b.ds};
-    if ((rc = product_simt<T, false>(p, HiddenGrad<T>{hid, dg, du, b.act}, st))) return rc;
+    if ((rc = product_simt<float, false>(p, HiddenGrad{hid, dg, du, b.act}, st))) return rc;
   }
   if (g.dx) {
     p.m = b.M; p.n = b.C; p.k[0] = p.k[1] = b.F; p.segments = 2;
     p.a[0] = Operand{dg, hid.pitch, 1}; p.a[1] = Operand{du, hid.pitch, 1};
     p.b[0] = Operand{b.wg, 1, b.gs}; p.b[1] = Operand{b.wu, 1, b.us};
-    if ((rc = product_simt<T, false>(p, Store<T>{static_cast<T*>(g.dx), b.C, nullptr}, st))) return rc;
+    if ((rc = product_simt<float, false>(p, Store{static_cast<float*>(g.dx), b.C, nullptr}, st))) return rc;
   }
   p.segments = 1;
   p.k[0] = (int)b.M;
@@ -165,12 +159,58 @@ template <typename T> int backward(const Block& b, const Hidden& hid, const Grad
     p.m = w.m; p.n = w.n;
     p.a[0] = Operand{w.a, 1, w.as};
     p.b[0] = Operand{w.b, 1, w.bs};
-    if ((rc = product_simt<T, false>(p, Store<T>{static_cast<T*>(w.to), w.n, nullptr}, st))) return rc;
+    if ((rc = product_simt<float, false>(p, Store{static_cast<float*>(w.to), w.n, nullptr}, st))) return rc;
   }
-  if (g.dbg && (rc = column_sums<T>(dg, b.M, b.F, hid.pitch, part, g.dbg, st))) return rc;
-  if (g.dbu && (rc = column_sums<T>(du, b.M, b.F, hid.pitch, part, g.dbu, st))) return rc;
-  if (g.dbd && (rc = column_sums<T>(g.dy, b.M, b.O, g.dys, part, g.dbd, st))) return rc;
+  if (g.dbg && (rc = column_sums<float>(dg, b.M, b.F, hid.pitch, part, g.dbg, st))) return rc;
+  if (g.dbu && (rc = column_sums<float>(du, b.M, b.F, hid.pitch, part, g.dbu, st))) return rc;
+  if (g.dbd && (rc = column_sums<float>(g.dy, b.M, b.O, g.dys, part, g.dbd, st))) return rc;
   return FOVI_OK;
+}
+
+// The three weight gradients as products over the tokens.
+void weight_tasks(const Block& b, const Hidden& hid, const Grads& g, const void* dg, const void* du, TcTask (&t)[3]) {
+  t[0] = TcTask{{dg, b.M, b.F, hid.pitch}, {b.x, b.M, b.C, b.xs}, b.F, b.C, g.dwg};
+  t[1] = TcTask{{du, b.M, b.F, hid.pitch}, {b.x, b.M, b.C, b.xs}, b.F, b.C, g.dwu};
+  t[2] = TcTask{{g.dy, b.M, b.O, g.dys}, {hid.h, b.M, b.F, hid.pitch}, b.O, b.F, g.dwd};
+}
+
+// Work of a bf16 backward pass: dg, du; then, one after another in the same place, the parts of dx, of the weight gradients, and of the biases' sums of dy.  The sums of
+// dg and du, which the first kernel leaves, have a place of their own.
+struct BackWork { int64_t sums, parts, bytes; };
+BackWork back_work(const Block& b, int64_t pitch) {
+  TcTask t[3];
+  weight_tasks(b, Hidden{}, Grads{}, nullptr, nullptr, t);
+  BackWork w;
+  w.sums = padded(2 * b.M * pitch * 2);
+  w.parts = w.sums + padded(fovi::tc_sum_rows(b.M) * 2 * pitch * 4);
+  w.bytes = w.parts + std::max({fovi::tc_linear_bytes(b.M, b.C, 2ll * b.F), fovi::tc_weight_grads_bytes(t, 3, b.M), (int64_t)STRIPS * b.O * 4});
+  return w;
+}
+
+int backward_bf16(const Block& b, const Hidden& hid, const Grads& g, char* work, cudaStream_t st) {
+  const BackWork at = back_work(b, hid.pitch);
+  __nv_bfloat16 *dg = reinterpret_cast<__nv_bfloat16*>(work), *du = dg + b.M * hid.pitch;
+  float *sums = reinterpret_cast<float*>(work + at.sums), *parts = reinterpret_cast<float*>(work + at.parts);
+  const TcMatrix dy{g.dy, b.M, b.O, g.dys}, wg{b.wg, b.F, b.C, b.gs}, wu{b.wu, b.F, b.C, b.us}, wd{b.wd, b.O, b.F, b.ds};
+  const TcMatrix dgm{dg, b.M, b.F, hid.pitch}, dum{du, b.M, b.F, hid.pitch};
+  int rc;
+  if (g.dx || g.dwg || g.dwu || g.dbg || g.dbu) {
+    if ((rc = fovi::tc_hidden_grad(dy, wd, hid, b.act, dg, du, g.dbg || g.dbu ? sums : nullptr, st))) return rc;
+  }
+  if (g.dx && (rc = fovi::tc_linear(dgm, wg, &dum, &wu, true, (int)b.M, b.C, nullptr, g.dx, parts, st))) return rc;
+  TcTask t[3];
+  weight_tasks(b, hid, g, dg, du, t);
+  if ((rc = fovi::tc_weight_grads(t, 3, b.M, parts, st))) return rc;
+  const int rows = (int)fovi::tc_sum_rows(b.M);
+  if (g.dbg && (rc = column_join<__nv_bfloat16>(sums, rows, b.F, 2 * hid.pitch, g.dbg, st))) return rc;
+  if (g.dbu && (rc = column_join<__nv_bfloat16>(sums + hid.pitch, rows, b.F, 2 * hid.pitch, g.dbu, st))) return rc;
+  if (g.dbd && (rc = column_sums<__nv_bfloat16>(g.dy, b.M, b.O, g.dys, parts, g.dbd, st))) return rc;
+  return FOVI_OK;
+}
+
+// bf16 rows as the tensor copies want them.
+bool aligned(const Block& b) {
+  return fovi::tc_takes(b.x, b.xs, 2) && fovi::tc_takes(b.wg, b.gs, 2) && fovi::tc_takes(b.wu, b.us, 2) && fovi::tc_takes(b.wd, b.ds, 2);
 }
 
 bool valid(int dtype, int64_t M, int C, int F, int O) { return fovi::valid_dtype(dtype) && M >= 0 && M <= (1 << 30) && C >= 1 && F >= 1 && O >= 1; }
@@ -182,10 +222,14 @@ extern "C" int64_t fovi_gated_ffn_saved_bytes(int dtype, int64_t tokens, int F) 
   return tokens * pitch_of(F) * (dtype == FOVI_BF16 ? 8 : 12);
 }
 
-extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int backward) {
-  if (!valid(dtype, tokens, C, F, O)) return -1;
+extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int phase) {
+  if (!valid(dtype, tokens, C, F, O) || phase < 0 || phase > 2) return -1;
   const int64_t n = tokens * pitch_of(F) * (int64_t)fovi::dtype_size(dtype);
-  return backward ? 2 * n + (int64_t)STRIPS * std::max(F, O) * 4 : n;
+  if (dtype == FOVI_F32) return phase == 1 ? 2 * n + (int64_t)STRIPS * std::max(F, O) * 4 : phase == 0 ? n : 0;
+  if (phase != 1) return (phase == 0 ? padded(n) : 0) + fovi::tc_linear_bytes(tokens, O, F);
+  Block b{};
+  b.M = tokens; b.C = C; b.F = F; b.O = O;
+  return back_work(b, pitch_of(F)).bytes;
 }
 
 extern "C" int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
@@ -194,11 +238,14 @@ extern "C" int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, 
   if (!valid(dtype, tokens, C, F, O) || activation < 0 || activation > 1 || x_stride < 0 || gate_stride < 0 || up_stride < 0 || down_stride < 0) return FOVI_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return FOVI_OK;
   if (!x || !gate_weight || !up_weight || !down_weight || !y) return FOVI_ERR_INVALID_ARGUMENT;
-  if (!saved && (!work || work_bytes < fovi_gated_ffn_workspace_bytes(dtype, tokens, C, F, O, 0))) return FOVI_ERR_INVALID_ARGUMENT;
+  const int64_t need = fovi_gated_ffn_workspace_bytes(dtype, tokens, C, F, O, saved ? 2 : 0);
+  if (work_bytes < need || (need && !work)) return FOVI_ERR_INVALID_ARGUMENT;
   const Block b{x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias, tokens, x_stride, gate_stride, up_stride, down_stride, C, F, O, activation};
   const Hidden h = hidden_at(saved ? saved : work, dtype, tokens, F, saved != nullptr);
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == FOVI_BF16 ? forward<__nv_bfloat16>(b, y, h, st) : forward<float>(b, y, h, st);
+  if (dtype == FOVI_F32) return forward_f32(b, y, h, st);
+  if (!aligned(b) || reinterpret_cast<uintptr_t>(y) % 16) return FOVI_ERR_ALIGNMENT;
+  return forward_bf16(b, y, h, static_cast<char*>(work) + (saved ? 0 : padded(tokens * h.pitch * 2)), st);
 }
 
 extern "C" int fovi_gated_ffn_backward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
@@ -221,5 +268,9 @@ extern "C" int fovi_gated_ffn_backward(const void* x, int dtype, int64_t tokens,
   const Block b{x, gate_weight, up_weight, down_weight, nullptr, nullptr, nullptr, tokens, x_stride, gate_stride, up_stride, down_stride, C, F, O, activation};
   const Hidden h = hidden_at(const_cast<void*>(saved), dtype, tokens, F, true);
   const Grads g{dy, dy_stride, dx, dgate_weight, dup_weight, ddown_weight, dgate_bias, dup_bias, ddown_bias};
-  return dtype == FOVI_BF16 ? backward<__nv_bfloat16>(b, h, g, static_cast<char*>(work), st) : backward<float>(b, h, g, static_cast<char*>(work), st);
+  if (dtype == FOVI_F32) return backward_f32(b, h, g, static_cast<char*>(work), st);
+  if (!aligned(b) || !fovi::tc_takes(dy, dy_stride, 2)) return FOVI_ERR_ALIGNMENT;
+  for (const void* p : {dx, dgate_weight, dup_weight, ddown_weight})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return FOVI_ERR_ALIGNMENT;
+  return backward_bf16(b, h, g, static_cast<char*>(work), st);
 }

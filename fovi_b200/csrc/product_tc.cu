@@ -1,0 +1,671 @@
+// Matrix products of a token block on the tensor cores.
+//
+//   D[256 rows, ct columns] = sum over k of A[row, k] B[column, k]          bf16 with float32 sums, or 8-bit integers with 32-bit integer sums
+//
+// A cluster of two CTAs shares a tile (tcgen05.mma with cta_group::2, M = 256): each stages its 128 rows of A and half of B's ct rows, 128 bytes of k (64 bf16, 128 integers) a stage,
+// by tensor copies.  An operand whose k is contiguous is K-major; one that lies the other way round (weights in the input gradients, both operands of a weight gradient) is read MN-major,
+// as 64-column boxes, so nothing is transposed in memory.  Two accumulators in tensor memory: a tile's epilogue runs under the next one's products.
+// Persistent: a pair takes every 74th tile.  Roles: warps 0-7 epilogue (a row per thread, the two halves take turns on 32-column chunks), warp 8 MMAs (of the pair's first CTA), warp 9 copies.
+// All waits are bounded.
+//
+// What becomes of a tile:
+//   GATED    accumulator columns of the first half are g, of the second u, since the first CTA stages rows of Wg and the second the same rows of Wu: h = act(g) u
+//   GRAD     the tile is dh; g and u are read, dg and du written
+//   STORE    bf16 result with a bias, or with k in parts a float32 part, joined by a second kernel in their order
+//   SCALED   integer sums times the scales
+#include <algorithm>
+
+#include "product_tc.cuh"
+#include "tc_common.cuh"
+
+using fovi::Hidden;
+using fovi::TcMatrix;
+using fovi::TcShape;
+using fovi::TcTask;
+
+namespace {
+
+__device__ int g_status;           // wait site at which a kernel gave up, see fovi_product_check: one word per device
+
+enum { GATED = 0, GRAD = 1, STORE = 2, SCALED = 3 };
+constexpr int EPI_WARPS = 8, PT_THREADS = (EPI_WARPS + 2) * 32;
+constexpr uint32_t A_BYTES = 16384, STAGE_BYTES = 2 * A_BYTES;      // a CTA's 128 rows of A and up to 128 rows of B
+constexpr int STAGES = 6, GROUPS = 3;
+constexpr uint32_t SCRATCH = 32 * 17 * 4;                            // of an epilogue warp: 32 rows x 16 columns (odd pitch), or 64 biases
+constexpr uint32_t PT_SMEM = 1024 + 1024 + EPI_WARPS * SCRATCH + STAGES * STAGE_BYTES;
+static_assert(PT_SMEM <= 227 * 1024 && SCRATCH * EPI_WARPS % 1024 == 0, "");
+
+struct PtMaps { CUtensorMap a[GROUPS], b[GROUPS]; };       // of each task, or of each segment of k
+
+struct PtArgs {
+  int tasks, first[GROUPS + 1];            // tiles first[t] .. first[t + 1] - 1 belong to task t
+  int n_mt[GROUPS], n_nt[GROUPS], m[GROUPS], n[GROUPS];
+  void* y[GROUPS];
+  int64_t part[GROUPS];                    // parts of k: where a task's begin in `work` (float32)
+  int kb0, kb, splits;                     // stages of the first segment of k, of all, parts
+  int ct;
+  const void *bias, *bias2; int act;
+  Hidden hidden; void *dg, *du; float* sums;
+  const float *scale, *wscale, *bias_f; int y_f32;
+  float* work;
+  int* status; uint32_t wait_limit; int skip_loads;
+};
+
+struct PtHeader {
+  uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__device__ __forceinline__ uint32_t pt_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t pt_map(uint32_t local, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void pt_sync() { asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void pt_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+template <bool I8> __device__ __forceinline__ void pt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (I8)
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pt_commit(uint32_t bar) {            // on the barrier at this offset in both CTAs
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void load_global_32(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+}
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ void st_global_32f(float* p, const uint32_t* v) {
+  const uint32_t w[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+  st_global_32(p, w);
+}
+
+// act(g) and act'(g), to a few units of float32: what is rounded to bf16 behind them.
+__device__ __forceinline__ float2 fast_act(float g, int act) {
+  if (act == fovi::ACT_SILU) {
+    const float p = __fdividef(1.f, 1.f + __expf(-g)), a = g * p;
+    return make_float2(a, fmaf(a, 1.f - p, p));
+  }
+  const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+  return make_float2(g * p, fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), p));
+}
+
+// Sums over the warp's 32 lanes (rows) of 32 columns, by halving exchanges: lane l ends with column l's.
+__device__ __forceinline__ float column_sums(float (&c)[32], int lane) {
+  const bool up16 = lane & 16, up8 = lane & 8, up4 = lane & 4, up2 = lane & 2, up1 = lane & 1;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) c[i] = (up16 ? c[i + 16] : c[i]) + __shfl_xor_sync(0xffffffffu, up16 ? c[i] : c[i + 16], 16);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = (up8 ? c[i + 8] : c[i]) + __shfl_xor_sync(0xffffffffu, up8 ? c[i] : c[i + 8], 8);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = (up4 ? c[i + 4] : c[i]) + __shfl_xor_sync(0xffffffffu, up4 ? c[i] : c[i + 4], 4);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) c[i] = (up2 ? c[i + 2] : c[i]) + __shfl_xor_sync(0xffffffffu, up2 ? c[i] : c[i + 2], 2);
+  return (up1 ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, up1 ? c[0] : c[1], 1);
+}
+
+struct Tile { int task, mt, nt, k0, k1, split; };
+__device__ __forceinline__ Tile tile_of(const PtArgs& a, int item) {
+  Tile t;
+  t.task = 0;
+  if (a.tasks > 1) t.task = item >= a.first[2] ? 2 : item >= a.first[1] ? 1 : 0;
+  int r = item - a.first[t.task];
+  t.nt = r % a.n_nt[t.task];
+  r /= a.n_nt[t.task];
+  t.mt = r % a.n_mt[t.task];
+  t.split = r / a.n_mt[t.task];
+  t.k0 = (int)((int64_t)a.kb * t.split / a.splits);
+  t.k1 = (int)((int64_t)a.kb * (t.split + 1) / a.splits);
+  return t;
+}
+
+// 32 columns of a row tile of 32 rows (a row per lane) into [m, n] with no alignment: through the warp's scratch, so that lanes write neighbouring columns.
+template <typename T> __device__ __forceinline__ void store_any(T* y, int64_t n, int64_t row0, int64_t m, int c0, const float* v, float* scratch, int lane) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) scratch[lane * 17 + i] = v[16 * h + i];
+    __syncwarp();
+    const int c = c0 + 16 * h + (lane & 15);
+    for (int r = lane >> 4; r < 32; r += 2)
+      if (row0 + r < m && c < n) y[(row0 + r) * n + c] = from_float<T>(scratch[r * 17 + (lane & 15)]);
+  }
+  __syncwarp();
+}
+
+template <int EPI, bool A_MN, bool B_MN, bool I8>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) product_tc_kernel(const __grid_constant__ PtMaps maps, const __grid_constant__ PtArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  PtHeader* hdr = reinterpret_cast<PtHeader*>(smem_raw + (base - raw));
+  const uint32_t stages0 = base + 1024u + EPI_WARPS * SCRATCH;
+  volatile int* abort_flag = &hdr->abort_flag;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = (int)pt_rank(), worker = blockIdx.x >> 1, workers = gridDim.x >> 1;
+  const int half = a.ct / 2, total = a.first[a.tasks];
+  constexpr int KS = I8 ? 128 : 64;               // values of k a stage
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->acc_full[i]), 1); mbar_init(smem_u32(&hdr->acc_empty[i]), 2 * EPI_WARPS); }
+    mbar_init(smem_u32(&hdr->drain), 1);
+    hdr->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == EPI_WARPS) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&hdr->tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  tc_fence_before();
+  pt_sync();
+  tc_fence_after();
+  const uint32_t tmem = hdr->tmem_base;
+
+  if (warp == EPI_WARPS + 1) {
+    // ------------------------------------------------------------ copies
+    const uint32_t b_bytes = B_MN ? (uint32_t)((half + 63) / 64) * 8192u : (uint32_t)half * 128u;
+    uint32_t s = 0, ph = 0;
+    bool ok = !a.skip_loads;
+    for (int item = worker; item < total && ok; item += workers) {
+      const Tile t = tile_of(a, item);
+      const int m0 = t.mt * 256 + rank * 128, n0 = EPI == GATED ? t.nt * half : t.nt * a.ct + rank * half;
+      for (int kb = t.k0; kb < t.k1; ++kb) {
+        ok = mbar_wait_warp(smem_u32(&hdr->empty[s]), ph ^ 1u, abort_flag, a.status, 41, a.wait_limit);
+        if (!ok) break;
+        const int seg = kb >= a.kb0 ? 1 : 0, k = (kb - (seg ? a.kb0 : 0)) * KS;
+        const CUtensorMap *ma = &maps.a[t.task + seg], *mb = &maps.b[EPI == GATED ? rank : t.task + seg];
+        const uint32_t full = pt_map(smem_u32(&hdr->full[s]), 0), sa = stages0 + s * STAGE_BYTES, sb = sa + A_BYTES;
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(smem_u32(&hdr->full[s]), 2u * (A_BYTES + b_bytes));      // of both CTAs
+          if (A_MN) {
+            pt_load(sa, ma, full, m0, k);
+            pt_load(sa + 8192u, ma, full, m0 + 64, k);
+          } else {
+            pt_load(sa, ma, full, k, m0);
+          }
+          if (B_MN) {
+            for (int j = 0; j < half; j += 64) pt_load(sb + j * 128u, mb, full, n0 + j, k);
+          } else {
+            pt_load(sb, mb, full, k, n0);
+          }
+        }
+        __syncwarp();
+        if (++s == STAGES) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (lane == 0 && *abort_flag) {
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);    // copies in flight land before this CTA's shared memory goes away
+    }
+  } else if (warp == EPI_WARPS) {
+    // ------------------------------------------------------------ products (see elect_one)
+    if (rank == 0) {
+      const uint32_t idesc = (I8 ? 2u << 4 : 1u << 4) | (1u << 7) | (1u << 10) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) | ((uint32_t)(a.ct >> 3) << 17) | (16u << 24);
+      const uint64_t desc_a = smem_desc(0, A_MN ? 8192u : 16u, 1024u, 2u), desc_b = smem_desc(0, B_MN ? 8192u : 16u, 1024u, 2u);
+      const uint32_t u_stages0 = warp_uniform(stages0), u_tmem = warp_uniform(tmem);
+      uint32_t s = 0, ph = 0, acc = 0, aph = 0;
+      bool ok = true;
+      for (int item = worker; item < total && ok; item += workers) {
+        const Tile t = tile_of(a, item);
+        const int steps = warp_uniform(t.k1 - t.k0);
+        ok = mbar_wait_warp(smem_u32(&hdr->acc_empty[acc]), aph ^ 1u, abort_flag, a.status, 42, a.wait_limit);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = u_tmem + acc * 256u;
+        for (int st = 0; st < steps; ++st) {
+          ok = mbar_wait_warp(smem_u32(&hdr->full[s]), ph, abort_flag, a.status, 43, a.wait_limit);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = u_stages0 + s * STAGE_BYTES;
+          const uint64_t da = desc_a + (sa >> 4), db = desc_b + ((sa + A_BYTES) >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) pt_mma<I8>(d, da + kk * (A_MN ? 128u : 2u), db + kk * (B_MN ? 128u : 2u), idesc, (st | kk) ? 1u : 0u);
+            pt_commit(smem_u32(&hdr->empty[s]));
+            if (st == steps - 1) pt_commit(smem_u32(&hdr->acc_full[acc]));
+          }
+          __syncwarp();
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
+        }
+        if (!ok) break;
+        if (++acc == 2) { acc = 0; aph ^= 1u; }
+      }
+      if (*abort_flag && elect_one()) {
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&hdr->drain)) : "memory");
+        for (uint32_t i = 0; i < (1u << 20); ++i)
+          if (mbar_try_wait(smem_u32(&hdr->drain), 0)) break;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, turn = warp >> 2;
+    float* scratch = reinterpret_cast<float*>(smem_raw + (base - raw) + 1024u + warp * SCRATCH);
+    uint32_t acc = 0, aph = 0;
+    for (int item = worker; item < total; item += workers) {
+      const Tile t = tile_of(a, item);
+      const int row0 = t.mt * 256 + rank * 128 + quarter * 32, row = row0 + lane;
+      const uint32_t t_base = tmem + ((uint32_t)(quarter * 32) << 16) + acc * 256u;
+      const int M = a.m[t.task], N = a.n[t.task];
+      const bool here = row < M;
+      // this warp's chunks of 32 columns: c = turn, turn + 2, ...
+      const int width = EPI == GATED ? half : a.ct, col0 = t.nt * width;
+      const int end = EPI == GATED || EPI == GRAD ? (int)a.hidden.pitch : N;          // columns from here on are not written
+      const int chunks = min(width / 32, (end - col0 + 31) / 32);
+      float rs = 0.f;
+      if (EPI == SCALED) rs = here ? __ldg(a.scale + row) : 0.f;
+      uint32_t gh[16], uh[16], gl[8], ul[8];
+      const int64_t hrow = (int64_t)row * a.hidden.pitch;
+      auto fetch = [&](int c) {                       // GRAD: g and u of a chunk
+        const int64_t at = hrow + col0 + 32 * c;
+        if (here && c < chunks) {
+          load_global_32(static_cast<const uint16_t*>(a.hidden.g) + at, *reinterpret_cast<uint32_t(*)[8]>(gh));
+          load_global_32(static_cast<const uint16_t*>(a.hidden.g) + at + 16, *reinterpret_cast<uint32_t(*)[8]>(gh + 8));
+          load_global_32(static_cast<const uint16_t*>(a.hidden.u) + at, *reinterpret_cast<uint32_t(*)[8]>(uh));
+          load_global_32(static_cast<const uint16_t*>(a.hidden.u) + at + 16, *reinterpret_cast<uint32_t(*)[8]>(uh + 8));
+          load_global_32(a.hidden.g_low + at, gl);
+          load_global_32(a.hidden.u_low + at, ul);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) gh[i] = uh[i] = 0u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) gl[i] = ul[i] = 0u;
+        }
+      };
+      if (EPI == GRAD) fetch(turn);
+      if (!mbar_wait_warp(smem_u32(&hdr->acc_full[acc]), aph, abort_flag, a.status, 44, a.wait_limit)) break;
+      tc_fence_after();
+      auto release = [&]() {                          // this warp has read the accumulator
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(pt_map(smem_u32(&hdr->acc_empty[acc]), 0)) : "memory");
+      };
+      if (turn >= chunks) release();
+      for (int c = turn; c < chunks; c += 2) {
+        const int c0 = col0 + 32 * c;
+        if (EPI == GATED) {
+          const int f = c0 + lane;
+          const __nv_bfloat16 *bg = static_cast<const __nv_bfloat16*>(a.bias), *bu = static_cast<const __nv_bfloat16*>(a.bias2);
+          const float b0 = bg && f < N ? __bfloat162float(__ldg(bg + f)) : 0.f, b1 = bu && f < N ? __bfloat162float(__ldg(bu + f)) : 0.f;
+          __syncwarp();
+          scratch[lane] = b0;
+          scratch[32 + lane] = b1;
+          __syncwarp();
+          uint32_t g[32], u[32];
+          tc_ld32(t_base + 32 * c, g);
+          tc_ld32(t_base + half + 32 * c, u);
+          tc_ld_wait();
+          if (c + 2 >= chunks) release();
+          uint32_t h[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float g0 = __uint_as_float(g[i]) + scratch[i], g1 = __uint_as_float(g[i + 1]) + scratch[i + 1];
+            const float u0 = __uint_as_float(u[i]) + scratch[32 + i], u1 = __uint_as_float(u[i + 1]) + scratch[33 + i];
+            g[i] = __float_as_uint(g0); g[i + 1] = __float_as_uint(g1);
+            u[i] = __float_as_uint(u0); u[i + 1] = __float_as_uint(u1);
+            h[i / 2] = bf16_pair(fast_act(g0, a.act).x * u0, fast_act(g1, a.act).x * u1);
+          }
+          if (here) {
+            const int64_t at = (int64_t)row * a.hidden.pitch + c0;
+            uint16_t* to = static_cast<uint16_t*>(a.hidden.h) + at;
+            st_global_32(to, *reinterpret_cast<uint32_t(*)[8]>(h));
+            st_global_32(to + 16, *reinterpret_cast<uint32_t(*)[8]>(h + 8));
+            if (a.hidden.g) {
+              auto keep = [&](const uint32_t* v, void* high, uint8_t* low) {
+                uint32_t hi[16], lo[8];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) hi[i] = __byte_perm(v[2 * i], v[2 * i + 1], 0x7632);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  lo[i] = __byte_perm(__byte_perm(v[4 * i], v[4 * i + 1], 0x0051), __byte_perm(v[4 * i + 2], v[4 * i + 3], 0x0051), 0x5410);
+                uint16_t* p = static_cast<uint16_t*>(high) + at;
+                st_global_32(p, *reinterpret_cast<uint32_t(*)[8]>(hi));
+                st_global_32(p + 16, *reinterpret_cast<uint32_t(*)[8]>(hi + 8));
+                st_global_32(low + at, lo);
+              };
+              keep(g, a.hidden.g, a.hidden.g_low);
+              keep(u, a.hidden.u, a.hidden.u_low);
+            }
+          }
+        } else if (EPI == GRAD) {
+          uint32_t r[32];
+          tc_ld32(t_base + 32 * c, r);
+          tc_ld_wait();
+          if (c + 2 >= chunks) release();
+          float dg[32], du[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float g = upper24(i & 1 ? gh[i / 2] >> 16 : gh[i / 2] & 0xffffu, gl[i / 4] >> (8 * (i & 3)) & 0xffu);
+            const float u = upper24(i & 1 ? uh[i / 2] >> 16 : uh[i / 2] & 0xffffu, ul[i / 4] >> (8 * (i & 3)) & 0xffu);
+            const float2 s = fast_act(g, a.act);
+            const float dh = __uint_as_float(r[i]);
+            dg[i] = dh * u * s.y;
+            du[i] = dh * s.x;
+          }
+          if (c + 2 < chunks) fetch(c + 2);
+          if (here) {
+            uint32_t w[16];
+            const int64_t at = hrow + c0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = bf16_pair(dg[2 * i], dg[2 * i + 1]);
+            st_global_32(static_cast<uint16_t*>(a.dg) + at, *reinterpret_cast<uint32_t(*)[8]>(w));
+            st_global_32(static_cast<uint16_t*>(a.dg) + at + 16, *reinterpret_cast<uint32_t(*)[8]>(w + 8));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = bf16_pair(du[2 * i], du[2 * i + 1]);
+            st_global_32(static_cast<uint16_t*>(a.du) + at, *reinterpret_cast<uint32_t(*)[8]>(w));
+            st_global_32(static_cast<uint16_t*>(a.du) + at + 16, *reinterpret_cast<uint32_t(*)[8]>(w + 8));
+          }
+          if (a.sums) {                               // rows behind the last token are zeros of dy, and so of dg and du
+            float* to = a.sums + (int64_t)(row0 >> 5) * 2 * a.hidden.pitch + c0 + lane;
+            to[0] = column_sums(dg, lane);
+            to[a.hidden.pitch] = column_sums(du, lane);
+          }
+        } else {
+          uint32_t r[32];
+          float v[32];
+          if (EPI == SCALED) {
+            const int n = c0 + lane;
+            const float ws = n < N ? __ldg(a.wscale + n) : 0.f, b = a.bias_f && n < N ? __ldg(a.bias_f + n) : 0.f;
+            __syncwarp();
+            scratch[lane] = ws;
+            scratch[32 + lane] = b;
+            __syncwarp();
+          } else if (a.splits == 1) {
+            const int n = c0 + lane;
+            const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(a.bias);
+            const float b = bias && n < N ? __bfloat162float(__ldg(bias + n)) : 0.f;
+            __syncwarp();
+            scratch[lane] = b;
+            __syncwarp();
+          }
+          tc_ld32(t_base + 32 * c, r);
+          tc_ld_wait();
+          if (c + 2 >= chunks) release();
+          if (EPI == STORE && a.splits > 1) {
+            if (here) {
+              const int64_t pitch = (N + 31) / 32 * 32;
+              float* to = a.work + a.part[t.task] + ((int64_t)t.split * M + row) * pitch + c0;
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) st_global_32f(to + i, r + i);
+            }
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = EPI == SCALED ? fmaf((float)(int)r[i] * rs, scratch[i], scratch[32 + i]) : __uint_as_float(r[i]) + scratch[i];
+          void* y = a.y[t.task];
+          const bool f32 = EPI == SCALED && a.y_f32;
+          if (f32 && N % 8 == 0) {
+            if (here) {
+              float* to = static_cast<float*>(y) + (int64_t)row * N + c0;
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[i + j]);
+                if (c0 + i < N) st_global_32(to + i, w);
+              }
+            }
+          } else if (!f32 && N % 16 == 0) {
+            if (here) {
+              uint16_t* to = static_cast<uint16_t*>(y) + (int64_t)row * N + c0;
+#pragma unroll
+              for (int i = 0; i < 32; i += 16) {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = bf16_pair(v[i + 2 * j], v[i + 2 * j + 1]);
+                if (c0 + i < N) st_global_32(to + i, w);
+              }
+            }
+          } else if (f32) {
+            store_any(static_cast<float*>(y), N, row0, M, c0, v, scratch, lane);
+          } else {
+            store_any(static_cast<__nv_bfloat16*>(y), N, row0, M, c0, v, scratch, lane);
+          }
+        }
+      }
+      if (++acc == 2) { acc = 0; aph ^= 1u; }
+    }
+  }
+  tc_fence_before();
+  pt_sync();
+  if (warp == EPI_WARPS) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// The parts of a product's k, added in their order, with the bias.  A thread for four columns.
+__global__ void __launch_bounds__(256) product_join_kernel(const float* part, int splits, int64_t m, int n, const __nv_bfloat16* bias, __nv_bfloat16* y) {
+  const int64_t pitch = (n + 31) / 32 * 32, per = pitch / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per;
+  const int c = (int)(i - row * per) * 4;
+  if (row >= m || c >= n) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = 0; p < splits; ++p) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(part + ((int64_t)p * m + row) * pitch + c));
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  const float v[4] = {s.x, s.y, s.z, s.w};
+  float b[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = v[e] + (bias && c + e < n ? __bfloat162float(__ldg(bias + c + e)) : 0.f);
+  __nv_bfloat16* to = y + row * n + c;
+  if (n % 4 == 0) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(bf16_pair(b[0], b[1]), bf16_pair(b[2], b[3]));
+  } else {
+    for (int e = 0; e < 4 && c + e < n; ++e) to[e] = __float2bfloat16_rn(b[e]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ host
+int pairs() { return std::max(1, fovi::sm_count() / 2); }
+
+// The cut with the least time by a count of clocks: 2 clocks a column and stage, about 1500 for a tile's start and end, and for k in parts their way through memory.
+// `columns` of a tile are divided among `share` matrices (GATED: 2).
+TcShape shape_of(const int64_t* m, const int* n, int tasks, int64_t kb, int share, bool may_split) {
+  TcShape best{256, 1};
+  double least = 1e300;
+  for (int ct = 256; ct >= 64; ct -= 64) {
+    int64_t tiles = 0, values = 0;
+    for (int t = 0; t < tasks; ++t) {
+      tiles += (m[t] + 255) / 256 * ((n[t] * (int64_t)share + ct - 1) / ct);
+      values += m[t] * ((n[t] + 31) / 32 * 32);
+    }
+    for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || kb / s >= 4); ++s) {
+      const double rounds = (double)((tiles * s + pairs() - 1) / pairs());
+      double clocks = rounds * ((double)((kb + s - 1) / s) * std::max(2 * ct, 200) + 1500);
+      if (s > 1) clocks += 5000 + (double)values * s * 8 / 3400;
+      if (clocks < least) { least = clocks; best = {ct, s}; }
+    }
+  }
+  return best;
+}
+
+int map_k(CUtensorMap* m, const TcMatrix& x, bool bytes, int rows) {
+  return fovi::encode_2d(m, x.p, bytes, (uint64_t)x.cols, (uint64_t)x.rows, (uint64_t)x.pitch * (bytes ? 1 : 2), bytes ? 128 : 64, (uint32_t)rows);
+}
+int map_mn(CUtensorMap* m, const TcMatrix& x) { return fovi::encode_2d(m, x.p, false, (uint64_t)x.cols, (uint64_t)x.rows, (uint64_t)x.pitch * 2, 64, 64); }
+
+template <int EPI, bool A_MN, bool B_MN, bool I8> int launch(const PtMaps& maps, PtArgs& a, bool selftest, cudaStream_t st) {
+  FOVI_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&a.status), g_status));
+  a.wait_limit = selftest ? 4096u : WAIT_LIMIT;
+  a.skip_loads = selftest;
+  const int grid = 2 * std::min(a.first[a.tasks], pairs());
+  auto kernel = product_tc_kernel<EPI, A_MN, B_MN, I8>;
+  FOVI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PT_SMEM));
+  FOVI_CUDA(fovi::launch_pdl(kernel, grid, PT_THREADS, PT_SMEM, st, maps, a));
+  return fovi::after_launch("product_tc_kernel");
+}
+
+// Tiles of each task, in order.
+int tiles_of(PtArgs& a, int share) {
+  int64_t at = 0;
+  for (int t = 0; t < a.tasks; ++t) {
+    a.first[t] = (int)at;
+    a.n_mt[t] = (a.m[t] + 255) / 256;
+    a.n_nt[t] = (int)(((int64_t)a.n[t] * share + a.ct - 1) / a.ct);
+    at += (int64_t)a.n_mt[t] * a.n_nt[t] * a.splits;
+  }
+  if (at >= (1ll << 31) - (1 << 16)) return FOVI_ERR_UNSUPPORTED;
+  for (int t = a.tasks; t <= GROUPS; ++t) a.first[t] = (int)at;
+  return FOVI_OK;
+}
+
+int join(const PtArgs& a, cudaStream_t st) {
+  for (int t = 0; t < a.tasks; ++t) {
+    const int64_t threads = (int64_t)a.m[t] * ((a.n[t] + 31) / 32 * 8);
+    product_join_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a.work + a.part[t], a.splits, a.m[t], a.n[t], static_cast<const __nv_bfloat16*>(a.bias),
+                                                                          static_cast<__nv_bfloat16*>(a.y[t]));
+    const int rc = fovi::after_launch("product_join_kernel");
+    if (rc) return rc;
+  }
+  return FOVI_OK;
+}
+
+int64_t stages_of(int64_t k) { return (k + 63) / 64; }
+
+}  // namespace
+
+int fovi::tc_gated(const TcMatrix& x, const TcMatrix& wg, const TcMatrix& wu, const void* bg, const void* bu, int act, const Hidden& to, cudaStream_t st) {
+  PtArgs a{};
+  PtMaps maps{};
+  const int64_t m = x.rows;
+  const int n = (int)wg.rows;
+  a.tasks = 1; a.m[0] = (int)m; a.n[0] = n;
+  a.kb0 = a.kb = (int)stages_of(x.cols);
+  a.splits = 1;
+  a.ct = shape_of(&m, &n, 1, a.kb, 2, false).ct;
+  a.bias = bg; a.bias2 = bu; a.act = act; a.hidden = to;
+  int rc = tiles_of(a, 2);
+  if (!rc) rc = map_k(&maps.a[0], x, false, 128);
+  if (!rc) rc = map_k(&maps.b[0], wg, false, a.ct / 2);
+  if (!rc) rc = map_k(&maps.b[1], wu, false, a.ct / 2);
+  return rc ? rc : launch<GATED, false, false, false>(maps, a, false, st);
+}
+
+int64_t fovi::tc_sum_rows(int64_t tokens) { return (tokens + 255) / 256 * 8; }
+
+int fovi::tc_hidden_grad(const TcMatrix& dy, const TcMatrix& wd, const Hidden& from, int act, void* dg, void* du, float* sums, cudaStream_t st) {
+  PtArgs a{};
+  PtMaps maps{};
+  const int64_t m = dy.rows;
+  const int n = (int)wd.cols;
+  a.tasks = 1; a.m[0] = (int)m; a.n[0] = n;
+  a.kb0 = a.kb = (int)stages_of(dy.cols);
+  a.splits = 1;
+  a.ct = shape_of(&m, &n, 1, a.kb, 1, false).ct;
+  a.act = act; a.hidden = from; a.dg = dg; a.du = du; a.sums = sums;
+  int rc = tiles_of(a, 1);
+  if (!rc) rc = map_k(&maps.a[0], dy, false, 128);
+  if (!rc) rc = map_mn(&maps.b[0], wd);
+  return rc ? rc : launch<GRAD, false, true, false>(maps, a, false, st);
+}
+
+int64_t fovi::tc_linear_bytes(int64_t m, int n, int64_t k) {
+  const TcShape s = shape_of(&m, &n, 1, stages_of(k), 1, true);
+  return s.splits > 1 ? (int64_t)s.splits * m * ((n + 31) / 32 * 32) * 4 : 0;
+}
+
+int fovi::tc_linear(const TcMatrix& am, const TcMatrix& bm, const TcMatrix* a2, const TcMatrix* b2, bool b_mn, int m, int n, const void* bias, void* y, void* work, cudaStream_t st) {
+  PtArgs a{};
+  PtMaps maps{};
+  a.tasks = 1; a.m[0] = m; a.n[0] = n; a.y[0] = y;
+  a.kb0 = (int)stages_of(am.cols);
+  a.kb = a.kb0 * (a2 ? 2 : 1);
+  const int64_t m64 = m;
+  const TcShape s = shape_of(&m64, &n, 1, a.kb, 1, true);
+  a.ct = s.ct; a.splits = s.splits; a.work = static_cast<float*>(work); a.bias = bias;
+  int rc = tiles_of(a, 1);
+  if (!rc) rc = map_k(&maps.a[0], am, false, 128);
+  if (!rc) rc = b_mn ? map_mn(&maps.b[0], bm) : map_k(&maps.b[0], bm, false, a.ct / 2);
+  if (!rc && a2) rc = map_k(&maps.a[1], *a2, false, 128);
+  if (!rc && a2) rc = b_mn ? map_mn(&maps.b[1], *b2) : map_k(&maps.b[1], *b2, false, a.ct / 2);
+  if (rc) return rc;
+  rc = b_mn ? launch<STORE, false, true, false>(maps, a, false, st) : launch<STORE, false, false, false>(maps, a, false, st);
+  return rc || a.splits == 1 ? rc : join(a, st);
+}
+
+// The cut follows from all the block's weights, so that a gradient has the same bits whichever are asked for.
+static TcShape grads_shape(const TcTask* tasks, int n, int64_t rows) {
+  int64_t m[GROUPS];
+  int cols[GROUPS];
+  for (int t = 0; t < n; ++t) { m[t] = tasks[t].m; cols[t] = tasks[t].n; }
+  return shape_of(m, cols, n, stages_of(rows), 1, true);
+}
+
+int64_t fovi::tc_weight_grads_bytes(const TcTask* tasks, int n, int64_t rows) {
+  const TcShape s = grads_shape(tasks, n, rows);
+  if (s.splits == 1) return 0;
+  int64_t bytes = 0;
+  for (int t = 0; t < n; ++t) bytes += (int64_t)s.splits * tasks[t].m * ((tasks[t].n + 31) / 32 * 32) * 4;
+  return bytes;
+}
+
+int fovi::tc_weight_grads(const TcTask* tasks, int n, int64_t rows, void* work, cudaStream_t st) {
+  PtArgs a{};
+  PtMaps maps{};
+  const TcShape s = grads_shape(tasks, n, rows);
+  a.ct = s.ct; a.splits = s.splits; a.work = static_cast<float*>(work);
+  a.kb0 = a.kb = (int)stages_of(rows);
+  int64_t at = 0;
+  int rc = FOVI_OK;
+  for (int t = 0; t < n && !rc; ++t) {
+    if (!tasks[t].y) continue;
+    const int i = a.tasks++;
+    a.m[i] = tasks[t].m; a.n[i] = tasks[t].n; a.y[i] = tasks[t].y; a.part[i] = at;
+    at += (int64_t)a.splits * tasks[t].m * ((tasks[t].n + 31) / 32 * 32);
+    rc = map_mn(&maps.a[i], tasks[t].a);
+    if (!rc) rc = map_mn(&maps.b[i], tasks[t].b);
+  }
+  if (rc || !a.tasks) return rc;
+  rc = tiles_of(a, 1);
+  if (!rc) rc = launch<STORE, true, true, false>(maps, a, false, st);
+  return rc || a.splits == 1 ? rc : join(a, st);
+}
+
+int fovi::tc_int8(const TcMatrix& q, const TcMatrix& w, const float* scale, const float* wscale, const float* bias, void* y, int y_dtype, bool selftest, cudaStream_t st) {
+  PtArgs a{};
+  PtMaps maps{};
+  const int64_t m = q.rows;
+  const int n = (int)w.rows;
+  a.tasks = 1; a.m[0] = (int)m; a.n[0] = n; a.y[0] = y; a.y_f32 = y_dtype == FOVI_F32;
+  a.kb0 = a.kb = (int)((q.cols + 127) / 128);
+  a.splits = 1;
+  a.ct = shape_of(&m, &n, 1, a.kb, 1, false).ct;
+  a.scale = scale; a.wscale = wscale; a.bias_f = bias;
+  int rc = tiles_of(a, 1);
+  if (!rc) rc = map_k(&maps.a[0], q, true, 128);
+  if (!rc) rc = map_k(&maps.b[0], w, true, a.ct / 2);
+  return rc ? rc : launch<SCALED, false, false, true>(maps, a, selftest, st);
+}
+
+extern "C" int fovi_product_check(void* stream) {
+  auto st = reinterpret_cast<cudaStream_t>(stream);
+  int site = 0;
+  FOVI_CUDA(cudaMemcpyFromSymbolAsync(&site, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+  FOVI_CUDA(cudaStreamSynchronize(st));
+  if (!site) return FOVI_OK;
+  const int zero = 0;
+  FOVI_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+  FOVI_CUDA(cudaStreamSynchronize(st));
+  fovi::g_last_cuda_error = "token product: wait site " + std::to_string(site) + " gave up";
+  return FOVI_ERR_DEVICE_TIMEOUT;
+}

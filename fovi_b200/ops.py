@@ -961,7 +961,7 @@ def _copy_rows(t, c, plain=False):
     t2, n, stride = _rows(t, c)
     per = 16 // t.element_size()
     if plain or (t2.data_ptr() % 16 == 0 and (n <= 1 or (stride % per == 0 and stride > 0))):
-        return t2, n, max(stride, -(-c // per) * per) if n <= 1 else stride
+        return t2, n, -(-c // per) * per if n <= 1 else stride
     buffer = torch.empty((n, -(-c // per) * per), dtype=t.dtype, device=t.device)
     buffer[:, :c] = t2.view(n, c) if t2.is_contiguous() else t2
     return buffer, n, buffer.shape[1]
@@ -1020,11 +1020,11 @@ def gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias=None, u
     dev = x.device
     y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=dev)
     saved = torch.empty(lib.fovi_gated_ffn_saved_bytes(dt, m, F), dtype=torch.uint8, device=dev) if want_saved else None
-    size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, 0)
-    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, 2 if want_saved else 0)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     with _on(dev):
         check(lib.fovi_gated_ffn_forward(_ptr(rows[0][0]), dt, m, c, F, o, rows[0][1], *(a for w, s in rows[1:] for a in (_ptr(w), s)), *(_opt(b) for b in biases),
-                                         ACTIVATIONS[activation], _ptr(y), _opt(saved), _ptr(work), size, _stream()), "fovi_gated_ffn_forward")
+                                         ACTIVATIONS[activation], _ptr(y), _opt(saved), _opt(work), size, _stream()), "fovi_gated_ffn_forward")
     return y, saved
 
 
@@ -1176,6 +1176,11 @@ def attention_backward(q, k, v, o, grad, lse, key_lengths=None, key_mask=None, s
 def attention_check():
     """Synchronise the current stream and raise if an attention launch on the current device gave up on a bounded wait since the last check."""
     check(lib.fovi_attention_check(_stream()), "fovi_attention_check")
+
+
+def product_check():
+    """The same of the tensor-core products of linear_int8 and gated_feed_forward."""
+    check(lib.fovi_product_check(_stream()), "fovi_product_check")
 
 
 def launch_count():

@@ -225,8 +225,12 @@ def gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias=None, u
 
 
 def check():
-    """Synchronise the current stream and raise if an attention launch on the current device since the last check, forward or backward, gave up on a bounded wait."""
-    ops.attention_check()
+    """Synchronise the current stream and raise if an attention launch, or a product of linear_int8 or gated_feed_forward, on the current device since the last check, forward or
+    backward, gave up on a bounded wait."""
+    try:
+        ops.attention_check()
+    finally:
+        ops.product_check()
 
 
 # ------------------------------------------------------------------------------------------------------------ modules

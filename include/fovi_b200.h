@@ -518,17 +518,24 @@ int fovi_rms_norm_backward(const void* t, int dtype, int64_t rows, int C, int64_
 int fovi_quantize_rows(const void* x, int dtype, int64_t rows, int C, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, void* stream);
 
 /* y[m, n] = scale[m] * weight_scale[n] * sum over k of q[m, k] * weight[n, k] + bias[n]: q [tokens, K], weight [N, K] 8-bit integers (rows q_stride, weight_stride bytes
- * apart), exact 32-bit sums (K < 131072); scale [tokens], weight_scale [N], bias [N] or NULL float32; y contiguous [tokens, N] float32 or bf16. */
+ * apart), exact 32-bit sums (K < 131072); scale [tokens], weight_scale [N], bias [N] or NULL float32; y contiguous [tokens, N] float32 or bf16.
+ * Rows of q and weight, and y, start on 16-byte boundaries. */
 int fovi_linear_int8(const int8_t* q, int64_t tokens, int K, int64_t q_stride, const float* scale, const int8_t* weight, int N, int64_t weight_stride,
                      const float* weight_scale, const float* bias, void* y, int y_dtype, void* stream);
+/* Synchronises `stream` and returns FOVI_ERR_DEVICE_TIMEOUT if a tensor-core product of fovi_linear_int8 or fovi_gated_ffn_* on the current device since the last check gave up on a
+ * bounded wait (its result is then incomplete); clears the word. */
+int fovi_product_check(void* stream);
+/* Diagnostic: fovi_linear_int8's tensor-core kernel with its loads withheld and a short wait limit, so that its first wait gives up; y is left unwritten or undefined. */
+int fovi_linear_int8_selftest_wait_timeout(const int8_t* q, int64_t tokens, int K, int64_t q_stride, const float* scale, const int8_t* weight, int N, int64_t weight_stride,
+                                           const float* weight_scale, const float* bias, void* y, int y_dtype, void* stream);
 
 /* Gated feed-forward block: g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) * u, y = h Wd^T + bd; x [tokens, C], Wg, Wu [F, C], Wd [O, F], biases [F], [F], [O] (contiguous) or NULL,
  * y contiguous [tokens, O], all of one type; strides: elements from one row to the next.  activation 0: act(g) = g / (1 + exp(-g)), 1: g times the normal distribution
- * function.  saved: fovi_gated_ffn_saved_bytes bytes for the backward pass, or NULL (then work holds fovi_gated_ffn_workspace_bytes(.., 0) bytes).
- * Backward: each gradient may be NULL; all are of the block's type, contiguous, and have the same bits every time, whichever are asked for.
- * work: fovi_gated_ffn_workspace_bytes(.., 1) bytes. */
+ * function.  bf16: rows, y and the gradients start on 16-byte boundaries.  saved: fovi_gated_ffn_saved_bytes bytes for the backward pass, or NULL; work:
+ * fovi_gated_ffn_workspace_bytes bytes of the phase (0: forward without `saved`, 2: with, 1: backward; 0 bytes: NULL), both on 32-byte boundaries.
+ * Backward: each gradient may be NULL; all are of the block's type, contiguous, and have the same bits every time, whichever are asked for. */
 int64_t fovi_gated_ffn_saved_bytes(int dtype, int64_t tokens, int F);
-int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int backward);
+int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int phase);
 int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
                            const void* up_weight, int64_t up_stride, const void* down_weight, int64_t down_stride, const void* gate_bias, const void* up_bias,
                            const void* down_bias, int activation, void* y, void* saved, void* work, int64_t work_bytes, void* stream);
