@@ -30,10 +30,7 @@ struct GateUp {       // g and u -> h
     g += bg ? __ldg(bg + n) : 0.f;
     u += bu ? __ldg(bu + n) : 0.f;
     const int64_t at = m * to.pitch + n;
-    if (to.g) {
-      static_cast<float*>(to.g)[at] = g;
-      static_cast<float*>(to.u)[at] = u;
-    }
+    if (to.g) { to.g[at] = g; to.u[at] = u; }
     static_cast<float*>(to.h)[at] = activate(g, act).x * u;
   }
 };
@@ -41,8 +38,8 @@ struct HiddenGrad {   // dh -> dg, du
   Hidden from; float *dg, *du; int act;
   __device__ __forceinline__ void operator()(int64_t m, int n, float dh, float) const {
     const int64_t at = m * from.pitch + n;
-    const float2 s = activate(static_cast<const float*>(from.g)[at], act);
-    dg[at] = dh * static_cast<const float*>(from.u)[at] * s.y;
+    const float2 s = activate(from.g[at], act);
+    dg[at] = dh * from.u[at] * s.y;
     du[at] = dh * s.x;
   }
 };
@@ -94,11 +91,12 @@ Hidden hidden_at(void* p, int dtype, int64_t M, int F, bool saved) {
   const int64_t n = M * h.pitch, size = fovi::dtype_size(dtype);
   char* at = static_cast<char*>(p);
   h.h = at;
-  if (saved) {
-    h.g = at + n * size;
-    h.u = at + 2 * n * size;
-    h.g_low = reinterpret_cast<uint8_t*>(at + 3 * n * size);
-    h.u_low = h.g_low + n;
+  if (saved && dtype == FOVI_F32) {
+    h.g = reinterpret_cast<float*>(at + n * size);
+    h.u = h.g + n;
+  } else if (saved) {
+    h.high = reinterpret_cast<uint16_t*>(at + n * size);
+    h.low = reinterpret_cast<uint8_t*>(h.high + 2 * n);
   }
   return h;
 }

@@ -492,14 +492,14 @@ int fovi::encode_4d(CUtensorMap* m, const void* ptr, const uint64_t (&dims)[4], 
   return FOVI_OK;
 }
 
-int fovi::encode_2d(CUtensorMap* m, const void* ptr, bool bytes, uint64_t d0, uint64_t d1, uint64_t stride_bytes, uint32_t b0, uint32_t b1) {
+int fovi::encode_2d(CUtensorMap* m, const void* ptr, bool bytes, uint64_t d0, uint64_t d1, uint64_t stride_bytes, uint32_t b0, uint32_t b1, bool swizzle64) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) { fovi::g_last_cuda_error = "cuTensorMapEncodeTiled entry point not available"; return FOVI_ERR_CUDA; }
   const cuuint64_t d[2] = {d0, d1}, st[1] = {stride_bytes};
   const cuuint32_t b[2] = {b0, b1}, estr[2] = {1, 1};
   auto encode = [&] {
     return fn(m, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+              swizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = encode();
   if (r == CUDA_ERROR_INVALID_CONTEXT && fovi::bind_context()) r = encode();

@@ -11,6 +11,8 @@
 // What becomes of a tile:
 //   GATED    accumulator columns of the first half are g, of the second u, since the first CTA stages rows of Wg and the second the same rows of Wu: h = act(g) u
 //   GRAD     the tile is dh; g and u are read, dg and du written
+//            Both move 8 and 10 bytes a hidden value, which is what bounds them where C is small, so their tiles go through shared memory as tensor copies, 32 rows x 32 columns of a warp at
+//            a time: with a row per thread in global memory every instruction touched 32 lines, and the load/store unit bound them (65792 x 384 x 1024: 227 and 293 us).
 //   STORE    bf16 result with a bias, or with k in parts a float32 part, joined by a second kernel in their order
 //   SCALED   integer sums times the scales
 #include <algorithm>
@@ -30,12 +32,17 @@ __device__ int g_status;           // wait site at which a kernel gave up, see f
 enum { GATED = 0, GRAD = 1, STORE = 2, SCALED = 3 };
 constexpr int EPI_WARPS = 8, PT_THREADS = (EPI_WARPS + 2) * 32;
 constexpr uint32_t A_BYTES = 16384, STAGE_BYTES = 2 * A_BYTES;      // a CTA's 128 rows of A and up to 128 rows of B
-constexpr int STAGES = 6, GROUPS = 3;
-constexpr uint32_t SCRATCH = 32 * 17 * 4;                            // of an epilogue warp: 32 rows x 16 columns (odd pitch), or 64 biases
-constexpr uint32_t PT_SMEM = 1024 + 1024 + EPI_WARPS * SCRATCH + STAGES * STAGE_BYTES;
-static_assert(PT_SMEM <= 227 * 1024 && SCRATCH * EPI_WARPS % 1024 == 0, "");
+constexpr int MOST_STAGES = 6, GROUPS = 3;
+// Shared memory of an epilogue warp.  GATED: a chunk's g and u (high 4 KB, low 2 KB) and h (2 KB) on their way out.  GRAD: two such places for g and u on their way in, dg and du go out from
+// over the high parts.  Otherwise: 32 rows x 16 columns (odd pitch), or 64 factors and biases.
+template <int EPI> struct Sizes {
+  static constexpr uint32_t SCRATCH = EPI == GATED ? 8192 : EPI == GRAD ? 12288 : 32 * 17 * 4;
+  static constexpr int STAGES = EPI == GATED ? 5 : EPI == GRAD ? 4 : MOST_STAGES;
+  static constexpr uint32_t SMEM = 1024 + 1024 + EPI_WARPS * SCRATCH + STAGES * STAGE_BYTES;
+  static_assert(SMEM <= 227 * 1024 && SCRATCH * EPI_WARPS % 1024 == 0, "");
+};
 
-struct PtMaps { CUtensorMap a[GROUPS], b[GROUPS]; };       // of each task, or of each segment of k
+struct PtMaps { CUtensorMap a[GROUPS], b[GROUPS], high, low, out[2]; };       // a, b: of each task, or of each segment of k; out: h, or dg and du
 
 struct PtArgs {
   int tasks, first[GROUPS + 1];            // tiles first[t] .. first[t + 1] - 1 belong to task t
@@ -52,7 +59,7 @@ struct PtArgs {
 };
 
 struct PtHeader {
-  uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain;
+  uint64_t full[MOST_STAGES], empty[MOST_STAGES], acc_full[2], acc_empty[2], drain, came[EPI_WARPS][2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -83,9 +90,32 @@ template <bool I8> __device__ __forceinline__ void pt_mma(uint32_t d, uint64_t a
 __device__ __forceinline__ void pt_commit(uint32_t bar) {            // on the barrier at this offset in both CTAs
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
-__device__ __forceinline__ void load_global_32(const void* p, uint32_t (&w)[8]) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+// Copies of a warp's chunk, issued by one lane.
+__device__ __forceinline__ void pt_load_own(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
 }
+__device__ __forceinline__ void pt_store(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }      // this thread's stores have read shared memory
+__device__ __forceinline__ void bulk_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void put16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void get16(uint32_t at, uint32_t* w) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t get4(uint32_t at) {
+  uint32_t w;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+  return w;
+}
+// Place of 16-byte piece c of row r in a tile of 128-byte or 64-byte rows, swizzled over that many bytes: eight rows' pieces lie in eight bank groups.
+__device__ __forceinline__ uint32_t at128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+__device__ __forceinline__ uint32_t at64(int r, int c) { return (uint32_t)(r * 64 + ((c ^ (r >> 1 & 3)) << 4)); }
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
@@ -104,20 +134,6 @@ __device__ __forceinline__ float2 fast_act(float g, int act) {
   }
   const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
   return make_float2(g * p, fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), p));
-}
-
-// Sums over the warp's 32 lanes (rows) of 32 columns, by halving exchanges: lane l ends with column l's.
-__device__ __forceinline__ float column_sums(float (&c)[32], int lane) {
-  const bool up16 = lane & 16, up8 = lane & 8, up4 = lane & 4, up2 = lane & 2, up1 = lane & 1;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) c[i] = (up16 ? c[i + 16] : c[i]) + __shfl_xor_sync(0xffffffffu, up16 ? c[i] : c[i + 16], 16);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = (up8 ? c[i + 8] : c[i]) + __shfl_xor_sync(0xffffffffu, up8 ? c[i] : c[i + 8], 8);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = (up4 ? c[i + 4] : c[i]) + __shfl_xor_sync(0xffffffffu, up4 ? c[i] : c[i + 4], 4);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) c[i] = (up2 ? c[i + 2] : c[i]) + __shfl_xor_sync(0xffffffffu, up2 ? c[i] : c[i + 2], 2);
-  return (up1 ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, up1 ? c[0] : c[1], 1);
 }
 
 struct Tile { int task, mt, nt, k0, k1, split; };
@@ -155,6 +171,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   PtHeader* hdr = reinterpret_cast<PtHeader*>(smem_raw + (base - raw));
+  constexpr uint32_t SCRATCH = Sizes<EPI>::SCRATCH;
+  constexpr int STAGES = Sizes<EPI>::STAGES;
   const uint32_t stages0 = base + 1024u + EPI_WARPS * SCRATCH;
   volatile int* abort_flag = &hdr->abort_flag;
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -166,6 +184,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
     for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&hdr->acc_full[i]), 1); mbar_init(smem_u32(&hdr->acc_empty[i]), 2 * EPI_WARPS); }
     mbar_init(smem_u32(&hdr->drain), 1);
+    if (EPI == GRAD)
+      for (int i = 0; i < 2 * EPI_WARPS; ++i) mbar_init(smem_u32(&hdr->came[0][0]) + 8 * i, 1);
     hdr->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -258,38 +278,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3, turn = warp >> 2;
     float* scratch = reinterpret_cast<float*>(smem_raw + (base - raw) + 1024u + warp * SCRATCH);
+    const uint32_t place = base + 1024u + warp * SCRATCH;
+    const int width = EPI == GATED ? half : a.ct;                     // columns of a tile; this warp's chunks of 32 are turn, turn + 2, ...
+    auto chunks_of = [&](const Tile& t) {                             // columns from the end on are not written
+      const int end = EPI == GATED || EPI == GRAD ? (int)a.hidden.pitch : a.n[t.task];
+      return min(width / 32, (end - t.nt * width + 31) / 32);
+    };
+    auto row_of = [&](const Tile& t) { return t.mt * 256 + rank * 128 + quarter * 32; };
     uint32_t acc = 0, aph = 0;
+    // GRAD: g and u of this warp's chunks, two on their way.  The next to be asked for is chunk next_c of next_item.
+    int next_item = worker, next_c = turn, asked = 0, taken = 0;
+    auto ask = [&]() {
+      Tile t{};
+      int chunks = 0;
+      for (; next_item < total; next_item += workers, next_c = turn) {
+        t = tile_of(a, next_item);
+        chunks = chunks_of(t);
+        if (next_c < chunks) break;
+      }
+      if (next_item >= total) return;
+      if (lane == 0) {
+        const uint32_t to = place + (asked & 1) * 6144u, bar = smem_u32(&hdr->came[warp][asked & 1]);
+        mbar_expect_tx(bar, 6144u);
+        const int c = t.nt * width + 32 * next_c;
+        pt_load_own(to, &maps.high, bar, 2 * c, row_of(t));
+        pt_load_own(to + 4096u, &maps.low, bar, 2 * c, row_of(t));
+      }
+      ++asked;
+      next_c += 2;
+    };
+    if (EPI == GRAD && !a.skip_loads) { ask(); ask(); }
     for (int item = worker; item < total; item += workers) {
       const Tile t = tile_of(a, item);
-      const int row0 = t.mt * 256 + rank * 128 + quarter * 32, row = row0 + lane;
+      const int row0 = row_of(t), row = row0 + lane;
       const uint32_t t_base = tmem + ((uint32_t)(quarter * 32) << 16) + acc * 256u;
       const int M = a.m[t.task], N = a.n[t.task];
       const bool here = row < M;
-      // this warp's chunks of 32 columns: c = turn, turn + 2, ...
-      const int width = EPI == GATED ? half : a.ct, col0 = t.nt * width;
-      const int end = EPI == GATED || EPI == GRAD ? (int)a.hidden.pitch : N;          // columns from here on are not written
-      const int chunks = min(width / 32, (end - col0 + 31) / 32);
+      const int col0 = t.nt * width, chunks = chunks_of(t);
       float rs = 0.f;
       if (EPI == SCALED) rs = here ? __ldg(a.scale + row) : 0.f;
-      uint32_t gh[16], uh[16], gl[8], ul[8];
-      const int64_t hrow = (int64_t)row * a.hidden.pitch;
-      auto fetch = [&](int c) {                       // GRAD: g and u of a chunk
-        const int64_t at = hrow + col0 + 32 * c;
-        if (here && c < chunks) {
-          load_global_32(static_cast<const uint16_t*>(a.hidden.g) + at, *reinterpret_cast<uint32_t(*)[8]>(gh));
-          load_global_32(static_cast<const uint16_t*>(a.hidden.g) + at + 16, *reinterpret_cast<uint32_t(*)[8]>(gh + 8));
-          load_global_32(static_cast<const uint16_t*>(a.hidden.u) + at, *reinterpret_cast<uint32_t(*)[8]>(uh));
-          load_global_32(static_cast<const uint16_t*>(a.hidden.u) + at + 16, *reinterpret_cast<uint32_t(*)[8]>(uh + 8));
-          load_global_32(a.hidden.g_low + at, gl);
-          load_global_32(a.hidden.u_low + at, ul);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) gh[i] = uh[i] = 0u;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) gl[i] = ul[i] = 0u;
-        }
-      };
-      if (EPI == GRAD) fetch(turn);
       if (!mbar_wait_warp(smem_u32(&hdr->acc_full[acc]), aph, abort_flag, a.status, 44, a.wait_limit)) break;
       tc_fence_after();
       auto release = [&]() {                          // this warp has read the accumulator
@@ -298,85 +325,121 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
         if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(pt_map(smem_u32(&hdr->acc_empty[acc]), 0)) : "memory");
       };
       if (turn >= chunks) release();
+      bool lost = false;
       for (int c = turn; c < chunks; c += 2) {
         const int c0 = col0 + 32 * c;
         if (EPI == GATED) {
           const int f = c0 + lane;
           const __nv_bfloat16 *bg = static_cast<const __nv_bfloat16*>(a.bias), *bu = static_cast<const __nv_bfloat16*>(a.bias2);
           const float b0 = bg && f < N ? __bfloat162float(__ldg(bg + f)) : 0.f, b1 = bu && f < N ? __bfloat162float(__ldg(bu + f)) : 0.f;
-          __syncwarp();
-          scratch[lane] = b0;
-          scratch[32 + lane] = b1;
-          __syncwarp();
           uint32_t g[32], u[32];
           tc_ld32(t_base + 32 * c, g);
           tc_ld32(t_base + half + 32 * c, u);
           tc_ld_wait();
           if (c + 2 >= chunks) release();
-          uint32_t h[16];
+          if (bg) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float g0 = __uint_as_float(g[i]) + scratch[i], g1 = __uint_as_float(g[i + 1]) + scratch[i + 1];
-            const float u0 = __uint_as_float(u[i]) + scratch[32 + i], u1 = __uint_as_float(u[i + 1]) + scratch[33 + i];
-            g[i] = __float_as_uint(g0); g[i + 1] = __float_as_uint(g1);
-            u[i] = __float_as_uint(u0); u[i + 1] = __float_as_uint(u1);
-            h[i / 2] = bf16_pair(fast_act(g0, a.act).x * u0, fast_act(g1, a.act).x * u1);
+            for (int i = 0; i < 32; ++i) g[i] = __float_as_uint(__uint_as_float(g[i]) + __shfl_sync(0xffffffffu, b0, i));
           }
-          if (here) {
-            const int64_t at = (int64_t)row * a.hidden.pitch + c0;
-            uint16_t* to = static_cast<uint16_t*>(a.hidden.h) + at;
-            st_global_32(to, *reinterpret_cast<uint32_t(*)[8]>(h));
-            st_global_32(to + 16, *reinterpret_cast<uint32_t(*)[8]>(h + 8));
-            if (a.hidden.g) {
-              auto keep = [&](const uint32_t* v, void* high, uint8_t* low) {
-                uint32_t hi[16], lo[8];
+          if (bu) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) hi[i] = __byte_perm(v[2 * i], v[2 * i + 1], 0x7632);
+            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) + __shfl_sync(0xffffffffu, b1, i));
+          }
+          if (lane == 0) bulk_read();                 // the chunk before has left this place
+          __syncwarp();
+          if (a.hidden.high) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  lo[i] = __byte_perm(__byte_perm(v[4 * i], v[4 * i + 1], 0x0051), __byte_perm(v[4 * i + 2], v[4 * i + 3], 0x0051), 0x5410);
-                uint16_t* p = static_cast<uint16_t*>(high) + at;
-                st_global_32(p, *reinterpret_cast<uint32_t(*)[8]>(hi));
-                st_global_32(p + 16, *reinterpret_cast<uint32_t(*)[8]>(hi + 8));
-                st_global_32(low + at, lo);
-              };
-              keep(g, a.hidden.g, a.hidden.g_low);
-              keep(u, a.hidden.u, a.hidden.u_low);
+            for (int m = 0; m < 2; ++m) {
+              const uint32_t* v = m ? u : g;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                put16(place + at128(lane, 4 * m + i), __byte_perm(v[8 * i], v[8 * i + 1], 0x7632), __byte_perm(v[8 * i + 2], v[8 * i + 3], 0x7632),
+                      __byte_perm(v[8 * i + 4], v[8 * i + 5], 0x7632), __byte_perm(v[8 * i + 6], v[8 * i + 7], 0x7632));
+              uint32_t lo[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                lo[i] = __byte_perm(__byte_perm(v[4 * i], v[4 * i + 1], 0x0051), __byte_perm(v[4 * i + 2], v[4 * i + 3], 0x0051), 0x5410);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) put16(place + 4096u + at64(lane, 2 * m + i), lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
             }
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int e = 8 * i + 2 * j;
+              h[j] = bf16_pair(fast_act(__uint_as_float(g[e]), a.act).x * __uint_as_float(u[e]), fast_act(__uint_as_float(g[e + 1]), a.act).x * __uint_as_float(u[e + 1]));
+            }
+            put16(place + 6144u + at64(lane, i), h[0], h[1], h[2], h[3]);
+          }
+          async_fence();
+          __syncwarp();
+          if (lane == 0) {                            // rows behind the last token are outside the tensors, and left out
+            if (a.hidden.high) {
+              pt_store(&maps.high, place, 2 * c0, row0);
+              pt_store(&maps.low, place + 4096u, 2 * c0, row0);
+            }
+            pt_store(&maps.out[0], place + 6144u, c0, row0);
+            bulk_commit();
+          }
         } else if (EPI == GRAD) {
-          uint32_t r[32];
+          const uint32_t from = place + (taken & 1) * 6144u;
+          if (!mbar_wait_warp(smem_u32(&hdr->came[warp][taken & 1]), taken >> 1 & 1, abort_flag, a.status, 45, a.wait_limit)) { lost = true; break; }
+          ++taken;
+          uint32_t r[32], gu[32], lo[16];             // gu: g of 32 columns, then u
           tc_ld32(t_base + 32 * c, r);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) get16(from + at128(lane, i), gu + 4 * i);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) get16(from + 4096u + at64(lane, i), lo + 4 * i);
           tc_ld_wait();
           if (c + 2 >= chunks) release();
-          float dg[32], du[32];
+          uint32_t dg[16], du[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float g = upper24(i & 1 ? gh[i / 2] >> 16 : gh[i / 2] & 0xffffu, gl[i / 4] >> (8 * (i & 3)) & 0xffu);
-            const float u = upper24(i & 1 ? uh[i / 2] >> 16 : uh[i / 2] & 0xffffu, ul[i / 4] >> (8 * (i & 3)) & 0xffu);
-            const float2 s = fast_act(g, a.act);
-            const float dh = __uint_as_float(r[i]);
-            dg[i] = dh * u * s.y;
-            du[i] = dh * s.x;
-          }
-          if (c + 2 < chunks) fetch(c + 2);
-          if (here) {
-            uint32_t w[16];
-            const int64_t at = hrow + c0;
+          for (int i = 0; i < 16; ++i) {
+            float x[2], y[2];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = bf16_pair(dg[2 * i], dg[2 * i + 1]);
-            st_global_32(static_cast<uint16_t*>(a.dg) + at, *reinterpret_cast<uint32_t(*)[8]>(w));
-            st_global_32(static_cast<uint16_t*>(a.dg) + at + 16, *reinterpret_cast<uint32_t(*)[8]>(w + 8));
+            for (int j = 0; j < 2; ++j) {
+              const int e = 2 * i + j;
+              const uint32_t pick = (j ? 0x3244u : 0x1044u) + ((uint32_t)(e & 3) << 4);      // [two high bytes, low byte, any]
+              const float g = __uint_as_float((__byte_perm(gu[i], lo[e / 4], pick) & 0xffffff00u) | 0x80u);
+              const float u = __uint_as_float((__byte_perm(gu[16 + i], lo[8 + e / 4], pick) & 0xffffff00u) | 0x80u);
+              const float dh = __uint_as_float(r[e]);
+              const float2 s = fast_act(g, a.act);
+              x[j] = dh * u * s.y;
+              y[j] = dh * s.x;
+            }
+            dg[i] = bf16_pair(x[0], x[1]);
+            du[i] = bf16_pair(y[0], y[1]);
+          }
+          __syncwarp();                               // every lane has its g and u
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = bf16_pair(du[2 * i], du[2 * i + 1]);
-            st_global_32(static_cast<uint16_t*>(a.du) + at, *reinterpret_cast<uint32_t(*)[8]>(w));
-            st_global_32(static_cast<uint16_t*>(a.du) + at + 16, *reinterpret_cast<uint32_t(*)[8]>(w + 8));
+          for (int i = 0; i < 4; ++i) {
+            put16(from + at64(lane, i), dg[4 * i], dg[4 * i + 1], dg[4 * i + 2], dg[4 * i + 3]);
+            put16(from + 2048u + at64(lane, i), du[4 * i], du[4 * i + 1], du[4 * i + 2], du[4 * i + 3]);
           }
-          if (a.sums) {                               // rows behind the last token are zeros of dy, and so of dg and du
-            float* to = a.sums + (int64_t)(row0 >> 5) * 2 * a.hidden.pitch + c0 + lane;
-            to[0] = column_sums(dg, lane);
-            to[a.hidden.pitch] = column_sums(du, lane);
+          async_fence();
+          __syncwarp();
+          if (lane == 0) {
+            pt_store(&maps.out[0], from, c0, row0);
+            pt_store(&maps.out[1], from + 2048u, c0, row0);
+            bulk_commit();
           }
+          if (a.sums) {                               // of this warp's 32 rows, two columns a lane; rows behind the last token are zeros of dy, and so of dg and du
+            float s0 = 0.f, s1 = 0.f;
+            const uint32_t mine = from + (lane >> 4) * 2048u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const uint32_t w = get4(mine + at64(i, lane >> 2 & 3) + (lane & 3) * 4u);
+              s0 += __uint_as_float(w << 16);
+              s1 += __uint_as_float(w & 0xffff0000u);
+            }
+            *reinterpret_cast<float2*>(a.sums + ((int64_t)(row0 >> 5) * 2 + (lane >> 4)) * a.hidden.pitch + c0 + 2 * (lane & 15)) = make_float2(s0, s1);
+          }
+          if (lane == 0) bulk_read();
+          __syncwarp();
+          ask();
         } else {
           uint32_t r[32];
           float v[32];
@@ -440,7 +503,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
           }
         }
       }
+      if (lost) break;
       if (++acc == 2) { acc = 0; aph ^= 1u; }
+    }
+    if ((EPI == GATED || EPI == GRAD) && lane == 0) bulk_done();
+    if (EPI == GRAD && *abort_flag && lane == 0) {
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);    // copies in flight, as above
     }
   }
   tc_fence_before();
@@ -510,10 +578,18 @@ template <int EPI, bool A_MN, bool B_MN, bool I8> int launch(const PtMaps& maps,
   a.skip_loads = selftest;
   const int grid = 2 * std::min(a.first[a.tasks], pairs());
   auto kernel = product_tc_kernel<EPI, A_MN, B_MN, I8>;
-  FOVI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PT_SMEM));
-  FOVI_CUDA(fovi::launch_pdl(kernel, grid, PT_THREADS, PT_SMEM, st, maps, a));
+  FOVI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sizes<EPI>::SMEM));
+  FOVI_CUDA(fovi::launch_pdl(kernel, grid, PT_THREADS, Sizes<EPI>::SMEM, st, maps, a));
   return fovi::after_launch("product_tc_kernel");
 }
+
+// Tensors of a row of hidden values a token, as boxes of 32 rows x 32 columns (high, low: of g and u side by side).
+int map_hidden(PtMaps& maps, const Hidden& h, int64_t m) {
+  if (!h.high) return FOVI_OK;
+  const int rc = fovi::encode_2d(&maps.high, h.high, false, 2 * h.pitch, m, 4 * h.pitch, 64, 32);
+  return rc ? rc : fovi::encode_2d(&maps.low, h.low, true, 2 * h.pitch, m, 2 * h.pitch, 64, 32, true);
+}
+int map_out(CUtensorMap* map, const void* p, int64_t pitch, int64_t m) { return fovi::encode_2d(map, p, false, pitch, m, 2 * pitch, 32, 32, true); }
 
 // Tiles of each task, in order.
 int tiles_of(PtArgs& a, int share) {
@@ -558,6 +634,8 @@ int fovi::tc_gated(const TcMatrix& x, const TcMatrix& wg, const TcMatrix& wu, co
   if (!rc) rc = map_k(&maps.a[0], x, false, 128);
   if (!rc) rc = map_k(&maps.b[0], wg, false, a.ct / 2);
   if (!rc) rc = map_k(&maps.b[1], wu, false, a.ct / 2);
+  if (!rc) rc = map_hidden(maps, to, m);
+  if (!rc) rc = map_out(&maps.out[0], to.h, to.pitch, m);
   return rc ? rc : launch<GATED, false, false, false>(maps, a, false, st);
 }
 
@@ -576,6 +654,9 @@ int fovi::tc_hidden_grad(const TcMatrix& dy, const TcMatrix& wd, const Hidden& f
   int rc = tiles_of(a, 1);
   if (!rc) rc = map_k(&maps.a[0], dy, false, 128);
   if (!rc) rc = map_mn(&maps.b[0], wd);
+  if (!rc) rc = map_hidden(maps, from, m);
+  if (!rc) rc = map_out(&maps.out[0], dg, from.pitch, m);
+  if (!rc) rc = map_out(&maps.out[1], du, from.pitch, m);
   return rc ? rc : launch<GRAD, false, true, false>(maps, a, false, st);
 }
 

@@ -235,8 +235,8 @@ int encode_3d(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_
               uint64_t stride2_bytes, uint32_t b0, uint32_t b1, uint32_t b2, bool swizzle128);
 // Tiled 4-D bf16 tensor map, without swizzle unless asked for (strides: bytes of dimensions 1 to 3).
 int encode_4d(CUtensorMap* m, const void* ptr, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4], bool swizzle128 = false);
-// Tiled 2-D tensor map of bf16 values or of bytes, 128-byte swizzle.
-int encode_2d(CUtensorMap* m, const void* ptr, bool bytes, uint64_t d0, uint64_t d1, uint64_t stride_bytes, uint32_t b0, uint32_t b1);
+// Tiled 2-D tensor map of bf16 values or of bytes, 128-byte swizzle, or 64-byte.
+int encode_2d(CUtensorMap* m, const void* ptr, bool bytes, uint64_t d0, uint64_t d1, uint64_t stride_bytes, uint32_t b0, uint32_t b1, bool swizzle64 = false);
 // CTA-pair variant of the 64-channel mode (knnconv_tc2.cu).  Returns FOVI_ERR_UNSUPPORTED when it does not apply.
 int launch_knnconv_tc_pair(const fovi_knnconv_plan* p, const void* X, const void* Wt, const float* bias, void* Y, int y_dtype,
                            int B, int relu, cudaStream_t st, int skip_loads, uint32_t wait_limit, const OutMode& om);
