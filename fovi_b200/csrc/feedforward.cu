@@ -4,6 +4,7 @@
 //   dh = dy Wd,  dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h,  and column sums of dg, du, dy for the biases.
 #include <algorithm>
 
+#include "product_few.cuh"
 #include "product_simt.cuh"
 #include "product_tc.cuh"
 
@@ -124,6 +125,10 @@ int forward_f32(const Block& b, void* y, const Hidden& hid, cudaStream_t st) {
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 int forward_bf16(const Block& b, void* y, const Hidden& hid, void* work, cudaStream_t st) {
+  if (b.M <= fovi::FEW_TOKENS && !hid.high) {
+    const int rc = fovi::few_gated({b.x, b.xs}, {b.wg, b.gs}, {b.wu, b.us}, (int)b.M, b.F, b.C, b.bg, b.bu, b.act, {hid.h, hid.pitch}, st);
+    return rc ? rc : fovi::few_linear({hid.h, hid.pitch}, {b.wd, b.ds}, (int)b.M, b.O, b.F, b.bd, y, true, st);
+  }
   const TcMatrix x{b.x, b.M, b.C, b.xs}, wg{b.wg, b.F, b.C, b.gs}, wu{b.wu, b.F, b.C, b.us}, wd{b.wd, b.O, b.F, b.ds}, h{hid.h, b.M, b.F, hid.pitch};
   const int rc = fovi::tc_gated(x, wg, wu, b.bg, b.bu, b.act, hid, st);
   return rc ? rc : fovi::tc_linear(h, wd, nullptr, nullptr, false, (int)b.M, b.O, b.bd, y, work, st);

@@ -1,0 +1,186 @@
+// Matrix products of up to 32 tokens, 16 a block: y[m, n] = sum over k of x[m, k] w[n, k], bf16 or 8-bit integers.
+//
+// What bounds them is how fast the weights come: each is used by up to 32 tokens and read once.  A block takes 16 rows of w (GATED: of both matrices) and divides k among its warps in
+// turns of 64 bytes a row; a warp's loads are 16 bytes a lane, four lanes side by side in a row, straight into the registers that the matrix instruction (m16n8k16 or m16n8k32: weights
+// are its 16 rows, tokens its 8 columns) takes them from.  That an instruction's k then is not consecutive does not matter, since tokens are loaded the same way.
+// Four turns of loads are on their way at a time.  The warps' sums are joined in shared memory in a fixed order, and a thread for each result ends it.
+// The tensor cores' large instructions (product_tc.cu) have 128 rows: with one token 5120 x 1280 8-bit weights take 8.8 us there.
+#include <algorithm>
+
+#include "product_few.cuh"
+#include "tc_common.cuh"
+
+using fovi::FewRows;
+
+namespace {
+
+enum { GATED = 0, LINEAR = 1, SCALED = 2 };
+constexpr int ROWS = 16, TURNS = 4;
+
+struct FewArgs {
+  const char *x, *w, *w2; int64_t x_pitch, w_pitch, w2_pitch;        // pitches in bytes
+  int m, n, k;                                                       // k in bytes
+  const __nv_bfloat16 *bias, *bias2; int act;
+  const float *scale, *wscale, *bias_f; int y_f32;
+  void* y; int64_t y_pitch;                                          // in values
+};
+
+__device__ __forceinline__ void mma_few(float (&d)[4], const uint32_t* a, const uint32_t* b, uint32_t a0, uint32_t a1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a0), "r"(a[1]), "r"(a1), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma_few(int (&d)[4], const uint32_t* a, const uint32_t* b, uint32_t a0, uint32_t a1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a0), "r"(a[1]), "r"(a1), "r"(b[0]), "r"(b[1]));
+}
+template <bool I8> struct SumT { using type = float; };
+template <> struct SumT<true> { using type = int; };
+
+struct Piece16 { uint32_t w[4]; };
+// 16 bytes of a row from byte `at` on, of which those behind the row's `end` are zeros whatever lies there.  No branches: the lanes of a warp stay together for the matrix instructions,
+// which are the whole warp's (with the loads in branches on a lane's row and column, lanes could reach them apart).  Weights: read once; tokens may come from the launch before: a load
+// that stays behind the wait for it.
+template <bool WEIGHTS> __device__ __forceinline__ Piece16 load16(const char* row, bool here, int at, int end) {
+  Piece16 p;
+  const int left = end - at, use = here && left > 0;
+  if (WEIGHTS)
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+                 " @p ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n}\n"
+                 : "=&r"(p.w[0]), "=&r"(p.w[1]), "=&r"(p.w[2]), "=&r"(p.w[3]) : "l"(row + at), "r"(use));
+  else
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+                 " @p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n}\n"
+                 : "=&r"(p.w[0]), "=&r"(p.w[1]), "=&r"(p.w[2]), "=&r"(p.w[3]) : "l"(row + at), "r"(use) : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p.w[i] &= (uint32_t)((1ull << 8 * min(max(left - 4 * i, 0), 4)) - 1ull);
+  return p;
+}
+
+template <int EPI, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) product_few_kernel(const __grid_constant__ FewArgs a, const int early) {
+  constexpr bool I8 = EPI == SCALED, TWO = EPI == GATED;
+  constexpr int MATS = TWO ? 2 : 1, COLS = NT * 8;
+  using S = typename SumT<I8>::type;
+  __shared__ S part[WARPS][MATS][ROWS][COLS + 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * ROWS, m0 = blockIdx.y * 16;
+  const bool low = n0 + r < a.n, high = n0 + r + 8 < a.n;
+  const char* w[MATS][2];
+  w[0][0] = a.w + (int64_t)(n0 + r) * a.w_pitch;
+  w[0][1] = w[0][0] + 8 * a.w_pitch;
+  if (TWO) {
+    w[MATS - 1][0] = a.w2 + (int64_t)(n0 + r) * a.w2_pitch;
+    w[MATS - 1][1] = w[MATS - 1][0] + 8 * a.w2_pitch;
+  }
+  Piece16 wp[TURNS][MATS][2], xp[TURNS][NT];
+  auto weights = [&](int turn, int at) {
+#pragma unroll
+    for (int q = 0; q < MATS; ++q) {
+      wp[turn][q][0] = load16<true>(w[q][0], low, at, a.k);
+      wp[turn][q][1] = load16<true>(w[q][1], high, at, a.k);
+    }
+  };
+  const int first = warp * 64, own = t * 16, step = WARPS * 64;
+  // The weights do not come from the launch before: where that is known to be this call's own, they are asked for in front of the wait for it.
+  if (early) {
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) weights(u, first + u * step + own);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  S d[MATS][NT][4] = {};
+  for (int at = first; at < a.k; at += TURNS * step) {            // (the same turns for all lanes, as the instruction is the warp's)
+    if (!early || at != first) {
+#pragma unroll
+      for (int u = 0; u < TURNS; ++u) weights(u, at + u * step + own);
+    }
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) xp[u][j] = load16<false>(a.x + (int64_t)(m0 + 8 * j + r) * a.x_pitch, m0 + 8 * j + r < a.m, at + u * step + own, a.k);
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+      for (int q = 0; q < MATS; ++q)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_few(d[q][j], wp[u][q][0].w, xp[u][j].w, wp[u][q][1].w[0], wp[u][q][1].w[1]);
+          mma_few(d[q][j], wp[u][q][0].w + 2, xp[u][j].w + 2, wp[u][q][1].w[2], wp[u][q][1].w[3]);
+        }
+  }
+#pragma unroll
+  for (int q = 0; q < MATS; ++q)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      part[warp][q][r][8 * j + 2 * t] = d[q][j][0];
+      part[warp][q][r][8 * j + 2 * t + 1] = d[q][j][1];
+      part[warp][q][r + 8][8 * j + 2 * t] = d[q][j][2];
+      part[warp][q][r + 8][8 * j + 2 * t + 1] = d[q][j][3];
+    }
+  __syncthreads();
+  for (int e = threadIdx.x; e < ROWS * COLS; e += WARPS * 32) {
+    const int i = e % ROWS, col = e / ROWS, m = m0 + col, n = n0 + i;               // neighbouring threads write neighbouring values
+    if (m >= a.m || n >= a.n) continue;
+    S s[MATS] = {};
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v)
+#pragma unroll
+      for (int q = 0; q < MATS; ++q) s[q] += part[v][q][i][col];
+    const int64_t at = m * a.y_pitch + n;
+    if (EPI == SCALED) {
+      const float y = fmaf((float)s[0] * __ldg(a.scale + m), __ldg(a.wscale + n), a.bias_f ? __ldg(a.bias_f + n) : 0.f);
+      if (a.y_f32) static_cast<float*>(a.y)[at] = y;
+      else static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(y);
+    } else if (EPI == GATED) {
+      const float g = s[0] + (a.bias ? __bfloat162float(__ldg(a.bias + n)) : 0.f), u = s[MATS - 1] + (a.bias2 ? __bfloat162float(__ldg(a.bias2 + n)) : 0.f);
+      const float p = a.act == fovi::ACT_SILU ? __fdividef(1.f, 1.f + __expf(-g)) : 0.5f * (1.f + erff(g * 0.70710678118654752f));
+      static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(g * p * u);
+    } else {
+      static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(s[0] + (a.bias ? __bfloat162float(__ldg(a.bias + n)) : 0.f));
+    }
+  }
+}
+
+template <int EPI, int NT, int WARPS> int launch(const FewArgs& a, bool early, cudaStream_t st) {
+  FOVI_CUDA(fovi::launch_pdl(product_few_kernel<EPI, NT, WARPS>, dim3((a.n + ROWS - 1) / ROWS, (a.m + 15) / 16), WARPS * 32, 0, st, a, (int)early));
+  return fovi::after_launch("product_few_kernel");
+}
+template <int EPI, int NT> int by_warps(const FewArgs& a, bool early, cudaStream_t st) {
+  // Fewer blocks than SMs: more warps each.
+  return (a.n + ROWS - 1) / ROWS * ((a.m + 15) / 16) < fovi::sm_count() ? launch<EPI, NT, 16>(a, early, st) : launch<EPI, NT, 8>(a, early, st);
+}
+template <int EPI> int by_tokens(const FewArgs& a, bool early, cudaStream_t st) {
+  return a.m <= 8 ? by_warps<EPI, 1>(a, early, st) : by_warps<EPI, 2>(a, early, st);
+}
+
+FewArgs args(const FewRows& x, const FewRows& w, int m, int n, int k, int size) {
+  FewArgs a{};
+  a.x = static_cast<const char*>(x.p); a.x_pitch = x.pitch * size;
+  a.w = static_cast<const char*>(w.p); a.w_pitch = w.pitch * size;
+  a.m = m; a.n = n; a.k = k * size;
+  return a;
+}
+
+}  // namespace
+
+int fovi::few_gated(const FewRows& x, const FewRows& wg, const FewRows& wu, int m, int n, int k, const void* bg, const void* bu, int act, const FewRows& h, cudaStream_t st) {
+  FewArgs a = args(x, wg, m, n, k, 2);
+  a.w2 = static_cast<const char*>(wu.p); a.w2_pitch = wu.pitch * 2;
+  a.bias = static_cast<const __nv_bfloat16*>(bg); a.bias2 = static_cast<const __nv_bfloat16*>(bu); a.act = act;
+  a.y = const_cast<void*>(h.p); a.y_pitch = h.pitch;
+  return by_tokens<GATED>(a, false, st);
+}
+
+int fovi::few_linear(const FewRows& x, const FewRows& w, int m, int n, int k, const void* bias, void* y, bool after_own, cudaStream_t st) {
+  FewArgs a = args(x, w, m, n, k, 2);
+  a.bias = static_cast<const __nv_bfloat16*>(bias);
+  a.y = y; a.y_pitch = n;
+  return by_tokens<LINEAR>(a, after_own, st);
+}
+
+int fovi::few_int8(const FewRows& q, const FewRows& w, int m, int n, int k, const float* scale, const float* wscale, const float* bias, void* y, int y_dtype, cudaStream_t st) {
+  FewArgs a = args(q, w, m, n, k, 1);
+  a.scale = scale; a.wscale = wscale; a.bias_f = bias; a.y_f32 = y_dtype == FOVI_F32;
+  a.y = y; a.y_pitch = n;
+  return by_tokens<SCALED>(a, false, st);
+}
