@@ -319,7 +319,10 @@ PyObject* connect(PyObject*, PyObject* dict) {
       {"fovi_layer_norm_forward", (void**)&tok.norm}, {"fovi_layer_norm_workspace_bytes", (void**)&tok.norm_work},
       {"fovi_layer_norm_backward", (void**)&tok.norm_back}, {"fovi_rotary", (void**)&tok.rotary},
       {"fovi_attention_workspace_bytes", (void**)&tok.attend_work}, {"fovi_attention_forward", (void**)&tok.attend},
-      {"fovi_attention_backward", (void**)&tok.attend_back}};
+      {"fovi_attention_backward", (void**)&tok.attend_back}, {"fovi_rms_norm_forward", (void**)&tok.rms}, {"fovi_rms_norm_workspace_bytes", (void**)&tok.rms_work},
+      {"fovi_rms_norm_backward", (void**)&tok.rms_back}, {"fovi_quantize_rows", (void**)&tok.quantize}, {"fovi_linear_int8", (void**)&tok.int8},
+      {"fovi_gated_ffn_saved_bytes", (void**)&tok.ffn_saved}, {"fovi_gated_ffn_workspace_bytes", (void**)&tok.ffn_work},
+      {"fovi_gated_ffn_forward", (void**)&tok.ffn}, {"fovi_gated_ffn_backward", (void**)&tok.ffn_back}};
   for (const auto& w : want) {
     PyObject* a = PyDict_GetItemString(dict, w.name);
     if (!a) { PyErr_Format(PyExc_KeyError, "%s", w.name); return nullptr; }
@@ -331,7 +334,8 @@ PyObject* connect(PyObject*, PyObject* dict) {
 
 #define FAST(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(sample), FAST(conv_forward), FAST(conv_forward_f32), FAST(pack_points), FAST(pack_slabs), FAST(weight_grad), FAST(block_forward),
-                         FAST(block_backward), FAST(layer_norm), FAST(rotary), FAST(attention), {"connect", connect, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         FAST(block_backward), FAST(layer_norm), FAST(rotary), FAST(attention), FAST(rms_norm), FAST(rms_norm_int8), FAST(quantize), FAST(linear_int8),
+                         FAST(gated_feed_forward), {"connect", connect, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

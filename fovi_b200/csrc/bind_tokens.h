@@ -28,6 +28,15 @@ struct TokenAbi {
   decltype(&fovi_attention_workspace_bytes) attend_work = nullptr;
   decltype(&fovi_attention_forward) attend = nullptr;
   decltype(&fovi_attention_backward) attend_back = nullptr;
+  decltype(&fovi_rms_norm_forward) rms = nullptr;
+  decltype(&fovi_rms_norm_workspace_bytes) rms_work = nullptr;
+  decltype(&fovi_rms_norm_backward) rms_back = nullptr;
+  decltype(&fovi_quantize_rows) quantize = nullptr;
+  decltype(&fovi_linear_int8) int8 = nullptr;
+  decltype(&fovi_gated_ffn_saved_bytes) ffn_saved = nullptr;
+  decltype(&fovi_gated_ffn_workspace_bytes) ffn_work = nullptr;
+  decltype(&fovi_gated_ffn_forward) ffn = nullptr;
+  decltype(&fovi_gated_ffn_backward) ffn_back = nullptr;
 } tok;
 
 // The stream that the engine has made current on this thread for the device of a backward call.
@@ -310,6 +319,297 @@ BODY(attention, 8)
     }
   }
   return status_or(rcode, o);
+END
+
+// ------------------------------------------------------------------------------------------------------------ root-mean-square norm
+PyObject* tuple_of(std::initializer_list<at::Tensor> all) {
+  Py_ssize_t n = 0, i = 0;
+  for (const auto& t : all) n += t.defined();
+  PyObject* tuple = PyTuple_New(n);
+  if (!tuple) return nullptr;
+  for (const auto& t : all)
+    if (t.defined()) PyTuple_SET_ITEM(tuple, i++, THPVariable_Wrap(t));
+  return tuple;
+}
+
+struct RmsNormNode : Node {                // inputs x, weight, residual; outputs y and, with a residual, the sum
+  SavedVariable t, w;
+  at::Tensor rstd;
+  at::DimVector shape;
+  bool sum = false;                        // t is the second output
+  std::string name() const override { return "FoviRmsNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    t.reset_data(); w.reset_data(); rstd.reset();
+  }
+  variable_list apply(variable_list&& in) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(3);
+    const at::Tensor own = sum ? in[1] : at::Tensor();
+    if (!in[0].defined()) {                // the sum alone was used
+      if (own.defined() && task_should_compute_output(0)) out[0] = own;
+      if (own.defined() && task_should_compute_output(2)) out[2] = own;
+      return out;
+    }
+    const at::Tensor tv = sum ? t.unpack(shared_from_this()) : t.unpack(), wv = w.unpack();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const at::ScalarType type = tv.scalar_type();
+      const at::Tensor g = in[0].to(type).contiguous(), d = own.defined() ? own.to(type).contiguous() : at::Tensor();
+      const int64_t C = tv.size(-1), rows = tv.numel() / C;
+      const int dev = tv.get_device();
+      const at::Tensor dx = task_should_compute_output(0) || task_should_compute_output(2) ? fresh(tv.sizes(), type, dev) : at::Tensor();
+      if (task_should_compute_output(1)) out[1] = fresh(shape, at::kFloat, dev);
+      const int64_t bytes = out[1].defined() ? tok.rms_work(rows, (int)C) : 0;
+      const at::Tensor work = bytes ? fresh({bytes}, at::kByte, dev) : at::Tensor();
+      launched(tok.rms_back(tv.const_data_ptr(), code_of(type), rows, (int)C, C, g.const_data_ptr(), C, d.defined() ? d.const_data_ptr() : nullptr, C,
+                            wv.defined() ? wv.const_data_ptr<float>() : nullptr, rstd.const_data_ptr<float>(), out_ptr(dx), (float*)out_ptr(out[1]), out_ptr(work), bytes,
+                            stream_of(tv)),
+               "fovi_rms_norm_backward");
+      if (task_should_compute_output(0)) out[0] = dx;
+      if (task_should_compute_output(2)) out[2] = dx;
+    }
+    once(out, {in[0], own, tv, wv}, "rms_norm");
+    return out;
+  }
+};
+
+// Arguments of both forms of the norm: x, weight or None, eps, residual or None.
+struct RmsIn { const at::Tensor *x = nullptr, *w = nullptr, *res = nullptr; const float* wp = nullptr; int64_t C = 0, rows = 0; float eps = 0.f; };
+// 1: taken, 0: not in the plain form, -1: an error is set
+int rms_in(PyObject* const* v, int dev, RmsIn* a) {
+  a->x = plain(v[0], dev);
+  if (!a->x || !real_type(*a->x) || a->x->dim() < 1 || a->x->numel() == 0 || !a->x->is_contiguous()) return 0;
+  a->C = a->x->size(-1);
+  a->rows = a->x->numel() / a->C;
+  if (a->C > INT32_MAX || !bias_arg(v[1], dev, a->C, &a->wp)) return 0;
+  const double eps = PyFloat_AsDouble(v[2]);
+  if (PyErr_Occurred()) return -1;
+  if (!(eps >= 0)) return 0;
+  a->eps = (float)eps;
+  if (v[3] != Py_None && (!(a->res = plain(v[3], dev)) || a->res->scalar_type() != a->x->scalar_type() || a->res->sizes() != a->x->sizes() || !a->res->is_contiguous())) return 0;
+  a->w = a->wp ? plain(v[1], dev) : nullptr;
+  return has_tangent(*a->x) || (a->w && has_tangent(*a->w)) || (a->res && has_tangent(*a->res)) ? 0 : 1;
+}
+
+// x, weight or None, eps, residual or None, device, stream
+BODY(rms_norm, 6)
+  RmsIn a;
+  const int ok = rms_in(v, dev, &a);
+  if (ok < 0) return nullptr;
+  if (!ok) GENERAL;
+  at::Tensor y, total;
+  int rcode;
+  {
+    Release r;
+    const bool graph = needs_graph(*a.x, a.w, a.res);
+    const at::ScalarType type = a.x->scalar_type();
+    at::Tensor rstd;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      y = fresh(a.x->sizes(), type, dev);
+      if (a.res) total = fresh(a.x->sizes(), type, dev);
+      if (graph) rstd = fresh({a.rows}, at::kFloat, dev);
+    }
+    rcode = tok.rms(a.x->const_data_ptr(), code_of(type), a.rows, (int)a.C, a.C, a.res ? a.res->const_data_ptr() : nullptr, a.C, a.wp, a.eps, out_ptr(total),
+                    y.mutable_data_ptr(), nullptr, 0, nullptr, (float*)out_ptr(rstd), st);
+    if (graph && !rcode) {
+      std::shared_ptr<RmsNormNode> node(new RmsNormNode(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(*a.x, or_none(a.w), or_none(a.res)));
+      node->w = SavedVariable(or_none(a.w), false);
+      if (a.w) node->shape = a.w->sizes();
+      node->rstd = rstd;
+      node->sum = a.res != nullptr;
+      torch::autograd::set_history(y, node);
+      if (a.res) torch::autograd::set_history(total, node);
+      node->t = a.res ? SavedVariable(total, true) : SavedVariable(*a.x, false);
+    }
+  }
+  if (rcode || !a.res) return status_or(rcode, y);
+  return tuple_of({y, total});
+END
+
+// Rows in 8 bits on 16-byte boundaries, as tokens.py lays them out.
+at::Tensor eight_bits(at::IntArrayRef shape, int64_t pitch, int dev) {
+  at::DimVector full(shape);
+  full.back() = pitch;
+  at::Tensor q = fresh(full, at::kChar, dev);
+  return pitch == shape.back() ? q : q.narrow(-1, 0, shape.back());
+}
+
+// x, weight or None, eps, residual or None, device, stream
+BODY(rms_norm_int8, 6)
+  RmsIn a;
+  const int ok = rms_in(v, dev, &a);
+  if (ok < 0) return nullptr;
+  if (!ok || needs_graph(*a.x, a.w, a.res)) GENERAL;
+  at::Tensor q, scale, total;
+  int rcode;
+  {
+    Release r;
+    const int64_t pitch = (a.C + 15) / 16 * 16;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      q = eight_bits(a.x->sizes(), pitch, dev);
+      scale = fresh(a.x->sizes().slice(0, a.x->dim() - 1), at::kFloat, dev);
+      if (a.res) total = fresh(a.x->sizes(), a.x->scalar_type(), dev);
+    }
+    rcode = tok.rms(a.x->const_data_ptr(), code_of(a.x->scalar_type()), a.rows, (int)a.C, a.C, a.res ? a.res->const_data_ptr() : nullptr, a.C, a.wp, a.eps, out_ptr(total), nullptr,
+                    (int8_t*)q.mutable_data_ptr(), pitch, (float*)scale.mutable_data_ptr(), nullptr, st);
+  }
+  if (rcode) return PyLong_FromLong(rcode);
+  return tuple_of({q, scale, total});
+END
+
+// x, device, stream
+BODY(quantize, 3)
+  const at::Tensor* x = plain(v[0], dev);
+  if (!x || !real_type(*x) || x->dim() < 1 || x->numel() == 0 || !x->is_contiguous() || x->size(-1) > INT32_MAX || needs_graph(*x) || has_tangent(*x)) GENERAL;
+  at::Tensor q, scale;
+  int rcode;
+  {
+    Release r;
+    const int64_t C = x->size(-1), pitch = (C + 15) / 16 * 16;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      q = eight_bits(x->sizes(), pitch, dev);
+      scale = fresh(x->sizes().slice(0, x->dim() - 1), at::kFloat, dev);
+    }
+    rcode = tok.quantize(x->const_data_ptr(), code_of(x->scalar_type()), x->numel() / C, (int)C, C, (int8_t*)q.mutable_data_ptr(), pitch, (float*)scale.mutable_data_ptr(), st);
+  }
+  if (rcode) return PyLong_FromLong(rcode);
+  return tuple_of({q, scale});
+END
+
+// Rows of a tensor [..., k] a fixed stride apart, on 16-byte boundaries: what the kernels take without a copy.
+bool rows_on_boundaries(const at::Tensor& t, int64_t* stride) {
+  const int64_t k = t.size(-1), per = 16 / (int64_t)t.element_size();
+  if ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) || (t.stride(-1) != 1 && k > 1)) return false;
+  if (t.dim() == 2) *stride = t.size(0) > 1 ? t.stride(0) : (k + per - 1) / per * per;
+  else if (t.is_contiguous()) *stride = k;
+  else return false;
+  return *stride >= k && *stride % per == 0;
+}
+
+// q, scale, weight, weight_scale, bias or None, out dtype or -2, device, stream
+BODY(linear_int8, 8)
+  const at::Tensor *q = plain(v[0], dev), *s = plain(v[1], dev), *w = plain(v[2], dev), *ws = plain(v[3], dev);
+  if (!q || !s || !w || !ws || q->scalar_type() != at::kChar || w->scalar_type() != at::kChar || s->scalar_type() != at::kFloat || ws->scalar_type() != at::kFloat || q->dim() < 1 ||
+      w->dim() != 2 || q->numel() == 0 || w->numel() == 0 || q->size(-1) != w->size(1) || s->sizes() != q->sizes().slice(0, q->dim() - 1) || ws->dim() != 1 ||
+      ws->size(0) != w->size(0) || !s->is_contiguous() || !ws->is_contiguous())
+    GENERAL;
+  const int64_t K = w->size(1), N = w->size(0), M = q->numel() / K;
+  const long type = num(v[5]);
+  if (PyErr_Occurred()) return nullptr;
+  const float* b;
+  int64_t qs, wstride;
+  if (type < 0 || K >= 131072 || N > INT32_MAX || !bias_arg(v[4], dev, N, &b) || !rows_on_boundaries(*q, &qs) || !rows_on_boundaries(*w, &wstride)) GENERAL;
+  const at::Tensor* bias = b ? plain(v[4], dev) : nullptr;
+  if (needs_graph(*s, ws, bias) || has_tangent(*s) || has_tangent(*ws) || (bias && has_tangent(*bias))) GENERAL;
+  at::Tensor y;
+  int rcode;
+  {
+    Release r;
+    at::DimVector shape(q->sizes());
+    shape.back() = N;
+    y = fresh(shape, type_of(type), dev);
+    rcode = tok.int8(q->const_data_ptr<int8_t>(), M, (int)K, qs, s->const_data_ptr<float>(), w->const_data_ptr<int8_t>(), (int)N, wstride, ws->const_data_ptr<float>(), b,
+                     y.mutable_data_ptr(), (int)type, st);
+  }
+  return status_or(rcode, y);
+END
+
+// ------------------------------------------------------------------------------------------------------------ gated feed-forward block
+struct FeedForwardNode : Node {            // inputs x, gate, up and down weights, their biases
+  SavedVariable t[4];
+  at::Tensor saved;
+  int act = 0;
+  std::string name() const override { return "FoviGatedFeedForwardBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& s : t) s.reset_data();
+    saved.reset();
+  }
+  variable_list apply(variable_list&& in) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(7);
+    if (!in[0].defined()) return out;
+    const at::Tensor x = t[0].unpack(), wg = t[1].unpack(), wu = t[2].unpack(), wd = t[3].unpack();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const at::ScalarType type = x.scalar_type();
+      const int64_t C = wg.size(1), F = wg.size(0), O = wd.size(0), M = x.numel() / C;
+      const int dev = x.get_device();
+      at::Tensor g = in[0].to(type).contiguous();
+      if (reinterpret_cast<uintptr_t>(g.const_data_ptr()) & 15) g = g.clone();
+      const at::DimVector vf{F}, vo{O};
+      const at::IntArrayRef shape[7] = {x.sizes(), wg.sizes(), wu.sizes(), wd.sizes(), vf, vf, vo};
+      for (int i = 0; i < 7; ++i)
+        if (task_should_compute_output(i)) out[i] = fresh(shape[i], type, dev);
+      const int64_t bytes = tok.ffn_work(code_of(type), M, (int)C, (int)F, (int)O, 1);
+      const at::Tensor work = fresh({bytes}, at::kByte, dev);
+      launched(tok.ffn_back(x.const_data_ptr(), code_of(type), M, (int)C, (int)F, (int)O, C, wg.const_data_ptr(), C, wu.const_data_ptr(), C, wd.const_data_ptr(), F, act,
+                            saved.const_data_ptr(), g.const_data_ptr(), O, out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]), out_ptr(out[3]), out_ptr(out[4]), out_ptr(out[5]),
+                            out_ptr(out[6]), work.mutable_data_ptr(), bytes, stream_of(x)),
+               "fovi_gated_ffn_backward");
+    }
+    once(out, {in[0], x, wg, wu, wd}, "gated_feed_forward");
+    return out;
+  }
+};
+
+// x, gate, up and down weights, their biases or None, activation, device, stream
+BODY(gated_feed_forward, 10)
+  const at::Tensor* t[7] = {};
+  for (int i = 0; i < 7; ++i) {
+    if (i > 3 && v[i] == Py_None) continue;
+    t[i] = plain(v[i], dev);
+    if (!t[i] || !t[i]->is_contiguous() || t[i]->numel() == 0 || t[i]->scalar_type() != t[0]->scalar_type() || has_tangent(*t[i])) GENERAL;
+  }
+  const at::Tensor &x = *t[0], &wg = *t[1], &wu = *t[2], &wd = *t[3];
+  const long act = num(v[7]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!real_type(x) || x.dim() < 1 || wg.dim() != 2 || wd.dim() != 2 || wu.sizes() != wg.sizes() || x.size(-1) != wg.size(1) || wd.size(1) != wg.size(0)) GENERAL;
+  const int64_t C = wg.size(1), F = wg.size(0), O = wd.size(0), M = x.numel() / C;
+  const int64_t length[3] = {F, F, O};
+  for (int i = 4; i < 7; ++i)
+    if (t[i] && (t[i]->dim() != 1 || t[i]->size(0) != length[i - 4])) GENERAL;
+  if (C > INT32_MAX || F > INT32_MAX || O > INT32_MAX || M > (1 << 30)) GENERAL;
+  if (x.scalar_type() == at::kBFloat16) {
+    if (C % 8 || F % 8 || O % 8) GENERAL;          // (O: the rows of the result's gradient)
+    for (int i = 0; i < 4; ++i)
+      if (reinterpret_cast<uintptr_t>(t[i]->const_data_ptr()) & 15) GENERAL;
+  }
+  at::Tensor y;
+  int rcode;
+  {
+    Release r;
+    bool graph = false;
+    for (const at::Tensor* p : t) graph = graph || (p && needs_graph(*p));
+    const int type = code_of(x.scalar_type());
+    const int64_t bytes = tok.ffn_work(type, M, (int)C, (int)F, (int)O, graph ? 2 : 0);
+    at::Tensor saved, work;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      at::DimVector shape(x.sizes());
+      shape.back() = O;
+      y = fresh(shape, x.scalar_type(), dev);
+      if (graph) saved = fresh({tok.ffn_saved(type, M, (int)F)}, at::kByte, dev);
+      if (bytes > 0) work = fresh({bytes}, at::kByte, dev);
+    }
+    auto bias = [&](int i) { return t[i] ? t[i]->const_data_ptr() : nullptr; };
+    rcode = tok.ffn(x.const_data_ptr(), type, M, (int)C, (int)F, (int)O, C, wg.const_data_ptr(), C, wu.const_data_ptr(), C, wd.const_data_ptr(), F, bias(4), bias(5), bias(6),
+                    (int)act, y.mutable_data_ptr(), out_ptr(saved), out_ptr(work), bytes, st);
+    if (graph && !rcode) {
+      std::shared_ptr<FeedForwardNode> node(new FeedForwardNode(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(x, wg, wu, wd, or_none(t[4]), or_none(t[5]), or_none(t[6])));
+      for (int i = 0; i < 4; ++i) node->t[i] = SavedVariable(*t[i], false);
+      node->saved = saved;
+      node->act = (int)act;
+      torch::autograd::set_history(y, node);
+    }
+  }
+  return status_or(rcode, y);
 END
 
 }  // namespace

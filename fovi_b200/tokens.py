@@ -161,6 +161,11 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None):
     """Root-mean-square norm over the last axis: y = t / sqrt(mean(t^2) + eps) * weight of t = x, or with `residual` (x's shape and type) of t = x + residual as their type holds it:
     then (y, t) is returned, the same values as from the addition and the norm one after the other.  x [..., C] float32 or bf16; weight [C] or None.  Statistics, sums and the
     weight's gradient are float32; gradients are the same bits every time."""
+    if ops._native is not None and x.is_cuda:
+        dev = ops._current_device()
+        got = ops._native.rms_norm(x, weight, eps, residual, dev, ops._raw_stream(dev))
+        if got is not None:
+            return ops._checked(got, "fovi_rms_norm_forward")
     _no_tangents("rms_norm", x, weight, residual)
     if _wants_grad(x, weight, residual):
         return _RmsNormFunction.apply(x, weight, eps, residual)
@@ -177,6 +182,11 @@ def rms_norm_int8(x, weight=None, eps=1e-6, residual=None):
     """rms_norm with its result in 8 bits for linear_int8: (q, scale), or (q, scale, t) with `residual`; y = q * scale to half a step.  q int8 [..., C], values of -127 .. 127 rounded
     from the unrounded y; scale float32 [...], max |y| / 127 of the row (at least the smallest normal number).  A row that holds infinity or not-a-number has one of them as its scale.
     No gradient."""
+    if ops._native is not None and x.is_cuda:
+        dev = ops._current_device()
+        got = ops._native.rms_norm_int8(x, weight, eps, residual, dev, ops._raw_stream(dev))
+        if got is not None:
+            return ops._checked(got, "fovi_rms_norm_forward")
     _no_tangents("rms_norm_int8", x, weight, residual)
     _no_gradient("rms_norm_int8", x, weight, residual)
     q, scale, total = ops.rms_norm_int8(x, weight, eps, residual)
@@ -186,6 +196,11 @@ def rms_norm_int8(x, weight=None, eps=1e-6, residual=None):
 def quantize(x):
     """Rows of x [..., C] (float32 or bf16) in 8 bits with a scale each, as rms_norm_int8 gives them: tokens for linear_int8, or a weight [N, K] with a scale for each
     output channel.  No gradient."""
+    if ops._native is not None and x.is_cuda:
+        dev = ops._current_device()
+        got = ops._native.quantize(x, dev, ops._raw_stream(dev))
+        if got is not None:
+            return ops._checked(got, "fovi_quantize_rows")
     _no_tangents("quantize", x)
     _no_gradient("quantize", x)
     return ops.quantize(x)
@@ -194,6 +209,11 @@ def quantize(x):
 def linear_int8(q, scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
     """y = scale * weight_scale * (q weight^T) + bias: q int8 [..., K] with scale float32 [...], weight int8 [N, K] with weight_scale float32 [N], both as ``quantize`` gives them (or
     any other int8 tensors), bias [N] or None; K up to 131071.  The sums are exact; the result [..., N] is float32 or bf16.  No gradient."""
+    if ops._native is not None and q.is_cuda:
+        dev = ops._current_device()
+        got = ops._native.linear_int8(q, scale, weight, weight_scale, bias, ops._DT.get(out_dtype, -2), dev, ops._raw_stream(dev))
+        if got is not None:
+            return ops._checked(got, "fovi_linear_int8")
     _no_tangents("linear_int8", scale, weight_scale, bias)
     _no_gradient("linear_int8", scale, weight_scale, bias)
     return ops.linear_int8(q, scale, weight, weight_scale, bias, out_dtype)
@@ -218,6 +238,11 @@ def gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias=None, u
     biases [F], [F], [O] or None, all float32 or all bf16; activation "silu" or "gelu" (with the error function).  Differentiable in all tensors.  Sums are float32; with bf16 the
     hidden values, and in the backward pass their gradients, are rounded to bf16 between the products.  Gradients are the same bits every time, whichever are asked for."""
     leaves = (x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias)
+    if ops._native is not None and x.is_cuda and activation in ops.ACTIVATIONS:
+        dev = ops._current_device()
+        got = ops._native.gated_feed_forward(*leaves, ops.ACTIVATIONS[activation], dev, ops._raw_stream(dev))
+        if got is not None:
+            return ops._checked(got, "fovi_gated_ffn_forward")
     _no_tangents("gated_feed_forward", *leaves)
     if _wants_grad(*leaves):
         return _FeedForwardFunction.apply(*leaves, activation)

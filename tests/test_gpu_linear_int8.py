@@ -8,6 +8,15 @@ pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True, params=["native", "python"])
+def launch_path(request, monkeypatch):
+    """Every test with the native launch path (csrc/bind_tokens.h) and with the Python one."""
+    from fovi_b200 import ops
+    assert ops._native is not None
+    if request.param == "python":
+        monkeypatch.setattr(ops, "_native", None)
+
+
 def _inputs(m, k, n, seed, low=-128):
     g = torch.Generator(device="cuda").manual_seed(seed)
     q, w = (torch.randint(low, 128, (r, k), generator=g, device="cuda", dtype=torch.int8) for r in (m, n))
