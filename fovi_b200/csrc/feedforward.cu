@@ -27,26 +27,38 @@ __device__ __forceinline__ float2 activate(float g, int act) {
 
 struct GateUp {       // g and u -> h
   Hidden to; const float *bg, *bu; int act;
-  __device__ __forceinline__ void operator()(int64_t m, int n, float g, float u) const {
-    g += bg ? __ldg(bg + n) : 0.f;
-    u += bu ? __ldg(bu + n) : 0.f;
+  __device__ __forceinline__ void operator()(int, int, int64_t m, int n, float (&g)[4], float (&u)[4], int left) const {
     const int64_t at = m * to.pitch + n;
-    if (to.g) { to.g[at] = g; to.u[at] = u; }
-    static_cast<float*>(to.h)[at] = activate(g, act).x * u;
+    float h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j < left) {
+        g[j] += bg ? __ldg(bg + n + j) : 0.f;
+        u[j] += bu ? __ldg(bu + n + j) : 0.f;
+      }
+      h[j] = activate(g[j], act).x * u[j];
+    }
+    if (to.g) {
+      store4(to.g + at, g, left, to.pitch);
+      store4(to.u + at, u, left, to.pitch);
+    }
+    store4(static_cast<float*>(to.h) + at, h, left, to.pitch);
   }
 };
 struct HiddenGrad {   // dh -> dg, du
   Hidden from; float *dg, *du; int act;
-  __device__ __forceinline__ void operator()(int64_t m, int n, float dh, float) const {
+  __device__ __forceinline__ void operator()(int, int, int64_t m, int n, float (&dh)[4], float (&du4)[4], int left) const {
     const int64_t at = m * from.pitch + n;
-    const float2 s = activate(from.g[at], act);
-    dg[at] = dh * from.u[at] * s.y;
-    du[at] = dh * s.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= left) continue;
+      const float2 s = activate(__ldg(from.g + at + j), act);
+      du4[j] = dh[j] * s.x;
+      dh[j] = dh[j] * __ldg(from.u + at + j) * s.y;
+    }
+    store4(dg + at, dh, left, from.pitch);
+    store4(du + at, du4, left, from.pitch);
   }
-};
-struct Store {
-  float* y; int64_t pitch; const float* bias;
-  __device__ __forceinline__ void operator()(int64_t m, int n, float v, float) const { y[m * pitch + n] = v + (bias ? __ldg(bias + n) : 0.f); }
 };
 
 // Column sums of [rows, n] in a fixed order: parts of strips of rows, then the parts of a column.
@@ -107,22 +119,38 @@ struct Block {
   int64_t M, xs, gs, us, ds; int C, F, O, act;
 };
 
-int forward_f32(const Block& b, void* y, const Hidden& hid, cudaStream_t st) {
-  SimtArgs p{};
-  p.m = b.M; p.n = b.F; p.k[0] = b.C; p.segments = 1;
-  p.a[0] = Operand{b.x, b.xs, 1};
-  p.b[0] = Operand{b.wg, b.gs, 1};
-  p.b2 = Operand{b.wu, b.us, 1};
-  int rc = product_simt<float, true>(p, GateUp{hid, static_cast<const float*>(b.bg), static_cast<const float*>(b.bu), b.act}, st);
-  if (rc) return rc;
-  p.n = b.O; p.k[0] = b.F;
-  p.a[0] = Operand{hid.h, hid.pitch, 1};
-  p.b[0] = Operand{b.wd, b.ds, 1};
-  return product_simt<float, false>(p, Store{static_cast<float*>(y), b.O, static_cast<const float*>(b.bd)}, st);
-}
-
 // The parts of a workspace, each on a boundary of 256 bytes.
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// The block's float32 products.
+SimtTask task(const Operand& a, const Operand& b, int64_t m, int n, int k) {
+  SimtTask t{};
+  t.a[0] = a; t.b[0] = b; t.m = m; t.n = n; t.k[0] = k;
+  return t;
+}
+SimtTask down_task(const Block& b, const Hidden& hid) { return task({hid.h, hid.pitch, 1}, {b.wd, b.ds, 1}, b.M, b.O, b.F); }
+SimtTask input_task(const Block& b, const float* dg, const float* du, int64_t pitch) {
+  SimtTask t = task({dg, pitch, 1}, {b.wg, 1, b.gs}, b.M, b.C, b.F);
+  t.a[1] = {du, pitch, 1}; t.b[1] = {b.wu, 1, b.us}; t.k[1] = b.F;
+  return t;
+}
+void weight_tasks_f32(const Block& b, const Hidden& hid, const void* dy, int64_t dys, const float* dg, const float* du, SimtTask (&t)[3]) {
+  t[0] = task({dg, 1, hid.pitch}, {b.x, 1, b.xs}, b.F, b.C, (int)b.M);
+  t[1] = task({du, 1, hid.pitch}, {b.x, 1, b.xs}, b.F, b.C, (int)b.M);
+  t[2] = task({dy, 1, dys}, {hid.h, 1, hid.pitch}, b.O, b.F, (int)b.M);
+}
+
+int forward_f32(const Block& b, void* y, const Hidden& hid, void* work, cudaStream_t st) {
+  SimtArgs p{};
+  p.tasks = p.segments = p.splits = 1;
+  p.t[0] = task({b.x, b.xs, 1}, {b.wg, b.gs, 1}, b.M, b.F, b.C);
+  p.t[0].b2 = Operand{b.wu, b.us, 1};
+  const int rc = product_simt<true>(p, GateUp{hid, static_cast<const float*>(b.bg), static_cast<const float*>(b.bu), b.act}, st);
+  if (rc) return rc;
+  const SimtTask t = down_task(b, hid);
+  float* to = static_cast<float*>(y);
+  return simt_store(&t, &to, 1, 1, static_cast<const float*>(b.bd), static_cast<float*>(work), st);
+}
 
 int forward_bf16(const Block& b, void* y, const Hidden& hid, void* work, cudaStream_t st) {
   if (b.M <= fovi::FEW_TOKENS && !hid.high) {
@@ -136,37 +164,41 @@ int forward_bf16(const Block& b, void* y, const Hidden& hid, void* work, cudaStr
 
 struct Grads { const void* dy; int64_t dys; void *dx, *dwg, *dwu, *dwd, *dbg, *dbu, *dbd; };
 
+// Work of a float32 backward pass: dg, du; then, one after another in the same place, the parts of dx, of the weight gradients, and of the biases' sums.
+struct BackWork { int64_t sums, parts, bytes; };
+BackWork back_work_f32(const Block& b, int64_t pitch) {
+  SimtTask t[3];
+  const SimtTask in = input_task(b, nullptr, nullptr, pitch);
+  Hidden h{};
+  h.pitch = pitch;
+  weight_tasks_f32(b, h, nullptr, 0, nullptr, nullptr, t);
+  BackWork w{};
+  w.parts = padded(2 * b.M * pitch * 4);
+  w.bytes = w.parts + std::max({simt_store_bytes(&in, 1, 2), simt_store_bytes(t, 3, 1), (int64_t)STRIPS * std::max(b.F, b.O) * 4});
+  return w;
+}
+
 int backward_f32(const Block& b, const Hidden& hid, const Grads& g, char* work, cudaStream_t st) {
-  float *dg = reinterpret_cast<float*>(work), *du = dg + b.M * hid.pitch, *part = du + b.M * hid.pitch;
+  float *dg = reinterpret_cast<float*>(work), *du = dg + b.M * hid.pitch, *parts = reinterpret_cast<float*>(work + back_work_f32(b, hid.pitch).parts);
   int rc;
-  SimtArgs p{};
-  p.segments = 1;
   if (g.dx || g.dwg || g.dwu || g.dbg || g.dbu) {
-    p.m = b.M; p.n = b.F; p.k[0] = b.O;
-    p.a[0] = Operand{g.dy, g.dys, 1};
-    p.b[0] = Operand{b.wd, 1, b.ds};
-    if ((rc = product_simt<float, false>(p, HiddenGrad{hid, dg, du, b.act}, st))) return rc;
+    SimtArgs p{};
+    p.tasks = p.segments = p.splits = 1;
+    p.t[0] = task({g.dy, g.dys, 1}, {b.wd, 1, b.ds}, b.M, b.F, b.O);
+    if ((rc = product_simt<false>(p, HiddenGrad{hid, dg, du, b.act}, st))) return rc;
   }
   if (g.dx) {
-    p.m = b.M; p.n = b.C; p.k[0] = p.k[1] = b.F; p.segments = 2;
-    p.a[0] = Operand{dg, hid.pitch, 1}; p.a[1] = Operand{du, hid.pitch, 1};
-    p.b[0] = Operand{b.wg, 1, b.gs}; p.b[1] = Operand{b.wu, 1, b.us};
-    if ((rc = product_simt<float, false>(p, Store{static_cast<float*>(g.dx), b.C, nullptr}, st))) return rc;
+    const SimtTask t = input_task(b, dg, du, hid.pitch);
+    float* to = static_cast<float*>(g.dx);
+    if ((rc = simt_store(&t, &to, 1, 2, nullptr, parts, st))) return rc;
   }
-  p.segments = 1;
-  p.k[0] = (int)b.M;
-  const struct { void* to; const void* a; int64_t as; int m; const void* b; int64_t bs; int n; } weights[3] = {
-      {g.dwg, dg, hid.pitch, b.F, b.x, b.xs, b.C}, {g.dwu, du, hid.pitch, b.F, b.x, b.xs, b.C}, {g.dwd, g.dy, g.dys, b.O, hid.h, hid.pitch, b.F}};
-  for (const auto& w : weights) {
-    if (!w.to) continue;
-    p.m = w.m; p.n = w.n;
-    p.a[0] = Operand{w.a, 1, w.as};
-    p.b[0] = Operand{w.b, 1, w.bs};
-    if ((rc = product_simt<float, false>(p, Store{static_cast<float*>(w.to), w.n, nullptr}, st))) return rc;
-  }
-  if (g.dbg && (rc = column_sums<float>(dg, b.M, b.F, hid.pitch, part, g.dbg, st))) return rc;
-  if (g.dbu && (rc = column_sums<float>(du, b.M, b.F, hid.pitch, part, g.dbu, st))) return rc;
-  if (g.dbd && (rc = column_sums<float>(g.dy, b.M, b.O, g.dys, part, g.dbd, st))) return rc;
+  SimtTask t[3];
+  weight_tasks_f32(b, hid, g.dy, g.dys, dg, du, t);
+  float* const to[3] = {static_cast<float*>(g.dwg), static_cast<float*>(g.dwu), static_cast<float*>(g.dwd)};
+  if ((rc = simt_store(t, to, 3, 1, nullptr, parts, st))) return rc;
+  if (g.dbg && (rc = column_sums<float>(dg, b.M, b.F, hid.pitch, parts, g.dbg, st))) return rc;
+  if (g.dbu && (rc = column_sums<float>(du, b.M, b.F, hid.pitch, parts, g.dbu, st))) return rc;
+  if (g.dbd && (rc = column_sums<float>(g.dy, b.M, b.O, g.dys, parts, g.dbd, st))) return rc;
   return FOVI_OK;
 }
 
@@ -179,7 +211,6 @@ void weight_tasks(const Block& b, const Hidden& hid, const Grads& g, const void*
 
 // Work of a bf16 backward pass: dg, du; then, one after another in the same place, the parts of dx, of the weight gradients, and of the biases' sums of dy.  The sums of
 // dg and du, which the first kernel leaves, have a place of their own.
-struct BackWork { int64_t sums, parts, bytes; };
 BackWork back_work(const Block& b, int64_t pitch) {
   TcTask t[3];
   weight_tasks(b, Hidden{}, Grads{}, nullptr, nullptr, t);
@@ -228,11 +259,11 @@ extern "C" int64_t fovi_gated_ffn_saved_bytes(int dtype, int64_t tokens, int F) 
 extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int phase) {
   if (!valid(dtype, tokens, C, F, O) || phase < 0 || phase > 2) return -1;
   const int64_t n = tokens * pitch_of(F) * (int64_t)fovi::dtype_size(dtype);
-  if (dtype == FOVI_F32) return phase == 1 ? 2 * n + (int64_t)STRIPS * std::max(F, O) * 4 : phase == 0 ? n : 0;
-  if (phase != 1) return (phase == 0 ? padded(n) : 0) + fovi::tc_linear_bytes(tokens, O, F);
   Block b{};
   b.M = tokens; b.C = C; b.F = F; b.O = O;
-  return back_work(b, pitch_of(F)).bytes;
+  if (phase == 1) return (dtype == FOVI_F32 ? back_work_f32(b, pitch_of(F)) : back_work(b, pitch_of(F))).bytes;
+  const SimtTask down = down_task(b, Hidden{});
+  return (phase == 0 ? padded(n) : 0) + (dtype == FOVI_F32 ? simt_store_bytes(&down, 1, 1) : fovi::tc_linear_bytes(tokens, O, F));
 }
 
 extern "C" int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
@@ -246,9 +277,10 @@ extern "C" int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, 
   const Block b{x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias, tokens, x_stride, gate_stride, up_stride, down_stride, C, F, O, activation};
   const Hidden h = hidden_at(saved ? saved : work, dtype, tokens, F, saved != nullptr);
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == FOVI_F32) return forward_f32(b, y, h, st);
+  char* parts = static_cast<char*>(work) + (saved ? 0 : padded(tokens * h.pitch * (int64_t)fovi::dtype_size(dtype)));
+  if (dtype == FOVI_F32) return forward_f32(b, y, h, parts, st);
   if (!aligned(b) || reinterpret_cast<uintptr_t>(y) % 16) return FOVI_ERR_ALIGNMENT;
-  return forward_bf16(b, y, h, static_cast<char*>(work) + (saved ? 0 : padded(tokens * h.pitch * 2)), st);
+  return forward_bf16(b, y, h, parts, st);
 }
 
 extern "C" int fovi_gated_ffn_backward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
