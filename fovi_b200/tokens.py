@@ -339,7 +339,8 @@ class TokenRMSNorm(nn.Module):
 
 
 class GatedFeedForward(nn.Module):
-    """A block's gated feed-forward half: `gate`, `up` and `down` are torch's Linear by parameters and state dict; their values are taken in x's type."""
+    """A block's gated feed-forward half: `gate`, `up` and `down` are torch's Linear by parameters and state dict; their values are taken in x's type, and both in autocast's where that
+    is on."""
 
     def __init__(self, dim, hidden, activation="silu", bias=True, device="cuda", dtype=None):
         super().__init__()
@@ -351,6 +352,8 @@ class GatedFeedForward(nn.Module):
 
     def forward(self, x):
         layers = (self.gate, self.up, self.down)
+        if torch.is_autocast_enabled("cuda"):
+            x = x.to(torch.get_autocast_dtype("cuda"))
         return gated_feed_forward(x, *(m.weight.to(x.dtype) for m in layers), *(None if m.bias is None else m.bias.to(x.dtype) for m in layers), activation=self.activation)
 
 
@@ -383,9 +386,10 @@ class FixationReader(nn.Module):
     """Reads images out through several fixations: sensor -> foveated patch embedding -> the tokens of all fixations as one set of states, each with its place (the fixation's number,
     and the height and width in the image at which the token looks) -> learned queries, in `depth` pre-norm cross-attention blocks -> class scores.
 
-    retina: RetinalTransform; embedding: KNNPatchEmbedding of `dim` channels that it feeds (not transposed)."""
+    retina: RetinalTransform; embedding: KNNPatchEmbedding of `dim` channels that it feeds (not transposed).  feed_forward: hidden channels of a gated feed-forward half behind each
+    block's attention, its norm fused with the addition of what the attention found; none by default."""
 
-    def __init__(self, retina, embedding, dim, heads, n_classes, queries=1, depth=1, kv_heads=None, device="cuda"):
+    def __init__(self, retina, embedding, dim, heads, n_classes, queries=1, depth=1, kv_heads=None, device="cuda", feed_forward=None):
         super().__init__()
         self.retina, self.embedding, self.dim = retina, embedding, dim
         self.rotary = AxialRotary(dim // heads, axes=3, units=[1.0, 2 * math.pi, 2 * math.pi], device=device)
@@ -393,6 +397,9 @@ class FixationReader(nn.Module):
         self.state_norm = TokenNorm(dim, device=device)
         self.norms = nn.ModuleList([TokenNorm(dim, device=device) for _ in range(depth)])
         self.blocks = nn.ModuleList([CrossAttention(dim, heads, kv_heads, rotary=self.rotary, device=device) for _ in range(depth)])
+        hidden = [] if feed_forward is None else [feed_forward] * depth
+        self.feed_forward_norms = nn.ModuleList([TokenRMSNorm(dim, device=device) for _ in hidden])
+        self.feed_forwards = nn.ModuleList([GatedFeedForward(dim, n, device=device) for n in hidden])
         self.norm = TokenNorm(dim, device=device)
         self.classifier = nn.Linear(dim, n_classes, device=device)
 
@@ -416,8 +423,12 @@ class FixationReader(nn.Module):
     def read(self, states, places, key_lengths=None, key_mask=None):
         """Class scores [B, n_classes] from the states; key_lengths / key_mask: as for cross_attention."""
         x = self.queries.to(states.dtype).expand(states.shape[0], -1, -1)
-        for norm, block in zip(self.norms, self.blocks):
-            x = x + block(norm(x), block.project_states(states, places), key_lengths=key_lengths, key_mask=key_mask)
+        for i, (norm, block) in enumerate(zip(self.norms, self.blocks)):
+            found = block(norm(x), block.project_states(states, places), key_lengths=key_lengths, key_mask=key_mask)
+            if self.feed_forwards:
+                normed, x = self.feed_forward_norms[i](found.to(x.dtype), residual=x)
+                found = self.feed_forwards[i](normed)
+            x = x + found
         return self.classifier(self.norm(x).mean(1))
 
     def forward(self, images, fix_loc, fixation_size=None, fixation_counts=None):
