@@ -51,7 +51,7 @@ struct PtArgs {
   int64_t part[GROUPS];                    // parts of k: where a task's begin in `work` (float32)
   int kb0, kb, splits;                     // stages of the first segment of k, of all, parts
   int ct;
-  const void *bias, *bias2; int act;
+  const void *bias, *bias2;
   Hidden hidden; void *dg, *du; float* sums;
   const float *scale, *wscale, *bias_f; int y_f32;
   float* work;
@@ -126,14 +126,23 @@ __device__ __forceinline__ void st_global_32f(float* p, const uint32_t* v) {
   st_global_32(p, w);
 }
 
-// act(g) and act'(g), to a few units of float32: what is rounded to bf16 behind them.
-__device__ __forceinline__ float2 fast_act(float g, int act) {
-  if (act == fovi::ACT_SILU) {
-    const float p = __fdividef(1.f, 1.f + __expf(-g)), a = g * p;
-    return make_float2(a, fmaf(a, 1.f - p, p));
+// act(g) and act'(g) of two values, to a few units of float32: what is rounded to bf16 behind them.  The logistic function takes an exponential each and one reciprocal for both,
+// 1/a = b/(ab), since those units are what bounds a tile's arithmetic; exponents are cut at 2^60, so that the product stays finite: there the function is below 1e-18.
+template <int ACT> __device__ __forceinline__ void act_pair(float g0, float g1, float2* value, float2* slope) {
+  if (ACT == fovi::ACT_SILU) {
+    float e0, e1, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(-1.4426950408889634f * g0, 60.f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(-1.4426950408889634f * g1, 60.f)));
+    e0 += 1.f; e1 += 1.f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e0 * e1));
+    const float p0 = r * e1, p1 = r * e0, a0 = g0 * p0, a1 = g1 * p1;
+    *value = make_float2(a0, a1);
+    if (slope) *slope = make_float2(fmaf(a0, 1.f - p0, p0), fmaf(a1, 1.f - p1, p1));
+  } else {
+    const float p0 = 0.5f * (1.f + erff(g0 * 0.70710678118654752f)), p1 = 0.5f * (1.f + erff(g1 * 0.70710678118654752f));
+    *value = make_float2(g0 * p0, g1 * p1);
+    if (slope) *slope = make_float2(fmaf(g0 * 0.39894228040143268f, __expf(-0.5f * g0 * g0), p0), fmaf(g1 * 0.39894228040143268f, __expf(-0.5f * g1 * g1), p1));
   }
-  const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-  return make_float2(g * p, fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), p));
 }
 
 struct Tile { int task, mt, nt, k0, k1, split; };
@@ -166,7 +175,7 @@ template <typename T> __device__ __forceinline__ void store_any(T* y, int64_t n,
   __syncwarp();
 }
 
-template <int EPI, bool A_MN, bool B_MN, bool I8>
+template <int EPI, bool A_MN, bool B_MN, bool I8, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) product_tc_kernel(const __grid_constant__ PtMaps maps, const __grid_constant__ PtArgs a) {
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -287,26 +296,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
     auto row_of = [&](const Tile& t) { return t.mt * 256 + rank * 128 + quarter * 32; };
     uint32_t acc = 0, aph = 0;
     // GRAD: g and u of this warp's chunks, two on their way.  The next to be asked for is chunk next_c of next_item.
-    int next_item = worker, next_c = turn, asked = 0, taken = 0;
-    auto ask = [&]() {
-      Tile t{};
-      int chunks = 0;
-      for (; next_item < total; next_item += workers, next_c = turn) {
-        t = tile_of(a, next_item);
-        chunks = chunks_of(t);
-        if (next_c < chunks) break;
+    int next_item = worker, next_c = turn, next_chunks = 0, next_col = 0, next_row = 0, asked = 0, taken = 0;
+    auto next_tile = [&]() {                         // on to a tile with a chunk for this warp
+      for (next_c = turn; next_item < total; next_item += workers) {
+        const Tile t = tile_of(a, next_item);
+        next_chunks = chunks_of(t);
+        next_col = t.nt * width;
+        next_row = row_of(t);
+        if (turn < next_chunks) return;
       }
+    };
+    auto ask = [&]() {
       if (next_item >= total) return;
       if (lane == 0) {
         const uint32_t to = place + (asked & 1) * 6144u, bar = smem_u32(&hdr->came[warp][asked & 1]);
         mbar_expect_tx(bar, 6144u);
-        const int c = t.nt * width + 32 * next_c;
-        pt_load_own(to, &maps.high, bar, 2 * c, row_of(t));
-        pt_load_own(to + 4096u, &maps.low, bar, 2 * c, row_of(t));
+        pt_load_own(to, &maps.high, bar, 2 * (next_col + 32 * next_c), next_row);
+        pt_load_own(to + 4096u, &maps.low, bar, 2 * (next_col + 32 * next_c), next_row);
       }
       ++asked;
       next_c += 2;
+      if (next_c >= next_chunks) { next_item += workers; next_tile(); }
     };
+    if (EPI == GRAD) next_tile();
     if (EPI == GRAD && !a.skip_loads) { ask(); ask(); }
     for (int item = worker; item < total; item += workers) {
       const Tile t = tile_of(a, item);
@@ -315,35 +327,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
       const int M = a.m[t.task], N = a.n[t.task];
       const bool here = row < M;
       const int col0 = t.nt * width, chunks = chunks_of(t);
-      float rs = 0.f;
+      float rs = 0.f, f0[4], f1[4];                   // asked for in front of the wait: the row's scale, and a column a lane of factors and biases for each of up to four chunks
       if (EPI == SCALED) rs = here ? __ldg(a.scale + row) : 0.f;
+#pragma unroll
+      for (int i = 0; i < (EPI == GATED ? 2 : 4); ++i) {
+        const int n = col0 + 32 * (turn + 2 * i) + lane;
+        const bool in = turn + 2 * i < chunks && n < N;
+        const __nv_bfloat16 *b0 = static_cast<const __nv_bfloat16*>(a.bias), *b1 = static_cast<const __nv_bfloat16*>(a.bias2);
+        f0[i] = f1[i] = 0.f;
+        if (EPI == SCALED) {
+          if (in) f0[i] = __ldg(a.wscale + n);
+          if (in && a.bias_f) f1[i] = __ldg(a.bias_f + n);
+        } else if (EPI == GATED || (EPI == STORE && a.splits == 1)) {
+          if (in && b0) f0[i] = __bfloat162float(__ldg(b0 + n));
+          if (EPI == GATED && in && b1) f1[i] = __bfloat162float(__ldg(b1 + n));
+        }
+      }
       if (!mbar_wait_warp(smem_u32(&hdr->acc_full[acc]), aph, abort_flag, a.status, 44, a.wait_limit)) break;
       tc_fence_after();
-      auto release = [&]() {                          // this warp has read the accumulator
+      auto release = [&]() {                          // this warp has read the accumulator (relaxed: a release would wait for the warp's stores to arrive in memory)
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(pt_map(smem_u32(&hdr->acc_empty[acc]), 0)) : "memory");
+        if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(pt_map(smem_u32(&hdr->acc_empty[acc]), 0)) : "memory");
       };
       if (turn >= chunks) release();
       bool lost = false;
-      for (int c = turn; c < chunks; c += 2) {
-        const int c0 = col0 + 32 * c;
+#pragma unroll
+      for (int ci = 0; ci < (EPI == GATED ? 2 : 4); ++ci) {
+        const int c = turn + 2 * ci, c0 = col0 + 32 * c;
+        if (c >= chunks) break;
         if (EPI == GATED) {
-          const int f = c0 + lane;
-          const __nv_bfloat16 *bg = static_cast<const __nv_bfloat16*>(a.bias), *bu = static_cast<const __nv_bfloat16*>(a.bias2);
-          const float b0 = bg && f < N ? __bfloat162float(__ldg(bg + f)) : 0.f, b1 = bu && f < N ? __bfloat162float(__ldg(bu + f)) : 0.f;
           uint32_t g[32], u[32];
           tc_ld32(t_base + 32 * c, g);
           tc_ld32(t_base + half + 32 * c, u);
           tc_ld_wait();
           if (c + 2 >= chunks) release();
-          if (bg) {
+          if (a.bias) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) g[i] = __float_as_uint(__uint_as_float(g[i]) + __shfl_sync(0xffffffffu, b0, i));
+            for (int i = 0; i < 32; ++i) g[i] = __float_as_uint(__uint_as_float(g[i]) + __shfl_sync(0xffffffffu, f0[ci], i));
           }
-          if (bu) {
+          if (a.bias2) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) + __shfl_sync(0xffffffffu, b1, i));
+            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) + __shfl_sync(0xffffffffu, f1[ci], i));
           }
           if (lane == 0) bulk_read();                 // the chunk before has left this place
           __syncwarp();
@@ -369,7 +394,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int e = 8 * i + 2 * j;
-              h[j] = bf16_pair(fast_act(__uint_as_float(g[e]), a.act).x * __uint_as_float(u[e]), fast_act(__uint_as_float(g[e + 1]), a.act).x * __uint_as_float(u[e + 1]));
+              float2 v;
+              act_pair<ACT>(__uint_as_float(g[e]), __uint_as_float(g[e + 1]), &v, nullptr);
+              h[j] = bf16_pair(v.x * __uint_as_float(u[e]), v.y * __uint_as_float(u[e + 1]));
             }
             put16(place + 6144u + at64(lane, i), h[0], h[1], h[2], h[3]);
           }
@@ -398,20 +425,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
           uint32_t dg[16], du[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float x[2], y[2];
+            float g[2], u[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int e = 2 * i + j;
               const uint32_t pick = (j ? 0x3244u : 0x1044u) + ((uint32_t)(e & 3) << 4);      // [two high bytes, low byte, any]
-              const float g = __uint_as_float((__byte_perm(gu[i], lo[e / 4], pick) & 0xffffff00u) | 0x80u);
-              const float u = __uint_as_float((__byte_perm(gu[16 + i], lo[8 + e / 4], pick) & 0xffffff00u) | 0x80u);
-              const float dh = __uint_as_float(r[e]);
-              const float2 s = fast_act(g, a.act);
-              x[j] = dh * u * s.y;
-              y[j] = dh * s.x;
+              g[j] = __uint_as_float((__byte_perm(gu[i], lo[e / 4], pick) & 0xffffff00u) | 0x80u);
+              u[j] = __uint_as_float((__byte_perm(gu[16 + i], lo[8 + e / 4], pick) & 0xffffff00u) | 0x80u);
             }
-            dg[i] = bf16_pair(x[0], x[1]);
-            du[i] = bf16_pair(y[0], y[1]);
+            float2 v, d;
+            act_pair<ACT>(g[0], g[1], &v, &d);
+            const float h0 = __uint_as_float(r[2 * i]), h1 = __uint_as_float(r[2 * i + 1]);
+            dg[i] = bf16_pair(h0 * u[0] * d.x, h1 * u[1] * d.y);
+            du[i] = bf16_pair(h0 * v.x, h1 * v.y);
           }
           __syncwarp();                               // every lane has its g and u
 #pragma unroll
@@ -443,21 +469,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
         } else {
           uint32_t r[32];
           float v[32];
-          if (EPI == SCALED) {
-            const int n = c0 + lane;
-            const float ws = n < N ? __ldg(a.wscale + n) : 0.f, b = a.bias_f && n < N ? __ldg(a.bias_f + n) : 0.f;
-            __syncwarp();
-            scratch[lane] = ws;
-            scratch[32 + lane] = b;
-            __syncwarp();
-          } else if (a.splits == 1) {
-            const int n = c0 + lane;
-            const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(a.bias);
-            const float b = bias && n < N ? __bfloat162float(__ldg(bias + n)) : 0.f;
-            __syncwarp();
-            scratch[lane] = b;
-            __syncwarp();
-          }
+          __syncwarp();
+          scratch[lane] = f0[ci];
+          if (EPI == SCALED) scratch[32 + lane] = f1[ci];
+          __syncwarp();
           tc_ld32(t_base + 32 * c, r);
           tc_ld_wait();
           if (c + 2 >= chunks) release();
@@ -572,12 +587,12 @@ int map_k(CUtensorMap* m, const TcMatrix& x, bool bytes, int rows) {
 }
 int map_mn(CUtensorMap* m, const TcMatrix& x) { return fovi::encode_2d(m, x.p, false, (uint64_t)x.cols, (uint64_t)x.rows, (uint64_t)x.pitch * 2, 64, 64); }
 
-template <int EPI, bool A_MN, bool B_MN, bool I8> int launch(const PtMaps& maps, PtArgs& a, bool selftest, cudaStream_t st) {
+template <int EPI, bool A_MN, bool B_MN, bool I8, int ACT = 0> int launch(const PtMaps& maps, PtArgs& a, bool selftest, cudaStream_t st) {
   FOVI_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&a.status), g_status));
   a.wait_limit = selftest ? 4096u : WAIT_LIMIT;
   a.skip_loads = selftest;
   const int grid = 2 * std::min(a.first[a.tasks], pairs());
-  auto kernel = product_tc_kernel<EPI, A_MN, B_MN, I8>;
+  auto kernel = product_tc_kernel<EPI, A_MN, B_MN, I8, ACT>;
   FOVI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sizes<EPI>::SMEM));
   FOVI_CUDA(fovi::launch_pdl(kernel, grid, PT_THREADS, Sizes<EPI>::SMEM, st, maps, a));
   return fovi::after_launch("product_tc_kernel");
@@ -629,14 +644,15 @@ int fovi::tc_gated(const TcMatrix& x, const TcMatrix& wg, const TcMatrix& wu, co
   a.kb0 = a.kb = (int)stages_of(x.cols);
   a.splits = 1;
   a.ct = shape_of(&m, &n, 1, a.kb, 2, false).ct;
-  a.bias = bg; a.bias2 = bu; a.act = act; a.hidden = to;
+  a.bias = bg; a.bias2 = bu; a.hidden = to;
   int rc = tiles_of(a, 2);
   if (!rc) rc = map_k(&maps.a[0], x, false, 128);
   if (!rc) rc = map_k(&maps.b[0], wg, false, a.ct / 2);
   if (!rc) rc = map_k(&maps.b[1], wu, false, a.ct / 2);
   if (!rc) rc = map_hidden(maps, to, m);
   if (!rc) rc = map_out(&maps.out[0], to.h, to.pitch, m);
-  return rc ? rc : launch<GATED, false, false, false>(maps, a, false, st);
+  if (rc) return rc;
+  return act == ACT_SILU ? launch<GATED, false, false, false, ACT_SILU>(maps, a, false, st) : launch<GATED, false, false, false, ACT_GELU>(maps, a, false, st);
 }
 
 int64_t fovi::tc_sum_rows(int64_t tokens) { return (tokens + 255) / 256 * 8; }
@@ -650,14 +666,15 @@ int fovi::tc_hidden_grad(const TcMatrix& dy, const TcMatrix& wd, const Hidden& f
   a.kb0 = a.kb = (int)stages_of(dy.cols);
   a.splits = 1;
   a.ct = shape_of(&m, &n, 1, a.kb, 1, false).ct;
-  a.act = act; a.hidden = from; a.dg = dg; a.du = du; a.sums = sums;
+  a.hidden = from; a.dg = dg; a.du = du; a.sums = sums;
   int rc = tiles_of(a, 1);
   if (!rc) rc = map_k(&maps.a[0], dy, false, 128);
   if (!rc) rc = map_mn(&maps.b[0], wd);
   if (!rc) rc = map_hidden(maps, from, m);
   if (!rc) rc = map_out(&maps.out[0], dg, from.pitch, m);
   if (!rc) rc = map_out(&maps.out[1], du, from.pitch, m);
-  return rc ? rc : launch<GRAD, false, true, false>(maps, a, false, st);
+  if (rc) return rc;
+  return act == ACT_SILU ? launch<GRAD, false, true, false, ACT_SILU>(maps, a, false, st) : launch<GRAD, false, true, false, ACT_GELU>(maps, a, false, st);
 }
 
 int64_t fovi::tc_linear_bytes(int64_t m, int n, int64_t k) {
