@@ -61,39 +61,82 @@ struct HiddenGrad {   // dh -> dg, du
   }
 };
 
-// Column sums of [rows, n] in a fixed order: parts of strips of rows, then the parts of a column.
+// Column sums of up to three matrices in a fixed order: parts of strips of rows, then the parts of each column; two launches for all.
+struct SumTask { const void* x; int64_t rows, pitch; int n; float* part; int parts; int64_t part_pitch; void* out; };      // part: given (x null), or to be made
+struct SumTasks { SumTask t[3]; };
+constexpr int SUM_COLS = 256, STRIPS = 128;
+
+// A block takes 256 columns of a strip of rows, a lane 8 neighbouring ones, its 8 warps a row each at a time.
 template <typename T>
-__global__ void __launch_bounds__(128) column_parts_kernel(const T* x, int64_t rows, int n, int64_t pitch, int strips, float* part) {
-  const int c = blockIdx.x * 128 + threadIdx.x;
-  if (c >= n) return;
-  float s = 0.f;
-  for (int64_t r = blockIdx.y; r < rows; r += strips) s += ld_as_float(x + r * pitch + c);
-  part[(size_t)blockIdx.y * n + c] = s;
+__global__ void __launch_bounds__(256) column_parts_kernel(const __grid_constant__ SumTasks tasks) {
+  const SumTask& t = tasks.t[blockIdx.z];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * SUM_COLS + 8 * lane;
+  if (!t.x || (int)blockIdx.y >= t.parts || blockIdx.x * SUM_COLS >= t.n) return;
+  __shared__ float red[8][SUM_COLS + 8];
+  const int64_t r0 = t.rows * blockIdx.y / t.parts, r1 = t.rows * (blockIdx.y + 1) / t.parts;
+  const T* x = static_cast<const T*>(t.x) + c;
+  float s[8] = {};
+  const bool whole = c + 8 <= t.n && t.pitch % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(t.x) & 15) == 0;
+  if (whole) {
+#pragma unroll 4
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      uint4 w[sizeof(T) / 2];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(x + r * t.pitch) + i);
+      const T* v = reinterpret_cast<const T*>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += (float)v[i];
+    }
+  } else {
+    for (int64_t r = r0 + warp; r < r1; r += 8)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < t.n) s[i] += ld_as_float(x + r * t.pitch + i);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[warp][8 * lane + i] = s[i];
+  __syncthreads();
+  const int col = blockIdx.x * SUM_COLS + threadIdx.x;
+  if (col >= t.n) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += red[w][threadIdx.x];
+  t.part[blockIdx.y * t.part_pitch + col] = sum;
 }
 template <typename T>
-__global__ void __launch_bounds__(1024) column_join_kernel(const float* part, int parts, int n, int64_t pitch, T* out) {
+__global__ void __launch_bounds__(1024) column_join_kernel(const __grid_constant__ SumTasks tasks) {
+  const SumTask& t = tasks.t[blockIdx.y];
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  if (!t.out || blockIdx.x * 32 >= t.n) return;
   float s = 0.f;
-  if (c < n)
-    for (int p = w; p < parts; p += 32) s += part[p * pitch + c];
+  if (c < t.n)
+    for (int p = w; p < t.parts; p += 32) s += t.part[p * t.part_pitch + c];
   red[w][lane] = s;
   __syncthreads();
-  if (w || c >= n) return;
+  if (w || c >= t.n) return;
   s = 0.f;
   for (int i = 0; i < 32; ++i) s += red[i][lane];
-  out[c] = from_float<T>(s);
+  static_cast<T*>(t.out)[c] = from_float<T>(s);
 }
-constexpr int STRIPS = 64;
-template <typename T> int column_join(const float* part, int parts, int n, int64_t pitch, void* out, cudaStream_t st) {
-  column_join_kernel<T><<<(n + 31) / 32, 1024, 0, st>>>(part, parts, n, pitch, static_cast<T*>(out));
+SumTask sum_task(const void* x, int64_t rows, int n, int64_t pitch, float* part, void* out) {
+  return {x, rows, pitch, n, part, (int)std::max<int64_t>(1, std::min<int64_t>(STRIPS, rows / 16)), n, out};
+}
+template <typename T> int column_sums(const SumTasks& tasks, cudaStream_t st) {
+  int most = 0, wide = 0, strips = 0;
+  for (const SumTask& t : tasks.t) {
+    if (!t.out) continue;
+    most = std::max(most, t.n);
+    if (t.x) { wide = std::max(wide, t.n); strips = std::max(strips, t.parts); }
+  }
+  if (!most) return FOVI_OK;
+  if (wide) {
+    column_parts_kernel<T><<<dim3((wide + SUM_COLS - 1) / SUM_COLS, strips, 3), 256, 0, st>>>(tasks);
+    const int rc = fovi::after_launch("column_parts_kernel");
+    if (rc) return rc;
+  }
+  column_join_kernel<T><<<dim3((most + 31) / 32, 3), 1024, 0, st>>>(tasks);
   return fovi::after_launch("column_join_kernel");
-}
-template <typename T> int column_sums(const void* x, int64_t rows, int n, int64_t pitch, float* part, void* out, cudaStream_t st) {
-  const int strips = (int)std::min<int64_t>(STRIPS, rows);
-  column_parts_kernel<T><<<dim3((n + 127) / 128, strips), 128, 0, st>>>(static_cast<const T*>(x), rows, n, pitch, strips, part);
-  const int rc = fovi::after_launch("column_parts_kernel");
-  return rc ? rc : column_join<T>(part, strips, n, n, out, st);
 }
 
 int64_t pitch_of(int F) { return ((int64_t)F + 31) / 32 * 32; }
@@ -174,7 +217,7 @@ BackWork back_work_f32(const Block& b, int64_t pitch) {
   weight_tasks_f32(b, h, nullptr, 0, nullptr, nullptr, t);
   BackWork w{};
   w.parts = padded(2 * b.M * pitch * 4);
-  w.bytes = w.parts + std::max({simt_store_bytes(&in, 1, 2), simt_store_bytes(t, 3, 1), (int64_t)STRIPS * std::max(b.F, b.O) * 4});
+  w.bytes = w.parts + std::max({simt_store_bytes(&in, 1, 2), simt_store_bytes(t, 3, 1), STRIPS * (2 * (int64_t)b.F + b.O) * 4});
   return w;
 }
 
@@ -196,10 +239,11 @@ int backward_f32(const Block& b, const Hidden& hid, const Grads& g, char* work, 
   weight_tasks_f32(b, hid, g.dy, g.dys, dg, du, t);
   float* const to[3] = {static_cast<float*>(g.dwg), static_cast<float*>(g.dwu), static_cast<float*>(g.dwd)};
   if ((rc = simt_store(t, to, 3, 1, nullptr, parts, st))) return rc;
-  if (g.dbg && (rc = column_sums<float>(dg, b.M, b.F, hid.pitch, parts, g.dbg, st))) return rc;
-  if (g.dbu && (rc = column_sums<float>(du, b.M, b.F, hid.pitch, parts, g.dbu, st))) return rc;
-  if (g.dbd && (rc = column_sums<float>(g.dy, b.M, b.O, g.dys, parts, g.dbd, st))) return rc;
-  return FOVI_OK;
+  SumTasks sums{};
+  if (g.dbg) sums.t[0] = sum_task(dg, b.M, b.F, hid.pitch, parts, g.dbg);
+  if (g.dbu) sums.t[1] = sum_task(du, b.M, b.F, hid.pitch, parts + (int64_t)STRIPS * b.F, g.dbu);
+  if (g.dbd) sums.t[2] = sum_task(g.dy, b.M, b.O, g.dys, parts + 2 * (int64_t)STRIPS * b.F, g.dbd);
+  return column_sums<float>(sums, st);
 }
 
 // The three weight gradients as products over the tokens.
@@ -235,11 +279,12 @@ int backward_bf16(const Block& b, const Hidden& hid, const Grads& g, char* work,
   TcTask t[3];
   weight_tasks(b, hid, g, dg, du, t);
   if ((rc = fovi::tc_weight_grads(t, 3, b.M, parts, st))) return rc;
+  SumTasks tasks{};
   const int rows = (int)fovi::tc_sum_rows(b.M);
-  if (g.dbg && (rc = column_join<__nv_bfloat16>(sums, rows, b.F, 2 * hid.pitch, g.dbg, st))) return rc;
-  if (g.dbu && (rc = column_join<__nv_bfloat16>(sums + hid.pitch, rows, b.F, 2 * hid.pitch, g.dbu, st))) return rc;
-  if (g.dbd && (rc = column_sums<__nv_bfloat16>(g.dy, b.M, b.O, g.dys, parts, g.dbd, st))) return rc;
-  return FOVI_OK;
+  if (g.dbg) tasks.t[0] = SumTask{nullptr, 0, 0, b.F, sums, rows, 2 * hid.pitch, g.dbg};
+  if (g.dbu) tasks.t[1] = SumTask{nullptr, 0, 0, b.F, sums + hid.pitch, rows, 2 * hid.pitch, g.dbu};
+  if (g.dbd) tasks.t[2] = sum_task(g.dy, b.M, b.O, g.dys, parts, g.dbd);
+  return column_sums<__nv_bfloat16>(tasks, st);
 }
 
 // bf16 rows as the tensor copies want them.

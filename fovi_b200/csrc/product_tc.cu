@@ -17,6 +17,7 @@
 //   SCALED   integer sums times the scales
 #include <algorithm>
 
+#include "pairs.cuh"
 #include "product_tc.cuh"
 #include "tc_common.cuh"
 
@@ -128,21 +129,26 @@ __device__ __forceinline__ void st_global_32f(float* p, const uint32_t* v) {
 
 // act(g) and act'(g) of two values, to a few units of float32: what is rounded to bf16 behind them.  The logistic function takes an exponential each and one reciprocal for both,
 // 1/a = b/(ab), since those units are what bounds a tile's arithmetic; exponents are cut at 2^60, so that the product stays finite: there the function is below 1e-18.
-template <int ACT> __device__ __forceinline__ void act_pair(float g0, float g1, float2* value, float2* slope) {
+template <int ACT> __device__ __forceinline__ float2 act_pair(float2 g, float2* slope) {
   if (ACT == fovi::ACT_SILU) {
-    float e0, e1, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(-1.4426950408889634f * g0, 60.f)));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(-1.4426950408889634f * g1, 60.f)));
-    e0 += 1.f; e1 += 1.f;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e0 * e1));
-    const float p0 = r * e1, p1 = r * e0, a0 = g0 * p0, a1 = g1 * p1;
-    *value = make_float2(a0, a1);
-    if (slope) *slope = make_float2(fmaf(a0, 1.f - p0, p0), fmaf(a1, 1.f - p1, p1));
-  } else {
-    const float p0 = 0.5f * (1.f + erff(g0 * 0.70710678118654752f)), p1 = 0.5f * (1.f + erff(g1 * 0.70710678118654752f));
-    *value = make_float2(g0 * p0, g1 * p1);
-    if (slope) *slope = make_float2(fmaf(g0 * 0.39894228040143268f, __expf(-0.5f * g0 * g0), p0), fmaf(g1 * 0.39894228040143268f, __expf(-0.5f * g1 * g1), p1));
+    const float2 x = mul2(g, both(-1.4426950408889634f));
+    float2 e;
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(x.x, 60.f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(x.y, 60.f)));
+    e = add2(e, both(1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e.x * e.y));
+    const float2 p = mul2(both(r), make_float2(e.y, e.x)), a = mul2(g, p);
+    if (slope) *slope = fma2(a, fma2(p, both(-1.f), both(1.f)), p);
+    return a;
   }
+  const float2 x = mul2(g, both(0.70710678118654752f));
+  const float2 p = fma2(make_float2(erff(x.x), erff(x.y)), both(0.5f), both(0.5f));
+  if (slope) {
+    const float2 q = mul2(mul2(g, both(-0.5f)), g);
+    *slope = fma2(mul2(g, both(0.39894228040143268f)), make_float2(__expf(q.x), __expf(q.y)), p);
+  }
+  return mul2(g, p);
 }
 
 struct Tile { int task, mt, nt, k0, k1, split; };
@@ -394,9 +400,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int e = 8 * i + 2 * j;
-              float2 v;
-              act_pair<ACT>(__uint_as_float(g[e]), __uint_as_float(g[e + 1]), &v, nullptr);
-              h[j] = bf16_pair(v.x * __uint_as_float(u[e]), v.y * __uint_as_float(u[e + 1]));
+              const float2 v = mul2(act_pair<ACT>(make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), nullptr),
+                                    make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])));
+              h[j] = bf16_pair(v.x, v.y);
             }
             put16(place + 6144u + at64(lane, i), h[0], h[1], h[2], h[3]);
           }
@@ -433,11 +439,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
               g[j] = __uint_as_float((__byte_perm(gu[i], lo[e / 4], pick) & 0xffffff00u) | 0x80u);
               u[j] = __uint_as_float((__byte_perm(gu[16 + i], lo[8 + e / 4], pick) & 0xffffff00u) | 0x80u);
             }
-            float2 v, d;
-            act_pair<ACT>(g[0], g[1], &v, &d);
-            const float h0 = __uint_as_float(r[2 * i]), h1 = __uint_as_float(r[2 * i + 1]);
-            dg[i] = bf16_pair(h0 * u[0] * d.x, h1 * u[1] * d.y);
-            du[i] = bf16_pair(h0 * v.x, h1 * v.y);
+            float2 d;
+            const float2 dh = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), v = mul2(dh, act_pair<ACT>(make_float2(g[0], g[1]), &d));
+            d = mul2(mul2(dh, make_float2(u[0], u[1])), d);
+            dg[i] = bf16_pair(d.x, d.y);
+            du[i] = bf16_pair(v.x, v.y);
           }
           __syncwarp();                               // every lane has its g and u
 #pragma unroll
@@ -453,15 +459,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
             bulk_commit();
           }
           if (a.sums) {                               // of this warp's 32 rows, two columns a lane; rows behind the last token are zeros of dy, and so of dg and du
-            float s0 = 0.f, s1 = 0.f;
+            float2 sum = both(0.f);
             const uint32_t mine = from + (lane >> 4) * 2048u;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const uint32_t w = get4(mine + at64(i, lane >> 2 & 3) + (lane & 3) * 4u);
-              s0 += __uint_as_float(w << 16);
-              s1 += __uint_as_float(w & 0xffff0000u);
+              sum = add2(sum, make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
             }
-            *reinterpret_cast<float2*>(a.sums + ((int64_t)(row0 >> 5) * 2 + (lane >> 4)) * a.hidden.pitch + c0 + 2 * (lane & 15)) = make_float2(s0, s1);
+            *reinterpret_cast<float2*>(a.sums + ((int64_t)(row0 >> 5) * 2 + (lane >> 4)) * a.hidden.pitch + c0 + 2 * (lane & 15)) = sum;
           }
           if (lane == 0) bulk_read();
           __syncwarp();
