@@ -196,7 +196,7 @@ int forward_f32(const Block& b, void* y, const Hidden& hid, void* work, cudaStre
 }
 
 int forward_bf16(const Block& b, void* y, const Hidden& hid, void* work, cudaStream_t st) {
-  if (b.M <= fovi::FEW_TOKENS && !hid.high) {
+  if (!hid.high && fovi::few_block(b.M, b.C, b.F, b.O)) {
     const int rc = fovi::few_gated({b.x, b.xs}, {b.wg, b.gs}, {b.wu, b.us}, (int)b.M, b.F, b.C, b.bg, b.bu, b.act, {hid.h, hid.pitch}, st);
     return rc ? rc : fovi::few_linear({hid.h, hid.pitch}, {b.wd, b.ds}, (int)b.M, b.O, b.F, b.bd, y, true, st);
   }

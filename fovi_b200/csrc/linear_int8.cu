@@ -14,7 +14,7 @@ int linear_int8(const int8_t* q, int64_t tokens, int K, int64_t q_stride, const 
   if (tokens == 0) return FOVI_OK;
   if (!q || !scale || !weight || !weight_scale || !y) return FOVI_ERR_INVALID_ARGUMENT;
   if (!fovi::tc_takes(q, q_stride, 1) || !fovi::tc_takes(weight, weight_stride, 1) || reinterpret_cast<uintptr_t>(y) % 16) return FOVI_ERR_ALIGNMENT;
-  if (tokens <= fovi::FEW_TOKENS && !selftest)
+  if (fovi::few_eight(tokens, K, N) && !selftest)
     return fovi::few_int8({q, q_stride}, {weight, weight_stride}, (int)tokens, N, K, scale, weight_scale, bias, y, y_dtype, reinterpret_cast<cudaStream_t>(stream));
   return fovi::tc_int8({q, tokens, K, q_stride}, {weight, N, K, weight_stride}, scale, weight_scale, bias, y, y_dtype, selftest, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -1,9 +1,10 @@
-// Matrix products of up to 32 tokens, 16 a block: y[m, n] = sum over k of x[m, k] w[n, k], bf16 or 8-bit integers.
+// Matrix products of few tokens, 16 a block: y[m, n] = sum over k of x[m, k] w[n, k], bf16 or 8-bit integers.
 //
-// What bounds them is how fast the weights come: each is used by up to 32 tokens and read once.  A block takes 16 rows of w (GATED: of both matrices) and divides k among its warps in
+// What bounds them is how fast the weights come: each is used by up to 16 tokens of a block.  A block takes 16 rows of w (GATED: of both matrices) and divides k among its warps in
 // turns of 64 bytes a row; a warp's loads are 16 bytes a lane, four lanes side by side in a row, straight into the registers that the matrix instruction (m16n8k16 or m16n8k32: weights
 // are its 16 rows, tokens its 8 columns) takes them from.  That an instruction's k then is not consecutive does not matter, since tokens are loaded the same way.
-// Four turns of loads are on their way at a time.  The warps' sums are joined in shared memory in a fixed order, and a thread for each result ends it.
+// Two turns' loads are on their way while two are worked on (GATED: one and one, so that three
+// blocks fit an SM and 5120 rows are one round of them: 1280 x 5120 channels, one token, 39 MB of weights 15.1 -> 12.7 us from memory, 10.0 -> 8.4 us from L2).  The warps' sums are joined in shared memory in a fixed order, and a thread for each result ends it.
 // The tensor cores' large instructions (product_tc.cu) have 128 rows: with one token 5120 x 1280 8-bit weights take 8.8 us there.
 #include <algorithm>
 
@@ -15,7 +16,7 @@ using fovi::FewRows;
 namespace {
 
 enum { GATED = 0, LINEAR = 1, SCALED = 2 };
-constexpr int ROWS = 16, TURNS = 4;
+constexpr int ROWS = 16;
 
 struct FewArgs {
   const char *x, *w, *w2; int64_t x_pitch, w_pitch, w2_pitch;        // pitches in bytes
@@ -57,56 +58,68 @@ template <bool WEIGHTS> __device__ __forceinline__ Piece16 load16(const char* ro
 }
 
 template <int EPI, int NT, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) product_few_kernel(const __grid_constant__ FewArgs a, const int early) {
+__global__ void __launch_bounds__(WARPS * 32, EPI == GATED && WARPS == 8 ? 3 : 1) product_few_kernel(const __grid_constant__ FewArgs a, const int early) {
   constexpr bool I8 = EPI == SCALED, TWO = EPI == GATED;
-  constexpr int MATS = TWO ? 2 : 1, COLS = NT * 8;
+  constexpr int MATS = TWO ? 2 : 1, COLS = NT * 8, TURNS = TWO ? 1 : 2;
   using S = typename SumT<I8>::type;
   __shared__ S part[WARPS][MATS][ROWS][COLS + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * ROWS, m0 = blockIdx.y * 16;
   const bool low = n0 + r < a.n, high = n0 + r + 8 < a.n;
-  const char* w[MATS][2];
+  const char *w[MATS][2], *x[NT];
   w[0][0] = a.w + (int64_t)(n0 + r) * a.w_pitch;
   w[0][1] = w[0][0] + 8 * a.w_pitch;
   if (TWO) {
     w[MATS - 1][0] = a.w2 + (int64_t)(n0 + r) * a.w2_pitch;
     w[MATS - 1][1] = w[MATS - 1][0] + 8 * a.w2_pitch;
   }
-  Piece16 wp[TURNS][MATS][2], xp[TURNS][NT];
-  auto weights = [&](int turn, int at) {
 #pragma unroll
-    for (int q = 0; q < MATS; ++q) {
-      wp[turn][q][0] = load16<true>(w[q][0], low, at, a.k);
-      wp[turn][q][1] = load16<true>(w[q][1], high, at, a.k);
-    }
-  };
-  const int first = warp * 64, own = t * 16, step = WARPS * 64;
-  // The weights do not come from the launch before: where that is known to be this call's own, they are asked for in front of the wait for it.
-  if (early) {
-#pragma unroll
-    for (int u = 0; u < TURNS; ++u) weights(u, first + u * step + own);
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  S d[MATS][NT][4] = {};
-  for (int at = first; at < a.k; at += TURNS * step) {            // (the same turns for all lanes, as the instruction is the warp's)
-    if (!early || at != first) {
-#pragma unroll
-      for (int u = 0; u < TURNS; ++u) weights(u, at + u * step + own);
-    }
+  for (int j = 0; j < NT; ++j) x[j] = a.x + (int64_t)(m0 + 8 * j + r) * a.x_pitch;
+  Piece16 wp[2][TURNS][MATS][2], xp[2][TURNS][NT];
+  constexpr int STEP = WARPS * 64, ROUND = TURNS * STEP;
+  const int first = warp * 64, own = t * 16;
+  auto weights = [&](int set, int at) {
 #pragma unroll
     for (int u = 0; u < TURNS; ++u)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) xp[u][j] = load16<false>(a.x + (int64_t)(m0 + 8 * j + r) * a.x_pitch, m0 + 8 * j + r < a.m, at + u * step + own, a.k);
+      for (int q = 0; q < MATS; ++q) {
+        wp[set][u][q][0] = load16<true>(w[q][0], low, at + u * STEP + own, a.k);
+        wp[set][u][q][1] = load16<true>(w[q][1], high, at + u * STEP + own, a.k);
+      }
+  };
+  auto tokens = [&](int set, int at) {
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) xp[set][u][j] = load16<false>(x[j], m0 + 8 * j + r < a.m, at + u * STEP + own, a.k);
+  };
+  S d[MATS][NT][4] = {};
+  auto products = [&](int set) {
 #pragma unroll
     for (int u = 0; u < TURNS; ++u)
 #pragma unroll
       for (int q = 0; q < MATS; ++q)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          mma_few(d[q][j], wp[u][q][0].w, xp[u][j].w, wp[u][q][1].w[0], wp[u][q][1].w[1]);
-          mma_few(d[q][j], wp[u][q][0].w + 2, xp[u][j].w + 2, wp[u][q][1].w[2], wp[u][q][1].w[3]);
+          const uint32_t *w0 = wp[set][u][q][0].w, *w1 = wp[set][u][q][1].w, *v = xp[set][u][j].w;
+          mma_few(d[q][j], w0, v, w1[0], w1[1]);
+          mma_few(d[q][j], w0 + 2, v + 2, w1[2], w1[3]);
         }
+  };
+  // The weights do not come from the launch before: where that is known to be this call's own, they are asked for in front of the wait for it.
+  if (early) weights(0, first);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!early) weights(0, first);
+  tokens(0, first);
+  for (int at = first; at < a.k; at += 2 * ROUND) {               // (the same turns for all lanes, as the instruction is the warp's)
+    weights(1, at + ROUND);
+    tokens(1, at + ROUND);
+    products(0);
+    if (at + ROUND >= a.k) break;
+    weights(0, at + 2 * ROUND);
+    tokens(0, at + 2 * ROUND);
+    products(1);
   }
 #pragma unroll
   for (int q = 0; q < MATS; ++q)

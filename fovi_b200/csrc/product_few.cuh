@@ -4,7 +4,12 @@
 
 namespace fovi {
 
-constexpr int FEW_TOKENS = 32;      // up to here these kernels take a product
+// Whether these kernels take a block's forward pass, or an 8-bit product: always for one block of 16 tokens; beyond, the weights come from L2 once for each block of 16, and the tensor
+// cores' kernels, which take a fixed time at first, are the faster ones where that is longer.  Both sides measured (us, these / those): block of 384 x 1024 channels, 64, 128, 192 and
+// 256 tokens 5.5 / 10.3, 7.2 / 10.6, 8.9 / 10.5, 11.7 / 10.6; 768 x 2048, 64, 96, 128: 9.8 / 14.7, 12.1 / 14.4, 16.0 / 14.4; 1280 x 5120, 32, 48, 64: 17.3 / 20, 21.9 / 20.6, 28 / 19.
+// 8-bit 384 -> 1024, 64, 96, 128 tokens: 2.5 / 3.9, 3.3 / 4.0, 3.9 / 4.0; 1280 -> 5120, 32, 48: 6.0 / 6.5, 8.0 / 6.6; 5120 -> 1280, 64, 96: 7.5 / 9.0, 9.4 / 9.1.
+inline bool few_block(int64_t m, int64_t c, int64_t f, int64_t o) { return m <= 16 || (m <= 1024 && (m + 15) / 16 * f * (2 * c + o) / 3 <= 2000000 + 2700 * (c + f)); }
+inline bool few_eight(int64_t m, int64_t k, int64_t n) { return m <= 16 || (m <= 1024 && (m + 15) / 16 * n * (k + 1500) <= 10000000 + 7300 * k + 2000 * n); }
 
 // Rows as in TcMatrix: `pitch` values apart, on 16-byte boundaries.
 struct FewRows { const void* p; int64_t pitch; };

@@ -163,12 +163,13 @@ struct Store {
     store4(y[task] + r * pitch[task] + n, v, left, pitch[task]);
   }
 };
-__global__ void __launch_bounds__(256) product_simt_join_kernel(const float* part, int splits, int64_t values, int n, const float* bias, float* y) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ void __launch_bounds__(256) product_simt_join_kernel(const __grid_constant__ Store a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, values = a.m[blockIdx.y] * a.pitch[blockIdx.y];
   if (i >= values) return;
+  const float* from = a.work + a.part[blockIdx.y] + i;
   float s = 0.f;
-  for (int p = 0; p < splits; ++p) s += __ldg(part + p * values + i);
-  y[i] = s + (bias ? __ldg(bias + i % n) : 0.f);
+  for (int p = 0; p < a.splits; ++p) s += __ldg(from + p * values);
+  a.y[blockIdx.y][i] = s + (a.bias ? __ldg(a.bias + i % a.pitch[blockIdx.y]) : 0.f);
 }
 
 // Tiles of the tasks, and how many parts k is cut into: what fills the SMs four blocks deep, of 64 of k and more.  (From every task's size, whether or not its result is wanted.)
@@ -217,13 +218,12 @@ inline int simt_store(const SimtTask* t, float* const* y, int n, int segments, c
     at += (int64_t)out.splits * t[i].m * t[i].n;
   }
   if (!p.tasks) return FOVI_OK;
-  int rc = product_simt<false>(p, out, st);
-  for (int q = 0; q < p.tasks && !rc && out.splits > 1; ++q) {
-    const int64_t values = out.m[q] * out.pitch[q];
-    product_simt_join_kernel<<<(unsigned)((values + 255) / 256), 256, 0, st>>>(work + out.part[q], out.splits, values, (int)out.pitch[q], bias, out.y[q]);
-    rc = fovi::after_launch("product_simt_join_kernel");
-  }
-  return rc;
+  const int rc = product_simt<false>(p, out, st);
+  if (rc || out.splits == 1) return rc;
+  int64_t most = 0;
+  for (int q = 0; q < p.tasks; ++q) most = std::max(most, out.m[q] * out.pitch[q]);
+  product_simt_join_kernel<<<dim3((unsigned)((most + 255) / 256), p.tasks), 256, 0, st>>>(out);
+  return fovi::after_launch("product_simt_join_kernel");
 }
 
 }  // namespace

@@ -33,12 +33,12 @@ __device__ int g_status;           // wait site at which a kernel gave up, see f
 enum { GATED = 0, GRAD = 1, STORE = 2, SCALED = 3 };
 constexpr int EPI_WARPS = 8, PT_THREADS = (EPI_WARPS + 2) * 32;
 constexpr uint32_t A_BYTES = 16384, STAGE_BYTES = 2 * A_BYTES;      // a CTA's 128 rows of A and up to 128 rows of B
-constexpr int MOST_STAGES = 6, GROUPS = 3;
+constexpr int MOST_STAGES = 5, GROUPS = 3;
 // Shared memory of an epilogue warp.  GATED: a chunk's g and u (high 4 KB, low 2 KB) and h (2 KB) on their way out.  GRAD: two such places for g and u on their way in, dg and du go out from
-// over the high parts.  Otherwise: 32 rows x 16 columns (odd pitch), or 64 factors and biases.
+// over the high parts.  Otherwise: 32 rows x 32 columns (odd pitch), or 64 factors and biases.
 template <int EPI> struct Sizes {
-  static constexpr uint32_t SCRATCH = EPI == GATED ? 8192 : EPI == GRAD ? 12288 : 32 * 17 * 4;
-  static constexpr int STAGES = EPI == GATED ? 5 : EPI == GRAD ? 4 : MOST_STAGES;
+  static constexpr uint32_t SCRATCH = EPI == GATED ? 8192 : EPI == GRAD ? 12288 : 32 * 33 * 4;
+  static constexpr int STAGES = EPI == GATED ? 5 : EPI == GRAD ? 4 : 5;
   static constexpr uint32_t SMEM = 1024 + 1024 + EPI_WARPS * SCRATCH + STAGES * STAGE_BYTES;
   static_assert(SMEM <= 227 * 1024 && SCRATCH * EPI_WARPS % 1024 == 0, "");
 };
@@ -168,15 +168,15 @@ __device__ __forceinline__ Tile tile_of(const PtArgs& a, int item) {
 
 // 32 columns of a row tile of 32 rows (a row per lane) into [m, n] with no alignment: through the warp's scratch, so that lanes write neighbouring columns.
 template <typename T> __device__ __forceinline__ void store_any(T* y, int64_t n, int64_t row0, int64_t m, int c0, const float* v, float* scratch, int lane) {
+  __syncwarp();
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) scratch[lane * 17 + i] = v[16 * h + i];
-    __syncwarp();
-    const int c = c0 + 16 * h + (lane & 15);
-    for (int r = lane >> 4; r < 32; r += 2)
-      if (row0 + r < m && c < n) y[(row0 + r) * n + c] = from_float<T>(scratch[r * 17 + (lane & 15)]);
+  for (int i = 0; i < 32; ++i) scratch[lane * 33 + i] = v[i];
+  __syncwarp();
+  if (c0 + lane < n) {
+    const int rows = (int)min((int64_t)32, m - row0);
+    T* to = y + row0 * n + c0 + lane;
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) to[r * n] = from_float<T>(scratch[r * 33 + lane]);
   }
   __syncwarp();
 }
@@ -540,22 +540,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
   }
 }
 
-// The parts of a product's k, added in their order, with the bias.  A thread for four columns.
-__global__ void __launch_bounds__(256) product_join_kernel(const float* part, int splits, int64_t m, int n, const __nv_bfloat16* bias, __nv_bfloat16* y) {
-  const int64_t pitch = (n + 31) / 32 * 32, per = pitch / 4;
+// The parts of the products' k, added in their order, with the bias.  A thread for four columns; y counts the products.
+struct JoinArgs { const float* part[GROUPS]; __nv_bfloat16* y[GROUPS]; int64_t m[GROUPS]; int n[GROUPS], splits; const __nv_bfloat16* bias; };
+__global__ void __launch_bounds__(256) product_join_kernel(const __grid_constant__ JoinArgs a) {
+  const int t = blockIdx.y, n = a.n[t];
+  const int64_t pitch = (n + 31) / 32 * 32, per = pitch / 4, m = a.m[t];
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per;
   const int c = (int)(i - row * per) * 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (row >= m || c >= n) return;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = 0; p < splits; ++p) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(part + ((int64_t)p * m + row) * pitch + c));
+  const float* from = a.part[t] + row * pitch + c;
+#pragma unroll 4
+  for (int p = 0; p < a.splits; ++p) {
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(from + p * m * pitch) : "memory");
     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
-  const float v[4] = {s.x, s.y, s.z, s.w};
-  float b[4];
+  float b[4] = {s.x, s.y, s.z, s.w};
+  if (a.bias) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) b[e] = v[e] + (bias && c + e < n ? __bfloat162float(__ldg(bias + c + e)) : 0.f);
-  __nv_bfloat16* to = y + row * n + c;
+    for (int e = 0; e < 4; ++e)
+      if (c + e < n) b[e] += __bfloat162float(__ldg(a.bias + c + e));
+  }
+  __nv_bfloat16* to = a.y[t] + row * n + c;
   if (n % 4 == 0) {
     *reinterpret_cast<uint2*>(to) = make_uint2(bf16_pair(b[0], b[1]), bf16_pair(b[2], b[3]));
   } else {
@@ -626,14 +634,16 @@ int tiles_of(PtArgs& a, int share) {
 }
 
 int join(const PtArgs& a, cudaStream_t st) {
+  JoinArgs j{};
+  int64_t threads = 0;
+  j.splits = a.splits;
+  j.bias = static_cast<const __nv_bfloat16*>(a.bias);
   for (int t = 0; t < a.tasks; ++t) {
-    const int64_t threads = (int64_t)a.m[t] * ((a.n[t] + 31) / 32 * 8);
-    product_join_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a.work + a.part[t], a.splits, a.m[t], a.n[t], static_cast<const __nv_bfloat16*>(a.bias),
-                                                                          static_cast<__nv_bfloat16*>(a.y[t]));
-    const int rc = fovi::after_launch("product_join_kernel");
-    if (rc) return rc;
+    j.part[t] = a.work + a.part[t]; j.y[t] = static_cast<__nv_bfloat16*>(a.y[t]); j.m[t] = a.m[t]; j.n[t] = a.n[t];
+    threads = std::max(threads, (int64_t)a.m[t] * ((a.n[t] + 31) / 32 * 8));
   }
-  return FOVI_OK;
+  FOVI_CUDA(fovi::launch_pdl(product_join_kernel, dim3((unsigned)((threads + 255) / 256), a.tasks), 256, 0, st, j));
+  return fovi::after_launch("product_join_kernel");
 }
 
 int64_t stages_of(int64_t k) { return (k + 63) / 64; }
