@@ -25,7 +25,7 @@ def _inputs(m, k, n, seed, low=-128):
 
 
 SIZES = [(1, 1, 1), (1, 16, 8), (1, 1280, 5120), (2, 384, 384), (5, 100, 33), (8, 1280, 1280), (9, 131, 64), (16, 48, 250), (17, 384, 1000), (31, 1003, 77), (33, 16, 16), (64, 4112, 96),
-         (65, 384, 384), (100, 37, 513), (128, 128, 256), (129, 1280, 384), (257, 640, 130), (300, 2000, 1031), (1031, 1003, 331), (2600, 384, 96), (777, 5120, 640)]
+         (65, 384, 384), (100, 37, 513), (128, 128, 256), (129, 1280, 384), (257, 640, 130), (300, 2000, 1031), (1031, 1003, 331), (2600, 384, 96), (777, 5120, 640), (48, 1280, 1280), (200, 96, 250), (1000, 64, 40), (1030, 48, 24)]
 
 
 @pytest.mark.parametrize("out_dtype", [BF, F32])
