@@ -21,7 +21,7 @@ LIB = os.path.join(HERE, "libfovi_b200.so")
 NATIVE = os.path.join(HERE, "_native" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 SOURCES = ["capi.cu", "sampler.cu", "knnconv.cu", "knnconv_tc.cu", "knnconv_tc2.cu", "knnconv_tcp.cu", "knnpool.cu", "knnnorm.cu", "blocktrain.cu", "fused.cu", "tables.cu", "geometry.cu", "grad.cu", "knnconv_dw.cu", "depthwise.cu",
            "layernorm.cu", "rotary.cu", "attention.cu", "attention_tc.cu",
-           "attention_tc_grad.cu", "rmsnorm.cu", "product_tc.cu", "product_few.cu", "feedforward.cu", "linear_int8.cu"]
+           "attention_tc_grad.cu", "rmsnorm.cu", "product_tc.cu", "product_few.cu", "product_split.cu", "feedforward.cu", "linear_int8.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 

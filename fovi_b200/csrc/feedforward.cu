@@ -6,10 +6,14 @@
 
 #include "product_few.cuh"
 #include "product_simt.cuh"
+#include "product_split.cuh"
 #include "product_tc.cuh"
 
 using fovi::Hidden;
 using fovi::Operand;
+using fovi::SplitMatrix;
+using fovi::SplitProduct;
+using fovi::SplitTask;
 using fovi::TcMatrix;
 using fovi::TcTask;
 
@@ -122,24 +126,38 @@ __global__ void __launch_bounds__(1024) column_join_kernel(const __grid_constant
 SumTask sum_task(const void* x, int64_t rows, int n, int64_t pitch, float* part, void* out) {
   return {x, rows, pitch, n, part, (int)std::max<int64_t>(1, std::min<int64_t>(STRIPS, rows / 16)), n, out};
 }
-template <typename T> int column_sums(const SumTasks& tasks, cudaStream_t st) {
-  int most = 0, wide = 0, strips = 0;
-  for (const SumTask& t : tasks.t) {
-    if (!t.out) continue;
-    most = std::max(most, t.n);
+// The parts of those tasks that have an x.
+template <typename T> int column_parts(const SumTasks& tasks, cudaStream_t st) {
+  int wide = 0, strips = 0;
+  for (const SumTask& t : tasks.t)
     if (t.x) { wide = std::max(wide, t.n); strips = std::max(strips, t.parts); }
-  }
+  if (!wide) return FOVI_OK;
+  column_parts_kernel<T><<<dim3((wide + SUM_COLS - 1) / SUM_COLS, strips, 3), 256, 0, st>>>(tasks);
+  return fovi::after_launch("column_parts_kernel");
+}
+template <typename T> int column_join(const SumTasks& tasks, cudaStream_t st) {
+  int most = 0;
+  for (const SumTask& t : tasks.t)
+    if (t.out) most = std::max(most, t.n);
   if (!most) return FOVI_OK;
-  if (wide) {
-    column_parts_kernel<T><<<dim3((wide + SUM_COLS - 1) / SUM_COLS, strips, 3), 256, 0, st>>>(tasks);
-    const int rc = fovi::after_launch("column_parts_kernel");
-    if (rc) return rc;
-  }
   column_join_kernel<T><<<dim3((most + 31) / 32, 3), 1024, 0, st>>>(tasks);
   return fovi::after_launch("column_join_kernel");
 }
+template <typename T> int column_sums(const SumTasks& tasks, cudaStream_t st) {
+  const int rc = column_parts<T>(tasks, st);
+  return rc ? rc : column_join<T>(tasks, st);
+}
 
+#ifndef SPLIT_TOKENS
+#define SPLIT_TOKENS 64
+#endif
+#ifndef SPLIT_WORK
+#define SPLIT_WORK 20000000
+#endif
 int64_t pitch_of(int F) { return ((int64_t)F + 31) / 32 * 32; }
+// Whether a float32 block takes the tensor cores (product_split.cu): its products have to be worth cutting the operands and a fixed time.
+bool split_block(int64_t M, int64_t C, int64_t F, int64_t O) { return M >= SPLIT_TOKENS && M * F * (2 * C + O) / 3 >= SPLIT_WORK; }
+
 // Where the parts of a buffer for the hidden values lie.
 Hidden hidden_at(void* p, int dtype, int64_t M, int F, bool saved) {
   Hidden h{};
@@ -246,6 +264,99 @@ int backward_f32(const Block& b, const Hidden& hid, const Grads& g, char* work, 
   return column_sums<float>(sums, st);
 }
 
+// ------------------------------------------------------------------------------------------------------------ float32 on the tensor cores
+// Where the float32 block's operands in parts lie: one behind the other from `at` on.
+struct Cut {
+  char* at;
+  int64_t used = 0;
+  SplitMatrix take(int64_t rows, int64_t cols, int64_t pitch) {
+    const SplitMatrix m{at ? at + used : nullptr, rows, cols, pitch};
+    used += padded(3 * rows * pitch * 2);
+    return m;
+  }
+  SplitMatrix take(int64_t rows, int64_t cols) { return take(rows, cols, fovi::split_pitch(cols)); }
+};
+struct SplitForward { SplitMatrix x, wg, wu, wd, h; int64_t parts, bytes; };
+SplitForward split_forward_at(const Block& b, bool saved, char* work) {
+  Cut c{work};
+  SplitForward f;
+  f.x = c.take(b.M, b.C);
+  f.wg = c.take(b.F, b.C);
+  f.wu = c.take(b.F, b.C);
+  f.wd = c.take(b.O, b.F);
+  if (!saved) f.h = c.take(b.M, b.F, pitch_of(b.F));
+  f.parts = c.used;
+  f.bytes = c.used + fovi::split_linear_bytes(b.M, b.O, b.F, 1);
+  return f;
+}
+// saved: g, u, then h in parts.
+SplitMatrix saved_parts(void* saved, const Block& b) {
+  const int64_t pitch = pitch_of(b.F);
+  return {static_cast<char*>(saved) + 8 * b.M * pitch, b.M, b.F, pitch};
+}
+
+int forward_split(const Block& b, void* y, void* saved, char* work, cudaStream_t st) {
+  SplitForward f = split_forward_at(b, saved != nullptr, work);
+  float *g = static_cast<float*>(saved), *u = saved ? g + b.M * pitch_of(b.F) : nullptr;
+  if (saved) f.h = saved_parts(saved, b);
+  const SplitTask cut[4] = {{static_cast<const float*>(b.x), b.xs, f.x}, {static_cast<const float*>(b.wg), b.gs, f.wg}, {static_cast<const float*>(b.wu), b.us, f.wu},
+                            {static_cast<const float*>(b.wd), b.ds, f.wd}};
+  int rc = fovi::split_matrices(cut, 4, st);
+  if (!rc) rc = fovi::split_gated(f.x, f.wg, f.wu, static_cast<const float*>(b.bg), static_cast<const float*>(b.bu), b.act, g, u, f.h, st);
+  return rc ? rc : fovi::split_linear(f.h, f.wd, nullptr, nullptr, false, (int)b.M, b.O, static_cast<const float*>(b.bd), static_cast<float*>(y), work + f.parts, st);
+}
+
+struct SplitBackward { SplitMatrix x, wg, wu, wd, dy, dg, du; SplitProduct t[3]; int64_t parts, bytes; };
+SplitBackward split_backward_at(const Block& b, const SplitMatrix& h, char* work) {
+  Cut c{work};
+  SplitBackward f;
+  f.x = c.take(b.M, b.C);
+  f.wg = c.take(b.F, b.C);
+  f.wu = c.take(b.F, b.C);
+  f.wd = c.take(b.O, b.F);
+  f.dy = c.take(b.M, b.O);
+  f.dg = c.take(b.M, b.F, pitch_of(b.F));
+  f.du = c.take(b.M, b.F, pitch_of(b.F));
+  f.t[0] = {f.dg, f.x, b.F, b.C, nullptr};
+  f.t[1] = {f.du, f.x, b.F, b.C, nullptr};
+  f.t[2] = {f.dy, h, b.O, b.F, nullptr};
+  f.parts = c.used;
+  f.bytes = c.used + std::max({fovi::split_linear_bytes(b.M, b.C, b.F, 2), fovi::split_weight_grads_bytes(f.t, 3, b.M), STRIPS * (2 * (int64_t)b.F + b.O) * 4});
+  return f;
+}
+
+int backward_split(const Block& b, const void* saved, const Grads& g, char* work, cudaStream_t st) {
+  SplitBackward f = split_backward_at(b, saved_parts(const_cast<void*>(saved), b), work);
+  const float *gv = static_cast<const float*>(saved), *uv = gv + b.M * pitch_of(b.F);
+  float* parts = reinterpret_cast<float*>(work + f.parts);
+  const bool hidden = g.dx || g.dwg || g.dwu || g.dbg || g.dbu;
+  SplitTask cut[5];
+  int n = 0;
+  if (hidden || g.dwd) cut[n++] = {static_cast<const float*>(g.dy), g.dys, f.dy};
+  if (hidden) cut[n++] = {static_cast<const float*>(b.wd), b.ds, f.wd};
+  if (g.dwg || g.dwu) cut[n++] = {static_cast<const float*>(b.x), b.xs, f.x};
+  if (g.dx) {
+    cut[n++] = {static_cast<const float*>(b.wg), b.gs, f.wg};
+    cut[n++] = {static_cast<const float*>(b.wu), b.us, f.wu};
+  }
+  int rc = n ? fovi::split_matrices(cut, n, st) : FOVI_OK;
+  if (!rc && hidden) rc = fovi::split_hidden_grad(f.dy, f.wd, gv, uv, b.act, f.dg, f.du, st);
+  if (!rc && g.dx) rc = fovi::split_linear(f.dg, f.wg, &f.du, &f.wu, true, (int)b.M, b.C, nullptr, static_cast<float*>(g.dx), parts, st);
+  f.t[0].y = static_cast<float*>(g.dwg); f.t[1].y = static_cast<float*>(g.dwu); f.t[2].y = static_cast<float*>(g.dwd);
+  if (!rc) rc = fovi::split_weight_grads(f.t, 3, b.M, parts, st);
+  if (rc) return rc;
+  // The biases' sums: of dg and du over the rows of all three parts, of dy as it is.
+  SumTasks hid{}, all{};
+  float* const at[3] = {parts, parts + (int64_t)STRIPS * b.F, parts + 2 * (int64_t)STRIPS * b.F};
+  if (g.dbg) hid.t[0] = all.t[0] = sum_task(f.dg.p, 3 * b.M, b.F, f.dg.pitch, at[0], g.dbg);
+  if (g.dbu) hid.t[1] = all.t[1] = sum_task(f.du.p, 3 * b.M, b.F, f.du.pitch, at[1], g.dbu);
+  SumTasks own{};
+  if (g.dbd) own.t[2] = all.t[2] = sum_task(g.dy, b.M, b.O, g.dys, at[2], g.dbd);
+  rc = column_parts<__nv_bfloat16>(hid, st);
+  if (!rc) rc = column_parts<float>(own, st);
+  return rc ? rc : column_join<float>(all, st);
+}
+
 // The three weight gradients as products over the tokens.
 void weight_tasks(const Block& b, const Hidden& hid, const Grads& g, const void* dg, const void* du, TcTask (&t)[3]) {
   t[0] = TcTask{{dg, b.M, b.F, hid.pitch}, {b.x, b.M, b.C, b.xs}, b.F, b.C, g.dwg};
@@ -298,7 +409,7 @@ bool valid(int dtype, int64_t M, int C, int F, int O) { return fovi::valid_dtype
 
 extern "C" int64_t fovi_gated_ffn_saved_bytes(int dtype, int64_t tokens, int F) {
   if (!valid(dtype, tokens, 1, F, 1)) return -1;
-  return tokens * pitch_of(F) * (dtype == FOVI_BF16 ? 8 : 12);
+  return tokens * pitch_of(F) * (dtype == FOVI_BF16 ? 8 : 14);          // (float32: g, u, h in 12 bytes, or in 14 where h is in parts)
 }
 
 extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int phase) {
@@ -306,6 +417,8 @@ extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int
   const int64_t n = tokens * pitch_of(F) * (int64_t)fovi::dtype_size(dtype);
   Block b{};
   b.M = tokens; b.C = C; b.F = F; b.O = O;
+  if (dtype == FOVI_F32 && split_block(tokens, C, F, O))
+    return phase == 1 ? split_backward_at(b, SplitMatrix{}, nullptr).bytes : split_forward_at(b, phase == 2, nullptr).bytes;
   if (phase == 1) return (dtype == FOVI_F32 ? back_work_f32(b, pitch_of(F)) : back_work(b, pitch_of(F))).bytes;
   const SimtTask down = down_task(b, Hidden{});
   return (phase == 0 ? padded(n) : 0) + (dtype == FOVI_F32 ? simt_store_bytes(&down, 1, 1) : fovi::tc_linear_bytes(tokens, O, F));
@@ -323,7 +436,10 @@ extern "C" int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, 
   const Hidden h = hidden_at(saved ? saved : work, dtype, tokens, F, saved != nullptr);
   auto st = reinterpret_cast<cudaStream_t>(stream);
   char* parts = static_cast<char*>(work) + (saved ? 0 : padded(tokens * h.pitch * (int64_t)fovi::dtype_size(dtype)));
-  if (dtype == FOVI_F32) return forward_f32(b, y, h, parts, st);
+  if (dtype == FOVI_F32) {
+    if (!split_block(tokens, C, F, O)) return forward_f32(b, y, h, parts, st);
+    return reinterpret_cast<uintptr_t>(y) % 16 ? FOVI_ERR_ALIGNMENT : forward_split(b, y, saved, static_cast<char*>(work), st);
+  }
   if (!aligned(b) || reinterpret_cast<uintptr_t>(y) % 16) return FOVI_ERR_ALIGNMENT;
   return forward_bf16(b, y, h, parts, st);
 }
@@ -348,9 +464,11 @@ extern "C" int fovi_gated_ffn_backward(const void* x, int dtype, int64_t tokens,
   const Block b{x, gate_weight, up_weight, down_weight, nullptr, nullptr, nullptr, tokens, x_stride, gate_stride, up_stride, down_stride, C, F, O, activation};
   const Hidden h = hidden_at(const_cast<void*>(saved), dtype, tokens, F, true);
   const Grads g{dy, dy_stride, dx, dgate_weight, dup_weight, ddown_weight, dgate_bias, dup_bias, ddown_bias};
-  if (dtype == FOVI_F32) return backward_f32(b, h, g, static_cast<char*>(work), st);
-  if (!aligned(b) || !fovi::tc_takes(dy, dy_stride, 2)) return FOVI_ERR_ALIGNMENT;
+  const bool split = split_block(tokens, C, F, O);
+  if (dtype == FOVI_F32 && !split) return backward_f32(b, h, g, static_cast<char*>(work), st);
+  if (dtype == FOVI_BF16 && (!aligned(b) || !fovi::tc_takes(dy, dy_stride, 2))) return FOVI_ERR_ALIGNMENT;
   for (const void* p : {dx, dgate_weight, dup_weight, ddown_weight})
     if (reinterpret_cast<uintptr_t>(p) % 16) return FOVI_ERR_ALIGNMENT;
+  if (dtype == FOVI_F32) return backward_split(b, saved, g, static_cast<char*>(work), st);
   return backward_bf16(b, h, g, static_cast<char*>(work), st);
 }

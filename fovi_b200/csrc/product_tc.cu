@@ -17,9 +17,9 @@
 //   SCALED   integer sums times the scales
 #include <algorithm>
 
-#include "pairs.cuh"
+#include "product_pair.cuh"
+#include "product_split.cuh"
 #include "product_tc.cuh"
-#include "tc_common.cuh"
 
 using fovi::Hidden;
 using fovi::TcMatrix;
@@ -65,32 +65,6 @@ struct PtHeader {
   int abort_flag;
 };
 
-__device__ __forceinline__ uint32_t pt_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t pt_map(uint32_t local, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void pt_sync() { asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ void pt_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
-}
-template <bool I8> __device__ __forceinline__ void pt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if (I8)
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  else
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void pt_commit(uint32_t bar) {            // on the barrier at this offset in both CTAs
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
 // Copies of a warp's chunk, issued by one lane.
 __device__ __forceinline__ void pt_load_own(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -117,16 +91,6 @@ __device__ __forceinline__ uint32_t get4(uint32_t at) {
 // Place of 16-byte piece c of row r in a tile of 128-byte or 64-byte rows, swizzled over that many bytes: eight rows' pieces lie in eight bank groups.
 __device__ __forceinline__ uint32_t at128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 __device__ __forceinline__ uint32_t at64(int r, int c) { return (uint32_t)(r * 64 + ((c ^ (r >> 1 & 3)) << 4)); }
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-__device__ __forceinline__ void st_global_32f(float* p, const uint32_t* v) {
-  const uint32_t w[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-  st_global_32(p, w);
-}
-
 // act(g) and act'(g) of two values, to a few units of float32: what is rounded to bf16 behind them.  The logistic function takes an exponential each and one reciprocal for both,
 // 1/a = b/(ab), since those units are what bounds a tile's arithmetic; exponents are cut at 2^60, so that the product stays finite: there the function is below 1e-18.
 template <int ACT> __device__ __forceinline__ float2 act_pair(float2 g, float2* slope) {
@@ -772,13 +736,15 @@ int fovi::tc_int8(const TcMatrix& q, const TcMatrix& w, const float* scale, cons
 
 extern "C" int fovi_product_check(void* stream) {
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  int site = 0;
-  FOVI_CUDA(cudaMemcpyFromSymbolAsync(&site, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+  int* words[2];
+  FOVI_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&words[0]), g_status));
+  int rc = fovi::split_status(&words[1]), sites[2] = {0, 0};
+  if (rc) return rc;
+  for (int i = 0; i < 2; ++i) FOVI_CUDA(cudaMemcpyAsync(&sites[i], words[i], sizeof(int), cudaMemcpyDeviceToHost, st));
   FOVI_CUDA(cudaStreamSynchronize(st));
-  if (!site) return FOVI_OK;
-  const int zero = 0;
-  FOVI_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+  if (!sites[0] && !sites[1]) return FOVI_OK;
+  for (int i = 0; i < 2; ++i) FOVI_CUDA(cudaMemsetAsync(words[i], 0, sizeof(int), st));
   FOVI_CUDA(cudaStreamSynchronize(st));
-  fovi::g_last_cuda_error = "token product: wait site " + std::to_string(site) + " gave up";
+  fovi::g_last_cuda_error = "token product: wait site " + std::to_string(sites[0] ? sites[0] : sites[1]) + " gave up";
   return FOVI_ERR_DEVICE_TIMEOUT;
 }

@@ -42,7 +42,7 @@ def _wanted(leaves, dy, activation):
 
 SIZES = [(1, 8, 8, 8), (1, 384, 1024, 384), (1, 1280, 5120, 1280), (3, 5, 7, 2), (1, 1, 1, 1), (8, 384, 1024, 384), (9, 40, 72, 24), (16, 100, 260, 100), (31, 384, 1021, 390), (33, 64, 64, 64),
          (65, 96, 130, 33), (65, 1280, 3416, 1280), (127, 136, 344, 136), (128, 128, 256, 128), (129, 384, 341, 384), (257, 1280, 24, 80), (300, 390, 520, 130), (700, 64, 1000, 64),
-         (2500, 48, 16, 40), (4200, 384, 1024, 384), (48, 384, 1024, 384), (200, 96, 256, 100), (1000, 40, 64, 48), (1030, 24, 40, 16), (513, 768, 2048, 768)]
+         (2500, 48, 16, 40), (4200, 384, 1024, 384), (48, 384, 1024, 384), (200, 96, 256, 100), (1000, 40, 64, 48), (1030, 24, 40, 16), (150, 301, 777, 203), (1028, 384, 1021, 384), (513, 768, 2048, 768)]
 
 
 @pytest.mark.autograd
