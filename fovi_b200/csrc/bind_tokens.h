@@ -520,6 +520,13 @@ BODY(linear_int8, 8)
 END
 
 // ------------------------------------------------------------------------------------------------------------ gated feed-forward block
+// Whether contiguous bf16 matrices need room for copies on 16-byte boundaries.
+int ffn_flag(std::initializer_list<const at::Tensor*> all) {
+  for (const at::Tensor* t : all)
+    if (t->scalar_type() == at::kBFloat16 && (t->size(-1) % 8 || (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15))) return FOVI_FFN_UNALIGNED;
+  return 0;
+}
+
 struct FeedForwardNode : Node {            // inputs x, gate, up and down weights, their biases
   SavedVariable t[4];
   at::Tensor saved;
@@ -540,13 +547,12 @@ struct FeedForwardNode : Node {            // inputs x, gate, up and down weight
       const at::ScalarType type = x.scalar_type();
       const int64_t C = wg.size(1), F = wg.size(0), O = wd.size(0), M = x.numel() / C;
       const int dev = x.get_device();
-      at::Tensor g = in[0].to(type).contiguous();
-      if (reinterpret_cast<uintptr_t>(g.const_data_ptr()) & 15) g = g.clone();
+      const at::Tensor g = in[0].to(type).contiguous();
       const at::DimVector vf{F}, vo{O};
       const at::IntArrayRef shape[7] = {x.sizes(), wg.sizes(), wu.sizes(), wd.sizes(), vf, vf, vo};
       for (int i = 0; i < 7; ++i)
         if (task_should_compute_output(i)) out[i] = fresh(shape[i], type, dev);
-      const int64_t bytes = tok.ffn_work(code_of(type), M, (int)C, (int)F, (int)O, 1);
+      const int64_t bytes = tok.ffn_work(code_of(type), M, (int)C, (int)F, (int)O, 1 | ffn_flag({&x, &wg, &wu, &wd, &g}));
       const at::Tensor work = fresh({bytes}, at::kByte, dev);
       launched(tok.ffn_back(x.const_data_ptr(), code_of(type), M, (int)C, (int)F, (int)O, C, wg.const_data_ptr(), C, wu.const_data_ptr(), C, wd.const_data_ptr(), F, act,
                             saved.const_data_ptr(), g.const_data_ptr(), O, out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]), out_ptr(out[3]), out_ptr(out[4]), out_ptr(out[5]),
@@ -575,11 +581,6 @@ BODY(gated_feed_forward, 10)
   for (int i = 4; i < 7; ++i)
     if (t[i] && (t[i]->dim() != 1 || t[i]->size(0) != length[i - 4])) GENERAL;
   if (C > INT32_MAX || F > INT32_MAX || O > INT32_MAX || M > (1 << 30)) GENERAL;
-  if (x.scalar_type() == at::kBFloat16) {
-    if (C % 8 || F % 8 || O % 8) GENERAL;          // (O: the rows of the result's gradient)
-    for (int i = 0; i < 4; ++i)
-      if (reinterpret_cast<uintptr_t>(t[i]->const_data_ptr()) & 15) GENERAL;
-  }
   at::Tensor y;
   int rcode;
   {
@@ -587,7 +588,7 @@ BODY(gated_feed_forward, 10)
     bool graph = false;
     for (const at::Tensor* p : t) graph = graph || (p && needs_graph(*p));
     const int type = code_of(x.scalar_type());
-    const int64_t bytes = tok.ffn_work(type, M, (int)C, (int)F, (int)O, graph ? 2 : 0);
+    const int64_t bytes = tok.ffn_work(type, M, (int)C, (int)F, (int)O, (graph ? 2 : 0) | ffn_flag({&x, &wg, &wu, &wd}));
     at::Tensor saved, work;
     {
       at::AutoDispatchBelowADInplaceOrView below;

@@ -5,12 +5,10 @@
 #include <algorithm>
 
 #include "product_few.cuh"
-#include "product_simt.cuh"
 #include "product_split.cuh"
 #include "product_tc.cuh"
 
 using fovi::Hidden;
-using fovi::Operand;
 using fovi::SplitMatrix;
 using fovi::SplitProduct;
 using fovi::SplitTask;
@@ -18,52 +16,6 @@ using fovi::TcMatrix;
 using fovi::TcTask;
 
 namespace {
-
-// act(g) and act'(g)
-__device__ __forceinline__ float2 activate(float g, int act) {
-  if (act == fovi::ACT_SILU) {
-    const float p = 1.f / (1.f + expf(-g)), a = g * p;
-    return make_float2(a, fmaf(a, 1.f - p, p));
-  }
-  const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-  return make_float2(g * p, fmaf(g * 0.39894228040143268f, expf(-0.5f * g * g), p));
-}
-
-struct GateUp {       // g and u -> h
-  Hidden to; const float *bg, *bu; int act;
-  __device__ __forceinline__ void operator()(int, int, int64_t m, int n, float (&g)[4], float (&u)[4], int left) const {
-    const int64_t at = m * to.pitch + n;
-    float h[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j < left) {
-        g[j] += bg ? __ldg(bg + n + j) : 0.f;
-        u[j] += bu ? __ldg(bu + n + j) : 0.f;
-      }
-      h[j] = activate(g[j], act).x * u[j];
-    }
-    if (to.g) {
-      store4(to.g + at, g, left, to.pitch);
-      store4(to.u + at, u, left, to.pitch);
-    }
-    store4(static_cast<float*>(to.h) + at, h, left, to.pitch);
-  }
-};
-struct HiddenGrad {   // dh -> dg, du
-  Hidden from; float *dg, *du; int act;
-  __device__ __forceinline__ void operator()(int, int, int64_t m, int n, float (&dh)[4], float (&du4)[4], int left) const {
-    const int64_t at = m * from.pitch + n;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j >= left) continue;
-      const float2 s = activate(__ldg(from.g + at + j), act);
-      du4[j] = dh[j] * s.x;
-      dh[j] = dh[j] * __ldg(from.u + at + j) * s.y;
-    }
-    store4(dg + at, dh, left, from.pitch);
-    store4(du + at, du4, left, from.pitch);
-  }
-};
 
 // Column sums of up to three matrices in a fixed order: parts of strips of rows, then the parts of each column; two launches for all.
 struct SumTask { const void* x; int64_t rows, pitch; int n; float* part; int parts; int64_t part_pitch; void* out; };      // part: given (x null), or to be made
@@ -148,29 +100,15 @@ template <typename T> int column_sums(const SumTasks& tasks, cudaStream_t st) {
   return rc ? rc : column_join<T>(tasks, st);
 }
 
-#ifndef SPLIT_TOKENS
-#define SPLIT_TOKENS 64
-#endif
-#ifndef SPLIT_WORK
-#define SPLIT_WORK 20000000
-#endif
 int64_t pitch_of(int F) { return ((int64_t)F + 31) / 32 * 32; }
-// Whether a float32 block takes the tensor cores (product_split.cu): its products have to be worth cutting the operands and a fixed time.
-bool split_block(int64_t M, int64_t C, int64_t F, int64_t O) { return M >= SPLIT_TOKENS && M * F * (2 * C + O) / 3 >= SPLIT_WORK; }
-
-// Where the parts of a buffer for the hidden values lie.
-Hidden hidden_at(void* p, int dtype, int64_t M, int F, bool saved) {
+// Where the parts of a bf16 block's buffer for the hidden values lie.
+Hidden hidden_at(void* p, int64_t M, int F, bool saved) {
   Hidden h{};
   h.pitch = pitch_of(F);
-  const int64_t n = M * h.pitch, size = fovi::dtype_size(dtype);
-  char* at = static_cast<char*>(p);
-  h.h = at;
-  if (saved && dtype == FOVI_F32) {
-    h.g = reinterpret_cast<float*>(at + n * size);
-    h.u = h.g + n;
-  } else if (saved) {
-    h.high = reinterpret_cast<uint16_t*>(at + n * size);
-    h.low = reinterpret_cast<uint8_t*>(h.high + 2 * n);
+  h.h = p;
+  if (saved) {
+    h.high = static_cast<uint16_t*>(p) + M * h.pitch;
+    h.low = reinterpret_cast<uint8_t*>(h.high + 2 * M * h.pitch);
   }
   return h;
 }
@@ -183,36 +121,6 @@ struct Block {
 // The parts of a workspace, each on a boundary of 256 bytes.
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// The block's float32 products.
-SimtTask task(const Operand& a, const Operand& b, int64_t m, int n, int k) {
-  SimtTask t{};
-  t.a[0] = a; t.b[0] = b; t.m = m; t.n = n; t.k[0] = k;
-  return t;
-}
-SimtTask down_task(const Block& b, const Hidden& hid) { return task({hid.h, hid.pitch, 1}, {b.wd, b.ds, 1}, b.M, b.O, b.F); }
-SimtTask input_task(const Block& b, const float* dg, const float* du, int64_t pitch) {
-  SimtTask t = task({dg, pitch, 1}, {b.wg, 1, b.gs}, b.M, b.C, b.F);
-  t.a[1] = {du, pitch, 1}; t.b[1] = {b.wu, 1, b.us}; t.k[1] = b.F;
-  return t;
-}
-void weight_tasks_f32(const Block& b, const Hidden& hid, const void* dy, int64_t dys, const float* dg, const float* du, SimtTask (&t)[3]) {
-  t[0] = task({dg, 1, hid.pitch}, {b.x, 1, b.xs}, b.F, b.C, (int)b.M);
-  t[1] = task({du, 1, hid.pitch}, {b.x, 1, b.xs}, b.F, b.C, (int)b.M);
-  t[2] = task({dy, 1, dys}, {hid.h, 1, hid.pitch}, b.O, b.F, (int)b.M);
-}
-
-int forward_f32(const Block& b, void* y, const Hidden& hid, void* work, cudaStream_t st) {
-  SimtArgs p{};
-  p.tasks = p.segments = p.splits = 1;
-  p.t[0] = task({b.x, b.xs, 1}, {b.wg, b.gs, 1}, b.M, b.F, b.C);
-  p.t[0].b2 = Operand{b.wu, b.us, 1};
-  const int rc = product_simt<true>(p, GateUp{hid, static_cast<const float*>(b.bg), static_cast<const float*>(b.bu), b.act}, st);
-  if (rc) return rc;
-  const SimtTask t = down_task(b, hid);
-  float* to = static_cast<float*>(y);
-  return simt_store(&t, &to, 1, 1, static_cast<const float*>(b.bd), static_cast<float*>(work), st);
-}
-
 int forward_bf16(const Block& b, void* y, const Hidden& hid, void* work, cudaStream_t st) {
   if (!hid.high && fovi::few_block(b.M, b.C, b.F, b.O)) {
     const int rc = fovi::few_gated({b.x, b.xs}, {b.wg, b.gs}, {b.wu, b.us}, (int)b.M, b.F, b.C, b.bg, b.bu, b.act, {hid.h, hid.pitch}, st);
@@ -224,45 +132,6 @@ int forward_bf16(const Block& b, void* y, const Hidden& hid, void* work, cudaStr
 }
 
 struct Grads { const void* dy; int64_t dys; void *dx, *dwg, *dwu, *dwd, *dbg, *dbu, *dbd; };
-
-// Work of a float32 backward pass: dg, du; then, one after another in the same place, the parts of dx, of the weight gradients, and of the biases' sums.
-struct BackWork { int64_t sums, parts, bytes; };
-BackWork back_work_f32(const Block& b, int64_t pitch) {
-  SimtTask t[3];
-  const SimtTask in = input_task(b, nullptr, nullptr, pitch);
-  Hidden h{};
-  h.pitch = pitch;
-  weight_tasks_f32(b, h, nullptr, 0, nullptr, nullptr, t);
-  BackWork w{};
-  w.parts = padded(2 * b.M * pitch * 4);
-  w.bytes = w.parts + std::max({simt_store_bytes(&in, 1, 2), simt_store_bytes(t, 3, 1), STRIPS * (2 * (int64_t)b.F + b.O) * 4});
-  return w;
-}
-
-int backward_f32(const Block& b, const Hidden& hid, const Grads& g, char* work, cudaStream_t st) {
-  float *dg = reinterpret_cast<float*>(work), *du = dg + b.M * hid.pitch, *parts = reinterpret_cast<float*>(work + back_work_f32(b, hid.pitch).parts);
-  int rc;
-  if (g.dx || g.dwg || g.dwu || g.dbg || g.dbu) {
-    SimtArgs p{};
-    p.tasks = p.segments = p.splits = 1;
-    p.t[0] = task({g.dy, g.dys, 1}, {b.wd, 1, b.ds}, b.M, b.F, b.O);
-    if ((rc = product_simt<false>(p, HiddenGrad{hid, dg, du, b.act}, st))) return rc;
-  }
-  if (g.dx) {
-    const SimtTask t = input_task(b, dg, du, hid.pitch);
-    float* to = static_cast<float*>(g.dx);
-    if ((rc = simt_store(&t, &to, 1, 2, nullptr, parts, st))) return rc;
-  }
-  SimtTask t[3];
-  weight_tasks_f32(b, hid, g.dy, g.dys, dg, du, t);
-  float* const to[3] = {static_cast<float*>(g.dwg), static_cast<float*>(g.dwu), static_cast<float*>(g.dwd)};
-  if ((rc = simt_store(t, to, 3, 1, nullptr, parts, st))) return rc;
-  SumTasks sums{};
-  if (g.dbg) sums.t[0] = sum_task(dg, b.M, b.F, hid.pitch, parts, g.dbg);
-  if (g.dbu) sums.t[1] = sum_task(du, b.M, b.F, hid.pitch, parts + (int64_t)STRIPS * b.F, g.dbu);
-  if (g.dbd) sums.t[2] = sum_task(g.dy, b.M, b.O, g.dys, parts + 2 * (int64_t)STRIPS * b.F, g.dbd);
-  return column_sums<float>(sums, st);
-}
 
 // ------------------------------------------------------------------------------------------------------------ float32 on the tensor cores
 // Where the float32 block's operands in parts lie: one behind the other from `at` on.
@@ -296,6 +165,11 @@ SplitMatrix saved_parts(void* saved, const Block& b) {
 }
 
 int forward_split(const Block& b, void* y, void* saved, char* work, cudaStream_t st) {
+  if (!saved && fovi::few_float(b.M, b.C, b.F, b.O)) {
+    auto f = [](const void* p) { return static_cast<const float*>(p); };
+    return fovi::few_block32(f(b.x), b.xs, f(b.wg), b.gs, f(b.wu), b.us, f(b.wd), b.ds, (int)b.M, b.C, b.F, b.O, f(b.bg), f(b.bu), f(b.bd), b.act, reinterpret_cast<float*>(work),
+                             pitch_of(b.F), static_cast<float*>(y), st);
+  }
   SplitForward f = split_forward_at(b, saved != nullptr, work);
   float *g = static_cast<float*>(saved), *u = saved ? g + b.M * pitch_of(b.F) : nullptr;
   if (saved) f.h = saved_parts(saved, b);
@@ -366,6 +240,7 @@ void weight_tasks(const Block& b, const Hidden& hid, const Grads& g, const void*
 
 // Work of a bf16 backward pass: dg, du; then, one after another in the same place, the parts of dx, of the weight gradients, and of the biases' sums of dy.  The sums of
 // dg and du, which the first kernel leaves, have a place of their own.
+struct BackWork { int64_t sums, parts, bytes; };
 BackWork back_work(const Block& b, int64_t pitch) {
   TcTask t[3];
   weight_tasks(b, Hidden{}, Grads{}, nullptr, nullptr, t);
@@ -398,9 +273,51 @@ int backward_bf16(const Block& b, const Hidden& hid, const Grads& g, char* work,
   return column_sums<__nv_bfloat16>(tasks, st);
 }
 
-// bf16 rows as the tensor copies want them.
-bool aligned(const Block& b) {
-  return fovi::tc_takes(b.x, b.xs, 2) && fovi::tc_takes(b.wg, b.gs, 2) && fovi::tc_takes(b.wu, b.us, 2) && fovi::tc_takes(b.wd, b.ds, 2);
+// Copies of bf16 matrices whose rows do not start on 16-byte boundaries, to where they do, up to five in one launch.  A thread for eight values of a row.
+struct PadTask { const uint16_t* x; int64_t stride; uint16_t* to; int64_t rows, cols, pitch; };
+struct PadArgs { PadTask t[5]; };
+__global__ void __launch_bounds__(256) pad_kernel(const __grid_constant__ PadArgs a) {
+  const PadTask& t = a.t[blockIdx.y];
+  const int64_t per = t.pitch / 8, all = t.rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per, c = 8 * (i - r * per);
+    const uint16_t* x = t.x + r * t.stride + c;
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < t.cols) w[j / 2] |= (uint32_t)__ldg(x + j) << (16 * (j & 1));
+    *reinterpret_cast<uint4*>(t.to + r * t.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+int64_t pad_bytes(int64_t rows, int64_t cols) { return padded(rows * fovi::split_pitch(cols) * 2); }
+int64_t pads_bytes(int64_t M, int64_t C, int64_t F, int64_t O, bool backward) {
+  return pad_bytes(M, C) + 2 * pad_bytes(F, C) + pad_bytes(O, F) + (backward ? pad_bytes(M, O) : 0);
+}
+bool boundaries(const Block& b, const Grads* g) {
+  return fovi::tc_takes(b.x, b.xs, 2) && fovi::tc_takes(b.wg, b.gs, 2) && fovi::tc_takes(b.wu, b.us, 2) && fovi::tc_takes(b.wd, b.ds, 2) && (!g || fovi::tc_takes(g->dy, g->dys, 2));
+}
+// The block (and dy) with copies in `at` for what does not lie on boundaries; moves `at` behind them.
+int pad(Block& b, Grads* g, char*& at, cudaStream_t st) {
+  PadArgs a{};
+  int n = 0;
+  int64_t most = 0;
+  auto one = [&](const void*& p, int64_t& stride, int64_t rows, int64_t cols) {
+    if (!fovi::tc_takes(p, stride, 2)) {
+      const int64_t pitch = fovi::split_pitch(cols);
+      a.t[n++] = PadTask{static_cast<const uint16_t*>(p), stride, reinterpret_cast<uint16_t*>(at), rows, cols, pitch};
+      most = std::max(most, rows * pitch / 8);
+      p = at;
+      stride = pitch;
+    }
+    at += pad_bytes(rows, cols);
+  };
+  one(b.x, b.xs, b.M, b.C);
+  one(b.wg, b.gs, b.F, b.C);
+  one(b.wu, b.us, b.F, b.C);
+  one(b.wd, b.ds, b.O, b.F);
+  if (g) one(g->dy, g->dys, b.M, b.O);
+  pad_kernel<<<dim3((unsigned)std::min<int64_t>((most + 255) / 256, 8 * fovi::sm_count()), n), 256, 0, st>>>(a);
+  return fovi::after_launch("pad_kernel");
 }
 
 bool valid(int dtype, int64_t M, int C, int F, int O) { return fovi::valid_dtype(dtype) && M >= 0 && M <= (1 << 30) && C >= 1 && F >= 1 && O >= 1; }
@@ -409,19 +326,19 @@ bool valid(int dtype, int64_t M, int C, int F, int O) { return fovi::valid_dtype
 
 extern "C" int64_t fovi_gated_ffn_saved_bytes(int dtype, int64_t tokens, int F) {
   if (!valid(dtype, tokens, 1, F, 1)) return -1;
-  return tokens * pitch_of(F) * (dtype == FOVI_BF16 ? 8 : 14);          // (float32: g, u, h in 12 bytes, or in 14 where h is in parts)
+  return tokens * pitch_of(F) * (dtype == FOVI_BF16 ? 8 : 14);
 }
 
 extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int phase) {
-  if (!valid(dtype, tokens, C, F, O) || phase < 0 || phase > 2) return -1;
-  const int64_t n = tokens * pitch_of(F) * (int64_t)fovi::dtype_size(dtype);
+  if (!valid(dtype, tokens, C, F, O) || phase < 0 || (phase & 3) > 2 || phase > 6) return -1;
+  const bool copies = phase & FOVI_FFN_UNALIGNED;
+  phase &= 3;
   Block b{};
   b.M = tokens; b.C = C; b.F = F; b.O = O;
-  if (dtype == FOVI_F32 && split_block(tokens, C, F, O))
-    return phase == 1 ? split_backward_at(b, SplitMatrix{}, nullptr).bytes : split_forward_at(b, phase == 2, nullptr).bytes;
-  if (phase == 1) return (dtype == FOVI_F32 ? back_work_f32(b, pitch_of(F)) : back_work(b, pitch_of(F))).bytes;
-  const SimtTask down = down_task(b, Hidden{});
-  return (phase == 0 ? padded(n) : 0) + (dtype == FOVI_F32 ? simt_store_bytes(&down, 1, 1) : fovi::tc_linear_bytes(tokens, O, F));
+  if (dtype == FOVI_F32) return phase == 1 ? split_backward_at(b, SplitMatrix{}, nullptr).bytes : split_forward_at(b, phase == 2, nullptr).bytes;
+  const int64_t extra = copies ? pads_bytes(tokens, C, F, O, phase == 1) : 0;
+  if (phase == 1) return extra + back_work(b, pitch_of(F)).bytes;
+  return extra + (phase == 0 ? padded(tokens * pitch_of(F) * 2) : 0) + fovi::tc_linear_bytes(tokens, O, F);
 }
 
 extern "C" int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
@@ -430,18 +347,21 @@ extern "C" int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, 
   if (!valid(dtype, tokens, C, F, O) || activation < 0 || activation > 1 || x_stride < 0 || gate_stride < 0 || up_stride < 0 || down_stride < 0) return FOVI_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return FOVI_OK;
   if (!x || !gate_weight || !up_weight || !down_weight || !y) return FOVI_ERR_INVALID_ARGUMENT;
-  const int64_t need = fovi_gated_ffn_workspace_bytes(dtype, tokens, C, F, O, saved ? 2 : 0);
+  Block b{x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias, tokens, x_stride, gate_stride, up_stride, down_stride, C, F, O, activation};
+  const bool copies = dtype == FOVI_BF16 && !boundaries(b, nullptr);
+  const int64_t need = fovi_gated_ffn_workspace_bytes(dtype, tokens, C, F, O, (saved ? 2 : 0) | (copies ? FOVI_FFN_UNALIGNED : 0));
   if (work_bytes < need || (need && !work)) return FOVI_ERR_INVALID_ARGUMENT;
-  const Block b{x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias, tokens, x_stride, gate_stride, up_stride, down_stride, C, F, O, activation};
-  const Hidden h = hidden_at(saved ? saved : work, dtype, tokens, F, saved != nullptr);
+  for (const void* p : {(const void*)y, (const void*)work, (const void*)saved})
+    if (reinterpret_cast<uintptr_t>(p) % (p == y ? 16 : 32)) return FOVI_ERR_ALIGNMENT;
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  char* parts = static_cast<char*>(work) + (saved ? 0 : padded(tokens * h.pitch * (int64_t)fovi::dtype_size(dtype)));
-  if (dtype == FOVI_F32) {
-    if (!split_block(tokens, C, F, O)) return forward_f32(b, y, h, parts, st);
-    return reinterpret_cast<uintptr_t>(y) % 16 ? FOVI_ERR_ALIGNMENT : forward_split(b, y, saved, static_cast<char*>(work), st);
+  char* at = static_cast<char*>(work);
+  if (dtype == FOVI_F32) return forward_split(b, y, saved, at, st);
+  if (copies) {
+    const int rc = pad(b, nullptr, at, st);
+    if (rc) return rc;
   }
-  if (!aligned(b) || reinterpret_cast<uintptr_t>(y) % 16) return FOVI_ERR_ALIGNMENT;
-  return forward_bf16(b, y, h, parts, st);
+  const Hidden h = hidden_at(saved ? saved : at, tokens, F, saved != nullptr);
+  return forward_bf16(b, y, h, at + (saved ? 0 : padded(tokens * h.pitch * 2)), st);
 }
 
 extern "C" int fovi_gated_ffn_backward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
@@ -459,16 +379,19 @@ extern "C" int fovi_gated_ffn_backward(const void* x, int dtype, int64_t tokens,
       if (z.p) FOVI_CUDA(cudaMemsetAsync(z.p, 0, z.n * size, st));
     return FOVI_OK;
   }
-  if (!x || !gate_weight || !up_weight || !down_weight || !saved || !dy || !work || work_bytes < fovi_gated_ffn_workspace_bytes(dtype, tokens, C, F, O, 1))
-    return FOVI_ERR_INVALID_ARGUMENT;
-  const Block b{x, gate_weight, up_weight, down_weight, nullptr, nullptr, nullptr, tokens, x_stride, gate_stride, up_stride, down_stride, C, F, O, activation};
-  const Hidden h = hidden_at(const_cast<void*>(saved), dtype, tokens, F, true);
-  const Grads g{dy, dy_stride, dx, dgate_weight, dup_weight, ddown_weight, dgate_bias, dup_bias, ddown_bias};
-  const bool split = split_block(tokens, C, F, O);
-  if (dtype == FOVI_F32 && !split) return backward_f32(b, h, g, static_cast<char*>(work), st);
-  if (dtype == FOVI_BF16 && (!aligned(b) || !fovi::tc_takes(dy, dy_stride, 2))) return FOVI_ERR_ALIGNMENT;
+  if (!x || !gate_weight || !up_weight || !down_weight || !saved || !dy || !work) return FOVI_ERR_INVALID_ARGUMENT;
+  Block b{x, gate_weight, up_weight, down_weight, nullptr, nullptr, nullptr, tokens, x_stride, gate_stride, up_stride, down_stride, C, F, O, activation};
+  Grads g{dy, dy_stride, dx, dgate_weight, dup_weight, ddown_weight, dgate_bias, dup_bias, ddown_bias};
+  const bool copies = dtype == FOVI_BF16 && !boundaries(b, &g);
+  if (work_bytes < fovi_gated_ffn_workspace_bytes(dtype, tokens, C, F, O, 1 | (copies ? FOVI_FFN_UNALIGNED : 0))) return FOVI_ERR_INVALID_ARGUMENT;
   for (const void* p : {dx, dgate_weight, dup_weight, ddown_weight})
     if (reinterpret_cast<uintptr_t>(p) % 16) return FOVI_ERR_ALIGNMENT;
-  if (dtype == FOVI_F32) return backward_split(b, saved, g, static_cast<char*>(work), st);
-  return backward_bf16(b, h, g, static_cast<char*>(work), st);
+  if (reinterpret_cast<uintptr_t>(work) % 32 || reinterpret_cast<uintptr_t>(saved) % 32) return FOVI_ERR_ALIGNMENT;
+  char* at = static_cast<char*>(work);
+  if (dtype == FOVI_F32) return backward_split(b, saved, g, at, st);
+  if (copies) {
+    const int rc = pad(b, &g, at, st);
+    if (rc) return rc;
+  }
+  return backward_bf16(b, hidden_at(const_cast<void*>(saved), tokens, F, true), g, at, st);
 }

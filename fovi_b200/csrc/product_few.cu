@@ -154,6 +154,115 @@ __global__ void __launch_bounds__(WARPS * 32, EPI == GATED && WARPS == 8 ? 3 : 1
   }
 }
 
+// ------------------------------------------------------------------------------------------------------------ float32
+// The same with multiply-adds: a block takes 16 rows and 8 tokens; a lane has 16 bytes of two rows (GATED: of each matrix) and their products with the eight tokens, whose values come
+// through L1; the four lanes of a row and the warps join their sums in a fixed order.
+struct Few32Args {
+  const float *x, *w, *w2; int64_t x_pitch, w_pitch, w2_pitch;
+  int m, n, k, act;
+  const float *bias, *bias2;
+  float* y; int64_t y_pitch;
+  int x_vec, w_vec;                // rows start on 16-byte boundaries
+};
+// Four values of a row from `at` on, of which those behind the row's end are zeros.
+__device__ __forceinline__ float4 load4(const float* row, bool here, int at, int end, bool vec, bool stream) {
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (here && at < end) {
+    if (vec && at + 4 <= end) {
+      if (stream) asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "l"(row + at));
+      else asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "l"(row + at) : "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at + i < end) asm volatile("ld.global.f32 %0, [%1];" : "=f"(v[i]) : "l"(row + at + i) : "memory");
+    }
+  }
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+template <bool TWO>
+__global__ void __launch_bounds__(256) product_few32_kernel(const __grid_constant__ Few32Args a) {
+  constexpr int MATS = TWO ? 2 : 1, WARPS = 8, TOK = 8;
+  __shared__ float part[WARPS][MATS][ROWS][TOK + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, n0 = blockIdx.x * ROWS, m0 = blockIdx.y * TOK;
+  const bool there[2] = {n0 + r < a.n, n0 + r + 8 < a.n};
+  const float* w[MATS][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    w[0][h] = a.w + (int64_t)(n0 + r + 8 * h) * a.w_pitch;
+    if (TWO) w[MATS - 1][h] = a.w2 + (int64_t)(n0 + r + 8 * h) * a.w2_pitch;
+  }
+  float d[MATS][2][TOK] = {};
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int STEP = WARPS * 16, TURNS = 2;           // two turns at a time, the next two on their way
+  float4 next[TURNS][MATS][2];
+  auto weights = [&](int at) {
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+      for (int q = 0; q < MATS; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) next[u][q][h] = load4(w[q][h], there[h], at + u * STEP, a.k, a.w_vec, true);
+  };
+  const float* x = a.x + (int64_t)m0 * a.x_pitch;
+  const int first = warp * 16 + 4 * t, tokens = a.m - m0;
+  weights(first);
+  for (int at = first; at < a.k; at += TURNS * STEP) {
+    float4 now[TURNS][MATS][2];
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+      for (int q = 0; q < MATS; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) now[u][q][h] = next[u][q][h];
+    weights(at + TURNS * STEP);
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) {
+      float4 v[TOK];
+#pragma unroll
+      for (int m = 0; m < TOK; ++m) v[m] = load4(x + m * a.x_pitch, m < tokens, at + u * STEP, a.k, a.x_vec, false);
+#pragma unroll
+      for (int m = 0; m < TOK; ++m) {
+        if (m > 0 && m >= tokens) break;
+#pragma unroll
+        for (int q = 0; q < MATS; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            d[q][h][m] = fmaf(now[u][q][h].w, v[m].w, fmaf(now[u][q][h].z, v[m].z, fmaf(now[u][q][h].y, v[m].y, fmaf(now[u][q][h].x, v[m].x, d[q][h][m]))));
+      }
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < MATS; ++q)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int m = 0; m < TOK; ++m) {
+        float s = d[q][h][m];
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        if (t == 0) part[warp][q][r + 8 * h][m] = s;
+      }
+  __syncthreads();
+  if (threadIdx.x >= ROWS * TOK) return;
+  const int i = threadIdx.x % ROWS, col = threadIdx.x / ROWS, m = m0 + col, n = n0 + i;
+  if (m >= a.m || n >= a.n) return;
+  float s[MATS] = {};
+#pragma unroll
+  for (int v = 0; v < WARPS; ++v)
+#pragma unroll
+    for (int q = 0; q < MATS; ++q) s[q] += part[v][q][i][col];
+  if (a.bias) s[0] += __ldg(a.bias + n);
+  if (TWO) {
+    if (a.bias2) s[MATS - 1] += __ldg(a.bias2 + n);
+    const float g = s[0], p = a.act == fovi::ACT_SILU ? 1.f / (1.f + expf(-g)) : 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    s[0] = g * p * s[MATS - 1];
+  }
+  a.y[m * a.y_pitch + n] = s[0];
+}
+
 template <int EPI, int NT, int WARPS> int launch(const FewArgs& a, bool early, cudaStream_t st) {
   FOVI_CUDA(fovi::launch_pdl(product_few_kernel<EPI, NT, WARPS>, dim3((a.n + ROWS - 1) / ROWS, (a.m + 15) / 16), WARPS * 32, 0, st, a, (int)early));
   return fovi::after_launch("product_few_kernel");
@@ -189,6 +298,19 @@ int fovi::few_linear(const FewRows& x, const FewRows& w, int m, int n, int k, co
   a.bias = static_cast<const __nv_bfloat16*>(bias);
   a.y = y; a.y_pitch = n;
   return by_tokens<LINEAR>(a, after_own, st);
+}
+
+int fovi::few_block32(const float* x, int64_t xs, const float* wg, int64_t gs, const float* wu, int64_t us, const float* wd, int64_t ds, int m, int c, int f, int o, const float* bg,
+                      const float* bu, const float* bd, int act, float* h, int64_t h_pitch, float* y, cudaStream_t st) {
+  auto vec = [](const float* p, int64_t pitch) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch % 4 == 0; };
+  const int tokens = (m + 7) / 8;
+  const Few32Args up{x, wg, wu, xs, gs, us, m, f, c, act, bg, bu, h, h_pitch, vec(x, xs), vec(wg, gs) && vec(wu, us)};
+  FOVI_CUDA(fovi::launch_pdl(product_few32_kernel<true>, dim3((f + ROWS - 1) / ROWS, tokens), 256, 0, st, up));
+  int rc = fovi::after_launch("product_few32_kernel");
+  if (rc) return rc;
+  const Few32Args down{h, wd, nullptr, h_pitch, ds, 0, m, o, f, act, bd, nullptr, y, o, vec(h, h_pitch), vec(wd, ds)};
+  FOVI_CUDA(fovi::launch_pdl(product_few32_kernel<false>, dim3((o + ROWS - 1) / ROWS, tokens), 256, 0, st, down));
+  return fovi::after_launch("product_few32_kernel");
 }
 
 int fovi::few_int8(const FewRows& q, const FewRows& w, int m, int n, int k, const float* scale, const float* wscale, const float* bias, void* y, int y_dtype, cudaStream_t st) {

@@ -9,6 +9,8 @@ namespace fovi {
 // 256 tokens 5.5 / 10.3, 7.2 / 10.6, 8.9 / 10.5, 11.7 / 10.6; 768 x 2048, 64, 96, 128: 9.8 / 14.7, 12.1 / 14.4, 16.0 / 14.4; 1280 x 5120, 32, 48, 64: 17.3 / 20, 21.9 / 20.6, 28 / 19.
 // 8-bit 384 -> 1024, 64, 96, 128 tokens: 2.5 / 3.9, 3.3 / 4.0, 3.9 / 4.0; 1280 -> 5120, 32, 48: 6.0 / 6.5, 8.0 / 6.6; 5120 -> 1280, 64, 96: 7.5 / 9.0, 9.4 / 9.1.
 inline bool few_block(int64_t m, int64_t c, int64_t f, int64_t o) { return m <= 16 || (m <= 1024 && (m + 15) / 16 * f * (2 * c + o) / 3 <= 2000000 + 2700 * (c + f)); }
+// A float32 block's, 8 tokens a block, against product_split.cu's: 1280 x 3416, 8 and 16 tokens 47 / 79 and 62 / 80, 32 tokens 118 / 81; 384 x 1024, 32 and 48 tokens 20 / 23 and 25 / 24.
+inline bool few_float(int64_t m, int64_t c, int64_t f, int64_t o) { return m <= 16 || (m <= 1024 && (m + 7) / 8 * f * (2 * c + o) / 3 <= 1600000); }
 inline bool few_eight(int64_t m, int64_t k, int64_t n) { return m <= 16 || (m <= 1024 && (m + 15) / 16 * n * (k + 1500) <= 10000000 + 7300 * k + 2000 * n); }
 
 // Rows as in TcMatrix: `pitch` values apart, on 16-byte boundaries.
@@ -18,6 +20,9 @@ struct FewRows { const void* p; int64_t pitch; };
 int few_gated(const FewRows& x, const FewRows& wg, const FewRows& wu, int m, int n, int k, const void* bg, const void* bu, int act, const FewRows& h, cudaStream_t st);
 // y = x W^T + bias, bf16.  after_own: the launch before it in the stream is few_gated's, with the same weights in the same call.
 int few_linear(const FewRows& x, const FewRows& w, int m, int n, int k, const void* bias, void* y, bool after_own, cudaStream_t st);
+// A float32 block's forward pass, rows of any alignment; h: [m, h_pitch] to work in.
+int few_block32(const float* x, int64_t xs, const float* wg, int64_t gs, const float* wu, int64_t us, const float* wd, int64_t ds, int m, int c, int f, int o, const float* bg,
+                const float* bu, const float* bd, int act, float* h, int64_t h_pitch, float* y, cudaStream_t st);
 // y = scale wscale (q W^T) + bias, y bf16 or float32.
 int few_int8(const FewRows& q, const FewRows& w, int m, int n, int k, const float* scale, const float* wscale, const float* bias, void* y, int y_dtype, cudaStream_t st);
 

@@ -956,11 +956,11 @@ def quantize(x):
     return q, scale
 
 
-def _copy_rows(t, c, plain=False):
-    """t [..., C] as (rows on 16-byte boundaries for the tensor copies, their number, the stride); a copy where its memory does not give that.  plain: boundaries do not matter."""
+def _copy_rows(t, c):
+    """t [..., C] as (rows on 16-byte boundaries for the tensor copies, their number, the stride); a copy where its memory does not give that."""
     t2, n, stride = _rows(t, c)
     per = 16 // t.element_size()
-    if plain or (t2.data_ptr() % 16 == 0 and (n <= 1 or (stride % per == 0 and stride > 0))):
+    if t2.data_ptr() % 16 == 0 and (n <= 1 or (stride % per == 0 and stride > 0)):
         return t2, n, -(-c // per) * per if n <= 1 else stride
     buffer = torch.empty((n, -(-c // per) * per), dtype=t.dtype, device=t.device)
     buffer[:, :c] = t2.view(n, c) if t2.is_contiguous() else t2
@@ -1006,10 +1006,17 @@ def _ffn_inputs(x, gate_weight, up_weight, down_weight, biases, activation):
             raise ValueError(f"the {name} bias has the shape {tuple(t.shape)}, {(n,)} is wanted")
     if any(t is not None and t.dtype != x.dtype for t in (gate_weight, up_weight, down_weight, *biases)):
         raise TypeError(f"x is {x.dtype}; weights and biases of the same type are wanted")
-    plain = x.dtype == torch.float32
-    xr, m, xs = _copy_rows(x, c, plain)
-    rows = [(xr, xs)] + [_copy_rows(w, w.shape[1], plain)[::2] for w in (gate_weight, up_weight, down_weight)]
+    xr, m, xs = _rows(x, c)
+    rows = [(xr, xs)] + [_rows(w, w.shape[1])[::2] for w in (gate_weight, up_weight, down_weight)]
     return rows, [None if t is None else t.contiguous() for t in biases], (m, c, F, o)
+
+
+def _ffn_work(dt, m, c, F, o, phase, rows, dev):
+    """Work of a feed-forward call: its bytes, and a tensor or None."""
+    if dt == BF16 and any(t.data_ptr() % 16 or s % 8 or s == 0 for t, s in rows):
+        phase |= 4                                       # FOVI_FFN_UNALIGNED: room for copies
+    size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, phase)
+    return size, torch.empty(size, dtype=torch.uint8, device=dev) if size else None
 
 
 def gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=None, down_bias=None, activation="silu", want_saved=False):
@@ -1020,8 +1027,7 @@ def gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias=None, u
     dev = x.device
     y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=dev)
     saved = torch.empty(lib.fovi_gated_ffn_saved_bytes(dt, m, F), dtype=torch.uint8, device=dev) if want_saved else None
-    size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, 2 if want_saved else 0)
-    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    size, work = _ffn_work(dt, m, c, F, o, 2 if want_saved else 0, rows, dev)
     with _on(dev):
         check(lib.fovi_gated_ffn_forward(_ptr(rows[0][0]), dt, m, c, F, o, rows[0][1], *(a for w, s in rows[1:] for a in (_ptr(w), s)), *(_opt(b) for b in biases),
                                          ACTIVATIONS[activation], _ptr(y), _opt(saved), _opt(work), size, _stream()), "fovi_gated_ffn_forward")
@@ -1038,15 +1044,14 @@ def gated_feed_forward_backward(x, gate_weight, up_weight, down_weight, saved, g
         raise ValueError(f"the gradient has the shape {tuple(grad.shape)}, the result {tuple(x.shape[:-1] + (o,))}")
     if saved.dtype != torch.uint8 or saved.numel() != lib.fovi_gated_ffn_saved_bytes(dt, m, F):
         raise ValueError("saved is not what gated_feed_forward gave for x")
-    gr, _, gs = _copy_rows(grad.to(x.dtype), o, x.dtype == torch.float32)
+    gr, _, gs = _rows(grad.to(x.dtype), o)
     dev = x.device
     shapes = (x.shape, gate_weight.shape, up_weight.shape, down_weight.shape, (F,), (F,), (o,))
     out = tuple(torch.empty(s, dtype=x.dtype, device=dev) if n else None for s, n in zip(shapes, need))
-    size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, 1)
-    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    size, work = _ffn_work(dt, m, c, F, o, 1, rows + [(gr, gs)], dev)
     with _on(dev):
         check(lib.fovi_gated_ffn_backward(_ptr(rows[0][0]), dt, m, c, F, o, rows[0][1], *(a for w, s in rows[1:] for a in (_ptr(w), s)), ACTIVATIONS[activation], _ptr(saved),
-                                          _ptr(gr), gs, *(_opt(t) for t in out), _ptr(work), size, _stream()), "fovi_gated_ffn_backward")
+                                          _ptr(gr), gs, *(_opt(t) for t in out), _opt(work), size, _stream()), "fovi_gated_ffn_backward")
     return out
 
 

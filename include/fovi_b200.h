@@ -531,9 +531,11 @@ int fovi_linear_int8_selftest_wait_timeout(const int8_t* q, int64_t tokens, int 
 
 /* Gated feed-forward block: g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) * u, y = h Wd^T + bd; x [tokens, C], Wg, Wu [F, C], Wd [O, F], biases [F], [F], [O] (contiguous) or NULL,
  * y contiguous [tokens, O], all of one type; strides: elements from one row to the next.  activation 0: act(g) = g / (1 + exp(-g)), 1: g times the normal distribution
- * function.  bf16: rows, y and the gradients start on 16-byte boundaries.  saved: fovi_gated_ffn_saved_bytes bytes for the backward pass, or NULL; work:
- * fovi_gated_ffn_workspace_bytes bytes of the phase (0: forward without `saved`, 2: with, 1: backward; 0 bytes: NULL), both on 32-byte boundaries.
+ * function.  saved: fovi_gated_ffn_saved_bytes bytes for the backward pass, or NULL; work: fovi_gated_ffn_workspace_bytes bytes of the phase (0: forward without `saved`, 2: with,
+ * 1: backward; plus FOVI_FFN_UNALIGNED where rows of x, a weight or dy of a bf16 block do not start on 16-byte boundaries: room for copies; 0 bytes: NULL).
+ * y and the gradients of x and the weights lie on 16-byte boundaries, saved and work on 32-byte ones.
  * Backward: each gradient may be NULL; all are of the block's type, contiguous, and have the same bits every time, whichever are asked for. */
+#define FOVI_FFN_UNALIGNED 4
 int64_t fovi_gated_ffn_saved_bytes(int dtype, int64_t tokens, int F);
 int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int C, int F, int O, int phase);
 int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,

@@ -39,11 +39,10 @@ def test_which_calls_it_takes(counted):
     plain = [lambda: tokens.rms_norm(x, w), lambda: tokens.rms_norm(x.view(4, 10, 64), residual=r.view(4, 10, 64)), lambda: tokens.rms_norm_int8(x, w, residual=r),
              lambda: tokens.rms_norm_int8(x[0]), lambda: tokens.quantize(x), lambda: tokens.linear_int8(q, s, q, s, s), lambda: tokens.linear_int8(q3, s3, q3, s3, out_dtype=torch.float32),
              lambda: tokens.linear_int8(q.view(4, 10, 64), s.view(4, 10), q, s), lambda: tokens.gated_feed_forward(*leaves), lambda: tokens.gated_feed_forward(*leaves[:4]),
-             lambda: tokens.gated_feed_forward(*plain32, activation="gelu")]
+             lambda: tokens.gated_feed_forward(*plain32, activation="gelu"), lambda: tokens.gated_feed_forward(*_block(BF, C=61)), lambda: tokens.gated_feed_forward(*_block(BF, F=33, O=5))]
     other = [lambda: tokens.rms_norm(x.t()), lambda: tokens.rms_norm(x, w.to(BF)), lambda: tokens.rms_norm(x[:0]), lambda: tokens.rms_norm(x, w, residual=r.t().contiguous().t()),
              lambda: tokens.rms_norm_int8(x[:, ::2]), lambda: tokens.quantize(x[:, ::2]), lambda: tokens.linear_int8(q[:, 1:], s, q[:, 1:].contiguous(), s),
              lambda: tokens.linear_int8(q, s, q, s, s.to(BF)), lambda: tokens.linear_int8(q[:0], s[:0], q, s), lambda: tokens.gated_feed_forward(leaves[0][:, ::2], *_block(BF, C=32)[1:]),
-             lambda: tokens.gated_feed_forward(*_block(BF, C=61)), lambda: tokens.gated_feed_forward(*_block(BF, F=33)), lambda: tokens.gated_feed_forward(*_block(BF, O=5)),
              lambda: tokens.gated_feed_forward(leaves[0][:0], *leaves[1:])]
     for call in plain:
         call()

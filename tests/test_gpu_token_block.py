@@ -204,16 +204,20 @@ def test_unaligned_pointers_are_refused_by_the_c_abi():
     from fovi_b200._lib import lib
     b = torch.zeros(4096, device="cuda", dtype=BF)
     p, st = b.data_ptr(), ops._stream()
-    args = [p, ops.BF16, 4, 16, 16, 16, 16, p, 16, p, 16, p, 16, None, None, None, 0, p, None, p, 8192, st]
-    for i in (0, 7, 9, 11, 17):
+    args = [p, ops.BF16, 4, 16, 16, 16, 16, p, 16, p, 16, p, 16, None, None, None, 0, p, None, p, 4096, st]
+    for i in (17, 19):                                                          # y, work
         bad = list(args)
-        bad[i] = p + 2
+        bad[i] = p + 8
         assert lib.fovi_gated_ffn_forward(*bad) == 5
-    for i in (6, 8, 10, 12):
+    for i, v in ((0, p + 2), (7, p + 2), (9, p + 2), (11, p + 2), (6, 17), (8, 17), (10, 17), (12, 17), (20, 8)):      # rows off boundaries: more work is needed than is there
         bad = list(args)
-        bad[i] = 17
-        assert lib.fovi_gated_ffn_forward(*bad) == 5
-    assert lib.fovi_gated_ffn_forward(*(args[:20] + [8] + args[21:])) == 1          # too little work
+        bad[i], bad[20] = v, lib.fovi_gated_ffn_workspace_bytes(ops.BF16, 4, 16, 16, 16, 0) - (i == 20)
+        assert lib.fovi_gated_ffn_forward(*bad) == 1
+    for i, v in ((1, 5), (2, -1), (3, 0), (4, 0), (5, 0), (6, -1), (16, 2), (16, -1), (0, None), (17, None), (19, None)):
+        bad = list(args)
+        bad[i] = v
+        assert lib.fovi_gated_ffn_forward(*bad) == 1
+    assert lib.fovi_gated_ffn_workspace_bytes(ops.BF16, 4, 16, 16, 16, 3) == -1 == lib.fovi_gated_ffn_workspace_bytes(ops.BF16, 4, 16, 16, 16, 7)
     assert lib.fovi_linear_int8(p + 1, 4, 16, 16, p, p, 16, 16, p, None, p, 0, st) == 5
     assert lib.fovi_linear_int8(p, 4, 16, 17, p, p, 16, 16, p, None, p, 0, st) == 5
     assert lib.fovi_linear_int8(p, 4, 131072, 131072, p, p, 16, 131072, p, None, p, 0, st) == 1
