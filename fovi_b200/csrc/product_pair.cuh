@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "pairs.cuh"
 #include "tc_common.cuh"
 
@@ -41,6 +43,26 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
 __device__ __forceinline__ void st_global_32f(float* p, const uint32_t* v) {
   const uint32_t w[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
   st_global_32(p, w);
+}
+
+// What a launch asks the runtime once for each device (of the first 64; of others every time): a kernel's shared memory, a status word's address.
+inline int device_slot() {
+  int dev = -1;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : -1;
+}
+template <typename Kernel> cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  const int dev = device_slot();
+  if (dev >= 0 && (done.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
+template <typename Symbol> cudaError_t word_of(int** word, Symbol& symbol, std::atomic<int*> (&known)[64]) {
+  const int dev = device_slot();
+  if (dev >= 0 && (*word = known[dev].load(std::memory_order_relaxed))) return cudaSuccess;
+  const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(word), symbol);
+  if (e == cudaSuccess && dev >= 0) known[dev].store(*word, std::memory_order_relaxed);
+  return e;
 }
 
 }  // namespace

@@ -426,7 +426,8 @@ template <int EPI, bool A_MN, bool B_MN, int ACT = 0> int launch(const PsMaps& m
   a.wait_limit = WAIT_LIMIT;
   const int grid = 2 * std::min(a.first[a.tasks], pairs());
   auto kernel = product_split_kernel<EPI, A_MN, B_MN, ACT>;
-  FOVI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PS_SMEM));
+  static std::atomic<uint64_t> done{0};
+  FOVI_CUDA(allow_shared(kernel, (int)PS_SMEM, done));
   FOVI_CUDA(fovi::launch_pdl(kernel, grid, PS_THREADS, PS_SMEM, st, maps, a));
   return fovi::after_launch("product_split_kernel");
 }
@@ -476,7 +477,8 @@ Shape grads_shape(const SplitProduct* tasks, int n, int64_t rows, int64_t* bytes
 }  // namespace
 
 int fovi::split_status(int** word) {
-  FOVI_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_status));
+  static std::atomic<int*> known[64];
+  FOVI_CUDA(word_of(word, g_status, known));
   return FOVI_OK;
 }
 

@@ -538,6 +538,11 @@ __global__ void __launch_bounds__(256) product_join_kernel(const __grid_constant
 // ------------------------------------------------------------------------------------------------------------ host
 int pairs() { return std::max(1, fovi::sm_count() / 2); }
 
+cudaError_t status_word(int** word) {
+  static std::atomic<int*> known[64];
+  return word_of(word, g_status, known);
+}
+
 // The cut with the least time by a count of clocks: 2 clocks a column and stage, about 1500 for a tile's start and end, and for k in parts their way through memory.
 // `columns` of a tile are divided among `share` matrices (GATED: 2).
 TcShape shape_of(const int64_t* m, const int* n, int tasks, int64_t kb, int share, bool may_split) {
@@ -565,12 +570,13 @@ int map_k(CUtensorMap* m, const TcMatrix& x, bool bytes, int rows) {
 int map_mn(CUtensorMap* m, const TcMatrix& x) { return fovi::encode_2d(m, x.p, false, (uint64_t)x.cols, (uint64_t)x.rows, (uint64_t)x.pitch * 2, 64, 64); }
 
 template <int EPI, bool A_MN, bool B_MN, bool I8, int ACT = 0> int launch(const PtMaps& maps, PtArgs& a, bool selftest, cudaStream_t st) {
-  FOVI_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&a.status), g_status));
+  static std::atomic<uint64_t> done{0};
+  FOVI_CUDA(status_word(&a.status));
   a.wait_limit = selftest ? 4096u : WAIT_LIMIT;
   a.skip_loads = selftest;
   const int grid = 2 * std::min(a.first[a.tasks], pairs());
   auto kernel = product_tc_kernel<EPI, A_MN, B_MN, I8, ACT>;
-  FOVI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sizes<EPI>::SMEM));
+  FOVI_CUDA(allow_shared(kernel, (int)Sizes<EPI>::SMEM, done));
   FOVI_CUDA(fovi::launch_pdl(kernel, grid, PT_THREADS, Sizes<EPI>::SMEM, st, maps, a));
   return fovi::after_launch("product_tc_kernel");
 }
@@ -737,7 +743,7 @@ int fovi::tc_int8(const TcMatrix& q, const TcMatrix& w, const float* scale, cons
 extern "C" int fovi_product_check(void* stream) {
   auto st = reinterpret_cast<cudaStream_t>(stream);
   int* words[2];
-  FOVI_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&words[0]), g_status));
+  FOVI_CUDA(status_word(&words[0]));
   int rc = fovi::split_status(&words[1]), sites[2] = {0, 0};
   if (rc) return rc;
   for (int i = 0; i < 2; ++i) FOVI_CUDA(cudaMemcpyAsync(&sites[i], words[i], sizeof(int), cudaMemcpyDeviceToHost, st));
