@@ -1,7 +1,7 @@
 // Float32 matrix products on the tensor cores.
 //
-// A float32 value is the sum of three bf16 values exactly (8 of its 24 bits each, cut off, not rounded, so that none leaves the range; infinity and not-a-number are the first part
-// alone).  Of the nine products of two values' parts the six largest are taken; what is left out is below 2^-24 of the product, a float32 product's own rounding.  They are exact in the
+// A float32 value is the sum of three bf16 values exactly: the value rounded to 8 bits, what is left rounded to 8 bits, and the rest (infinity and not-a-number: the first part alone).
+// Of the nine products of two values' parts the six largest are taken; what is left out is at most 2^-24 of the product, a float32 product's own rounding.  The six are exact in the
 // tensor cores, whose sums lose up to a unit of float32 at each step: so a sum runs over 64 of k only (24 steps), and the sums of 64 are added in registers with float32's rounding.
 //   bound: six bf16 products for one, 375 of 2250 TFLOP/s, where the multiply-add units give 74.
 // The kernel is that of product_tc.cu with these differences: a stage is 64 of k of all three parts of both operands (96 KB of a CTA, two stages), six products are taken from it, least
@@ -72,9 +72,13 @@ struct Parts { uint32_t w[3]; };
 __device__ __forceinline__ void cut(float x, uint32_t (&p)[3]) {
   const uint32_t b = __float_as_uint(x);
   const bool finite = (b & 0x7f800000u) != 0x7f800000u;
-  const float r1 = x - __uint_as_float(b & 0xffff0000u), r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
-  p[0] = finite ? b >> 16 : (b >> 16) | ((b & 0x007fffffu) ? 0x40u : 0u);          // (not-a-number stays that)
-  p[1] = finite ? __float_as_uint(r1) >> 16 : 0u;
+  uint32_t b0 = b + 0x8000u;
+  if ((b0 & 0x7f800000u) == 0x7f800000u) b0 = b;                                     // (rounding up would leave the range)
+  const float r1 = x - __uint_as_float(b0 & 0xffff0000u);
+  const uint32_t b1 = __float_as_uint(r1) + 0x8000u;
+  const float r2 = r1 - __uint_as_float(b1 & 0xffff0000u);
+  p[0] = finite ? b0 >> 16 : (b >> 16) | ((b & 0x007fffffu) ? 0x40u : 0u);           // (not-a-number stays that)
+  p[1] = finite ? b1 >> 16 : 0u;
   p[2] = finite ? __float_as_uint(r2) >> 16 : 0u;
 }
 __device__ __forceinline__ Parts cut_pair(float x, float y) {
