@@ -20,7 +20,7 @@ namespace {
 // Column sums of up to three matrices in a fixed order: parts of strips of rows, then the parts of each column; two launches for all.
 struct SumTask { const void* x; int64_t rows, pitch; int n; float* part; int parts; int64_t part_pitch; void* out; };      // part: given (x null), or to be made
 struct SumTasks { SumTask t[3]; };
-constexpr int SUM_COLS = 256, STRIPS = 128;
+constexpr int SUM_COLS = 256, STRIPS = 512;
 
 // A block takes 256 columns of a strip of rows, a lane 8 neighbouring ones, its 8 warps a row each at a time.
 template <typename T>
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(1024) column_join_kernel(const __grid_constant
   static_cast<T*>(t.out)[c] = from_float<T>(s);
 }
 SumTask sum_task(const void* x, int64_t rows, int n, int64_t pitch, float* part, void* out) {
-  return {x, rows, pitch, n, part, (int)std::max<int64_t>(1, std::min<int64_t>(STRIPS, rows / 16)), n, out};
+  return {x, rows, pitch, n, part, (int)std::max<int64_t>(1, std::min<int64_t>(STRIPS, rows / 32)), n, out};
 }
 // The parts of those tasks that have an x.
 template <typename T> int column_parts(const SumTasks& tasks, cudaStream_t st) {
@@ -278,9 +278,10 @@ struct PadTask { const uint16_t* x; int64_t stride; uint16_t* to; int64_t rows, 
 struct PadArgs { PadTask t[5]; };
 __global__ void __launch_bounds__(256) pad_kernel(const __grid_constant__ PadArgs a) {
   const PadTask& t = a.t[blockIdx.y];
-  const int64_t per = t.pitch / 8, all = t.rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per, c = 8 * (i - r * per);
+  const uint32_t per = (uint32_t)(t.pitch / 8);
+  const uint64_t all = t.rows * per;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+    const int64_t r = i >> 32 ? i / per : (uint32_t)i / per, c = 8 * (int64_t)(i - r * per);
     const uint16_t* x = t.x + r * t.stride + c;
     uint32_t w[4] = {};
 #pragma unroll

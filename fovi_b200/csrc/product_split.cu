@@ -361,34 +361,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PS_THREADS, 1) produ
   }
 }
 
-// The parts of the products' k, added in their order, with the bias.  A thread for a value; y counts the products.
+// The parts of the products' k, added in their order, with the bias.  A thread for four columns; y counts the products.
 struct JoinArgs { const float* part[GROUPS]; float* y[GROUPS]; int64_t m[GROUPS]; int n[GROUPS], splits; const float* bias; };
 __global__ void __launch_bounds__(256) product_split_join_kernel(const __grid_constant__ JoinArgs a) {
   const int t = blockIdx.y, n = a.n[t];
-  const int64_t pitch = (n + 31) / 32 * 32, i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / n, c = i - row * n;
+  const uint32_t pitch = (n + 31) / 32 * 32, per = pitch / 4;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x, row = i >> 32 ? i / per : (uint32_t)i / per;
+  const int c = (int)(i - row * per) * 4;
+  const int64_t m = a.m[t];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (row >= a.m[t]) return;
-  float s = 0.f;
+  if ((int64_t)row >= m || c >= n) return;
+  const float* from = a.part[t] + row * pitch + c;
+  float s[4] = {};
+#pragma unroll 4
   for (int p = 0; p < a.splits; ++p) {
-    float v;
-    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(a.part[t] + ((int64_t)p * a.m[t] + row) * pitch + c) : "memory");
-    s += v;
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(from + p * m * pitch) : "memory");
+    s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
   }
-  a.y[t][i] = s + (a.bias ? __ldg(a.bias + c) : 0.f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (a.bias && c + e < n) s[e] += __ldg(a.bias + c + e);
+  float* to = a.y[t] + (int64_t)row * n + c;
+  if (n % 4 == 0) {
+    *reinterpret_cast<float4*>(to) = make_float4(s[0], s[1], s[2], s[3]);
+  } else {
+    for (int e = 0; e < 4 && c + e < n; ++e) to[e] = s[e];
+  }
 }
 
 struct CutArgs { SplitTask t[fovi::SPLITS_MOST]; };
-// A thread for two neighbouring values of a row.
+// A thread for eight neighbouring values of a row.
 __global__ void __launch_bounds__(256) cut_kernel(const __grid_constant__ CutArgs a) {
   const SplitTask& t = a.t[blockIdx.y];
-  const int64_t per = (t.to.cols + 1) / 2, all = t.to.rows * per, part = t.to.rows * t.to.pitch;
+  const uint32_t per = (uint32_t)(t.to.pitch / 8);
+  const uint64_t all = t.to.rows * per;
+  const int64_t part = t.to.rows * t.to.pitch;
+  const bool vec = t.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(t.x) & 15) == 0;
   uint16_t* to = static_cast<uint16_t*>(t.to.p);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per, c = 2 * (i - r * per);
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+    const uint64_t r = i >> 32 ? i / per : (uint32_t)i / per;
+    const int64_t c = 8 * (int64_t)(i - r * per);
     const float* x = t.x + r * t.stride + c;
-    const Parts p = cut_pair(__ldg(x), c + 1 < t.to.cols ? __ldg(x + 1) : 0.f);          // (a row's pitch is even: its second value has a place)
+    float v[8];
+    if (vec && c + 8 <= t.to.cols) {
+      const float4 lo = __ldg(reinterpret_cast<const float4*>(x)), hi = __ldg(reinterpret_cast<const float4*>(x) + 1);
+      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+    } else {
 #pragma unroll
-    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(to + q * part + r * t.to.pitch + c) = p.w[q];
+      for (int j = 0; j < 8; ++j) v[j] = c + j < t.to.cols ? __ldg(x + j) : 0.f;
+    }
+    uint32_t w[3][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Parts p = cut_pair(v[2 * j], v[2 * j + 1]);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) w[q][j] = p.w[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * part + r * t.to.pitch + c) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
   }
 }
 
@@ -456,7 +487,7 @@ int join(const PsArgs& a, cudaStream_t st) {
   j.bias = a.bias;
   for (int t = 0; t < a.tasks; ++t) {
     j.part[t] = a.work + a.part[t]; j.y[t] = a.y[t]; j.m[t] = a.m[t]; j.n[t] = a.n[t];
-    threads = std::max(threads, (int64_t)a.m[t] * a.n[t]);
+    threads = std::max(threads, (int64_t)a.m[t] * ((a.n[t] + 31) / 32 * 8));
   }
   FOVI_CUDA(fovi::launch_pdl(product_split_join_kernel, dim3((unsigned)((threads + 255) / 256), a.tasks), 256, 0, st, j));
   return fovi::after_launch("product_split_join_kernel");
@@ -491,7 +522,7 @@ int fovi::split_matrices(const SplitTask* t, int n, cudaStream_t st) {
   int64_t most = 0;
   for (int i = 0; i < n; ++i) {
     a.t[i] = t[i];
-    most = std::max(most, t[i].to.rows * ((t[i].to.cols + 1) / 2));
+    most = std::max(most, t[i].to.rows * (t[i].to.pitch / 8));
   }
   cut_kernel<<<dim3((unsigned)std::min<int64_t>((most + 255) / 256, 8 * fovi::sm_count()), n), 256, 0, st>>>(a);
   return fovi::after_launch("cut_kernel");

@@ -508,8 +508,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
 struct JoinArgs { const float* part[GROUPS]; __nv_bfloat16* y[GROUPS]; int64_t m[GROUPS]; int n[GROUPS], splits; const __nv_bfloat16* bias; };
 __global__ void __launch_bounds__(256) product_join_kernel(const __grid_constant__ JoinArgs a) {
   const int t = blockIdx.y, n = a.n[t];
-  const int64_t pitch = (n + 31) / 32 * 32, per = pitch / 4, m = a.m[t];
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per;
+  const uint32_t pitch = (n + 31) / 32 * 32, per = pitch / 4;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t m = a.m[t], row = i >> 32 ? i / per : (uint32_t)i / per;
   const int c = (int)(i - row * per) * 4;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (row >= m || c >= n) return;
