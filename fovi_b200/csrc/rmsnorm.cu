@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(1024) rms_norm_join_kernel(const float* part, 
 // ------------------------------------------------------------------------------------------------------------ rows in registers
 // A row is held in registers by a team of threads (rows.cuh), a warp or, where it is too long for one, a block; the next row's loads are issued before this row's sums.  One pass over memory
 // in both directions: the residual's sum, its norm and the 8-bit form with its scale come from the same registers, and the backward kernel keeps every column's part of dw over all its rows.
+// What bounds it is memory: 263168 x 384 bf16 with the residual 124 us forward (6.5 TB/s) and 151 backward (5.4), 65792 x 1280 into 8 bits 103 (5.7).
 template <typename T, int VEC> __device__ __forceinline__ void store_eight(int8_t* p, const float* v, float inv) {
   if constexpr (VEC == 1) {
     p[0] = (int8_t)eight_bits(v[0], inv);
@@ -349,22 +350,27 @@ __global__ void __launch_bounds__(BLOCK ? BLOCK_MOST<VEC> : 256) rms_norm_grad_r
   for (int c = threadIdx.x; c < C; c += blockDim.x) mine[c] = joined[c];
 }
 
+// Values a thread of a warp's row.  In 8 bits a block would pass two barriers a row, its sum of squares and its largest value: a warp holds up to 40 of bf16 (us of 78000 x 1280 with a residual:
+// block 142, warp 123; of 130000 x 768: 140, 111), 24 where pieces have four values.  Otherwise of bf16 up to 16 (forward at 768 channels: block 126, warp 137; backward 146, 150), of float32 24 (backward at 512: block
+// 142, warp 124).
+constexpr int MOST_EIGHT = 40, MOST_BF16 = 16, MOST_F32 = 24;
 // How a row is held: pieces of `vec` values, `ch` of them a thread, teams of `threads` (0: the kernels above, which read a row several times).
 struct Shape { int vec, ch, threads; bool block; };
 
 // Every operand is (address, stride of rows in values, size of a value).
 struct Rows { const void* p; int64_t stride; int size; };
-template <int N> Shape shape_of(const Rows (&all)[N], int C, int size) {
+// most: how many values a thread of a warp holds at most; beyond, a block holds the row, 8 values a thread (bf16 from 8192 and float32 from 4096 channels on more threads than a block has: none).
+template <int N> Shape shape_of(const Rows (&all)[N], int C, int size, int most) {
   auto fits = [&](int v) {
     if (C % v) return false;
     for (const Rows& o : all)
       if (o.p && (o.stride % v || reinterpret_cast<uintptr_t>(o.p) % (v * o.size))) return false;
     return true;
   };
-  // 16 bytes a piece; of bf16 8 below 512 channels, where lanes would stay idle
-  const int vec = size == 2 && C >= 512 && fits(8) ? 8 : fits(4) ? 4 : 1;
-  // A warp holds up to 16 values a thread (12 of float32, one by one 8); beyond, a block does, 8 values a thread.
-  const int ch = (C + 32 * vec - 1) / (32 * vec), most = vec == 1 ? 8 : size == 4 ? 12 : 16;
+  // 16 bytes a piece; of bf16 8 below 256 channels, where lanes would stay idle (260000 x 384, with a residual: 16 bytes 128 us forward and 122 into 8 bits, 8 bytes 140 and 131)
+  const int vec = size == 2 && C >= 256 && fits(8) ? 8 : fits(4) ? 4 : 1;
+  const int ch = (C + 32 * vec - 1) / (32 * vec);
+  most = vec == 1 ? 8 : vec == 4 ? std::min(most, 24) : most;
   if (ch * vec <= most) return {vec, vec == 1 ? (ch + 3) / 4 * 4 : ch, 32, false};
   const int per = 8 / vec, threads = ((C + 7) / 8 + 31) / 32 * 32;
   if (threads <= (vec == 1 ? BLOCK_MOST<1> : BLOCK_MOST<4>)) return {vec, per, threads, true};
@@ -375,11 +381,10 @@ template <int N> Shape shape_of(const Rows (&all)[N], int C, int size) {
 template <typename T, typename F> int with(const Shape& s, const F& f) {
 #define FOVI_ROWS(V, N, B) if (s.vec == V && s.ch == N && s.block == B) return f(std::integral_constant<int, V>(), std::integral_constant<int, N>(), std::bool_constant<B>())
   if constexpr (sizeof(T) == 2) {
-    FOVI_ROWS(8, 1, true);
-    FOVI_ROWS(8, 2, false);
-    FOVI_ROWS(4, 4, false);
+    FOVI_ROWS(8, 1, true); FOVI_ROWS(8, 1, false); FOVI_ROWS(8, 2, false); FOVI_ROWS(8, 3, false);
+    FOVI_ROWS(8, 4, false); FOVI_ROWS(8, 5, false);
   }
-  FOVI_ROWS(4, 1, false); FOVI_ROWS(4, 2, false); FOVI_ROWS(4, 3, false); FOVI_ROWS(4, 2, true);
+  FOVI_ROWS(4, 1, false); FOVI_ROWS(4, 2, false); FOVI_ROWS(4, 3, false); FOVI_ROWS(4, 4, false); FOVI_ROWS(4, 5, false); FOVI_ROWS(4, 6, false); FOVI_ROWS(4, 2, true);
   FOVI_ROWS(1, 4, false); FOVI_ROWS(1, 8, false); FOVI_ROWS(1, 8, true);
 #undef FOVI_ROWS
   return FOVI_ERR_UNSUPPORTED;
@@ -412,7 +417,7 @@ int strips_of(int64_t rows) { return (int)(rows < 512 ? (rows + 15) / 16 : 64); 
 
 template <typename T, bool NORM> int forward(const RmsArgs& a, cudaStream_t st) {
   const int size = sizeof(T);
-  const Shape s = shape_of<5>({{a.x, a.x_stride, size}, {a.res, a.r_stride, size}, {a.total, a.C, size}, {a.y, a.C, size}, {a.q, a.q_stride, 1}}, a.C, size);
+  const Shape s = shape_of<5>({{a.x, a.x_stride, size}, {a.res, a.r_stride, size}, {a.total, a.C, size}, {a.y, a.C, size}, {a.q, a.q_stride, 1}}, a.C, size, a.q ? MOST_EIGHT : size == 2 ? MOST_BF16 : MOST_F32);
   if (s.threads) {
     if constexpr (!NORM) return rows_forward<T, ROWS>(a, s, st);
     else return a.q ? rows_forward<T, EIGHT>(a, s, st) : rows_forward<T, PLAIN>(a, s, st);
@@ -424,7 +429,7 @@ template <typename T, bool NORM> int forward(const RmsArgs& a, cudaStream_t st) 
 
 template <typename T> int backward(const RmsGradArgs& a, float* dw, cudaStream_t st) {
   const int size = sizeof(T);
-  const Shape s = shape_of<4>({{a.t, a.t_stride, size}, {a.dy, a.dy_stride, size}, {a.dt, a.dt_stride, size}, {a.dx, a.C, size}}, a.C, size);
+  const Shape s = shape_of<4>({{a.t, a.t_stride, size}, {a.dy, a.dy_stride, size}, {a.dt, a.dt_stride, size}, {a.dx, a.C, size}}, a.C, size, size == 2 ? MOST_BF16 : MOST_F32);
   int parts = strips_of(a.rows);
   if (s.threads) {
     const int rc = with<T>(s, [&](auto vec, auto ch, auto block) {
