@@ -35,6 +35,12 @@ template <bool I8> __device__ __forceinline__ void pt_mma(uint32_t d, uint64_t a
 __device__ __forceinline__ void pt_commit(uint32_t bar) {            // on the barrier at this offset in both CTAs
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
+// Behind tc_ld_wait: what reads the loaded registers stays behind the wait, which does not name them.
+__device__ __forceinline__ void pt_loaded(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));

@@ -238,6 +238,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PS_THREADS, 1) produ
               uint32_t r[32];
               tc_ld32(t_base + q * half + 32 * c, r);
               tc_ld_wait();
+              pt_loaded(r);
 #pragma unroll
               for (int i = 0; i < 16; ++i) sum[ci][q][i] = add2(sum[ci][q][i], make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])));
             }

@@ -331,6 +331,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
           tc_ld32(t_base + 32 * c, g);
           tc_ld32(t_base + half + 32 * c, u);
           tc_ld_wait();
+          pt_loaded(g);
+          pt_loaded(u);
           if (c + 2 >= chunks) release();
           if (a.bias) {
 #pragma unroll
@@ -391,6 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
 #pragma unroll
           for (int i = 0; i < 4; ++i) get16(from + 4096u + at64(lane, i), lo + 4 * i);
           tc_ld_wait();
+          pt_loaded(r);
           if (c + 2 >= chunks) release();
           uint32_t dg[16], du[16];
 #pragma unroll
@@ -444,6 +447,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
           __syncwarp();
           tc_ld32(t_base + 32 * c, r);
           tc_ld_wait();
+          pt_loaded(r);
           if (c + 2 >= chunks) release();
           if (EPI == STORE && a.splits > 1) {
             if (here) {
