@@ -91,8 +91,15 @@ __device__ __forceinline__ uint32_t get4(uint32_t at) {
 // Place of 16-byte piece c of row r in a tile of 128-byte or 64-byte rows, swizzled over that many bytes: eight rows' pieces lie in eight bank groups.
 __device__ __forceinline__ uint32_t at128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 __device__ __forceinline__ uint32_t at64(int r, int c) { return (uint32_t)(r * 64 + ((c ^ (r >> 1 & 3)) << 4)); }
+// The larger of two, not a number where one is not.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // act(g) and act'(g) of two values, to a few units of float32: what is rounded to bf16 behind them.  The logistic function takes an exponential each and one reciprocal for both,
-// 1/a = b/(ab), since those units are what bounds a tile's arithmetic; exponents are cut at 2^60, so that the product stays finite: there the function is below 1e-18.
+// 1/a = b/(ab), since those units are what bounds a tile's arithmetic.  Exponents are cut at 2^60, so that the product stays finite, and the factor g with them, at -60 ln 2: from there on
+// value and slope stand still, at -4e-17.  The exponent's cut drops what is not a number, as the pair shares its reciprocal; the factor's keeps it.
 template <int ACT> __device__ __forceinline__ float2 act_pair(float2 g, float2* slope) {
   if (ACT == fovi::ACT_SILU) {
     const float2 x = mul2(g, both(-1.4426950408889634f));
@@ -102,7 +109,7 @@ template <int ACT> __device__ __forceinline__ float2 act_pair(float2 g, float2* 
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(x.y, 60.f)));
     e = add2(e, both(1.f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e.x * e.y));
-    const float2 p = mul2(both(r), make_float2(e.y, e.x)), a = mul2(g, p);
+    const float2 p = mul2(both(r), make_float2(e.y, e.x)), a = mul2(make_float2(max_nan(g.x, -41.588831f), max_nan(g.y, -41.588831f)), p);
     if (slope) *slope = fma2(a, fma2(p, both(-1.f), both(1.f)), p);
     return a;
   }

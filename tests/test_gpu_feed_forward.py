@@ -202,3 +202,32 @@ def test_refusals():
     first, = torch.autograd.grad(y, x, torch.ones_like(y, requires_grad=True), create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(first.sum(), x)
+
+
+@pytest.mark.autograd
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M", [4, 16, 300])
+def test_gates_far_from_zero(M, dtype, activation):
+    """Gates from -1e20 to 1e3 with an up value of one, taken out unchanged: below -40 the value and the slope are zeros."""
+    F = 64
+    x = torch.zeros(M, F, device="cuda", dtype=dtype)
+    x[:, 0], x[:, 1] = 1e10, 1
+    gates = torch.tensor([-1e10, -1e3, -1e-5, -1e-8, -4e-9, -1e-9, 1e-10, 1e-7], device="cuda").repeat(F // 8)
+    wg, wu = torch.zeros(F, F, device="cuda", dtype=dtype), torch.zeros(F, F, device="cuda", dtype=dtype)
+    wg[:, 0], wu[:, 1] = gates.to(dtype), 1
+    leaves = [x, wg, wu, torch.eye(F, device="cuda", dtype=dtype)] + [None] * 3
+    with torch.no_grad():
+        from fovi_b200 import tokens
+        few = tokens.gated_feed_forward(*leaves, activation=activation)
+    y, _, dwg, dwu, _ = _grads(leaves, torch.ones(M, F, device="cuda", dtype=dtype), activation)
+    g = (x[0, 0].detach().double() * wg.detach()[:, 0].double()).requires_grad_(True)
+    h = torch.nn.functional.silu(g) if activation == "silu" else torch.nn.functional.gelu(g)
+    slope, = torch.autograd.grad(h.sum(), g)
+    # Two roundings each, of h and y or of dg or du and the weight's gradient; the gate is kept to 2^-17 of its value, which moves a value and a slope by no more than 41 (|g| where they
+    # are not zeros) times that.  The rest is zero to 1e-16 (value and slope below -41: 41.6 x 2^-60), a gradient's to that times the rows.
+    near = dict(rtol=2 ** -7 + 2 ** -11, atol=1e-16)
+    for got in (few, y):
+        torch.testing.assert_close(got.double(), h.detach().expand(M, F), **near)
+    torch.testing.assert_close(dwg[:, 1].double(), M * slope, rtol=near["rtol"], atol=M * 1e-16)
+    torch.testing.assert_close(dwu[:, 1].double(), M * h.detach(), rtol=near["rtol"], atol=M * 1e-16)
