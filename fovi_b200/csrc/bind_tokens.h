@@ -382,7 +382,7 @@ int rms_in(PyObject* const* v, int dev, RmsIn* a) {
   if (!a->x || !real_type(*a->x) || a->x->dim() < 1 || a->x->numel() == 0 || !a->x->is_contiguous()) return 0;
   a->C = a->x->size(-1);
   a->rows = a->x->numel() / a->C;
-  if (a->C > INT32_MAX || !bias_arg(v[1], dev, a->C, &a->wp)) return 0;
+  if (a->C > (1 << 30) || !bias_arg(v[1], dev, a->C, &a->wp)) return 0;
   const double eps = PyFloat_AsDouble(v[2]);
   if (PyErr_Occurred()) return -1;
   if (!(eps >= 0)) return 0;
@@ -464,7 +464,7 @@ END
 // x, device, stream
 BODY(quantize, 3)
   const at::Tensor* x = plain(v[0], dev);
-  if (!x || !real_type(*x) || x->dim() < 1 || x->numel() == 0 || !x->is_contiguous() || x->size(-1) > INT32_MAX || needs_graph(*x) || has_tangent(*x)) GENERAL;
+  if (!x || !real_type(*x) || x->dim() < 1 || x->numel() == 0 || !x->is_contiguous() || x->size(-1) > (1 << 30) || needs_graph(*x) || has_tangent(*x)) GENERAL;
   at::Tensor q, scale;
   int rcode;
   {
@@ -503,7 +503,7 @@ BODY(linear_int8, 8)
   if (PyErr_Occurred()) return nullptr;
   const float* b;
   int64_t qs, wstride;
-  if (type < 0 || K >= 131072 || N > INT32_MAX || !bias_arg(v[4], dev, N, &b) || !rows_on_boundaries(*q, &qs) || !rows_on_boundaries(*w, &wstride)) GENERAL;
+  if (type < 0 || K >= 131072 || N > (1 << 30) || M > (1 << 30) || !bias_arg(v[4], dev, N, &b) || !rows_on_boundaries(*q, &qs) || !rows_on_boundaries(*w, &wstride)) GENERAL;
   const at::Tensor* bias = b ? plain(v[4], dev) : nullptr;
   if (needs_graph(*s, ws, bias) || has_tangent(*s) || has_tangent(*ws) || (bias && has_tangent(*bias))) GENERAL;
   at::Tensor y;
@@ -580,7 +580,7 @@ BODY(gated_feed_forward, 10)
   const int64_t length[3] = {F, F, O};
   for (int i = 4; i < 7; ++i)
     if (t[i] && (t[i]->dim() != 1 || t[i]->size(0) != length[i - 4])) GENERAL;
-  if (C > INT32_MAX || F > INT32_MAX || O > INT32_MAX || M > (1 << 30)) GENERAL;
+  if (C > (1 << 24) || F > (1 << 24) || O > (1 << 24) || M > (1 << 30)) GENERAL;
   at::Tensor y;
   int rcode;
   {

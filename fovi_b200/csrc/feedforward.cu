@@ -321,7 +321,11 @@ int pad(Block& b, Grads* g, char*& at, cudaStream_t st) {
   return fovi::after_launch("pad_kernel");
 }
 
-bool valid(int dtype, int64_t M, int C, int F, int O) { return fovi::valid_dtype(dtype) && M >= 0 && M <= (1 << 30) && C >= 1 && F >= 1 && O >= 1; }
+// Rows and channels are counted in 32 bits, twice the hidden channels' bytes too; and a tile's waits are bounded, which its steps of 64 channels have to stay well below.
+constexpr int MOST_CHANNELS = 1 << 24;
+bool valid(int dtype, int64_t M, int C, int F, int O) {
+  return fovi::valid_dtype(dtype) && M >= 0 && M <= (1 << 30) && C >= 1 && C <= MOST_CHANNELS && F >= 1 && F <= MOST_CHANNELS && O >= 1 && O <= MOST_CHANNELS;
+}
 
 }  // namespace
 

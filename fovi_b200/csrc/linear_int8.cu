@@ -9,8 +9,8 @@ namespace {
 
 int linear_int8(const int8_t* q, int64_t tokens, int K, int64_t q_stride, const float* scale, const int8_t* weight, int N, int64_t weight_stride, const float* weight_scale,
                 const float* bias, void* y, int y_dtype, bool selftest, void* stream) {
-  // (-128)^2 K has to stay below 2^31
-  if (tokens < 0 || tokens > (1 << 30) || K < 1 || K >= 131072 || N < 1 || q_stride < 0 || weight_stride < 0 || !fovi::valid_dtype(y_dtype)) return FOVI_ERR_INVALID_ARGUMENT;
+  // (-128)^2 K has to stay below 2^31; rows and columns are counted in 32 bits, a tile beyond the last ones
+  if (tokens < 0 || tokens > (1 << 30) || K < 1 || K >= 131072 || N < 1 || N > (1 << 30) || q_stride < 0 || weight_stride < 0 || !fovi::valid_dtype(y_dtype)) return FOVI_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return FOVI_OK;
   if (!q || !scale || !weight || !weight_scale || !y) return FOVI_ERR_INVALID_ARGUMENT;
   if (!fovi::tc_takes(q, q_stride, 1) || !fovi::tc_takes(weight, weight_stride, 1) || reinterpret_cast<uintptr_t>(y) % 16) return FOVI_ERR_ALIGNMENT;

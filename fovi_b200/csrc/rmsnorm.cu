@@ -16,6 +16,7 @@ namespace {
 constexpr int GEN_THREADS = 256;
 constexpr int STRIP_COLS = 128;      // columns of a CTA of the weight-gradient pass
 constexpr float TINY = 1.17549435e-38f;
+constexpr int MOST_CHANNELS = 1 << 30;     // columns are counted in 32 bits, a block's width beyond the last one
 
 struct RmsArgs {
   const void *x, *res; int64_t rows; int C; int64_t x_stride, r_stride;
@@ -463,7 +464,7 @@ template <typename T> int backward(const RmsGradArgs& a, float* dw, cudaStream_t
 
 extern "C" int fovi_rms_norm_forward(const void* x, int dtype, int64_t rows, int C, int64_t x_stride, const void* residual, int64_t residual_stride, const float* weight,
                                      float eps, void* total, void* y, int8_t* q, int64_t q_stride, float* scale, float* rstd, void* stream) {
-  if (rows < 0 || C < 1 || x_stride < 0 || residual_stride < 0 || !(eps >= 0.f) || !fovi::valid_dtype(dtype)) return FOVI_ERR_INVALID_ARGUMENT;
+  if (rows < 0 || C < 1 || C > MOST_CHANNELS || x_stride < 0 || residual_stride < 0 || !(eps >= 0.f) || !fovi::valid_dtype(dtype)) return FOVI_ERR_INVALID_ARGUMENT;
   if (rows == 0) return FOVI_OK;
   if (!x || (y != nullptr) == (q != nullptr) || (q && (!scale || q_stride < C)) || (residual != nullptr) != (total != nullptr)) return FOVI_ERR_INVALID_ARGUMENT;
   const RmsArgs a{x, residual, rows, C, x_stride, residual_stride, weight, eps, total, y, q, q_stride, scale, rstd};
@@ -472,7 +473,7 @@ extern "C" int fovi_rms_norm_forward(const void* x, int dtype, int64_t rows, int
 }
 
 extern "C" int fovi_quantize_rows(const void* x, int dtype, int64_t rows, int C, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, void* stream) {
-  if (rows < 0 || C < 1 || x_stride < 0 || q_stride < C || !fovi::valid_dtype(dtype)) return FOVI_ERR_INVALID_ARGUMENT;
+  if (rows < 0 || C < 1 || C > MOST_CHANNELS || x_stride < 0 || q_stride < C || !fovi::valid_dtype(dtype)) return FOVI_ERR_INVALID_ARGUMENT;
   if (rows == 0) return FOVI_OK;
   if (!x || !q || !scale) return FOVI_ERR_INVALID_ARGUMENT;
   const RmsArgs a{x, nullptr, rows, C, x_stride, 0, nullptr, 0.f, nullptr, nullptr, q, q_stride, scale, nullptr};
@@ -481,13 +482,13 @@ extern "C" int fovi_quantize_rows(const void* x, int dtype, int64_t rows, int C,
 }
 
 extern "C" int64_t fovi_rms_norm_workspace_bytes(int64_t rows, int C) {
-  if (rows < 0 || C < 1) return -1;
+  if (rows < 0 || C < 1 || C > MOST_CHANNELS) return -1;
   return std::max<int64_t>(std::min<int64_t>(rows, GRAD_BLOCKS), strips_of(rows)) * C * 4;
 }
 
 extern "C" int fovi_rms_norm_backward(const void* t, int dtype, int64_t rows, int C, int64_t t_stride, const void* dy, int64_t dy_stride, const void* dt, int64_t dt_stride,
                                       const float* weight, const float* rstd, void* dx, float* dweight, void* work, int64_t work_bytes, void* stream) {
-  if (rows < 0 || C < 1 || t_stride < 0 || dy_stride < 0 || dt_stride < 0 || !fovi::valid_dtype(dtype)) return FOVI_ERR_INVALID_ARGUMENT;
+  if (rows < 0 || C < 1 || C > MOST_CHANNELS || t_stride < 0 || dy_stride < 0 || dt_stride < 0 || !fovi::valid_dtype(dtype)) return FOVI_ERR_INVALID_ARGUMENT;
   auto st = reinterpret_cast<cudaStream_t>(stream);
   if (rows == 0) {
     if (dweight) FOVI_CUDA(cudaMemsetAsync(dweight, 0, (size_t)C * 4, st));

@@ -877,8 +877,8 @@ def layer_norm_backward(x, grad, weight, stats, need=(True, True, True)):
 def _rms_inputs(x, weight, eps, residual):
     """Checked arguments of a root-mean-square norm: weight in float32, rows of x and of the residual, their number and length."""
     _same_device(x, weight, residual)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"rms norm needs a last axis of at least one value, got the shape {tuple(x.shape)}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 30:
+        raise ValueError(f"rms norm needs a last axis of at least one value and at most 2^30, got the shape {tuple(x.shape)}")
     if not eps >= 0:
         raise ValueError(f"eps is {eps}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
@@ -946,8 +946,8 @@ def rms_norm_int8(x, weight=None, eps=1e-6, residual=None):
 def quantize(x):
     """Rows x [..., C] (float32 or bf16) in 8 bits: (q int8 [..., C], scale float32 [...]), x = q * scale to half a step."""
     _need_cuda(x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"quantize needs a last axis of at least one value, got the shape {tuple(x.shape)}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 30:
+        raise ValueError(f"quantize needs a last axis of at least one value and at most 2^30, got the shape {tuple(x.shape)}")
     c = x.shape[-1]
     xr, n, stride = _rows(x, c)
     q, scale = _eight_bits(x.shape, x.device), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
@@ -978,6 +978,8 @@ def linear_int8(q, scale, weight, weight_scale, bias=None, out_dtype=torch.bfloa
     if scale.shape != q.shape[:-1] or weight_scale.shape != weight.shape[:1]:
         raise ValueError(f"scale {tuple(scale.shape)}, weight_scale {tuple(weight_scale.shape)}: one for each of {tuple(q.shape[:-1])} rows and {weight.shape[0]} channels")
     (n, k), dt = weight.shape, _dt(out_dtype)
+    if max(n, q.numel() // k) > 1 << 30:
+        raise ValueError(f"q {tuple(q.shape)}, weight {tuple(weight.shape)}: up to 2^30 rows each")
     b = _f32_param(bias, n, "bias")
     qr, m, q_stride = _copy_rows(q, k)
     wr, _, w_stride = _copy_rows(weight, k)
@@ -1001,6 +1003,8 @@ def _ffn_inputs(x, gate_weight, up_weight, down_weight, biases, activation):
         raise ValueError(f"x {tuple(x.shape)}, gate, up and down weights {tuple(gate_weight.shape)}, {tuple(up_weight.shape)}, {tuple(down_weight.shape)}: [..., C], [F, C], [F, C], [O, F] "
                          "are wanted")
     (F, c), o = gate_weight.shape, down_weight.shape[0]
+    if max(c, F, o) > 1 << 24 or x.numel() // c > 1 << 30:
+        raise ValueError(f"x {tuple(x.shape)}, {F} hidden channels, {o} of the result: up to 2^24 channels each and 2^30 tokens")
     for t, n, name in zip(biases, (F, F, o), ("gate", "up", "down")):
         if t is not None and t.shape != (n,):
             raise ValueError(f"the {name} bias has the shape {tuple(t.shape)}, {(n,)} is wanted")

@@ -505,7 +505,7 @@ int fovi_attention_backward_selftest_wait_timeout(const void* q, const void* k, 
 /* Root-mean-square norm over the last axis of `rows` rows of C elements (dtype; x_stride elements apart), of x or, with residual (same type, rows residual_stride
  * apart), of total = x + residual rounded to their type, which is written (contiguous; NULL where residual is):  y = t / sqrt(mean(t^2) + eps) * weight.
  * weight: DEVICE float32 [C] or NULL.  Either y (contiguous, same type), or q and scale: the result in 8 bits, y = q * scale, scale = max(max |y| / 127, smallest normal
- * number) of the row, q rounded from the unrounded y; rows of q q_stride bytes apart.  A row that holds infinity or not-a-number has one of them as its scale.
+ * number) of the row, q rounded from the unrounded y; rows of q q_stride bytes apart.  C up to 2^30.  A row that holds infinity or not-a-number has one of them as its scale.
  * rstd: float32 [rows], 1 / sqrt(mean(t^2) + eps), or NULL. */
 int fovi_rms_norm_forward(const void* x, int dtype, int64_t rows, int C, int64_t x_stride, const void* residual, int64_t residual_stride, const float* weight, float eps,
                           void* total, void* y, int8_t* q, int64_t q_stride, float* scale, float* rstd, void* stream);
@@ -518,7 +518,7 @@ int fovi_rms_norm_backward(const void* t, int dtype, int64_t rows, int C, int64_
 int fovi_quantize_rows(const void* x, int dtype, int64_t rows, int C, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, void* stream);
 
 /* y[m, n] = scale[m] * weight_scale[n] * sum over k of q[m, k] * weight[n, k] + bias[n]: q [tokens, K], weight [N, K] 8-bit integers (rows q_stride, weight_stride bytes
- * apart), exact 32-bit sums (K < 131072); scale [tokens], weight_scale [N], bias [N] or NULL float32; y contiguous [tokens, N] float32 or bf16.
+ * apart), exact 32-bit sums (K < 131072; up to 2^30 tokens and N); scale [tokens], weight_scale [N], bias [N] or NULL float32; y contiguous [tokens, N] float32 or bf16.
  * Rows of q and weight, and y, start on 16-byte boundaries. */
 int fovi_linear_int8(const int8_t* q, int64_t tokens, int K, int64_t q_stride, const float* scale, const int8_t* weight, int N, int64_t weight_stride,
                      const float* weight_scale, const float* bias, void* y, int y_dtype, void* stream);
@@ -533,7 +533,7 @@ int fovi_linear_int8_selftest_wait_timeout(const int8_t* q, int64_t tokens, int 
  * y contiguous [tokens, O], all of one type; strides: elements from one row to the next.  activation 0: act(g) = g / (1 + exp(-g)), 1: g times the normal distribution
  * function.  saved: fovi_gated_ffn_saved_bytes bytes for the backward pass, or NULL; work: fovi_gated_ffn_workspace_bytes bytes of the phase (0: forward without `saved`, 2: with,
  * 1: backward; plus FOVI_FFN_UNALIGNED where rows of x, a weight or dy of a bf16 block do not start on 16-byte boundaries: room for copies; 0 bytes: NULL).
- * y and the gradients of x and the weights lie on 16-byte boundaries, saved and work on 32-byte ones.
+ * y and the gradients of x and the weights lie on 16-byte boundaries, saved and work on 32-byte ones.  C, F and O up to 2^24, up to 2^30 tokens.
  * Backward: each gradient may be NULL; all are of the block's type, contiguous, and have the same bits every time, whichever are asked for. */
 #define FOVI_FFN_UNALIGNED 4
 int64_t fovi_gated_ffn_saved_bytes(int dtype, int64_t tokens, int F);

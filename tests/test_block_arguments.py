@@ -109,3 +109,40 @@ def test_parts_of_a_float32_value():
     far = (x.abs() > 3.39e38) | (x.flip(0).abs() > 3.39e38)                 # cut off, not rounded: a second part of up to 2^-7, a third of up to 2^-15 of the value
     # |second| <= 2^-8, |third| <= 2^-17 of the value: left out are two products of a second and a third part, and one of two third ones
     assert ((six - whole).abs() <= torch.where(far, 2.0 ** -21, 2.0 ** -24 + 2.0 ** -33) * whole.abs()).all()
+
+
+def test_sizes_that_32_bits_do_not_count():
+    """Refused before anything is read or launched: columns are counted in 32 bits, with a block's or a tile's width beyond the last one."""
+    lib = _lib()
+    for c in ((1 << 30) + 1, (1 << 31) - 1):
+        for rows in (0, 1):
+            assert lib.fovi_rms_norm_forward(P, 1, rows, c, c, None, 0, None, 1e-6, None, P, None, 0, None, None, None) == BAD
+            assert lib.fovi_rms_norm_backward(P, 1, rows, c, c, P, c, None, 0, None, P, P, None, None, 0, None) == BAD
+            assert lib.fovi_quantize_rows(P, 1, rows, c, c, P, c, P, None) == BAD
+            assert lib.fovi_linear_int8(P, rows, 32, 32, P, P, c, 32, P, None, P, 1, None) == BAD
+        assert lib.fovi_rms_norm_workspace_bytes(1, c) == -1
+    for c in ((1 << 24) + 1, (1 << 31) - 1):
+        for sizes in ((c, 8, 8), (8, c, 8), (8, 8, c)):
+            for dtype in (0, 1):
+                assert all(lib.fovi_gated_ffn_workspace_bytes(dtype, 1, *sizes, phase) == -1 for phase in (0, 1, 2))
+                for tokens in (0, 1):
+                    assert lib.fovi_gated_ffn_forward(P, dtype, tokens, *sizes, c, P, c, P, c, P, c, None, None, None, 0, P, None, P, 1 << 50, None) == BAD
+                    assert lib.fovi_gated_ffn_backward(P, dtype, tokens, *sizes, c, P, c, P, c, P, c, 0, P, P, c, P, P, P, P, P, P, P, P, 1 << 50, None) == BAD
+        assert lib.fovi_gated_ffn_saved_bytes(1, 1, c) == -1
+
+
+def test_sizes_that_python_refuses(monkeypatch):
+    from fovi_b200 import ops
+    monkeypatch.setattr(ops, "_need_cuda", lambda *a: None)
+    BF, F32, I8 = torch.bfloat16, torch.float32, torch.int8
+
+    def t(dtype, *s): return torch.empty(*s, dtype=dtype, device="meta")
+    n = (1 << 30) + 1
+    for call in (lambda: ops.rms_norm(t(BF, 1, n)), lambda: ops.quantize(t(BF, 1, n)), lambda: ops.linear_int8(t(I8, 4, 16), t(F32, 4), t(I8, n, 16), t(F32, n)),
+                 lambda: ops.linear_int8(t(I8, n, 16), t(F32, n), t(I8, 4, 16), t(F32, 4))):
+        with pytest.raises(ValueError, match="2.30"):
+            call()
+    n = (1 << 24) + 1
+    for c, h, o in ((n, 8, 8), (8, n, 8), (8, 8, n)):
+        with pytest.raises(ValueError, match="2.24"):
+            ops.gated_feed_forward(t(BF, 1, c), t(BF, h, c), t(BF, h, c), t(BF, o, h))
