@@ -1,6 +1,6 @@
 // Float32 matrix products on the tensor cores.
 //
-// A float32 value is the sum of three bf16 values exactly: the value rounded to 8 bits, what is left rounded to 8 bits, and the rest (infinity and not-a-number: the first part alone).
+// A float32 value is the sum of three bf16 values exactly: the value rounded to 8 bits, what is left rounded to 8 bits, and the rest.
 // Of the nine products of two values' parts the six largest are taken; what is left out is at most 2^-24 of the product, a float32 product's own rounding.  The six are exact in the
 // tensor cores, whose sums lose up to a unit of float32 at each step: so a sum runs over 64 of k only (24 steps), and the sums of 64 are added in registers with float32's rounding.
 //   bound: six bf16 products for one, 375 of 2250 TFLOP/s, where the multiply-add units give 74.
@@ -67,25 +67,24 @@ __device__ __forceinline__ Tile tile_of(const PsArgs& a, int item) {
   return t;
 }
 
-// The three parts of two values, as pairs.
+// The three parts of two values, as pairs.  The first two are rounded without leaving the range, so that a value that would round up to infinity keeps its rest, and infinity is the
+// third part, which meets no other than a first one.
 struct Parts { uint32_t w[3]; };
-__device__ __forceinline__ void cut(float x, uint32_t (&p)[3]) {
-  const uint32_t b = __float_as_uint(x);
-  const bool finite = (b & 0x7f800000u) != 0x7f800000u;
-  uint32_t b0 = b + 0x8000u;
-  if ((b0 & 0x7f800000u) == 0x7f800000u) b0 = b;                                     // (rounding up would leave the range)
-  const float r1 = x - __uint_as_float(b0 & 0xffff0000u);
-  const uint32_t b1 = __float_as_uint(r1) + 0x8000u;
-  const float r2 = r1 - __uint_as_float(b1 & 0xffff0000u);
-  p[0] = finite ? b0 >> 16 : (b >> 16) | ((b & 0x007fffffu) ? 0x40u : 0u);           // (not-a-number stays that)
-  p[1] = finite ? b1 >> 16 : 0u;
-  p[2] = finite ? __float_as_uint(r2) >> 16 : 0u;
+__device__ __forceinline__ uint32_t bf16_pair_finite(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
 }
+__device__ __forceinline__ float2 wide(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 __device__ __forceinline__ Parts cut_pair(float x, float y) {
-  uint32_t p[3], q[3];
-  cut(x, p);
-  cut(y, q);
-  return {{p[0] | q[0] << 16, p[1] | q[1] << 16, p[2] | q[2] << 16}};
+  Parts p;
+  float2 v = make_float2(x, y);
+  p.w[0] = bf16_pair_finite(x, y);
+  v = fma2(wide(p.w[0]), both(-1.f), v);
+  p.w[1] = bf16_pair_finite(v.x, v.y);
+  v = fma2(wide(p.w[1]), both(-1.f), v);
+  p.w[2] = bf16_pair(v.x, v.y);
+  return p;
 }
 
 // act(g) and act'(g)
@@ -255,71 +254,77 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PS_THREADS, 1) produ
         const int c = turn + 2 * ci, c0 = col0 + 32 * c;
         if (c >= chunks) break;
         const int64_t at = (int64_t)row * a.pitch + c0;
-        auto put_parts = [&](uint16_t* to, const float* v) {
+        auto put_parts = [&](uint16_t* to, int i, const float* v) {       // of 16 columns from i on
+          uint32_t w[3][8];
 #pragma unroll
-          for (int i = 0; i < 32; i += 16) {
-            uint32_t w[3][8];
+          for (int j = 0; j < 8; ++j) {
+            const Parts p = cut_pair(v[2 * j], v[2 * j + 1]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const Parts p = cut_pair(v[i + 2 * j], v[i + 2 * j + 1]);
-#pragma unroll
-              for (int q = 0; q < 3; ++q) w[q][j] = p.w[q];
-            }
-#pragma unroll
-            for (int q = 0; q < 3; ++q) st_global_32(to + q * a.part_of + at + i, w[q]);
+            for (int q = 0; q < 3; ++q) w[q][j] = p.w[q];
           }
-        };
-        auto put32 = [&](float* to, const float* v) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
+          for (int q = 0; q < 3; ++q) st_global_32(to + q * a.part_of + at + i, w[q]);
+        };
+        auto put32 = [&](float* to, const float* v, int n) {
+#pragma unroll
+          for (int i = 0; i < n; i += 8) {
             uint32_t w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[i + j]);
             st_global_32(to + i, w);
           }
         };
+        // 16 columns at a time, which registers hold beside the sums.
         if (EPI == GATED) {
-          float g[32], u[32];
           const int n = c0 + lane;
           __syncwarp();
           scratch[lane] = a.bias && n < N ? __ldg(a.bias + n) : 0.f;
           scratch[32 + lane] = a.bias2 && n < N ? __ldg(a.bias2 + n) : 0.f;
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            g[i] = (i & 1 ? sum[ci][0][i / 2].y : sum[ci][0][i / 2].x) + scratch[i];
-            u[i] = (i & 1 ? sum[ci][SETS - 1][i / 2].y : sum[ci][SETS - 1][i / 2].x) + scratch[32 + i];
-          }
-          if (here) {
-            if (a.g) { put32(a.g + at, g); put32(a.u + at, u); }
+          for (int i0 = 0; i0 < 32; i0 += 16) {
+            float g[16], u[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] *= act32<ACT>(g[i]).x;
-            put_parts(a.h, u);
+            for (int i = 0; i < 16; ++i) {
+              const int e = i0 + i;
+              g[i] = (e & 1 ? sum[ci][0][e / 2].y : sum[ci][0][e / 2].x) + scratch[e];
+              u[i] = (e & 1 ? sum[ci][SETS - 1][e / 2].y : sum[ci][SETS - 1][e / 2].x) + scratch[32 + e];
+            }
+            if (here) {
+              if (a.g) { put32(a.g + at + i0, g, 16); put32(a.u + at + i0, u, 16); }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) u[i] *= act32<ACT>(g[i]).x;
+              put_parts(a.h, i0, u);
+            }
           }
         } else if (EPI == GRAD) {
           if (here) {
-            float x[32], y[32];
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 g = *reinterpret_cast<const float4*>(a.g + at + i), u = *reinterpret_cast<const float4*>(a.u + at + i);
-              const float gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
+            for (int i0 = 0; i0 < 32; i0 += 16) {
+              float x[16], y[16];                  // g and u, then dg and du
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 s = act32<ACT>(gv[j]);
-                const float dh = (i + j) & 1 ? sum[ci][0][(i + j) / 2].y : sum[ci][0][(i + j) / 2].x;
-                x[i + j] = dh * uv[j] * s.y;
-                y[i + j] = dh * s.x;
+              for (int i = 0; i < 16; i += 4) {
+                *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(a.g + at + i0 + i);
+                *reinterpret_cast<float4*>(y + i) = *reinterpret_cast<const float4*>(a.u + at + i0 + i);
               }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int e = i0 + i;
+                const float2 s = act32<ACT>(x[i]);
+                const float dh = e & 1 ? sum[ci][0][e / 2].y : sum[ci][0][e / 2].x;
+                x[i] = dh * y[i] * s.y;
+                y[i] = dh * s.x;
+              }
+              put_parts(a.dg, i0, x);
+              put_parts(a.du, i0, y);
             }
-            put_parts(a.dg, x);
-            put_parts(a.du, y);
           }
         } else {
           float v[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = i & 1 ? sum[ci][0][i / 2].y : sum[ci][0][i / 2].x;
           if (a.splits > 1) {
-            if (here) put32(a.work + a.part[t.task] + ((int64_t)t.split * M + row) * ((N + 31) / 32 * 32) + c0, v);
+            if (here) put32(a.work + a.part[t.task] + ((int64_t)t.split * M + row) * ((N + 31) / 32 * 32) + c0, v, 32);
             continue;
           }
           const float b = a.bias && c0 + lane < N ? __ldg(a.bias + c0 + lane) : 0.f;

@@ -221,3 +221,35 @@ def test_unaligned_pointers_are_refused_by_the_c_abi():
     assert lib.fovi_linear_int8(p + 1, 4, 16, 16, p, p, 16, 16, p, None, p, 0, st) == 5
     assert lib.fovi_linear_int8(p, 4, 16, 17, p, p, 16, 16, p, None, p, 0, st) == 5
     assert lib.fovi_linear_int8(p, 4, 131072, 131072, p, p, 16, 131072, p, None, p, 0, st) == 1
+
+
+@pytest.mark.autograd
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("rows", [5, 700])
+def test_three_streams_at_once(rows, dtype):
+    """Calls that run beside one another give the bits that they give alone."""
+    from fovi_b200 import tokens
+
+    def inputs(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        def n(*s, scale=1.0): return (torch.randn(*s, generator=g, device="cuda") * scale).to(dtype).requires_grad_(True)
+        return [n(rows, 96), n(rows, 96), n(96), n(344, 96, scale=0.1), n(344, 96, scale=0.1), n(96, 344, scale=0.1)]
+
+    def step(t):
+        y, total = tokens.rms_norm(t[0], t[2], residual=t[1])
+        out = tokens.gated_feed_forward(y, *t[3:]) + total
+        with torch.no_grad():
+            eight = tokens.linear_int8(*tokens.rms_norm_int8(t[0], t[2]), *tokens.quantize(t[3]))
+        return [out, eight, *torch.autograd.grad(out, t, out.detach())]
+    sets = [inputs(i) for i in range(3)]
+    want = [step(t) for t in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for stream, t in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                got.append(step(t))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for a, b in zip(got, want) for p, q in zip(a, b))
+    tokens.check()
