@@ -438,6 +438,7 @@ struct Shape { int ct, splits; };
 Shape shape_of(const int64_t* m, const int* n, int tasks, int64_t kb, int share, bool may_split) {
   Shape best{256, 1};
   double least = 1e300;
+  const int64_t at_once = pairs();
   for (int ct = 256; ct >= 64; ct -= 64) {
     int64_t tiles = 0, values = 0;
     for (int t = 0; t < tasks; ++t) {
@@ -445,9 +446,9 @@ Shape shape_of(const int64_t* m, const int* n, int tasks, int64_t kb, int share,
       values += m[t] * ((n[t] + 31) / 32 * 32);
     }
     for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || kb / s >= 2); ++s) {
-      const double rounds = (double)((tiles * s + pairs() - 1) / pairs());
-      double clocks = rounds * ((double)((kb + s - 1) / s) * std::max(12 * ct, 1500) + 3000);
-      if (s > 1) clocks += 5000 + (double)values * s * 8 / 3400;
+      const double ways = s > 1 ? 5000 + (double)values * s * 8 / 3400 : 0;
+      if (ways >= least) break;
+      const double clocks = ways + (double)((tiles * s + at_once - 1) / at_once) * ((double)((kb + s - 1) / s) * std::max(12 * ct, 1500) + 3000);
       if (clocks < least) { least = clocks; best = {ct, s}; }
     }
   }
