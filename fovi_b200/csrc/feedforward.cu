@@ -18,17 +18,13 @@ using fovi::TcTask;
 namespace {
 
 // Column sums of up to three matrices in a fixed order: parts of strips of rows, then the parts of each column; two launches for all.
-struct SumTask { const void* x; int64_t rows, pitch; int n; float* part; int parts; int64_t part_pitch; void* out; };      // part: given (x null), or to be made
+struct SumTask { const void* x; int64_t rows, pitch; int n; float* part; int parts; int64_t part_pitch; void* out; bool bf16; };      // part: given (x null), or to be made; bf16: x's type
 struct SumTasks { SumTask t[3]; };
 constexpr int SUM_COLS = 256, STRIPS = 512;
 
 // A block takes 256 columns of a strip of rows, a lane 8 neighbouring ones, its 8 warps a row each at a time.
-template <typename T>
-__global__ void __launch_bounds__(256) column_parts_kernel(const __grid_constant__ SumTasks tasks) {
-  const SumTask& t = tasks.t[blockIdx.z];
+template <typename T> __device__ __forceinline__ void column_parts(const SumTask& t, float (&red)[8][SUM_COLS + 8]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * SUM_COLS + 8 * lane;
-  if (!t.x || (int)blockIdx.y >= t.parts || blockIdx.x * SUM_COLS >= t.n) return;
-  __shared__ float red[8][SUM_COLS + 8];
   const int64_t r0 = t.rows * blockIdx.y / t.parts, r1 = t.rows * (blockIdx.y + 1) / t.parts;
   const T* x = static_cast<const T*>(t.x) + c;
   float s[8] = {};
@@ -59,6 +55,13 @@ __global__ void __launch_bounds__(256) column_parts_kernel(const __grid_constant
   for (int w = 0; w < 8; ++w) sum += red[w][threadIdx.x];
   t.part[blockIdx.y * t.part_pitch + col] = sum;
 }
+__global__ void __launch_bounds__(256) column_parts_kernel(const __grid_constant__ SumTasks tasks) {
+  __shared__ float red[8][SUM_COLS + 8];
+  const SumTask& t = tasks.t[blockIdx.z];
+  if (!t.x || (int)blockIdx.y >= t.parts || blockIdx.x * SUM_COLS >= t.n) return;
+  if (t.bf16) column_parts<__nv_bfloat16>(t, red);
+  else column_parts<float>(t, red);
+}
 template <typename T>
 __global__ void __launch_bounds__(1024) column_join_kernel(const __grid_constant__ SumTasks tasks) {
   const SumTask& t = tasks.t[blockIdx.y];
@@ -75,29 +78,24 @@ __global__ void __launch_bounds__(1024) column_join_kernel(const __grid_constant
   for (int i = 0; i < 32; ++i) s += red[i][lane];
   static_cast<T*>(t.out)[c] = from_float<T>(s);
 }
-SumTask sum_task(const void* x, int64_t rows, int n, int64_t pitch, float* part, void* out) {
-  return {x, rows, pitch, n, part, (int)std::max<int64_t>(1, std::min<int64_t>(STRIPS, rows / 32)), n, out};
+SumTask sum_task(const void* x, int64_t rows, int n, int64_t pitch, float* part, void* out, bool bf16) {
+  return {x, rows, pitch, n, part, (int)std::max<int64_t>(1, std::min<int64_t>(STRIPS, rows / 32)), n, out, bf16};
 }
-// The parts of those tasks that have an x.
-template <typename T> int column_parts(const SumTasks& tasks, cudaStream_t st) {
-  int wide = 0, strips = 0;
-  for (const SumTask& t : tasks.t)
-    if (t.x) { wide = std::max(wide, t.n); strips = std::max(strips, t.parts); }
-  if (!wide) return FOVI_OK;
-  column_parts_kernel<T><<<dim3((wide + SUM_COLS - 1) / SUM_COLS, strips, 3), 256, 0, st>>>(tasks);
-  return fovi::after_launch("column_parts_kernel");
-}
-template <typename T> int column_join(const SumTasks& tasks, cudaStream_t st) {
-  int most = 0;
-  for (const SumTask& t : tasks.t)
+// T: the sums' type.
+template <typename T> int column_sums(const SumTasks& tasks, cudaStream_t st) {
+  int wide = 0, strips = 0, most = 0;
+  for (const SumTask& t : tasks.t) {
     if (t.out) most = std::max(most, t.n);
+    if (t.out && t.x) { wide = std::max(wide, t.n); strips = std::max(strips, t.parts); }
+  }
+  if (wide) {
+    column_parts_kernel<<<dim3((wide + SUM_COLS - 1) / SUM_COLS, strips, 3), 256, 0, st>>>(tasks);
+    const int rc = fovi::after_launch("column_parts_kernel");
+    if (rc) return rc;
+  }
   if (!most) return FOVI_OK;
   column_join_kernel<T><<<dim3((most + 31) / 32, 3), 1024, 0, st>>>(tasks);
   return fovi::after_launch("column_join_kernel");
-}
-template <typename T> int column_sums(const SumTasks& tasks, cudaStream_t st) {
-  const int rc = column_parts<T>(tasks, st);
-  return rc ? rc : column_join<T>(tasks, st);
 }
 
 int64_t pitch_of(int F) { return ((int64_t)F + 31) / 32 * 32; }
@@ -220,15 +218,12 @@ int backward_split(const Block& b, const void* saved, const Grads& g, char* work
   if (!rc) rc = fovi::split_weight_grads(f.t, 3, b.M, parts, st);
   if (rc) return rc;
   // The biases' sums: of dg and du over the rows of all three parts, of dy as it is.
-  SumTasks hid{}, all{};
+  SumTasks tasks{};
   float* const at[3] = {parts, parts + (int64_t)STRIPS * b.F, parts + 2 * (int64_t)STRIPS * b.F};
-  if (g.dbg) hid.t[0] = all.t[0] = sum_task(f.dg.p, 3 * b.M, b.F, f.dg.pitch, at[0], g.dbg);
-  if (g.dbu) hid.t[1] = all.t[1] = sum_task(f.du.p, 3 * b.M, b.F, f.du.pitch, at[1], g.dbu);
-  SumTasks own{};
-  if (g.dbd) own.t[2] = all.t[2] = sum_task(g.dy, b.M, b.O, g.dys, at[2], g.dbd);
-  rc = column_parts<__nv_bfloat16>(hid, st);
-  if (!rc) rc = column_parts<float>(own, st);
-  return rc ? rc : column_join<float>(all, st);
+  if (g.dbg) tasks.t[0] = sum_task(f.dg.p, 3 * b.M, b.F, f.dg.pitch, at[0], g.dbg, true);
+  if (g.dbu) tasks.t[1] = sum_task(f.du.p, 3 * b.M, b.F, f.du.pitch, at[1], g.dbu, true);
+  if (g.dbd) tasks.t[2] = sum_task(g.dy, b.M, b.O, g.dys, at[2], g.dbd, false);
+  return column_sums<float>(tasks, st);
 }
 
 // The three weight gradients as products over the tokens.
@@ -267,9 +262,9 @@ int backward_bf16(const Block& b, const Hidden& hid, const Grads& g, char* work,
   if ((rc = fovi::tc_weight_grads(t, 3, b.M, parts, st))) return rc;
   SumTasks tasks{};
   const int rows = (int)fovi::tc_sum_rows(b.M);
-  if (g.dbg) tasks.t[0] = SumTask{nullptr, 0, 0, b.F, sums, rows, 2 * hid.pitch, g.dbg};
-  if (g.dbu) tasks.t[1] = SumTask{nullptr, 0, 0, b.F, sums + hid.pitch, rows, 2 * hid.pitch, g.dbu};
-  if (g.dbd) tasks.t[2] = sum_task(g.dy, b.M, b.O, g.dys, parts, g.dbd);
+  if (g.dbg) tasks.t[0] = SumTask{nullptr, 0, 0, b.F, sums, rows, 2 * hid.pitch, g.dbg, false};
+  if (g.dbu) tasks.t[1] = SumTask{nullptr, 0, 0, b.F, sums + hid.pitch, rows, 2 * hid.pitch, g.dbu, false};
+  if (g.dbd) tasks.t[2] = sum_task(g.dy, b.M, b.O, g.dys, parts, g.dbd, true);
   return column_sums<__nv_bfloat16>(tasks, st);
 }
 
