@@ -122,7 +122,7 @@ int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 int forward_bf16(const Block& b, void* y, const Hidden& hid, void* work, cudaStream_t st) {
   if (!hid.high && fovi::few_block(b.M, b.C, b.F, b.O)) {
     const int rc = fovi::few_gated({b.x, b.xs}, {b.wg, b.gs}, {b.wu, b.us}, (int)b.M, b.F, b.C, b.bg, b.bu, b.act, {hid.h, hid.pitch}, st);
-    return rc ? rc : fovi::few_linear({hid.h, hid.pitch}, {b.wd, b.ds}, (int)b.M, b.O, b.F, b.bd, y, true, st);
+    return rc ? rc : fovi::few_down({hid.h, hid.pitch}, {b.wd, b.ds}, (int)b.M, b.O, b.F, b.bd, y, st);
   }
   const TcMatrix x{b.x, b.M, b.C, b.xs}, wg{b.wg, b.F, b.C, b.gs}, wu{b.wu, b.F, b.C, b.us}, wd{b.wd, b.O, b.F, b.ds}, h{hid.h, b.M, b.F, hid.pitch};
   const int rc = fovi::tc_gated(x, wg, wu, b.bg, b.bu, b.act, hid, st);
@@ -338,6 +338,7 @@ extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int
   if (dtype == FOVI_F32) return phase == 1 ? split_backward_at(b, SplitMatrix{}, nullptr).bytes : split_forward_at(b, phase == 2, nullptr).bytes;
   const int64_t extra = copies ? pads_bytes(tokens, C, F, O, phase == 1) : 0;
   if (phase == 1) return extra + back_work(b, pitch_of(F)).bytes;
+  if (phase == 0 && fovi::few_block(tokens, C, F, O)) return extra + tokens * pitch_of(F) * 4;
   return extra + (phase == 0 ? padded(tokens * pitch_of(F) * 2) : 0) + fovi::tc_linear_bytes(tokens, O, F);
 }
 

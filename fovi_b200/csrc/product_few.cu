@@ -20,6 +20,7 @@ constexpr int ROWS = 16;
 
 struct FewArgs {
   const char *x, *w, *w2; int64_t x_pitch, w_pitch, w2_pitch;        // pitches in bytes
+  int64_t rest;                                                      // LINEAR, GATED: bytes from h to its rest
   int m, n, k;                                                       // k in bytes
   const __nv_bfloat16 *bias, *bias2; int act;
   const float *scale, *wscale, *bias_f; int y_f32;
@@ -60,7 +61,7 @@ template <bool WEIGHTS> __device__ __forceinline__ Piece16 load16(const char* ro
 template <int EPI, int NT, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, EPI == GATED && WARPS == 8 ? 3 : 1) product_few_kernel(const __grid_constant__ FewArgs a, const int early) {
   constexpr bool I8 = EPI == SCALED, TWO = EPI == GATED;
-  constexpr int MATS = TWO ? 2 : 1, COLS = NT * 8, TURNS = TWO ? 1 : 2;
+  constexpr int MATS = TWO ? 2 : 1, COLS = NT * 8, TURNS = TWO ? 1 : 2, PARTS = EPI == LINEAR ? 2 : 1;
   using S = typename SumT<I8>::type;
   __shared__ S part[WARPS][MATS][ROWS][COLS + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(WARPS * 32, EPI == GATED && WARPS == 8 ? 3 : 1
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) x[j] = a.x + (int64_t)(m0 + 8 * j + r) * a.x_pitch;
-  Piece16 wp[2][TURNS][MATS][2], xp[2][TURNS][NT];
+  Piece16 wp[2][TURNS][MATS][2], xp[2][TURNS][PARTS][NT];
   constexpr int STEP = WARPS * 64, ROUND = TURNS * STEP;
   const int first = warp * 64, own = t * 16;
   auto weights = [&](int set, int at) {
@@ -91,7 +92,9 @@ __global__ void __launch_bounds__(WARPS * 32, EPI == GATED && WARPS == 8 ? 3 : 1
 #pragma unroll
     for (int u = 0; u < TURNS; ++u)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) xp[set][u][j] = load16<false>(x[j], m0 + 8 * j + r < a.m, at + u * STEP + own, a.k);
+      for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) xp[set][u][p][j] = load16<false>(x[j] + p * a.rest, m0 + 8 * j + r < a.m, at + u * STEP + own, a.k);
   };
   S d[MATS][NT][4] = {};
   auto products = [&](int set) {
@@ -101,9 +104,12 @@ __global__ void __launch_bounds__(WARPS * 32, EPI == GATED && WARPS == 8 ? 3 : 1
       for (int q = 0; q < MATS; ++q)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const uint32_t *w0 = wp[set][u][q][0].w, *w1 = wp[set][u][q][1].w, *v = xp[set][u][j].w;
-          mma_few(d[q][j], w0, v, w1[0], w1[1]);
-          mma_few(d[q][j], w0 + 2, v + 2, w1[2], w1[3]);
+#pragma unroll
+          for (int p = PARTS - 1; p >= 0; --p) {
+            const uint32_t *w0 = wp[set][u][q][0].w, *w1 = wp[set][u][q][1].w, *v = xp[set][u][p][j].w;
+            mma_few(d[q][j], w0, v, w1[0], w1[1]);
+            mma_few(d[q][j], w0 + 2, v + 2, w1[2], w1[3]);
+          }
         }
   };
   // The weights do not come from the launch before: where that is known to be this call's own, they are asked for in front of the wait for it.
@@ -147,7 +153,10 @@ __global__ void __launch_bounds__(WARPS * 32, EPI == GATED && WARPS == 8 ? 3 : 1
     } else if (EPI == GATED) {
       const float g = s[0] + (a.bias ? __bfloat162float(__ldg(a.bias + n)) : 0.f), u = s[MATS - 1] + (a.bias2 ? __bfloat162float(__ldg(a.bias2 + n)) : 0.f);
       const float p = a.act == fovi::ACT_SILU ? __fdividef(1.f, 1.f + __expf(-g)) : 0.5f * (1.f + erff(g * 0.70710678118654752f));
-      static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(g * p * u);
+      const float h = g * p * u, high = fminf(fmaxf(h, -3.38953139e38f), 3.38953139e38f);       // the largest bf16 value: infinity is the rest
+      const __nv_bfloat16 part = __float2bfloat16_rn(high);
+      static_cast<__nv_bfloat16*>(a.y)[at] = part;
+      reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(a.y) + a.rest)[at] = __float2bfloat16_rn(h - __bfloat162float(part));
     } else {
       static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(s[0] + (a.bias ? __bfloat162float(__ldg(a.bias + n)) : 0.f));
     }
@@ -289,15 +298,16 @@ int fovi::few_gated(const FewRows& x, const FewRows& wg, const FewRows& wu, int 
   FewArgs a = args(x, wg, m, n, k, 2);
   a.w2 = static_cast<const char*>(wu.p); a.w2_pitch = wu.pitch * 2;
   a.bias = static_cast<const __nv_bfloat16*>(bg); a.bias2 = static_cast<const __nv_bfloat16*>(bu); a.act = act;
-  a.y = const_cast<void*>(h.p); a.y_pitch = h.pitch;
+  a.y = const_cast<void*>(h.p); a.y_pitch = h.pitch; a.rest = m * h.pitch * 2;
   return by_tokens<GATED>(a, false, st);
 }
 
-int fovi::few_linear(const FewRows& x, const FewRows& w, int m, int n, int k, const void* bias, void* y, bool after_own, cudaStream_t st) {
-  FewArgs a = args(x, w, m, n, k, 2);
+int fovi::few_down(const FewRows& h, const FewRows& w, int m, int n, int k, const void* bias, void* y, cudaStream_t st) {
+  FewArgs a = args(h, w, m, n, k, 2);
   a.bias = static_cast<const __nv_bfloat16*>(bias);
+  a.rest = m * h.pitch * 2;
   a.y = y; a.y_pitch = n;
-  return by_tokens<LINEAR>(a, after_own, st);
+  return by_tokens<LINEAR>(a, true, st);
 }
 
 int fovi::few_block32(const float* x, int64_t xs, const float* wg, int64_t gs, const float* wu, int64_t us, const float* wd, int64_t ds, int m, int c, int f, int o, const float* bg,

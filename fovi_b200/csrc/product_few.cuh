@@ -16,10 +16,11 @@ inline bool few_eight(int64_t m, int64_t k, int64_t n) { return m <= 16 || (m <=
 // Rows as in TcMatrix: `pitch` values apart, on 16-byte boundaries.
 struct FewRows { const void* p; int64_t pitch; };
 
-// h = act(x Wg^T + bg) (x Wu^T + bu), bf16.
+// h = act(x Wg^T + bg) (x Wu^T + bu) as the sum of two bf16 values, [2][m][pitch]: h rounded to bf16 would put as much into the block's error as its rounded result does, and its rest costs
+// few_down no weights.
 int few_gated(const FewRows& x, const FewRows& wg, const FewRows& wu, int m, int n, int k, const void* bg, const void* bu, int act, const FewRows& h, cudaStream_t st);
-// y = x W^T + bias, bf16.  after_own: the launch before it in the stream is few_gated's, with the same weights in the same call.
-int few_linear(const FewRows& x, const FewRows& w, int m, int n, int k, const void* bias, void* y, bool after_own, cudaStream_t st);
+// y = h W^T + bias, bf16; the launch before it in the stream is few_gated's of the same call.
+int few_down(const FewRows& h, const FewRows& w, int m, int n, int k, const void* bias, void* y, cudaStream_t st);
 // A float32 block's forward pass, rows of any alignment; h: [m, h_pitch] to work in.
 int few_block32(const float* x, int64_t xs, const float* wg, int64_t gs, const float* wu, int64_t us, const float* wd, int64_t ds, int m, int c, int f, int o, const float* bg,
                 const float* bu, const float* bd, int act, float* h, int64_t h_pitch, float* y, cudaStream_t st);

@@ -231,3 +231,47 @@ def test_gates_far_from_zero(M, dtype, activation):
         torch.testing.assert_close(got.double(), h.detach().expand(M, F), **near)
     torch.testing.assert_close(dwg[:, 1].double(), M * slope, rtol=near["rtol"], atol=M * 1e-16)
     torch.testing.assert_close(dwu[:, 1].double(), M * h.detach(), rtol=near["rtol"], atol=M * 1e-16)
+
+
+def _in_64_bits(leaves, activation):
+    x, wg, wu, wd, bg, bu, bd = (t.detach().double() for t in leaves)
+    g, u = x @ wg.T + bg, x @ wu.T + bu
+    h = (torch.nn.functional.silu(g) if activation == "silu" else torch.nn.functional.gelu(g)) * u
+    return g, u, h, wd, bd
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("M,C,F,O", [(1, 1280, 5120, 1280), (3, 115, 312, 115), (1, 1280, 18, 1280), (8, 118, 320, 118), (16, 40, 24, 40), (40, 96, 256, 96)])
+def test_few_tokens_are_rounded_once(M, C, F, O, activation):
+    """Without gradients few tokens' hidden values keep 16 bits and more: what is left is the result's own rounding."""
+    from fovi_b200 import tokens
+    leaves, _ = _inputs(M, C, F, O, BF, 3 * M + F)
+    with torch.no_grad():
+        y = tokens.gated_feed_forward(*leaves, activation=activation).double()
+    _, _, h, wd, bd = _in_64_bits(leaves, activation)
+    # Half a step of the result; a hidden value's parts leave 2^-17 of it, its logistic function (approximate exponential and quotient) 2^-20; and float32 sums: of F products for the
+    # result, of C for g and u, which an activation's slope of up to 1.13 hands on times u, and act(g), at most |g|, times u's.
+    x, wg, wu, _, bg, bu, _ = (t.detach().double().abs() for t in leaves)
+    size, sum_g, sum_u = h.abs() @ wd.abs().T + bd.abs(), x @ wg.T + bg, x @ wu.T + bu
+    hidden = 2.0 ** -16 * h.abs() + 2.2 * C * 2.0 ** -24 * sum_g * sum_u
+    assert ((y - (h @ wd.T + bd)).abs() <= 2 ** -8 * (h @ wd.T + bd).abs() + hidden @ wd.abs().T + F * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.autograd
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("M,C,F", [(2, 384, 1536), (77, 22, 88), (314, 1280, 14), (525, 129, 344), (5000, 96, 79)])
+def test_gradients_of_biases_are_rounded_once(M, C, F, activation):
+    leaves, dy = _inputs(M, C, F, C, BF, M + F)
+    _, _, _, _, _, dbg, dbu, dbd = _grads(leaves, dy, activation)
+    g, u, h, wd, _ = _in_64_bits(leaves, activation)
+    g.requires_grad_(True)
+    a = torch.nn.functional.silu(g) if activation == "silu" else torch.nn.functional.gelu(g)
+    slope, = torch.autograd.grad(a.sum(), g)
+    a, dh = a.detach(), dy.double() @ wd
+    # Half a step of the result; g and u are kept to 2^-17, which a slope (its own slope is at most 0.8, |g| up to 8 or the slope is flat) takes as 2^-14; sums of C and M products in float32.
+    far = 2 ** -13 + (C + M) * 2 ** -24
+    size = dy.double().abs() @ wd.abs()
+    for got, each, most in ((dbg, dh * u * slope, size * (u.abs() + 1)), (dbu, dh * a, size * (a.abs() + 1))):
+        want = each.sum(0)
+        assert ((got.double() - want).abs() <= 2 ** -8 * want.abs() + far * most.sum(0)).all()
+    torch.testing.assert_close(dbd.double(), dy.double().sum(0), rtol=2 ** -8, atol=M * 2 ** -24 * dy.abs().sum(0).max().item())
