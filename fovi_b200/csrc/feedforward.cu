@@ -1,7 +1,9 @@
 // Gated feed-forward block on tokens x [tokens, C]:
 //   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) u,  y = h Wd^T + bd          Wg, Wu [F, C], Wd [O, F]; act(g) = g s(g) (s: logistic) or g Phi(g) (Phi: normal distribution)
-// and its gradients
+// and, from g and u in 24 bits and h in bf16 (float32: in 32, h in parts), which the forward pass keeps, its gradients
 //   dh = dy Wd,  dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h,  and column sums of dg, du, dy for the biases.
+// bf16: sums are float32; h, dg and du are rounded to bf16 between the products, as the tensor cores take them (few tokens without gradients: h as two bf16 values).  With 24 bits of g and u
+// what gradients lose by them is below those roundings; 16 would put two more into each.
 #include <algorithm>
 
 #include "product_few.cuh"

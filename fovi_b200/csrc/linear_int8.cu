@@ -1,7 +1,8 @@
 // Product of 8-bit tokens with 8-bit weights:
 //   y[m, n] = scale[m] weight_scale[n] sum over k of q[m, k] w[n, k] + bias[n]
 // The sums are exact, in 32-bit integers; what follows is float32, rounded once to y's type.
-// Bound by the tensor cores' integer rate for many tokens, by the weights' bytes for few.
+// Bound by the tensor cores' integer rate and their operands' way through L2 for many tokens (16448 x 1280 -> 5120: 97 us, 2.2 P a second), by the weights' bytes for few (one token
+// 1280 -> 5120: 3.0 to 4.5 us for 6.6 MB).
 #include "product_few.cuh"
 #include "product_tc.cuh"
 

@@ -3,9 +3,10 @@
 // What bounds them is how fast the weights come: each is used by up to 16 tokens of a block.  A block takes 16 rows of w (GATED: of both matrices) and divides k among its warps in
 // turns of 64 bytes a row; a warp's loads are 16 bytes a lane, four lanes side by side in a row, straight into the registers that the matrix instruction (m16n8k16 or m16n8k32: weights
 // are its 16 rows, tokens its 8 columns) takes them from.  That an instruction's k then is not consecutive does not matter, since tokens are loaded the same way.
-// Two turns' loads are on their way while two are worked on (GATED: one and one, so that three
-// blocks fit an SM and 5120 rows are one round of them: 1280 x 5120 channels, one token, 39 MB of weights 15.1 -> 12.7 us from memory, 10.0 -> 8.4 us from L2).  The warps' sums are joined in shared memory in a fixed order, and a thread for each result ends it.
-// The tensor cores' large instructions (product_tc.cu) have 128 rows: with one token 5120 x 1280 8-bit weights take 8.8 us there.
+// Two turns' loads are on their way while two are worked on (GATED: one and one, so that three blocks fit an SM and 5120 rows are one round of them).  The warps' sums are joined in shared
+// memory in a fixed order, and a thread for each result ends it.
+// One token through 1280 x 5120 channels, 39 MB of weights: 13.3 us from memory (3.0 TB/s; 12.8 with h in one part), 8.4 from L2.
+// The tensor cores' large instructions (product_tc.cu) have 128 rows: with one token 5120 x 1280 8-bit weights take 8.8 us there, 3.0 to 4.5 here.
 #include <algorithm>
 
 #include "product_few.cuh"

@@ -5,10 +5,14 @@
 namespace fovi {
 
 // Whether these kernels take a block's forward pass, or an 8-bit product: always for one block of 16 tokens; beyond, the weights come from L2 once for each block of 16, and the tensor
-// cores' kernels, which take a fixed time at first, are the faster ones where that is longer.  Both sides measured (us, these / those): block of 384 x 1024 channels, 64, 128, 192 and
-// 256 tokens 5.5 / 10.3, 7.2 / 10.6, 8.9 / 10.5, 11.7 / 10.6; 768 x 2048, 64, 96, 128: 9.8 / 14.7, 12.1 / 14.4, 16.0 / 14.4; 1280 x 5120, 32, 48, 64: 17.3 / 20, 21.9 / 20.6, 28 / 19.
+// cores' kernels, which take a fixed time at first, are the faster ones where that is longer.  Both sides measured (us, these / those): block of 96 x 256 channels, 512 and 1024 tokens
+// 6.5 / 8.0, 9.9 / 8.0; 384 x 1024, 64, 128 and 192 tokens 6.4 / 10.3, 9.6 / 10.5, 11.6 / 10.5; 768 x 2048, 64 and 96: 13.0 / 14.6, 16.0 / 14.4; 1280 x 1280, 32 and 64: 10.4 / 16.9,
+// 14.9 / 14.1; 1280 x 5120, 16 and 32: 14.0 / 19.6, 22.2 / 19.3.
 // 8-bit 384 -> 1024, 64, 96, 128 tokens: 2.5 / 3.9, 3.3 / 4.0, 3.9 / 4.0; 1280 -> 5120, 32, 48: 6.0 / 6.5, 8.0 / 6.6; 5120 -> 1280, 64, 96: 7.5 / 9.0, 9.4 / 9.1.
-inline bool few_block(int64_t m, int64_t c, int64_t f, int64_t o) { return m <= 16 || (m <= 1024 && (m + 15) / 16 * f * (2 * c + o) / 3 <= 2000000 + 2700 * (c + f)); }
+inline bool few_block(int64_t m, int64_t c, int64_t f, int64_t o) {
+  const int64_t channels = c + f < 5000 ? c + f : 5000;
+  return m <= 16 || (m <= 1024 && (m + 15) / 16 * f * (2 * c + o) / 3 <= 700000 + 2000 * channels);
+}
 // A float32 block's, 8 tokens a block, against product_split.cu's: 1280 x 3416, 8 and 16 tokens 47 / 79 and 62 / 80, 32 tokens 118 / 81; 384 x 1024, 32 and 48 tokens 20 / 23 and 25 / 24.
 inline bool few_float(int64_t m, int64_t c, int64_t f, int64_t o) { return m <= 16 || (m <= 1024 && (m + 7) / 8 * f * (2 * c + o) / 3 <= 1600000); }
 inline bool few_eight(int64_t m, int64_t k, int64_t n) { return m <= 16 || (m <= 1024 && (m + 15) / 16 * n * (k + 1500) <= 10000000 + 7300 * k + 2000 * n); }

@@ -12,9 +12,13 @@
 //   GATED    accumulator columns of the first half are g, of the second u, since the first CTA stages rows of Wg and the second the same rows of Wu: h = act(g) u
 //   GRAD     the tile is dh; g and u are read, dg and du written
 //            Both move 8 and 10 bytes a hidden value, which is what bounds them where C is small, so their tiles go through shared memory as tensor copies, 32 rows x 32 columns of a warp at
-//            a time: with a row per thread in global memory every instruction touched 32 lines, and the load/store unit bound them (65792 x 384 x 1024: 227 and 293 us).
+//            a time: with a row per thread in global memory every instruction touched 32 lines, and the load/store unit bound them (65792 x 384 x 1024: 227 and 293 us, now 124 and 132:
+//            5.4 TB/s of theirs).
 //   STORE    bf16 result with a bias, or with k in parts a float32 part, joined by a second kernel in their order
 //   SCALED   integer sums times the scales
+// Where C is large the power limit bounds it: 16448 tokens, 1280 x 5120 channels, projections 1.30 PFLOP/s, down 1.32, input gradients 1.26, weight gradients 1.36 (from 1.2 to 1.3 sustained
+// for library products of these sizes), hidden gradients 0.95, whose tiles' arithmetic is longer than their products.  8-bit 16448 x 1280 -> 5120 in 97 us, 2.2 P a second: a stage's 64 KB
+// through L2 take as long as its products.
 #include <algorithm>
 
 #include "product_pair.cuh"

@@ -236,7 +236,7 @@ class _FeedForwardFunction(torch.autograd.Function):
 def gated_feed_forward(x, gate_weight, up_weight, down_weight, gate_bias=None, up_bias=None, down_bias=None, activation="silu"):
     """The gated feed-forward block of a transformer: (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd.  x [..., C], weights as torch's Linear has them (Wg, Wu [F, C], Wd [O, F]),
     biases [F], [F], [O] or None, all float32 or all bf16; activation "silu" or "gelu" (with the error function).  Differentiable in all tensors.  Sums are float32; with bf16 the
-    hidden values, and in the backward pass their gradients, are rounded to bf16 between the products.  Gradients are the same bits every time, whichever are asked for."""
+    hidden values, and in the backward pass their gradients, are rounded to bf16 between the products (few tokens without gradients: hidden values keep twice the bits).  Gradients are the same bits every time, whichever are asked for."""
     leaves = (x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias)
     if ops._native is not None and x.is_cuda and activation in ops.ACTIVATIONS:
         dev = ops._current_device()
