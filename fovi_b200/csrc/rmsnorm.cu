@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(1024) rms_norm_join_kernel(const float* part, 
 // ------------------------------------------------------------------------------------------------------------ rows in registers
 // A row is held in registers by a team of threads (rows.cuh), a warp or, where it is too long for one, a block; the next row's loads are issued before this row's sums.  One pass over memory
 // in both directions: the residual's sum, its norm and the 8-bit form with its scale come from the same registers, and the backward kernel keeps every column's part of dw over all its rows.
-// What bounds it is memory: 263168 x 384 bf16 with the residual 124 us forward (6.5 TB/s) and 151 backward (5.4), 65792 x 1280 into 8 bits 103 (5.7).
+// What bounds it is memory: 263168 x 384 bf16 with the residual 124 us forward (6.5 TB/s) and 129 to 151 backward (5.4 and more), 65792 x 1280 into 8 bits 101 (5.8).
 template <typename T, int VEC> __device__ __forceinline__ void store_eight(int8_t* p, const float* v, float inv) {
   if constexpr (VEC == 1) {
     p[0] = (int8_t)eight_bits(v[0], inv);
