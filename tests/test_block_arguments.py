@@ -92,10 +92,7 @@ def test_parts_of_a_float32_value():
     def parts(v):
         out = []
         for _ in range(3):
-            b = v.view(torch.int32)
-            up = b + 0x8000
-            b = torch.where((up & 0x7f800000) == 0x7f800000, b, up)
-            p = (b & -65536).view(torch.float32)
+            p = v.clamp(-torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).max).to(torch.bfloat16).float()      # rounded without leaving the range
             out.append(p)
             v = v - p
         assert not v.any()
@@ -106,7 +103,7 @@ def test_parts_of_a_float32_value():
     assert torch.equal(sum(a), x.double())
     six = sum(a[i] * b[j] for i in range(3) for j in range(3) if i + j < 3)
     whole = x.double() * x.flip(0).double()
-    far = (x.abs() > 3.39e38) | (x.flip(0).abs() > 3.39e38)                 # cut off, not rounded: a second part of up to 2^-7, a third of up to 2^-15 of the value
+    far = (x.abs() > 3.39e38) | (x.flip(0).abs() > 3.39e38)                 # cut off where rounding would leave the range: a second part of up to 2^-7, a third of up to 2^-15 of the value
     # |second| <= 2^-8, |third| <= 2^-17 of the value: left out are two products of a second and a third part, and one of two third ones
     assert ((six - whole).abs() <= torch.where(far, 2.0 ** -21, 2.0 ** -24 + 2.0 ** -33) * whole.abs()).all()
 
