@@ -275,3 +275,18 @@ def test_gradients_of_biases_are_rounded_once(M, C, F, activation):
         want = each.sum(0)
         assert ((got.double() - want).abs() <= 2 ** -8 * want.abs() + far * most.sum(0)).all()
     torch.testing.assert_close(dbd.double(), dy.double().sum(0), rtol=2 ** -8, atol=M * 2 ** -24 * dy.abs().sum(0).max().item())
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M", [4, 300])
+def test_infinity_stays_infinity(M, dtype, activation):
+    """Weights above zero: a token with infinity in it has an infinite result, with and without what a backward pass keeps; the others' are finite."""
+    from fovi_b200 import ops
+    leaves, _ = _inputs(M, 96, 200, 80, dtype, M, bias=False)
+    x, *weights = leaves[:4]
+    weights = [w.abs() + 0.125 for w in weights]
+    x[1, 5] = float("inf")
+    for saved in (False, True):
+        y, _ = ops.gated_feed_forward(x, *weights, activation=activation, want_saved=saved)
+        assert (y[1] == float("inf")).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all()
