@@ -244,7 +244,7 @@ BackWork back_work(const Block& b, int64_t pitch) {
   BackWork w;
   w.sums = padded(2 * b.M * pitch * 2);
   w.parts = w.sums + padded(fovi::tc_sum_rows(b.M) * 2 * pitch * 4);
-  w.bytes = w.parts + std::max({fovi::tc_linear_bytes(b.M, b.C, 2ll * b.F), fovi::tc_weight_grads_bytes(t, 3, b.M), (int64_t)STRIPS * b.O * 4});
+  w.bytes = w.parts + std::max({fovi::tc_linear_bytes(b.M, b.C, b.F, 2), fovi::tc_weight_grads_bytes(t, 3, b.M), (int64_t)STRIPS * b.O * 4});
   return w;
 }
 
@@ -341,7 +341,7 @@ extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int
   const int64_t extra = copies ? pads_bytes(tokens, C, F, O, phase == 1) : 0;
   if (phase == 1) return extra + back_work(b, pitch_of(F)).bytes;
   if (phase == 0 && fovi::few_block(tokens, C, F, O)) return extra + tokens * pitch_of(F) * 4;
-  return extra + (phase == 0 ? padded(tokens * pitch_of(F) * 2) : 0) + fovi::tc_linear_bytes(tokens, O, F);
+  return extra + (phase == 0 ? padded(tokens * pitch_of(F) * 2) : 0) + fovi::tc_linear_bytes(tokens, O, F, 1);
 }
 
 extern "C" int fovi_gated_ffn_forward(const void* x, int dtype, int64_t tokens, int C, int F, int O, int64_t x_stride, const void* gate_weight, int64_t gate_stride,

@@ -573,7 +573,10 @@ int fovi::split_hidden_grad(const SplitMatrix& dy, const SplitMatrix& wd, const 
   return act == ACT_SILU ? launch<GRAD, false, true, ACT_SILU>(maps, a, st) : launch<GRAD, false, true, ACT_GELU>(maps, a, st);
 }
 
-int64_t fovi::split_linear_bytes(int64_t m, int n, int64_t k, int segments) { return part_bytes(&m, &n, 1, shape_of(&m, &n, 1, segments * stages_of(k), 1, true).splits); }
+// As in product_tc.cu: one cut for a launch and for its workspace.
+static Shape linear_shape(int64_t m, int n, int64_t k, int segments) { return shape_of(&m, &n, 1, segments * stages_of(k), 1, true); }
+
+int64_t fovi::split_linear_bytes(int64_t m, int n, int64_t k, int segments) { return part_bytes(&m, &n, 1, linear_shape(m, n, k, segments).splits); }
 
 int fovi::split_linear(const SplitMatrix& am, const SplitMatrix& bm, const SplitMatrix* a2, const SplitMatrix* b2, bool b_mn, int m, int n, const float* bias, float* y, void* work,
                        cudaStream_t st) {
@@ -582,8 +585,7 @@ int fovi::split_linear(const SplitMatrix& am, const SplitMatrix& bm, const Split
   a.tasks = 1; a.m[0] = m; a.n[0] = n; a.y[0] = y;
   a.kb0 = (int)stages_of(am.cols);
   a.kb = a.kb0 * (a2 ? 2 : 1);
-  const int64_t m64 = m;
-  const Shape s = shape_of(&m64, &n, 1, a.kb, 1, true);
+  const Shape s = linear_shape(m, n, am.cols, a2 ? 2 : 1);
   a.ct = s.ct; a.splits = s.splits; a.work = static_cast<float*>(work); a.bias = bias;
   int rc = tiles_of(a, 1);
   if (!rc) rc = map_k(&maps.a[0], am, 128);

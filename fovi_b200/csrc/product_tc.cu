@@ -713,8 +713,11 @@ int fovi::tc_hidden_grad(const TcMatrix& dy, const TcMatrix& wd, const Hidden& f
   return act == ACT_SILU ? launch<GRAD, false, true, false, ACT_SILU>(maps, a, false, st) : launch<GRAD, false, true, false, ACT_GELU>(maps, a, false, st);
 }
 
-int64_t fovi::tc_linear_bytes(int64_t m, int n, int64_t k) {
-  const TcShape s = shape_of(&m, &n, 1, stages_of(k), 1, true);
+// The cut of y = A B^T over `segments` pairs of matrices of k each, every one in whole stages: what a launch takes and what its workspace is counted by.
+static TcShape linear_shape(int64_t m, int n, int64_t k, int segments) { return shape_of(&m, &n, 1, segments * stages_of(k), 1, true); }
+
+int64_t fovi::tc_linear_bytes(int64_t m, int n, int64_t k, int segments) {
+  const TcShape s = linear_shape(m, n, k, segments);
   return s.splits > 1 ? (int64_t)s.splits * m * ((n + 31) / 32 * 32) * 4 : 0;
 }
 
@@ -724,8 +727,7 @@ int fovi::tc_linear(const TcMatrix& am, const TcMatrix& bm, const TcMatrix* a2, 
   a.tasks = 1; a.m[0] = m; a.n[0] = n; a.y[0] = y;
   a.kb0 = (int)stages_of(am.cols);
   a.kb = a.kb0 * (a2 ? 2 : 1);
-  const int64_t m64 = m;
-  const TcShape s = shape_of(&m64, &n, 1, a.kb, 1, true);
+  const TcShape s = linear_shape(m, n, am.cols, a2 ? 2 : 1);
   a.ct = s.ct; a.splits = s.splits; a.work = static_cast<float*>(work); a.bias = bias;
   int rc = tiles_of(a, 1);
   if (!rc) rc = map_k(&maps.a[0], am, false, 128);

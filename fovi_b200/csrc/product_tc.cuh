@@ -19,8 +19,8 @@ int tc_gated(const TcMatrix& x, const TcMatrix& wg, const TcMatrix& wu, const vo
 // dg, du from dh = dy Wd and the saved g, u; with `sums` also the column sums of each 32 rows of dg and du, [ceil(rows / 32) to whole tiles][2][pitch].
 int tc_hidden_grad(const TcMatrix& dy, const TcMatrix& wd, const Hidden& from, int act, void* dg, void* du, float* sums, cudaStream_t st);
 int64_t tc_sum_rows(int64_t tokens);
-// y = A B^T + bias, bf16; k runs over a and b, then over a2 and b2 where there are any.  b_mn: B lies as [k, n].
-int64_t tc_linear_bytes(int64_t m, int n, int64_t k);
+// y = A B^T + bias, bf16; k runs over a and b, then over a2 and b2 where there are any (two segments of k each).  b_mn: B lies as [k, n].
+int64_t tc_linear_bytes(int64_t m, int n, int64_t k, int segments);
 int tc_linear(const TcMatrix& a, const TcMatrix& b, const TcMatrix* a2, const TcMatrix* b2, bool b_mn, int m, int n, const void* bias, void* y, void* work, cudaStream_t st);
 // Up to three products y = A^T B over the rows of A and B: weight gradients over `rows` tokens.  A task with y null is left out.
 int64_t tc_weight_grads_bytes(const TcTask* tasks, int n, int64_t rows);

@@ -1,0 +1,68 @@
+"""GPU: the gated feed-forward block where its sizes and values are at an edge: workspaces, infinities, large gates, hooks on what it saves."""
+import pytest
+import torch
+
+from oracle import block_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(autouse=True, params=["native", "python"])
+def launch_path(request, monkeypatch):
+    """Every test with the native launch path (csrc/bind_tokens.h) and with the Python one."""
+    from fovi_b200 import ops
+    assert ops._native is not None
+    if request.param == "python":
+        monkeypatch.setattr(ops, "_native", None)
+
+
+def _inputs(M, C, F, O, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    def n(*s, scale=1.0): return (torch.randn(*s, generator=g, device="cuda") * scale).to(dtype)
+    leaves = [n(M, C), n(F, C, scale=1.5 * C ** -0.5), n(F, C, scale=C ** -0.5), n(O, F, scale=F ** -0.5), n(F), n(F, scale=0.3), n(O, scale=0.3)]
+    return leaves, n(M, O)
+
+
+def _grads(leaves, dy, activation="silu"):
+    from fovi_b200 import tokens
+    for t in leaves:
+        t.requires_grad_(True)
+    y = tokens.gated_feed_forward(*leaves, activation=activation)
+    return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+
+# Hidden channels that leave 1 to 32 in their last 64: input gradients have one stage of k more in two pieces than in one.
+LAST = [(885, 384, 1736, 384), (532, 768, 2080, 768), (233, 1280, 2968, 1280), (300, 64, 961, 64)]
+
+
+@pytest.mark.autograd
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M,C,F,O", LAST)
+def test_gradients_of_uneven_hidden_channels(M, C, F, O, dtype):
+    leaves, dy = _inputs(M, C, F, O, dtype, M)
+    want = oracle.feed_forward(*[t.detach() for t in leaves], "silu", dy)
+    for g, w in zip(_grads(leaves, dy), want, strict=True):
+        oracle.near(g, w)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M,C,F,O", LAST + [(40, 96, 1000, 96), (5, 384, 1021, 384)])
+def test_nothing_is_written_behind_the_workspace(monkeypatch, M, C, F, O, dtype):
+    from fovi_b200 import ops
+    made, plain = [], ops._ffn_work
+
+    def with_a_tail(*args):
+        size, _ = plain(*args)
+        made.append((size, torch.full((size + 65536,), 0xA5, dtype=torch.uint8, device="cuda")))
+        return made[-1]
+    monkeypatch.setattr(ops, "_ffn_work", with_a_tail)
+    leaves, dy = _inputs(M, C, F, O, dtype, M)
+    ops.gated_feed_forward(*leaves)
+    _, saved = ops.gated_feed_forward(*leaves, want_saved=True)
+    ops.gated_feed_forward_backward(*leaves[:4], saved, dy)
+    for need in range(7):
+        ops.gated_feed_forward_backward(*leaves[:4], saved, dy, need=[j == need for j in range(7)])
+    assert len(made) == 10
+    for size, work in made:
+        assert (work[size:] == 0xA5).all()
