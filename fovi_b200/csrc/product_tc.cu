@@ -103,18 +103,19 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 // act(g) and act'(g) of two values, to a few units of float32: what is rounded to bf16 behind them.  The logistic function takes an exponential each and one reciprocal for both,
 // 1/a = b/(ab), since those units are what bounds a tile's arithmetic.  Exponents are cut at 2^60, so that the product stays finite, and the factor g with them, at -60 ln 2: from there on
-// value and slope stand still, at -4e-17.  The exponent's cut drops what is not a number, as the pair shares its reciprocal; the factor's keeps it.
+// value and slope stand still, at -4e-17.  In the slope p + a (1 - p) the last factor is exp(-g) p: from p itself it would be its error, 2^-23, which a gate of 1e5 and more makes
+// a slope of.  The exponent's cut drops what is not a number, as the pair shares its reciprocal; the factor's keeps it.
 template <int ACT> __device__ __forceinline__ float2 act_pair(float2 g, float2* slope) {
   if (ACT == fovi::ACT_SILU) {
     const float2 x = mul2(g, both(-1.4426950408889634f));
-    float2 e;
+    float2 q;
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(x.x, 60.f)));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(x.y, 60.f)));
-    e = add2(e, both(1.f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q.x) : "f"(fminf(x.x, 60.f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q.y) : "f"(fminf(x.y, 60.f)));
+    const float2 e = add2(q, both(1.f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e.x * e.y));
     const float2 p = mul2(both(r), make_float2(e.y, e.x)), a = mul2(make_float2(max_nan(g.x, -41.588831f), max_nan(g.y, -41.588831f)), p);
-    if (slope) *slope = fma2(a, fma2(p, both(-1.f), both(1.f)), p);
+    if (slope) *slope = fma2(a, mul2(q, p), p);
     return a;
   }
   const float2 x = mul2(g, both(0.70710678118654752f));

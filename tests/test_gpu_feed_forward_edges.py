@@ -66,3 +66,31 @@ def test_nothing_is_written_behind_the_workspace(monkeypatch, M, C, F, O, dtype)
     assert len(made) == 10
     for size, work in made:
         assert (work[size:] == 0xA5).all()
+
+
+@pytest.mark.autograd
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M", [1, 3, 300])
+def test_slope_of_large_gates(M, dtype, activation):
+    """The slope is one there, whatever the hidden channel beside it has for its gate, and the value the gate itself."""
+    F = 128
+    x = torch.ones(M, F, device="cuda", dtype=dtype)
+    zero, eye = torch.zeros(F, F, device="cuda", dtype=dtype), torch.eye(F, device="cuda", dtype=dtype)
+    wu = zero.clone()
+    wu[:, 0] = 1
+    large = 2.0 ** torch.arange(5, 5 + F // 2, device="cuda")                # 32 to 2^68
+    gate = torch.stack([large, torch.linspace(-3, 5, F // 2, device="cuda")], 1).flatten().to(dtype)
+    leaves = [x, zero, wu, eye, gate, None, None]
+    for t in leaves[:5]:
+        t.requires_grad_(True)
+    from fovi_b200 import tokens
+    y = tokens.gated_feed_forward(*leaves, activation=activation)
+    dbg, = torch.autograd.grad(y, gate, torch.ones_like(y))
+    g = gate.detach().double().requires_grad_(True)
+    h = torch.nn.functional.silu(g) if activation == "silu" else torch.nn.functional.gelu(g)
+    slope, = torch.autograd.grad(h.sum(), g)
+    # bf16: a rounding each of h and y, and of dg and the bias's gradient, and the gate to 2^-16, which moves a slope of up to 1.13 by no more than 2^-16 |g| of the small ones; else float32's
+    near = dict(rtol=2 ** -7 + 2 ** -11, atol=2 ** -12) if dtype is BF else dict(rtol=2 ** -19, atol=2 ** -20)
+    torch.testing.assert_close(y.detach().double(), h.detach().expand(M, F), **near)
+    torch.testing.assert_close(dbg.double(), M * slope, rtol=near["rtol"], atol=M * near["atol"])
