@@ -8,7 +8,7 @@ namespace fovi {
 
 enum { ACT_SILU = 0, ACT_GELU = 1 };
 
-// What a bf16 gated projection writes: h = act(g) u and, for the backward pass, g and u as the upper 24 of their 32 bits, 16 in one tensor and 8 in another: as bf16 their rounding would be
+// What a bf16 gated projection writes: h = act(g) u and, for the backward pass, g and u rounded to the upper 24 of their 32 bits, 16 in one tensor and 8 in another: as bf16 their rounding would be
 // a third one in every gradient (0.0034 off in place of 0.0023, of which 0.0017 is a result's own rounding).
 struct Hidden {
   void* h;                       // [tokens, pitch]

@@ -127,6 +127,9 @@ template <int ACT> __device__ __forceinline__ float2 act_pair(float2 g, float2* 
   return mul2(g, p);
 }
 
+// A value whose upper 24 bits are it, rounded: infinity and not-a-number stay what they are, and finite values from the largest of 24 bits on (0x1.fffep127) finite.
+__device__ __forceinline__ uint32_t upper24(uint32_t v) { return fabsf(__uint_as_float(v)) < 0x1.fffep127f ? v + 0x80u : v; }
+
 // Sums of 32 columns over the lanes, a column at a time: column c's value of every lane goes in, and after the last the sum of column `lane` comes out.  Two neighbours' sums are halved at
 // each level: a lane keeps the one whose number has its bit.  31 exchanges in all, in a fixed order.
 struct ColumnSums {
@@ -377,7 +380,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
           if (a.hidden.high) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-              const uint32_t* v = m ? u : g;
+              uint32_t v[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = upper24(m ? u[i] : g[i]);
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 put16(place + at128(lane, 4 * m + i), __byte_perm(v[8 * i], v[8 * i + 1], 0x7632), __byte_perm(v[8 * i + 2], v[8 * i + 3], 0x7632),
@@ -435,8 +440,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
             for (int j = 0; j < 2; ++j) {
               const int e = 2 * i + j;
               const uint32_t pick = (j ? 0x3244u : 0x1044u) + ((uint32_t)(e & 3) << 4);      // [two high bytes, low byte, any]
-              g[j] = __uint_as_float((__byte_perm(gu[i], lo[e / 4], pick) & 0xffffff00u) | 0x80u);
-              u[j] = __uint_as_float((__byte_perm(gu[16 + i], lo[8 + e / 4], pick) & 0xffffff00u) | 0x80u);
+              g[j] = __uint_as_float(__byte_perm(gu[i], lo[e / 4], pick) & 0xffffff00u);
+              u[j] = __uint_as_float(__byte_perm(gu[16 + i], lo[8 + e / 4], pick) & 0xffffff00u);
             }
             float2 d;
             const float2 dh = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), v = mul2(dh, act_pair<ACT>(make_float2(g[0], g[1]), &d));

@@ -94,3 +94,63 @@ def test_slope_of_large_gates(M, dtype, activation):
     near = dict(rtol=2 ** -7 + 2 ** -11, atol=2 ** -12) if dtype is BF else dict(rtol=2 ** -19, atol=2 ** -20)
     torch.testing.assert_close(y.detach().double(), h.detach().expand(M, F), **near)
     torch.testing.assert_close(dbg.double(), M * slope, rtol=near["rtol"], atol=M * near["atol"])
+
+
+def _by_definition(x, wg, wu, wd, bg, bu, bd, activation, dy):
+    """Result and gradients in 64 bits, infinities and all, on the CPU."""
+    x, wg, wu, wd, bg, bu, bd, dy = (t.detach().double().cpu() for t in (x, wg, wu, wd, bg, bu, bd, dy))
+    g, u = x @ wg.T + bg, x @ wu.T + bu
+    if activation == "silu":
+        p = torch.sigmoid(g)
+        slope = p * (1 + g * (1 - p))
+    else:
+        p = 0.5 * torch.erfc(-g / 2 ** 0.5)
+        slope = p + g * torch.exp(-g * g / 2) / (2 * torch.pi) ** 0.5
+    a = g * p
+    h, dh = a * u, dy @ wd
+    dg, du = dh * u * slope, dh * a
+    return h @ wd.T + bd, dg @ wg + du @ wu, dg.T @ x, du.T @ x, dy.T @ h, dg.sum(0), du.sum(0), dy.sum(0)
+
+
+@pytest.mark.autograd
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("where", ["gate", "up"])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M", [1, 2, 300])
+def test_infinity_in_the_gradients(M, dtype, value, where, activation):
+    """A hidden channel that is infinite, or not a number: results and gradients are so exactly where the definition's are.  Tokens and the gradient of the result are positive, so that a
+    gradient that sums infinities of one sign over the tokens stays infinite.  (The gate at -infinity is left out: the definition has 0 times infinity there.)"""
+    if where == "gate" and value == -float("inf"):
+        return
+    leaves, dy = _inputs(M, 40, 100, 24, dtype, 3)
+    leaves[0], dy = leaves[0].abs() + 0.125, dy.abs() + 0.125
+    leaves[3] = leaves[3].abs() + 0.125
+    leaves[4 if where == "gate" else 5][37] = value
+    want = _by_definition(*leaves, activation, dy)
+    infinite = 0
+    for got, w in zip(_grads(leaves, dy, activation), want, strict=True):
+        got, w = got.cpu().double(), w.to(dtype).double()
+        assert torch.equal(got.isnan(), w.isnan())
+        assert torch.equal(got.isinf(), w.isinf()) and torch.equal(got[w.isinf()], w[w.isinf()])
+        infinite += w.isinf().sum().item()
+    assert value != value or infinite >= 80
+
+
+@pytest.mark.autograd
+def test_the_largest_hidden_values():
+    """Gates and up values near bf16's and float32's largest stay finite in what is kept for the backward pass."""
+    from fovi_b200 import ops
+    leaves, dy = _inputs(2, 8, 64, 8, BF, 5)
+    x, wg, wu, wd = (torch.zeros_like(t) for t in leaves[:4])
+    x[:, 0], wu[:, 0], wg[:, 1] = 1, 3.3895313892515355e38, 0
+    x[:, 1], wu[:, 1] = 1, 1.3e36                                    # their sum: above bf16's largest value, below float32's
+    wd[0, :] = 2.0 ** -126
+    gate = torch.full((64,), 2.0, device="cuda", dtype=BF)
+    _, saved = ops.gated_feed_forward(x, wg, wu, wd, gate, None, None, want_saved=True)
+    grads = ops.gated_feed_forward_backward(x, wg, wu, wd, saved, torch.ones_like(dy))
+    u, g = x.double() @ wu.double().T, gate.double()
+    s = torch.sigmoid(g)
+    dg = 2.0 ** -126 * u * s * (1 + g * (1 - s))
+    # u kept to 2^-15, dg rounded to bf16, the sum of two tokens rounded once more
+    torch.testing.assert_close(grads[4].double(), dg.sum(0), rtol=2 ** -7, atol=0)
