@@ -337,6 +337,7 @@ extern "C" int64_t fovi_gated_ffn_workspace_bytes(int dtype, int64_t tokens, int
   phase &= 3;
   Block b{};
   b.M = tokens; b.C = C; b.F = F; b.O = O;
+  if (dtype == FOVI_F32 && phase == 0 && fovi::few_float(tokens, C, F, O)) return tokens * pitch_of(F) * 4;
   if (dtype == FOVI_F32) return phase == 1 ? split_backward_at(b, SplitMatrix{}, nullptr).bytes : split_forward_at(b, phase == 2, nullptr).bytes;
   const int64_t extra = copies ? pads_bytes(tokens, C, F, O, phase == 1) : 0;
   if (phase == 1) return extra + back_work(b, pitch_of(F)).bytes;

@@ -59,3 +59,25 @@ def test_backward(dtype):
     for sizes in NAMED + last + any_size:
         have, need = lib.fovi_gated_ffn_workspace_bytes(dtype, *sizes, 1), _backward(dtype, *sizes)
         assert have >= need, (sizes, have, need)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("tokens", [1, 7, 16])
+def test_few_tokens_want_room_for_their_hidden_values_only(dtype, tokens):
+    """Float32 hidden values, or two bf16 parts of each; the weights are read where they lie."""
+    from fovi_b200._lib import lib
+    for C, F, O in ((1280, 5120, 1280), (384, 1021, 384), (8, 40, 24)):
+        assert lib.fovi_gated_ffn_workspace_bytes(dtype, tokens, C, F, O, 0) == tokens * _up(F, 32) * 32 * 4
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_forward(dtype):
+    """Of many tokens: h (float32: where it is not kept; and the operands, in three parts each), then the parts of the result."""
+    from fovi_b200._lib import lib
+    for M, C, F, O in NAMED + [(2000, 40, 65, 7), (4000, 384, 1021, 384), (16448, 1280, 5120, 1280), (5000, 1, 1, 1)]:
+        if M <= 1024:
+            continue
+        parts, pitch = _parts([(M, O)], _up(F, 64), dtype == 0), _up(F, 32) * 32
+        cut = sum(_padded(6 * rows * _up(cols, 8) * 8) for rows, cols in ((M, C), (F, C), (F, C), (O, F))) if dtype == 0 else 0
+        for phase, h in ((0, _padded((6 if dtype == 0 else 2) * M * pitch)), (2, 0)):
+            assert lib.fovi_gated_ffn_workspace_bytes(dtype, M, C, F, O, phase) >= cut + h + parts
