@@ -67,16 +67,23 @@ bool needs_graph(const at::Tensor& a, const at::Tensor* b = nullptr, const at::T
 // A tensor with a tangent: the Python path names the derivative that is not built, where this one would lose it.
 bool has_tangent(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
 at::Tensor or_none(const at::Tensor* t) { return t ? *t : at::Tensor(); }
+// What a node keeps goes through SavedVariable, so that hooks on saved tensors (offloading, checkpoints) see all of it.  A tensor that only the node made is held to what it was, as the
+// kernels take its size and type on trust.
+at::Tensor kept(const SavedVariable& s, at::ScalarType type, int64_t n, const at::Tensor& beside) {
+  const at::Tensor t = s.unpack();
+  TORCH_CHECK(t.defined() && t.scalar_type() == type && t.numel() == n && t.device() == beside.device() && t.is_contiguous(),
+              "a saved-tensor hook did not return the tensor that it was given");
+  return t;
+}
 
 // ------------------------------------------------------------------------------------------------------------ layer norm
 struct LayerNormNode : Node {
-  SavedVariable x, w;
-  at::Tensor stats;
+  SavedVariable x, w, stats;
   at::DimVector shape[2];                // of the weight and the bias: C values, in whatever shape
   std::string name() const override { return "FoviLayerNormBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    x.reset_data(); w.reset_data(); stats.reset();
+    x.reset_data(); w.reset_data(); stats.reset_data();
   }
   variable_list apply(variable_list&& in) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -89,6 +96,7 @@ struct LayerNormNode : Node {
       const at::Tensor g = in[0].contiguous();
       const int64_t C = xv.size(-1), rows = xv.numel() / C;
       const int dev = xv.get_device();
+      const at::Tensor st = kept(stats, at::kFloat, 2 * rows, xv);
       if (task_should_compute_output(0)) out[0] = fresh(xv.sizes(), xv.scalar_type(), dev);
       for (int i = 1; i < 3; ++i)
         if (task_should_compute_output(i)) out[i] = fresh(shape[i - 1], at::kFloat, dev);
@@ -96,7 +104,7 @@ struct LayerNormNode : Node {
       const int64_t bytes = sums ? tok.norm_work(rows, (int)C) : 0;
       const at::Tensor work = sums ? fresh({bytes}, at::kByte, dev) : at::Tensor();
       launched(tok.norm_back(xv.const_data_ptr(), code_of(xv.scalar_type()), rows, (int)C, C, g.const_data_ptr(), code_of(g.scalar_type()), C,
-                             wv.defined() ? wv.const_data_ptr<float>() : nullptr, stats.const_data_ptr<float>(), out_ptr(out[0]), (float*)out_ptr(out[1]),
+                             wv.defined() ? wv.const_data_ptr<float>() : nullptr, st.const_data_ptr<float>(), out_ptr(out[0]), (float*)out_ptr(out[1]),
                              (float*)out_ptr(out[2]), out_ptr(work), bytes, stream_of(xv)),
                "fovi_layer_norm_backward");
     }
@@ -137,7 +145,7 @@ BODY(layer_norm, 6)
       node->w = SavedVariable(or_none(w), false);
       if (w) node->shape[0] = w->sizes();
       if (b) node->shape[1] = b->sizes();
-      node->stats = stats;
+      node->stats = SavedVariable(stats, false);
       torch::autograd::set_history(y, node);
     }
   }
@@ -235,13 +243,12 @@ bool rows_plain(const at::Tensor& t) {
 void put_strides(int64_t* s, const at::Tensor& t) { for (int i = 0; i < 3; ++i) s[i] = t.stride(i); }
 
 struct AttentionNode : Node {
-  SavedVariable q, k, v, o, lengths, mask;
-  at::Tensor lse;
+  SavedVariable q, k, v, o, lse, lengths, mask;
   float scale = 0.f;
   std::string name() const override { return "FoviAttentionBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    q.reset_data(); k.reset_data(); v.reset_data(); o.reset_data(); lengths.reset_data(); mask.reset_data(); lse.reset();
+    q.reset_data(); k.reset_data(); v.reset_data(); o.reset_data(); lse.reset_data(); lengths.reset_data(); mask.reset_data();
   }
   variable_list apply(variable_list&& in) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -257,13 +264,14 @@ struct AttentionNode : Node {
       at::Tensor dv;
       if (task_should_compute_output(1)) out[1] = fresh(kv.sizes(), kv.scalar_type(), dev);
       if (out[1].defined() || task_should_compute_output(2)) dv = fresh(kv.sizes(), kv.scalar_type(), dev);
+      const at::Tensor ls = kept(lse, at::kFloat, (int64_t)B * H * Lq, qv);
       const int64_t bytes = tok.attend_work(type, B, Lq, Lk, H, Hkv, D, 1);
       const at::Tensor work = fresh({bytes}, at::kByte, dev);
       int64_t s[12];
       put_strides(s, qv); put_strides(s + 3, kv); put_strides(s + 6, vv); put_strides(s + 9, g);
       launched(tok.attend_back(qv.const_data_ptr(), kv.const_data_ptr(), vv.const_data_ptr(), ov.const_data_ptr(), g.const_data_ptr(), type, B, Lq, Lk, H, Hkv, D, s,
                                len.defined() ? len.const_data_ptr<int32_t>() : nullptr, mk.defined() ? (const uint8_t*)mk.const_data_ptr() : nullptr, scale,
-                               lse.const_data_ptr<float>(), out_ptr(out[0]), out_ptr(out[1]), out_ptr(dv), work.mutable_data_ptr(), bytes, stream_of(qv)),
+                               ls.const_data_ptr<float>(), out_ptr(out[0]), out_ptr(out[1]), out_ptr(dv), work.mutable_data_ptr(), bytes, stream_of(qv)),
                "fovi_attention_backward");
       if (task_should_compute_output(2)) out[2] = dv;
     }
@@ -313,7 +321,7 @@ BODY(attention, 8)
       node->set_next_edges(torch::autograd::collect_next_edges(*q, *k, *s));
       node->q = SavedVariable(*q, false); node->k = SavedVariable(*k, false); node->v = SavedVariable(*s, false);
       node->lengths = SavedVariable(or_none(len), false); node->mask = SavedVariable(or_none(mask), false);
-      node->lse = lse; node->scale = (float)scale;
+      node->lse = SavedVariable(lse, false); node->scale = (float)scale;
       torch::autograd::set_history(o, node);
       node->o = SavedVariable(o, true);
     }
@@ -333,14 +341,13 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> all) {
 }
 
 struct RmsNormNode : Node {                // inputs x, weight, residual; outputs y and, with a residual, the sum
-  SavedVariable t, w;
-  at::Tensor rstd;
+  SavedVariable t, w, rstd;
   at::DimVector shape;
   bool sum = false;                        // t is the second output
   std::string name() const override { return "FoviRmsNormBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    t.reset_data(); w.reset_data(); rstd.reset();
+    t.reset_data(); w.reset_data(); rstd.reset_data();
   }
   variable_list apply(variable_list&& in) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -358,12 +365,13 @@ struct RmsNormNode : Node {                // inputs x, weight, residual; output
       const at::Tensor g = in[0].to(type).contiguous(), d = own.defined() ? own.to(type).contiguous() : at::Tensor();
       const int64_t C = tv.size(-1), rows = tv.numel() / C;
       const int dev = tv.get_device();
+      const at::Tensor rs = kept(rstd, at::kFloat, rows, tv);
       const at::Tensor dx = task_should_compute_output(0) || task_should_compute_output(2) ? fresh(tv.sizes(), type, dev) : at::Tensor();
       if (task_should_compute_output(1)) out[1] = fresh(shape, at::kFloat, dev);
       const int64_t bytes = out[1].defined() ? tok.rms_work(rows, (int)C) : 0;
       const at::Tensor work = bytes ? fresh({bytes}, at::kByte, dev) : at::Tensor();
       launched(tok.rms_back(tv.const_data_ptr(), code_of(type), rows, (int)C, C, g.const_data_ptr(), C, d.defined() ? d.const_data_ptr() : nullptr, C,
-                            wv.defined() ? wv.const_data_ptr<float>() : nullptr, rstd.const_data_ptr<float>(), out_ptr(dx), (float*)out_ptr(out[1]), out_ptr(work), bytes,
+                            wv.defined() ? wv.const_data_ptr<float>() : nullptr, rs.const_data_ptr<float>(), out_ptr(dx), (float*)out_ptr(out[1]), out_ptr(work), bytes,
                             stream_of(tv)),
                "fovi_rms_norm_backward");
       if (task_should_compute_output(0)) out[0] = dx;
@@ -418,7 +426,7 @@ BODY(rms_norm, 6)
       node->set_next_edges(torch::autograd::collect_next_edges(*a.x, or_none(a.w), or_none(a.res)));
       node->w = SavedVariable(or_none(a.w), false);
       if (a.w) node->shape = a.w->sizes();
-      node->rstd = rstd;
+      node->rstd = SavedVariable(rstd, false);
       node->sum = a.res != nullptr;
       torch::autograd::set_history(y, node);
       if (a.res) torch::autograd::set_history(total, node);
@@ -528,14 +536,13 @@ int ffn_flag(std::initializer_list<const at::Tensor*> all) {
 }
 
 struct FeedForwardNode : Node {            // inputs x, gate, up and down weights, their biases
-  SavedVariable t[4];
-  at::Tensor saved;
+  SavedVariable t[4], saved;
   int act = 0;
   std::string name() const override { return "FoviGatedFeedForwardBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     for (auto& s : t) s.reset_data();
-    saved.reset();
+    saved.reset_data();
   }
   variable_list apply(variable_list&& in) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -547,7 +554,7 @@ struct FeedForwardNode : Node {            // inputs x, gate, up and down weight
       const at::ScalarType type = x.scalar_type();
       const int64_t C = wg.size(1), F = wg.size(0), O = wd.size(0), M = x.numel() / C;
       const int dev = x.get_device();
-      const at::Tensor g = in[0].to(type).contiguous();
+      const at::Tensor g = in[0].to(type).contiguous(), hidden = kept(saved, at::kByte, tok.ffn_saved(code_of(type), M, (int)F), x);
       const at::DimVector vf{F}, vo{O};
       const at::IntArrayRef shape[7] = {x.sizes(), wg.sizes(), wu.sizes(), wd.sizes(), vf, vf, vo};
       for (int i = 0; i < 7; ++i)
@@ -555,7 +562,7 @@ struct FeedForwardNode : Node {            // inputs x, gate, up and down weight
       const int64_t bytes = tok.ffn_work(code_of(type), M, (int)C, (int)F, (int)O, 1 | ffn_flag({&x, &wg, &wu, &wd, &g}));
       const at::Tensor work = fresh({bytes}, at::kByte, dev);
       launched(tok.ffn_back(x.const_data_ptr(), code_of(type), M, (int)C, (int)F, (int)O, C, wg.const_data_ptr(), C, wu.const_data_ptr(), C, wd.const_data_ptr(), F, act,
-                            saved.const_data_ptr(), g.const_data_ptr(), O, out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]), out_ptr(out[3]), out_ptr(out[4]), out_ptr(out[5]),
+                            hidden.const_data_ptr(), g.const_data_ptr(), O, out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]), out_ptr(out[3]), out_ptr(out[4]), out_ptr(out[5]),
                             out_ptr(out[6]), work.mutable_data_ptr(), bytes, stream_of(x)),
                "fovi_gated_ffn_backward");
     }
@@ -605,7 +612,7 @@ BODY(gated_feed_forward, 10)
       std::shared_ptr<FeedForwardNode> node(new FeedForwardNode(), torch::autograd::deleteNode);
       node->set_next_edges(torch::autograd::collect_next_edges(x, wg, wu, wd, or_none(t[4]), or_none(t[5]), or_none(t[6])));
       for (int i = 0; i < 4; ++i) node->t[i] = SavedVariable(*t[i], false);
-      node->saved = saved;
+      node->saved = SavedVariable(saved, false);
       node->act = (int)act;
       torch::autograd::set_history(y, node);
     }
