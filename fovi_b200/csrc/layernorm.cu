@@ -351,19 +351,13 @@ template <typename TX, typename TY> struct Run {
     if (!backward) {
       auto k = layer_norm_rows_kernel<TX, TY, VEC, CH, BLOCK>;
       const int64_t want = BLOCK ? rows : (rows + 7) / 8;
-      k<<<(int)std::min(want, resident<VEC, CH, BLOCK>(k, threads)), threads, 0, st>>>((const TX*)x, rows, C, stride, w, b, eps, (TY*)y, (float2*)stats);
+      static std::atomic<int> known[33];
+      k<<<(int)std::min(want, resident(k, threads, 0, known[threads / 32])), threads, 0, st>>>((const TX*)x, rows, C, stride, w, b, eps, (TY*)y, (float2*)stats);
       return fovi::after_launch("layer_norm_rows_kernel");
     }
     auto k = layer_norm_grad_rows_kernel<TX, TY, VEC, CH, BLOCK>;
     k<<<grad_blocks(s, rows), threads, BLOCK ? 0 : 2 * C * sizeof(float), st>>>((const TX*)x, rows, C, stride, (const TY*)dy, dy_stride, w, (const float2*)stats, (TX*)dx, part);
     return fovi::after_launch("layer_norm_grad_rows_kernel");
-  }
-  // As many blocks as are on the SMs at once: every team then takes the same number of rows.
-  template <int VEC, int CH, bool BLOCK, typename Kernel> static int64_t resident(Kernel k, int threads) {
-    static int per_sm[33] = {};
-    int& n = per_sm[threads / 32];
-    if (!n && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, threads, 0) != cudaSuccess || n < 1)) n = 1;
-    return (int64_t)fovi::sm_count() * n;
   }
   template <int VEC, int MOST, int STEP = 1, int CH = STEP> int warp(const Shape& s, bool backward) const {
     if constexpr (CH * VEC <= MOST) return s.ch == CH ? go<VEC, CH, false>(s, backward) : warp<VEC, MOST, STEP, CH + STEP>(s, backward);

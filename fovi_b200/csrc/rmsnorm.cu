@@ -391,21 +391,15 @@ template <typename T, typename F> int with(const Shape& s, const F& f) {
   return FOVI_ERR_UNSUPPORTED;
 }
 
-// As many blocks as the SMs hold at once, at most what the rows need: every team then takes the same number of rows.
-template <typename Kernel> int64_t resident(Kernel k, int threads, size_t smem, int* known) {
-  if (!*known && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(known, k, threads, smem) != cudaSuccess || *known < 1)) *known = 1;
-  return (int64_t)fovi::sm_count() * *known;
-}
-
 template <typename T, int FORM> int rows_forward(const RmsArgs& a, const Shape& s, cudaStream_t st) {
   return with<T>(s, [&](auto vec, auto ch, auto block) {
-    auto go = [&](auto kernel, int* known) {
+    auto go = [&](auto kernel, std::atomic<int>* known) {
       const int threads = s.block ? s.threads : 256;
       const int64_t want = s.block ? a.rows : (a.rows + 7) / 8;
-      kernel<<<(int)std::min(want, resident(kernel, threads, 0, known + threads / 32)), threads, 0, st>>>(a);
+      kernel<<<(int)std::min(want, resident(kernel, threads, 0, known[threads / 32])), threads, 0, st>>>(a);
       return fovi::after_launch("rms_norm_rows_kernel");
     };
-    static int known[2][33] = {};
+    static std::atomic<int> known[2][33];
     if constexpr (FORM != ROWS) {
       if (a.res) return go(rms_norm_rows_kernel<T, decltype(vec)::value, decltype(ch)::value, decltype(block)::value, true, FORM>, known[1]);
     }
@@ -434,12 +428,12 @@ template <typename T> int backward(const RmsGradArgs& a, float* dw, cudaStream_t
   int parts = strips_of(a.rows);
   if (s.threads) {
     const int rc = with<T>(s, [&](auto vec, auto ch, auto block) {
-      static int known[33] = {};
+      static std::atomic<int> known[33];
       auto kernel = rms_norm_grad_rows_kernel<T, decltype(vec)::value, decltype(ch)::value, decltype(block)::value>;
       const int threads = s.block ? s.threads : 256;
       const size_t smem = s.block ? 0 : a.C * sizeof(float);
       const int64_t want = s.block ? a.rows : (a.rows + 7) / 8;
-      parts = (int)std::min({want, resident(kernel, threads, smem, known + threads / 32), (int64_t)GRAD_BLOCKS});
+      parts = (int)std::min({want, resident(kernel, threads, smem, known[threads / 32]), (int64_t)GRAD_BLOCKS});
       kernel<<<parts, threads, smem, st>>>(a);
       return fovi::after_launch("rms_norm_grad_rows_kernel");
     });

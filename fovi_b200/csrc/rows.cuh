@@ -4,6 +4,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
+#include "common.cuh"
 #include "pairs.cuh"
 
 namespace {
@@ -72,6 +75,16 @@ template <int VEC, bool BLOCK> struct Team {
 
 // Threads of the largest block: single values take more instructions and more registers.
 template <int VEC> constexpr int BLOCK_MOST = VEC == 1 ? 512 : 1024;
+
+// As many blocks as the SMs hold at once: every team then takes the same number of rows.  `known`: the answer for one SM, which threads that ask at once all store.
+template <typename Kernel> int64_t resident(Kernel k, int threads, size_t smem, std::atomic<int>& known) {
+  int n = known.load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, threads, smem) != cudaSuccess || n < 1) n = 1;
+    known.store(n, std::memory_order_relaxed);
+  }
+  return (int64_t)fovi::sm_count() * n;
+}
 
 // Values two by two, for the instructions that take two.
 template <int E> struct Pairs {
