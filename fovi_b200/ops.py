@@ -1016,10 +1016,11 @@ def _ffn_inputs(x, gate_weight, up_weight, down_weight, biases, activation):
 
 
 def _ffn_work(dt, m, c, F, o, phase, rows, dev):
-    """Work of a feed-forward call: its bytes, and a tensor or None."""
+    """Work of a feed-forward call: its bytes, which depend on the device's SMs, and a tensor or None."""
     if dt == BF16 and any(t.data_ptr() % 16 or s % 8 or s == 0 for t, s in rows):
         phase |= 4                                       # FOVI_FFN_UNALIGNED: room for copies
-    size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, phase)
+    with _on(dev):
+        size = lib.fovi_gated_ffn_workspace_bytes(dt, m, c, F, o, phase)
     return size, torch.empty(size, dtype=torch.uint8, device=dev) if size else None
 
 
@@ -1148,9 +1149,9 @@ def attention(q, k, v, key_lengths=None, key_mask=None, scale=None, want_lse=Fal
     dev, dt = q.device, _dt(q.dtype)
     o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=dev) if want_lse else None
-    size = lib.fovi_attention_workspace_bytes(dt, *dims, 0)
-    work = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
     with _on(dev):
+        size = lib.fovi_attention_workspace_bytes(dt, *dims, 0)
+        work = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
         check(lib.fovi_attention_forward(_ptr(q), _ptr(k), _ptr(v), dt, *dims, _I64x9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
                                          None if lengths is None else _ptr(lengths), None if mask is None else _ptr(mask), scale, _ptr(o),
                                          None if lse is None else _ptr(lse), None if work is None else _ptr(work), size, _stream()), "fovi_attention_forward")
@@ -1171,9 +1172,9 @@ def attention_backward(q, k, v, o, grad, lse, key_lengths=None, key_mask=None, s
     grad = _rows_for_copies(grad)
     dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev) if need[0] else None
     dk, dv = (torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev) if m else None for m in (need[1], need[1] or need[2]))
-    size = lib.fovi_attention_workspace_bytes(dt, *dims, 1)
-    work = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
     with _on(dev):
+        size = lib.fovi_attention_workspace_bytes(dt, *dims, 1)
+        work = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
         check(lib.fovi_attention_backward(_ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(grad), dt, *dims,
                                           _I64x12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *grad.stride()[:3]),
                                           None if lengths is None else _ptr(lengths), None if mask is None else _ptr(mask), scale, _ptr(lse),
