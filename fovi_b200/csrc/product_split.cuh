@@ -7,7 +7,6 @@ namespace fovi {
 // A float32 matrix in three bf16 parts, x = p0 + p1 + p2: each `rows` rows of `cols` values, `pitch` values apart (a multiple of 8), one part behind the other.
 struct SplitMatrix { void* p; int64_t rows, cols, pitch; };
 inline int64_t split_pitch(int64_t cols) { return (cols + 7) / 8 * 8; }
-inline int64_t split_bytes(int64_t rows, int64_t cols) { return 3 * rows * split_pitch(cols) * 2; }
 
 // The parts of up to five matrices, in one launch.
 constexpr int SPLITS_MOST = 5;

@@ -57,7 +57,7 @@ struct PtArgs {
   int kb0, kb, splits;                     // stages of the first segment of k, of all, parts
   int ct;
   const void *bias, *bias2;
-  Hidden hidden; void *dg, *du; float* sums;
+  Hidden hidden; float* sums;
   const float *scale, *wscale, *bias_f; int y_f32;
   float* work;
   int* status; uint32_t wait_limit; int skip_loads;
@@ -704,7 +704,7 @@ int fovi::tc_hidden_grad(const TcMatrix& dy, const TcMatrix& wd, const Hidden& f
   a.kb0 = a.kb = (int)stages_of(dy.cols);
   a.splits = 1;
   a.ct = shape_of(&m, &n, 1, a.kb, 1, false).ct;
-  a.hidden = from; a.dg = dg; a.du = du; a.sums = sums;
+  a.hidden = from; a.sums = sums;
   int rc = tiles_of(a, 1);
   if (!rc) rc = map_k(&maps.a[0], dy, false, 128);
   if (!rc) rc = map_mn(&maps.b[0], wd);
