@@ -1,6 +1,7 @@
 // Float32 matrix products on the tensor cores.
 //
-// A float32 value is the sum of three bf16 values exactly: the value rounded to 8 bits, what is left rounded to 8 bits, and the rest.
+// A float32 value is the sum of three bf16 values exactly: the value rounded to 8 bits, what is left rounded to 8 bits, and the rest.  (Below 2^-110 the rest is below bf16's smallest value:
+// such values are taken to 2^-134.)
 // Of the nine products of two values' parts the six largest are taken; what is left out is at most 2^-24 of the product, a float32 product's own rounding.  The six are exact in the
 // tensor cores, whose sums lose up to a unit of float32 at each step: so a sum runs over 64 of k only (24 steps), and the sums of 64 are added in registers with float32's rounding.
 //   bound: six bf16 products for one, 375 of 2250 TFLOP/s, where the multiply-add units give 74.  1028 tokens, 384 x 1021 channels (one round of 40 tiles and less): projections 23 us,
@@ -244,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PS_THREADS, 1) produ
             }
           }
         }
-        tc_fence_before();
+        tc_fence_before();                         // (relaxed: see product_tc.cu)
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(pt_map(smem_u32(&hdr->acc_empty[acc]), 0)) : "memory");
         if (++acc == 2) { acc = 0; aph ^= 1u; }

@@ -5,7 +5,7 @@
 // A cluster of two CTAs shares a tile (tcgen05.mma with cta_group::2, M = 256): each stages its 128 rows of A and half of B's ct rows, 128 bytes of k (64 bf16, 128 integers) a stage,
 // by tensor copies.  An operand whose k is contiguous is K-major; one that lies the other way round (weights in the input gradients, both operands of a weight gradient) is read MN-major,
 // as 64-column boxes, so nothing is transposed in memory.  Two accumulators in tensor memory: a tile's epilogue runs under the next one's products.
-// Persistent: a pair takes every 74th tile.  Roles: warps 0-7 epilogue (a row per thread, the two halves take turns on 32-column chunks), warp 8 MMAs (of the pair's first CTA), warp 9 copies.
+// Persistent: of n pairs each takes every n-th tile.  Roles: warps 0-7 epilogue (a row per thread, the two halves take turns on 32-column chunks), warp 8 MMAs (of the pair's first CTA), warp 9 copies.
 // All waits are bounded.
 //
 // What becomes of a tile:
@@ -17,8 +17,8 @@
 //   STORE    bf16 result with a bias, or with k in parts a float32 part, joined by a second kernel in their order
 //   SCALED   integer sums times the scales
 // Where C is large the power limit bounds it: 16448 tokens, 1280 x 5120 channels, projections 1.30 PFLOP/s, down 1.32, input gradients 1.26, weight gradients 1.36 (from 1.2 to 1.3 sustained
-// for library products of these sizes), hidden gradients 0.95, whose tiles' arithmetic is longer than their products.  8-bit 16448 x 1280 -> 5120 in 97 us, 2.2 P a second: a stage's 64 KB
-// through L2 take as long as its products.
+// for library products of these sizes), hidden gradients 0.95, whose tiles' arithmetic is longer than their products.  8-bit 16448 x 1280 -> 5120 in 86 to 97 us, 2.2 to 2.5 P a
+// second: bound by the epilogue's stores, a row a thread in pieces of 32 bytes, 32 lines an instruction (62 us without them, 512 clocks a stage of 256 columns).
 #include <algorithm>
 
 #include "product_pair.cuh"
@@ -348,7 +348,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
       }
       if (!mbar_wait_warp(smem_u32(&hdr->acc_full[acc]), aph, abort_flag, a.status, 44, a.wait_limit)) break;
       tc_fence_after();
-      auto release = [&]() {                          // this warp has read the accumulator (relaxed: a release would wait for the warp's stores to arrive in memory)
+      // This warp has read the accumulator.  The arrival hands over tensor memory alone: the wait for the loads has put their values into registers, and the fences on both sides order the next products behind it.
+      // So it is relaxed: a release would also wait for the warp's stores to arrive in memory, which nobody behind this barrier reads.
+      auto release = [&]() {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(pt_map(smem_u32(&hdr->acc_empty[acc]), 0)) : "memory");

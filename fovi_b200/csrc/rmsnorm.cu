@@ -2,7 +2,8 @@
 //   y  = t * rstd * w                       rstd = 1 / sqrt(mean(t^2) + eps)
 //   dt = rstd * (g - th * mean(g * th)) + (the stream's own gradient)          g = dy * w, th = t * rstd;  dx = dresidual = dt
 //   dw = sum over rows of dy * th
-// or y in 8 bits: q = round(y / scale), scale = max(max |y| of the row / 127, the smallest normal number).  Sums and statistics are float32; y is not rounded before it is quantised.
+// or y in 8 bits: scale = max(max |y| of the row / 127, the smallest normal number), q = round(y * (1 / scale)): a reciprocal a row and a product a value,
+// beside a half one step from round(y / scale).  Sums and statistics are float32; y is not rounded before it is quantised.
 #include <algorithm>
 #include <type_traits>
 
@@ -133,7 +134,8 @@ __global__ void __launch_bounds__(1024) rms_norm_join_kernel(const float* part, 
 // ------------------------------------------------------------------------------------------------------------ rows in registers
 // A row is held in registers by a team of threads (rows.cuh), a warp or, where it is too long for one, a block; the next row's loads are issued before this row's sums.  One pass over memory
 // in both directions: the residual's sum, its norm and the 8-bit form with its scale come from the same registers, and the backward kernel keeps every column's part of dw over all its rows.
-// What bounds it is memory: 263168 x 384 bf16 with the residual 124 us forward (6.5 TB/s) and 129 to 151 backward (5.4 and more), 65792 x 1280 into 8 bits 101 (5.8).
+// What bounds it is memory: 263168 x 384 bf16 with the residual 124 us forward (6.5 TB/s) and 129 to 151 backward (5.4 and more), 65792 x 1280 into 8 bits 101 (5.8);
+// quantised without a norm 40 (6.3), from float32 81 (5.2).
 template <typename T, int VEC> __device__ __forceinline__ void store_eight(int8_t* p, const float* v, float inv) {
   if constexpr (VEC == 1) {
     p[0] = (int8_t)eight_bits(v[0], inv);
@@ -360,7 +362,8 @@ struct Shape { int vec, ch, threads; bool block; };
 
 // Every operand is (address, stride of rows in values, size of a value).
 struct Rows { const void* p; int64_t stride; int size; };
-// most: how many values a thread of a warp holds at most; beyond, a block holds the row, 8 values a thread (bf16 from 8192 and float32 from 4096 channels on more threads than a block has: none).
+// most: how many values a thread of a warp holds at most; beyond, a block holds the row, 8 values a thread: up to 8192 channels in pieces of four or eight values, up to 4096 in single ones (the threads that
+// a block has), in either type; above that none.
 template <int N> Shape shape_of(const Rows (&all)[N], int C, int size, int most) {
   auto fits = [&](int v) {
     if (C % v) return false;

@@ -506,7 +506,7 @@ int fovi_attention_backward_selftest_wait_timeout(const void* q, const void* k, 
  * apart), of total = x + residual rounded to their type, which is written (contiguous; NULL where residual is):  y = t / sqrt(mean(t^2) + eps) * weight.
  * weight: DEVICE float32 [C] or NULL.  Either y (contiguous, same type), or q and scale: the result in 8 bits, y = q * scale, scale = max(max |y| / 127, smallest normal
  * number) of the row, q rounded from the unrounded y; rows of q q_stride bytes apart.  C up to 2^30.  A row that holds infinity or not-a-number has one of them as its scale.
- * rstd: float32 [rows], 1 / sqrt(mean(t^2) + eps), or NULL. */
+ * rstd: float32 [rows], 1 / sqrt(mean(t^2) + eps), or NULL.  What is written overlaps nothing that is read (long rows are read several times). */
 int fovi_rms_norm_forward(const void* x, int dtype, int64_t rows, int C, int64_t x_stride, const void* residual, int64_t residual_stride, const float* weight, float eps,
                           void* total, void* y, int8_t* q, int64_t q_stride, float* scale, float* rstd, void* stream);
 /* Its gradients from t (x, or total), dy (rows dy_stride apart), the gradient dt of total itself (or NULL) and the forward's rstd, all of one type: dx (contiguous; the residual's
